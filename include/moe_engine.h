@@ -217,6 +217,11 @@ typedef struct moe_layer_desc {
   const void *shared;    /* device: resident shared expert in slot layout, or NULL */
 } moe_layer_desc;
 int moe_set_layer(moe_engine *eng, int layer, const moe_layer_desc *desc);
+/* After moe_set_layer: the layer routes by this rule (moe_group_topk) instead of route_mode; bias: device fp32 [num_expert]
+ * or NULL, kept valid by the caller as long as the layer runs.  NULL rule: back to route_mode, as a new moe_set_layer does.
+ * The layer's decode steps take their gate logits and the routing as launches of their own.  The reference leaves routers to
+ * the model's own module. */
+int moe_set_layer_routing(moe_engine *eng, int layer, const moe_route_rule *rule_host, const float *bias);
 /* allocate the forward workspace for up to max_tokens tokens per call */
 int moe_forward_prepare(moe_engine *eng, int max_tokens);
 /* y[T,H] = MoE layer `layer` applied to x[T,H] (device bf16) on the compute stream:

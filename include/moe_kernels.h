@@ -104,6 +104,25 @@ int moe_gate_logits_pair(const void *x_bf16, const void *wg_bf16, const float *b
 int moe_topk(const float *logits, int T, int E, int ldl, int k, int mode, int *idx, float *w,
              void *stream);
 
+/* k1b for routers with groups of experts, sigmoid scores or a selection bias (E <= 256, k <= 32, n_group <= 64 groups of
+ * E / n_group consecutive experts each).  Scores s: softmax over E, or sigmoid.  The experts are ordered by c = s + bias (bias
+ * [E] fp32 or NULL).  A group is worth its largest c, or the sum of its two largest; the topk_group groups worth most are
+ * kept, and the k largest c in them are chosen, descending.  w = s of the choice, / their sum if renorm, * scale.  Ties: the
+ * lower group, the lower expert.  Scores and comparisons are in 64 bits, w is rounded once.
+ * A NaN logit counts as -inf; a row of nothing else has weights 0 under softmax.  A c that is NaN (a NaN bias, +inf under
+ * softmax, whose scores and weights are NaN) is ordered behind the others.  k different experts come out in every case.
+ * No reference counterpart (its routers are torch's). */
+#define MOE_SCORES_SOFTMAX 0
+#define MOE_SCORES_SIGMOID 1
+#define MOE_GROUP_MAX 0
+#define MOE_GROUP_TOP2 1 /* groups of at least two experts */
+typedef struct moe_route_rule {
+  int scores, n_group, topk_group, group_value, renorm;
+  float scale;
+} moe_route_rule;
+int moe_group_topk(const float *logits, int T, int E, int ldl, int k, const moe_route_rule *rule_host, const float *bias,
+                   int *idx, float *w, void *stream);
+
 /* one active routed expert of a layer call */
 typedef struct moe_unit {
   int32_t expert; /* expert id, -1 = unused entry */
@@ -161,6 +180,13 @@ int moe_topk_dispatch(const float *logits, int T, int E, int ldl, int k, int mod
                       moe_unit *units, int *n_active, int64_t *active_ids, int max_units,
                       moe_unit *units_host_out, int *n_active_host_out, int *seq_host_out, int seq_value,
                       void *stream);
+
+/* moe_topk_dispatch with a rule (moe_group_topk): one launch for T <= 64, T*k <= 512; the arrays of moe_dispatch. */
+int moe_group_topk_dispatch(const float *logits, int T, int E, int ldl, int k, const moe_route_rule *rule_host,
+                            const float *bias, int *idx, float *w, int *counts, int *offsets, int *sorted_pair,
+                            int *pos_of_pair, int *sorted_tok, moe_unit *units, int *n_active, int64_t *active_ids,
+                            int max_units, moe_unit *units_host_out, int *n_active_host_out, int *seq_host_out,
+                            int seq_value, void *stream);
 
 /* k1a + k1b + k2 in one launch for decode batches (2 <= T <= 32, E <= 256, T*k <= 512): same results, bit for
  * bit, as moe_gate_logits + moe_topk_dispatch (reference: the gate's linear layer, the top-k and the expert
@@ -443,6 +469,32 @@ int moe_combine_splits(const float *part_r, const float *part_s, const float *to
 int moe_combine_windows(const float *part_r, const float *part_s, const float *topk_w,
                         const int *pos_of_pair, const float *shared_gate_logit, int sg_stride, void *y_bf16,
                         int T, int H, int k, int n_routed_splits, int n_shared_splits, void *stream);
+
+/* Products of the dense layers between the sparse blocks (the reference leaves them to torch):
+ *   moe_linear        y = act(x W^T + bias) + residual
+ *   moe_linear_gated  y = act(x Wg^T + b_gate) * (x Wu^T + b_up)
+ * x [M, K], W [N, K], biases [N], residual [M, N] all bf16 or all fp16 (dtype); y [M, N] of that type or fp32 (y_fp32).
+ * Sums, biases, activation, product and residual in fp32, one rounding at the end.  Rows are ldx, ldw, ldr and ldy elements apart
+ * (both matrices of a pair ldw).  K, ldx and ldw multiples of 8, ldx and ldw below 2^21, x and the matrices on 16-byte boundaries; M
+ * and N are any, 0 included.  bias, b_gate, b_up and residual may be NULL; residual may be y itself (same rows and type), y must not
+ * overlap anything else.
+ * ws: moe_linear_workspace_bytes(M, N, K, gated) of device memory, not shared by calls that overlap, with no contents to keep; a
+ * smaller one or NULL is refused where that number is not 0. */
+#define MOE_DT_BF16 0
+#define MOE_DT_FP16 1
+#define MOE_ACT_NONE 0
+#define MOE_ACT_SILU 1      /* v / (1 + e^-v) */
+#define MOE_ACT_GELU 2      /* v (1 + erf(v / sqrt 2)) / 2 */
+#define MOE_ACT_GELU_TANH 3 /* v (1 + tanh(sqrt(2 / pi) (v + 0.044715 v^3))) / 2 */
+#define MOE_ACT_RELU 4
+#define MOE_ACT_RELU2 5     /* max(v, 0)^2 */
+int64_t moe_linear_workspace_bytes(int M, int N, int K, int gated);
+int moe_linear(const void *x, int64_t ldx, const void *w, int64_t ldw, const void *bias, const void *residual, int64_t ldr,
+               void *y, int64_t ldy, int M, int N, int K, int dtype, int act, int y_fp32, void *ws, int64_t ws_bytes,
+               void *stream);
+int moe_linear_gated(const void *x, int64_t ldx, const void *w_gate, const void *w_up, int64_t ldw, const void *b_gate,
+                     const void *b_up, void *y, int64_t ldy, int M, int N, int K, int dtype, int act, int y_fp32, void *ws,
+                     int64_t ws_bytes, void *stream);
 
 /* Per-kernel timing with HIP events recorded on the launch stream around every kernel
  * the launchers below start (no reference counterpart; used by the benchmark to report

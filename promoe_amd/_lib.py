@@ -22,6 +22,10 @@ lib = C.CDLL(LIB_PATH)
 
 MOE_OK, MOE_EINVAL, MOE_EHIP, MOE_ESTATE, MOE_ENOMEM, MOE_ENOTRESIDENT = 0, -1, -2, -3, -4, -5
 ROUTE_SOFTMAX_TOPK, ROUTE_SOFTMAX_TOPK_RENORM, ROUTE_TOPK_SOFTMAX = 0, 1, 2
+DTYPES = {torch.bfloat16: 0, torch.float16: 1}
+ACTS = {"none": 0, "silu": 1, "gelu": 2, "gelu_tanh": 3, "relu": 4, "relu2": 5}
+SCORES = {"softmax": 0, "sigmoid": 1}
+GROUP_VALUES = {"max": 0, "top2": 1}
 FMT_INT4_G128, FMT_BF16, FMT_Q4K = 0, 1, 2
 
 vp, i32, i64, u64 = C.c_void_p, C.c_int, C.c_int64, C.c_uint64
@@ -30,6 +34,11 @@ vp, i32, i64, u64 = C.c_void_p, C.c_int, C.c_int64, C.c_uint64
 class Int4Layout(C.Structure):
     _fields_ = [(n, i64) for n in ("off13_q", "off13_s", "off13_z", "off2_q", "off2_s", "off2_z",
                                    "total_bytes")]
+
+
+class RouteRule(C.Structure):
+    _fields_ = [("scores", i32), ("n_group", i32), ("topk_group", i32), ("group_value", i32), ("renorm", i32),
+                ("scale", C.c_float)]
 
 
 class MoeError(RuntimeError):
@@ -45,6 +54,11 @@ def _sig(name, argtypes, restype=i32):
 
 _sig("moe_last_error", [], C.c_char_p)
 _sig("moe_int4_layout_make", [i32, i32, C.POINTER(Int4Layout)])
+_sig("moe_linear_workspace_bytes", [i32, i32, i32, i32], i64)
+_sig("moe_linear", [vp, i64, vp, i64, vp, vp, i64, vp, i64, i32, i32, i32, i32, i32, i32, vp, i64, vp])
+_sig("moe_linear_gated", [vp, i64, vp, vp, i64, vp, vp, vp, i64, i32, i32, i32, i32, i32, i32, vp, i64, vp])
+_sig("moe_group_topk", [vp, i32, i32, i32, i32, vp, vp, vp, vp, vp])
+_sig("moe_group_topk_dispatch", [vp, i32, i32, i32, i32, vp] + [vp] * 11 + [i32, vp, vp, vp, i32, vp])
 _sig("moe_gate_logits", [vp, vp, vp, vp, i32, i32, i32, i32, vp])
 _sig("moe_gate_logits_bias_rows", [vp, vp, vp, i32, vp, i32, i32, i32, i32, vp])
 _sig("moe_gate_logits_pair", [vp, vp, vp, vp, i32, i32, i32, i32, vp, vp, vp, i32, i32, vp])
@@ -177,6 +191,7 @@ _sig("moe_drain", [vp])
 _sig("moe_get_counters", [vp, C.POINTER(Counters)])
 _sig("moe_report", [vp, i32, C.c_char_p, i32])
 _sig("moe_set_layer", [vp, i32, C.POINTER(LayerDesc)])
+_sig("moe_set_layer_routing", [vp, i32, vp, vp])
 _sig("moe_forward_prepare", [vp, i32])
 _sig("moe_forward", [vp, i32, vp, i32, vp])
 _sig("moe_last_routing", [vp, pp, pp, pp])

@@ -676,6 +676,7 @@ extern "C" int moe_engine_create(const moe_cfg *cfg, int backend, void *compute_
   eng->layer_complete.assign(L, 0);
   eng->budget = cfg->max_prefetch_layer_distance;
   eng->layer_desc.resize(L);
+  eng->layer_routing.resize(L);
   for (auto &d : eng->layer_desc) memset(&d, 0, sizeof d);
   *out = eng;
   return MOE_OK;

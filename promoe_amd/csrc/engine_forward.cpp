@@ -104,6 +104,7 @@ extern "C" int moe_set_layer(moe_engine *eng, int layer, const moe_layer_desc *d
     return MOE_EINVAL;
   }
   eng->layer_desc[layer] = *d;
+  eng->layer_routing[layer] = LayerRouting();
   return MOE_OK;
 }
 
@@ -373,12 +374,12 @@ static int gate_parts_env() {
   static const int v = [] { const char *e = getenv("MOE_GATE_ROUTE"); return e ? atoi(e) : 1; }();
   return v;
 }
-static int route_batch(const moe_layer_desc &d, LayerState *s, const void *x, int T, int E, int k, int n_gate_rows, int ldl,
+static int route_batch(const moe_layer_desc &d, const LayerRouting &lr, LayerState *s, const void *x, int T, int E, int k, int n_gate_rows, int ldl,
                        int max_units, int layer, moe_unit *host_units, int *host_n, int *host_seq, int seq_val,
                        hipStream_t st) {
   int rc;
   const int parts = gate_parts_env();
-  if (T >= 2 && d.H % 8 == 0 && (parts == 1 || parts == 8) &&
+  if (!lr.set && T >= 2 && d.H % 8 == 0 && (parts == 1 || parts == 8) &&
       moe_gate_route_ws_bytes(T, n_gate_rows) <= (int64_t)s->gate_ws_bytes) {
     s->gate_seq = s->gate_seq < 0x7fffffff ? s->gate_seq + 1 : 1;
     return moe_gate_topk_dispatch(x, d.gate_w, d.gate_bias, d.gate_bias ? E : 0, s->logits, T, d.H, E, n_gate_rows, ldl, k,
@@ -388,6 +389,10 @@ static int route_batch(const moe_layer_desc &d, LayerState *s, const void *x, in
   }
   // the bias covers the routed experts only; the shared-gate row (row E) has none
   if ((rc = moe_gate_logits_bias_rows(x, d.gate_w, d.gate_bias, E, s->logits, T, d.H, n_gate_rows, ldl, st))) return rc;
+  if (lr.set)
+    return lr.topk_dispatch(s->logits, T, E, ldl, k, &lr.rule, lr.bias, s->idx, s->topk_w, s->counts, s->offsets, s->sorted_pair,
+                            s->pos_of_pair, s->sorted_tok, s->units, s->n_active, s->active_ids, max_units, host_units, host_n,
+                            host_seq, seq_val, st);
   return moe_topk_dispatch(s->logits, T, E, ldl, k, d.route_mode, s->idx, s->topk_w, s->counts, s->offsets,
                            s->sorted_pair, s->pos_of_pair, s->sorted_tok, s->units, s->n_active, s->active_ids,
                            max_units, host_units, host_n, host_seq, seq_val, st);
@@ -410,9 +415,9 @@ static int route_batch(const moe_layer_desc &d, LayerState *s, const void *x, in
 //   1024 x 512, 16 experts top-2                 21.5 / 16.6   20.8 / 17.8    27.6 / 23.8
 //   4096 x 14336, 8 experts top-2               123.5 / 118.1 329.4 / 330.2  389.5 / 388.6  390.7 / 397.1   436.8 / 441.4
 //   2048 x 768, 128 experts top-8                34.7 / 30.7   70.7 / 68.6    94.8 / 95.1   111.9 / 116.6   143.0 / 147.9
-static bool batch_routes_in_w13(const moe_layer_desc &d, const LayerState *s, int T, int E, int k, int n_gate_rows) {
+static bool batch_routes_in_w13(const moe_layer_desc &d, const LayerRouting &lr, const LayerState *s, int T, int E, int k, int n_gate_rows) {
   static const bool on = [] { const char *e = getenv("MOE_BATCH_ROUTE"); return !e || atoi(e) != 0; }();
-  if (!on || moe_gate_route_ws_bytes(T, n_gate_rows) > (int64_t)s->gate_ws_bytes) return false;
+  if (!on || lr.set || moe_gate_route_ws_bytes(T, n_gate_rows) > (int64_t)s->gate_ws_bytes) return false;
   if (d.fmt == MOE_FMT_BF16)
     return T <= 32 && T * k <= 512 && (T <= 4 || (E <= 64 && (T <= 8 || d.I_sh > 0))) &&
            moe_decode_batch_int4_gate_fits(2, E, k, d.H, d.I, d.I_sh, n_gate_rows);
@@ -426,6 +431,7 @@ extern "C" int moe_forward(moe_engine *eng, int layer, const void *x, int T, voi
   if (layer < 0 || layer >= eng->cfg.num_layer || !x || !y || T <= 0) { moe_set_error("moe_forward: bad argument"); return MOE_EINVAL; }
   LayerState *s = eng->fw;
   const moe_layer_desc &d = eng->layer_desc[layer];
+  const LayerRouting &lr = eng->layer_routing[layer];  // (its routing is a launch of its own: no launch that routes by itself)
   if (!s || !d.gate_w) { moe_set_error("moe_forward: layer %d not described or workspace not prepared", layer); return MOE_ESTATE; }
   if (T > s->max_tokens) { moe_set_error("moe_forward: T=%d exceeds the prepared workspace (%d)", T, s->max_tokens); return MOE_EINVAL; }
   if (!eng->launched) { moe_set_error("engine not launched"); return MOE_ESTATE; }
@@ -438,7 +444,7 @@ extern "C" int moe_forward(moe_engine *eng, int layer, const void *x, int T, voi
   // the layer hook's pre_forward: this block's input (decode: what the built-in predictor reads)
   if ((rc = moe_forward_check_kernels(eng))) return rc;  // of earlier calls: the words arrive without a copy
   // (a one-token step that will launch its gate kernel below takes the predictor's score rows into that launch)
-  const bool token_kernels = T == 1 && d.fmt == MOE_FMT_INT4_G128 && E <= 256 && k <= 32 &&
+  const bool token_kernels = T == 1 && !lr.set && d.fmt == MOE_FMT_INT4_G128 && E <= 256 && k <= 32 &&
                              eng->cfg.early_preempt && eng->cfg.reorder_experts && (size_t)d.H * 2 + 8192 <= 60 * 1024;
   const void *pred_w = nullptr; const float *pred_b = nullptr; float *pred_out = nullptr; int pred_rows = 0;
   bool pred_fused = token_kernels && moe_predictor_fused_rows(eng, layer, d.H, &pred_w, &pred_b, &pred_out, &pred_rows);
@@ -457,7 +463,7 @@ extern "C" int moe_forward(moe_engine *eng, int layer, const void *x, int T, voi
     all_resident = eng->cfg.per_layer_cache && eng->cfg.early_preempt && (int)eng->group_of(layer).full_len == E &&
                    eng->layer_complete[layer] == E && !eng->predictor_attached;
   }
-  if (all_resident && T == 1 && d.fmt == MOE_FMT_INT4_G128 && E <= 256 && k <= 32 && (size_t)d.H * 2 + 8192 <= 60 * 1024) {
+  if (all_resident && T == 1 && !lr.set && d.fmt == MOE_FMT_INT4_G128 && E <= 256 && k <= 32 && (size_t)d.H * 2 + 8192 <= 60 * 1024) {
     // one token: the w13 launch computes the gate logits in its first workgroups and routes by itself (no gate,
     // top-k or dispatch launches): two launches per step
     const uint64_t *table = nullptr;
@@ -665,7 +671,7 @@ extern "C" int moe_forward(moe_engine *eng, int layer, const void *x, int T, voi
   }
   bool routed_by_tail = false, w13_publishes = false;
   int tail_seq = 0, host_seq = 0;  // host_seq != 0: the unit list comes to units_host with this value in *opt_seq
-  if (all_resident && batch_routes_in_w13(d, s, T, E, k, n_gate_rows)) {
+  if (all_resident && batch_routes_in_w13(d, lr, s, T, E, k, n_gate_rows)) {
     // 2 to 16 tokens (bf16: 1 to 32), nothing for the host to decide: the w13 launch sums the gate rows, routes by itself and hands
     // the unit list to the host through the pending slot's pinned memory; then w2 and the combine (three launches)
     LayerState::Pending &p = s->pend[s->pend_head];
@@ -713,7 +719,7 @@ extern "C" int moe_forward(moe_engine *eng, int layer, const void *x, int T, voi
   // time is in the copies, which start no earlier this way, and the recomputed units cost more than the wait saved:
   // 16 tokens at cache rate 0.375 370 -> 379 us per step, at 0.97 85 -> 77)
   if (!all_resident && batch_spec_on && eng->cfg.early_preempt && eng->cfg.reorder_experts &&
-      d.fmt == MOE_FMT_INT4_G128 && (T <= 8 || s->late_last[layer] <= 1) && batch_routes_in_w13(d, s, T, E, k, n_gate_rows)) {
+      d.fmt == MOE_FMT_INT4_G128 && (T <= 8 || s->late_last[layer] <= 1) && batch_routes_in_w13(d, lr, s, T, E, k, n_gate_rows)) {
     // 2 to 16 tokens that may meet non-resident experts: as for one token, the expert launches go out BEFORE the host
     // knows the routing.  The self-routing w13 launch and the w2 launch behind it compute what is resident (a unit
     // whose table entry is 0 is skipped and raises the loose error word) and hand the unit list to the host, which
@@ -819,7 +825,7 @@ extern "C" int moe_forward(moe_engine *eng, int layer, const void *x, int T, voi
     // the unit list reaches the host from the w13 launch where that one can carry it (its stores to pinned memory
     // hold the routing launch for about 2 us, and nothing in the w13 launch waits for them), else from here
     w13_publishes = launch_publishes(d, T, max_units);
-    if ((rc = route_batch(d, s, x, T, E, k, n_gate_rows, ldl, max_units, layer, w13_publishes ? nullptr : pn.units,
+    if ((rc = route_batch(d, lr, s, x, T, E, k, n_gate_rows, ldl, max_units, layer, w13_publishes ? nullptr : pn.units,
                           w13_publishes ? nullptr : pn.n_active, w13_publishes ? nullptr : pn.seq, tail_seq, st)))
       return rc;
     routed_by_tail = true;
@@ -828,13 +834,18 @@ extern "C" int moe_forward(moe_engine *eng, int layer, const void *x, int T, voi
     // top-k + dispatch in one launch that stores the unit list into pinned host memory and, behind it, a sequence
     // word; the host polls the word below.  Two copies, an event and a blocking wait for it took 15-20 us per step.
     host_seq = ++s->seq_counter;
-    if ((rc = route_batch(d, s, x, T, E, k, n_gate_rows, ldl, max_units, layer, s->units_host, s->n_active_host, s->opt_seq,
+    if ((rc = route_batch(d, lr, s, x, T, E, k, n_gate_rows, ldl, max_units, layer, s->units_host, s->n_active_host, s->opt_seq,
                           host_seq, st)))
       return rc;
   } else {
     // the bias covers the routed experts only; the shared-gate row (row E) has none
     if ((rc = moe_gate_logits_bias_rows(x, d.gate_w, d.gate_bias, E, s->logits, T, d.H, n_gate_rows, ldl, st))) return rc;
-    if ((rc = moe_topk_dispatch_ws(s->logits, T, E, ldl, k, d.route_mode, s->idx, s->topk_w, s->counts, s->offsets,
+    if (lr.set) {
+      if ((rc = lr.topk(s->logits, T, E, ldl, k, &lr.rule, lr.bias, s->idx, s->topk_w, st))) return rc;
+      if ((rc = moe_dispatch_ws(s->idx, T, k, E, s->counts, s->offsets, s->sorted_pair, s->pos_of_pair, s->sorted_tok, s->units,
+                                s->n_active, s->active_ids, max_units, s->disp_ws, s->disp_ws_bytes, s->err_host + layer, st)))
+        return rc;
+    } else if ((rc = moe_topk_dispatch_ws(s->logits, T, E, ldl, k, d.route_mode, s->idx, s->topk_w, s->counts, s->offsets,
                                    s->sorted_pair, s->pos_of_pair, s->sorted_tok, s->units, s->n_active, s->active_ids,
                                    max_units, s->disp_ws, s->disp_ws_bytes, s->err_host + layer, st)))
       return rc;

@@ -203,6 +203,16 @@ struct Series { std::vector<uint64_t> v; };
 struct LayerState;  // forward workspace, engine_forward.cpp
 struct PredictorState;  // built-in predictor, engine_predict.cpp
 
+// A layer whose router has groups of experts, sigmoid scores or a selection bias (moe_set_layer_routing): the rule, and the launches
+// that follow it, which the layer brings along (a build without device code has neither)
+struct LayerRouting {
+  bool set = false;
+  moe_route_rule rule{};
+  const float *bias = nullptr;
+  decltype(&moe_group_topk) topk = nullptr;
+  decltype(&moe_group_topk_dispatch) topk_dispatch = nullptr;
+};
+
 struct moe_engine {
   moe_cfg cfg;
   std::unique_ptr<Backend> be;
@@ -252,6 +262,7 @@ struct moe_engine {
 
   // fused forward
   std::vector<moe_layer_desc> layer_desc;
+  std::vector<LayerRouting> layer_routing;
   LayerState *fw = nullptr;
   PredictorState *pred = nullptr;
 

@@ -5,6 +5,8 @@ hand-written HIP kernel from libmoe_engine.so on torch's current stream.
 """
 from __future__ import annotations
 
+from ctypes import byref
+
 import torch
 
 from . import _lib as L
@@ -54,6 +56,78 @@ def topk(logits: torch.Tensor, k: int, mode: int = L.ROUTE_SOFTMAX_TOPK, E: int 
     check(lib.moe_topk(ptr(_dev(logits)), T, E, logits.stride(0), k, mode, ptr(idx), ptr(w),
                        cur_stream()), "moe_topk")
     return idx, w
+
+
+class RouteRule(L.RouteRule):
+    """How group_topk routes.  scores: "softmax" (over all experts) or "sigmoid"; n_group groups of consecutive experts of which
+    the topk_group best are kept, by their largest score plus bias ("max") or the sum of the two largest ("top2"); renorm: the
+    weights are divided by their sum; scale multiplies them."""
+
+    def __init__(self, scores: str = "softmax", n_group: int = 1, topk_group: int = 1, group_value: str = "max",
+                 renorm: bool = False, scale: float = 1.0):
+        if scores not in L.SCORES or group_value not in L.GROUP_VALUES:
+            raise L.MoeError("RouteRule: scores must be one of %s and group_value one of %s" % (sorted(L.SCORES),
+                                                                                               sorted(L.GROUP_VALUES)))
+        super().__init__(L.SCORES[scores], n_group, topk_group, L.GROUP_VALUES[group_value], int(bool(renorm)), scale)
+
+
+def _operands(what: str, *tensors):
+    """Tensors of a call (None among them): on one GPU, and none that a gradient is expected of."""
+    dev = tensors[0].device
+    if dev.type != "cuda":
+        raise L.MoeError("%s: tensors of a GPU are needed, not of %s" % (what, dev))
+    for t in tensors:
+        if t is None:
+            continue
+        if t.device != dev:
+            raise L.MoeError("%s: tensors of %s and of %s" % (what, dev, t.device))
+        if t.requires_grad and torch.is_grad_enabled():
+            raise L.MoeError("%s has no gradient: call it under torch.no_grad() or with detached tensors" % what)
+    return dev
+
+
+def _route_args(what, logits, k, rule, bias):
+    """(device, T, E, row stride) of a routing call."""
+    if logits.dim() != 2 or logits.dtype != torch.float32 or (logits.shape[1] > 1 and logits.stride(1) != 1):
+        raise L.MoeError("%s: logits must be fp32 [T, E] with the experts of a row side by side" % what)
+    if not isinstance(rule, L.RouteRule):
+        raise L.MoeError("%s: rule must be a RouteRule" % what)
+    dev = _operands(what, logits, bias)
+    T, E = logits.shape
+    if bias is not None and (bias.dtype != torch.float32 or bias.shape != (E,) or not bias.is_contiguous()):
+        raise L.MoeError("%s: bias must be fp32 [%d], contiguous" % (what, E))
+    return dev, T, E, logits.stride(0) if T > 1 else E
+
+
+def group_topk(logits: torch.Tensor, k: int, rule: RouteRule, bias: torch.Tensor | None = None):
+    """Routing with groups of experts and a selection bias (moe_group_topk): logits fp32 [T, E] (rows may be further apart: a
+    slice in front of a shared expert's gate column) -> (idx [T, k] int32, w [T, k] fp32).  The bias [E] takes part in the
+    choice, not in the weights."""
+    dev, T, E, ldl = _route_args("group_topk", logits, k, rule, bias)
+    if dev.index != torch.cuda.current_device():
+        with torch.cuda.device(dev):
+            return group_topk(logits, k, rule, bias)
+    idx = torch.empty(T, k, dtype=torch.int32, device=dev)
+    w = torch.empty(T, k, dtype=torch.float32, device=dev)
+    check(lib.moe_group_topk(logits.data_ptr(), T, E, ldl, k, byref(rule), ptr(bias), idx.data_ptr(), w.data_ptr(), cur_stream()),
+          "moe_group_topk")
+    return idx, w
+
+
+def group_topk_dispatch(logits: torch.Tensor, k: int, rule: RouteRule, bias: torch.Tensor | None = None):
+    """group_topk and the stable dispatch in one launch for T <= 64 and T*k <= 512.  Returns (idx, w, Dispatch)."""
+    dev, T, E, ldl = _route_args("group_topk_dispatch", logits, k, rule, bias)
+    if dev.index != torch.cuda.current_device():
+        with torch.cuda.device(dev):
+            return group_topk_dispatch(logits, k, rule, bias)
+    idx = torch.empty(T, k, dtype=torch.int32, device=dev)
+    w = torch.empty(T, k, dtype=torch.float32, device=dev)
+    d = Dispatch(T, k, E, min(E, T * k), dev)
+    check(lib.moe_group_topk_dispatch(logits.data_ptr(), T, E, ldl, k, byref(rule), ptr(bias), ptr(idx), ptr(w), ptr(d.counts),
+                                      ptr(d.offsets), ptr(d.sorted_pair), ptr(d.pos_of_pair), ptr(d.sorted_tok), ptr(d.units),
+                                      ptr(d.n_active), ptr(d.active_ids), d.max_units, 0, 0, 0, 0, cur_stream()),
+          "moe_group_topk_dispatch")
+    return idx, w, d
 
 
 class Dispatch:
@@ -406,3 +480,74 @@ def combine(part_r, part_s, topk_w, pos_of_pair, shared_gate_logit, T: int, H: i
                                   ptr(shared_gate_logit), sg_stride, ptr(out), T, H, k, routed_pieces, n_splits, cur_stream()),
           "moe_combine")
     return out
+
+
+def _rows(what: str, t: torch.Tensor, cols: int) -> int:
+    """Elements between the rows of a [R, cols] matrix whose rows are whole."""
+    if t.dim() != 2 or t.shape[1] != cols or (cols > 1 and t.stride(1) != 1):
+        raise L.MoeError("%s: a matrix of whole rows of %d columns is needed, not %s with strides %s"
+                         % (what, cols, tuple(t.shape), t.stride()))
+    return t.stride(0) if t.shape[0] > 1 else cols
+
+
+def _product(what, x, mats, biases, act, residual, out, out_dtype):
+    dt = L.DTYPES.get(x.dtype)
+    if dt is None or act not in L.ACTS:
+        raise L.MoeError("%s: bf16 or fp16 operands and one of the activations %s" % (what, sorted(L.ACTS)))
+    dev = _operands(what, x, *mats, *biases, residual, out)
+    if dev.index != torch.cuda.current_device():
+        with torch.cuda.device(dev):
+            return _product(what, x, mats, biases, act, residual, out, out_dtype)
+    if x.dim() != 2 or mats[0].dim() != 2:
+        raise L.MoeError("%s: x must be [M, K] and a matrix [N, K]" % what)
+    M, K = x.shape
+    N = mats[0].shape[0]
+    ldx, ldw = _rows(what, x, K), _rows(what, mats[0], K)
+    for m in mats:
+        if m.dtype != x.dtype or m.shape != (N, K) or _rows(what, m, K) != ldw:
+            raise L.MoeError("%s: matrices of one shape, row stride and type (%s)" % (what, x.dtype))
+    for b in biases:
+        if b is not None and (b.dtype != x.dtype or b.shape != (N,) or not b.is_contiguous()):
+            raise L.MoeError("%s: a bias must be %s [%d], contiguous" % (what, x.dtype, N))
+    ldr = 0
+    if residual is not None:
+        if residual.dtype != x.dtype or residual.dim() != 2 or residual.shape[0] != M:
+            raise L.MoeError("%s: the residual must be %s [%d, %d]" % (what, x.dtype, M, N))
+        ldr = _rows(what, residual, N)
+    if out is None:
+        out = torch.empty(M, N, dtype=out_dtype or x.dtype, device=dev)
+    elif out.dim() != 2 or out.shape[0] != M or (out_dtype is not None and out.dtype != out_dtype):
+        raise L.MoeError("%s: out must be [%d, %d] of the type asked for" % (what, M, N))
+    if out.dtype != x.dtype and out.dtype != torch.float32:
+        raise L.MoeError("%s: results are %s or fp32" % (what, x.dtype))
+    ldy = _rows(what, out, N)
+    ws = None
+    n_ws = lib.moe_linear_workspace_bytes(M, N, K, len(mats) - 1)
+    if n_ws:
+        ws = torch.empty(n_ws, dtype=torch.uint8, device=dev)
+    y32 = out.dtype == torch.float32
+    if len(mats) == 1:
+        check(lib.moe_linear(x.data_ptr(), ldx, mats[0].data_ptr(), ldw, ptr(biases[0]), ptr(residual), ldr, out.data_ptr(), ldy,
+                             M, N, K, dt, L.ACTS[act], y32, ptr(ws), n_ws, cur_stream()), "moe_linear")
+    else:
+        check(lib.moe_linear_gated(x.data_ptr(), ldx, mats[0].data_ptr(), mats[1].data_ptr(), ldw, ptr(biases[0]), ptr(biases[1]),
+                                   out.data_ptr(), ldy, M, N, K, dt, L.ACTS[act], y32, ptr(ws), n_ws, cur_stream()),
+              "moe_linear_gated")
+    return out
+
+
+def linear(x: torch.Tensor, w: torch.Tensor, bias: torch.Tensor | None = None, act: str = "none",
+           residual: torch.Tensor | None = None, out: torch.Tensor | None = None, out_dtype: torch.dtype | None = None):
+    """act(x w^T + bias) + residual in one pass (moe_linear): x [M, K], w [N, K], bias [N] and residual [M, N] all bf16 or all
+    fp16; act one of none, silu, gelu, gelu_tanh, relu, relu2.  Sums and epilogue in fp32, rounded once to the type of x (or left
+    in fp32: out_dtype).  K and the row strides of x and w are multiples of 8; rows of x, w, residual and out may be further apart
+    than they are long.  out may be the residual itself (added in place)."""
+    return _product("linear", x, (w,), (bias,), act, residual, out, out_dtype)
+
+
+def linear_gated(x: torch.Tensor, w_gate: torch.Tensor, w_up: torch.Tensor, b_gate: torch.Tensor | None = None,
+                 b_up: torch.Tensor | None = None, act: str = "silu", out: torch.Tensor | None = None,
+                 out_dtype: torch.dtype | None = None):
+    """act(x w_gate^T + b_gate) * (x w_up^T + b_up) in one pass (moe_linear_gated): the first half of a gated dense layer.  Types,
+    strides and activations as in linear."""
+    return _product("linear_gated", x, (w_gate, w_up), (b_gate, b_up), act, None, out, out_dtype)
