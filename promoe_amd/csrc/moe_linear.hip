@@ -3,6 +3,7 @@
 // fp32 sums, which are rounded once, to the type of y.
 #include <hip/hip_runtime.h>
 #include <stdint.h>
+#include <type_traits>
 
 #include "moe_common.h"
 #include "moe_kernels.h"
@@ -10,12 +11,21 @@
 
 typedef __bf16 bf16x8_t __attribute__((ext_vector_type(8)));
 typedef float f32x4_t __attribute__((ext_vector_type(4)));
+typedef float f32x16_t __attribute__((ext_vector_type(16)));
+typedef int lt_rsrc_t __attribute__((ext_vector_type(4)));
+// raw buffer resource over the 2 GiB from p on, as four scalars for the assembly below
+static __device__ __forceinline__ lt_rsrc_t lt_rsrc(const void *p) {
+  const unsigned long long u = (unsigned long long)p;
+  return lt_rsrc_t{(int)(u32)u, (int)(u32)(u >> 32), 0x7fffff00, 0x00020000};
+}
 
 struct LinArgs {
   const uint16_t *x, *w[2], *bias[2], *res;  // w[1]: the second matrix of a gated pair
   void *y;
   long long ldx, ldw, ldr, ldy;              // elements
   int M, N, K, act, y32;
+  int nm, nn;                                // tiles
+  int whole;                                 // rows of y and of the residual start on 16-byte boundaries
 };
 
 template <bool F16>
@@ -38,79 +48,225 @@ static __device__ __forceinline__ f32x4_t lin_mfma16(u32x4_t a, u32x4_t b, f32x4
 static __device__ __forceinline__ float lin_sigmoid(float v) {
   return __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(v * -1.44269504088896f));
 }
-static __device__ __forceinline__ float lin_act(int act, float v) {
+static __device__ __forceinline__ void lin_act8(int act, float (&v)[8]) {
   switch (act) {
-    case MOE_ACT_SILU: return v * lin_sigmoid(v);
-    case MOE_ACT_GELU: return 0.5f * v * erfcf(v * -0.70710678118654752f);
-    // (1 + tanh z) / 2 = 1 / (1 + e^-2z), z = sqrt(2 / pi) (v + 0.044715 v^3)
-    case MOE_ACT_GELU_TANH: return v * lin_sigmoid(1.5957691216057308f * v * fmaf(0.044715f * v, v, 1.f));
-    case MOE_ACT_RELU: return v <= 0.f ? 0.f : v;  // (a NaN stays one)
-    case MOE_ACT_RELU2: return v <= 0.f ? 0.f : v * v;
-    default: return v;
+    case MOE_ACT_SILU:
+#pragma unroll
+      for (int i = 0; i < 8; ++i) v[i] = v[i] * lin_sigmoid(v[i]);
+      break;
+    case MOE_ACT_GELU:
+      for (int i = 0; i < 8; ++i) v[i] = 0.5f * v[i] * erfcf(v[i] * -0.70710678118654752f);
+      break;
+    case MOE_ACT_GELU_TANH:  // (1 + tanh z) / 2 = 1 / (1 + e^-2z), z = sqrt(2 / pi) (v + 0.044715 v^3)
+#pragma unroll
+      for (int i = 0; i < 8; ++i) v[i] = v[i] * lin_sigmoid(1.5957691216057308f * v[i] * fmaf(0.044715f * v[i], v[i], 1.f));
+      break;
+    case MOE_ACT_RELU:       // (a NaN stays one)
+#pragma unroll
+      for (int i = 0; i < 8; ++i) v[i] = v[i] <= 0.f ? 0.f : v[i];
+      break;
+    case MOE_ACT_RELU2:
+#pragma unroll
+      for (int i = 0; i < 8; ++i) v[i] = v[i] <= 0.f ? 0.f : v[i] * v[i];
+      break;
+    default: break;
   }
 }
 
-// bias, activation, gate, residual and the one rounding of element (m, n)
+// Eight adjacent columns of the result from column n on (past N: left out): bias, activation, gate, residual and the one rounding
 template <bool F16, bool GATED>
-static __device__ __forceinline__ void lin_store(const LinArgs &a, int m, int n, float s0, float s1) {
-  if (a.bias[0]) s0 += lin_f32<F16>(a.bias[0][n]);
-  float v = lin_act(a.act, s0);
-  if constexpr (GATED) {
-    if (a.bias[1]) s1 += lin_f32<F16>(a.bias[1][n]);
-    v *= s1;
-  }
-  if (a.res) v += lin_f32<F16>(a.res[m * a.ldr + n]);
-  if (a.y32) ((float *)a.y)[m * a.ldy + n] = v;
-  else ((uint16_t *)a.y)[m * a.ldy + n] = lin_bits<F16>(v);
-}
-
-// A workgroup of four waves on a tile of 64 x 64 (gated: of both matrices), 32 columns of K at a time through LDS.  Rows past the
-// end read the last one and are not stored; columns past K are zeros on both sides.
-#define LN_T 64
-#define LN_K 32
-template <bool F16, bool GATED>
-__global__ __launch_bounds__(256) void k_linear(const LinArgs a) {
-  constexpr int NM = GATED ? 2 : 1;
-  __shared__ u32x4_t sx[LN_T][5], sw[NM][LN_T][5];  // four of five 16-byte chunks in use: rows 80 bytes apart
-  const int tid = threadIdx.x, lane = tid & 63, wv = tid >> 6, r = lane & 15, q = lane >> 4;
-  const int m0 = blockIdx.y * LN_T, n0 = blockIdx.x * LN_T, wm = (wv & 1) * 32, wn = (wv >> 1) * 32;
-  f32x4_t acc[NM][2][2] = {};
-  const int lr = tid >> 2, lc = tid & 3;  // the row and chunk this thread brings
-  const uint16_t *px = a.x + min(m0 + lr, a.M - 1) * a.ldx + 8 * lc;
-  const uint16_t *pw[NM];
+struct LinColumns {
+  int n, count;
+  float b0[8], b1[8];
+  __device__ __forceinline__ LinColumns(const LinArgs &a, int n_) : n(n_), count(min(8, a.N - n_)) {
 #pragma unroll
-  for (int i = 0; i < NM; ++i) pw[i] = a.w[i] + min(n0 + lr, a.N - 1) * a.ldw + 8 * lc;
-  for (int k = 0; k < a.K; k += LN_K) {
-    const bool in = k + 8 * lc < a.K;
-    const u32x4_t zero = {0, 0, 0, 0};
-    const u32x4_t vx = in ? *(const u32x4_t *)(px + k) : zero;
-    u32x4_t vw[NM];
-#pragma unroll
-    for (int i = 0; i < NM; ++i) vw[i] = in ? *(const u32x4_t *)(pw[i] + k) : zero;
-    __syncthreads();
-    sx[lr][lc] = vx;
-#pragma unroll
-    for (int i = 0; i < NM; ++i) sw[i][lr][lc] = vw[i];
-    __syncthreads();
-#pragma unroll
-    for (int bm = 0; bm < 2; ++bm) {
-      const u32x4_t fx = sx[wm + 16 * bm + r][q];
-#pragma unroll
-      for (int i = 0; i < NM; ++i)
-#pragma unroll
-        for (int bn = 0; bn < 2; ++bn) acc[i][bm][bn] = lin_mfma16<F16>(sw[i][wn + 16 * bn + r][q], fx, acc[i][bm][bn]);
+    for (int i = 0; i < 8; ++i) {
+      b0[i] = a.bias[0] && i < count ? lin_f32<F16>(a.bias[0][n + i]) : 0.f;
+      b1[i] = GATED && a.bias[1] && i < count ? lin_f32<F16>(a.bias[1][n + i]) : 0.f;
     }
   }
-  // element i of a lane: column 4 q + i of W's block, row r of x's
+  // s0, s1: the sums of row m (s1: of the second matrix)
+  __device__ __forceinline__ void store(const LinArgs &a, int m, const float *s0, const float *s1) const {
+    if (count <= 0) return;
+    float v[8];
 #pragma unroll
-  for (int bm = 0; bm < 2; ++bm)
+    for (int i = 0; i < 8; ++i) v[i] = s0[i] + b0[i];
+    lin_act8(a.act, v);
+    if constexpr (GATED) {
 #pragma unroll
-    for (int bn = 0; bn < 2; ++bn)
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const int m = m0 + wm + 16 * bm + r, n = n0 + wn + 16 * bn + 4 * q + i;
-        if (m < a.M && n < a.N) lin_store<F16, GATED>(a, m, n, acc[0][bm][bn][i], acc[NM - 1][bm][bn][i]);
+      for (int i = 0; i < 8; ++i) v[i] *= s1[i] + b1[i];
+    }
+    if (count == 8 && a.whole) {  // whole rows of 16-byte pieces
+      if (a.res) {
+        const u32x4_t r = *(const u32x4_t *)(a.res + m * a.ldr + n);
+        v[0] += lin_f32<F16>((uint16_t)r.x); v[1] += lin_f32<F16>((uint16_t)(r.x >> 16));
+        v[2] += lin_f32<F16>((uint16_t)r.y); v[3] += lin_f32<F16>((uint16_t)(r.y >> 16));
+        v[4] += lin_f32<F16>((uint16_t)r.z); v[5] += lin_f32<F16>((uint16_t)(r.z >> 16));
+        v[6] += lin_f32<F16>((uint16_t)r.w); v[7] += lin_f32<F16>((uint16_t)(r.w >> 16));
       }
+      if (a.y32) {
+        float *y = (float *)a.y + m * a.ldy + n;
+        *(f32x4_t *)y = f32x4_t{v[0], v[1], v[2], v[3]};
+        *(f32x4_t *)(y + 4) = f32x4_t{v[4], v[5], v[6], v[7]};
+      } else {
+        u32x4_t r;
+        r.x = lin_bits<F16>(v[0]) | (u32)lin_bits<F16>(v[1]) << 16; r.y = lin_bits<F16>(v[2]) | (u32)lin_bits<F16>(v[3]) << 16;
+        r.z = lin_bits<F16>(v[4]) | (u32)lin_bits<F16>(v[5]) << 16; r.w = lin_bits<F16>(v[6]) | (u32)lin_bits<F16>(v[7]) << 16;
+        *(u32x4_t *)((uint16_t *)a.y + m * a.ldy + n) = r;
+      }
+      return;
+    }
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+      if (i < count) {
+        if (a.res) v[i] += lin_f32<F16>(a.res[m * a.ldr + n + i]);
+        if (a.y32) ((float *)a.y)[m * a.ldy + n + i] = v[i];
+        else ((uint16_t *)a.y)[m * a.ldy + n + i] = lin_bits<F16>(v[i]);
+      }
+  }
+};
+
+// ---- tile kernel --------------------------------------------------------------------------------------------------------------
+// Four waves (2 x 2), wave (wm, wn) on WM x WN blocks of 32 x 32: a tile of 64 WM rows of x by 64 WN rows of W.  A gated pair's W
+// blocks alternate between the two matrices (block b: matrix b & 1, its columns 32 (b >> 1) ..), so that a lane holds both sums
+// of a column.  K advances 64 at a time (a slab); slabs go global -> LDS directly, two of them in LDS.
+#define LT_K 64
+#define LT_ROW 128  // bytes of a row of a slab: 8 chunks of 16, chunk c of row r in slot c ^ ((r >> 1) & 7)
+#define LT_OUT 0x7fffff00
+template <bool F16>
+static __device__ __forceinline__ f32x16_t lin_mfma32(u32x4_t a, u32x4_t b, f32x16_t c) {
+  if constexpr (F16) return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8_t, a), __builtin_bit_cast(f16x8_t, b), c, 0, 0, 0);
+  else return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8_t, a), __builtin_bit_cast(bf16x8_t, b), c, 0, 0, 0);
+}
+// s_waitcnt for all vector-memory operations and nothing else; for all LDS operations and nothing else
+#define LT_VM0() __builtin_amdgcn_s_waitcnt(0x0f70)
+#define LT_LGKM0() __builtin_amdgcn_s_waitcnt(0xc07f)
+
+template <bool F16, bool GATED, int WM, int WN>
+__global__ __launch_bounds__(256, WM * WN > 8 ? 1 : 2) void k_linear_tile(const LinArgs a) {
+  constexpr int BM = 64 * WM, BN = 64 * WN, NX = 2 * WM, NW = 2 * WN, SLAB = (BM + BN) * LT_ROW, NG = WM * WN;
+  __shared__ __align__(2 * SLAB) unsigned char s_ring[2 * SLAB];
+  const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6), wm = w & 1, wn = w >> 1;
+  const int fr = lane & 31, q = lane >> 5;
+  int mt, nt;
+  {  // workgroup i runs on XCD i % 8: each XCD takes a contiguous run of tiles, four rows of tiles wide
+    const int per = (int)gridDim.x >> 3, b = (blockIdx.x & 7) * per + (blockIdx.x >> 3);
+    if (b >= a.nm * a.nn) return;
+    const int group = b / (4 * a.nn), r = b - group * 4 * a.nn, rows = min(4, a.nm - 4 * group);
+    mt = 4 * group + r % rows;
+    nt = r / rows;
+  }
+  constexpr int NC = GATED ? BN / 2 : BN;  // columns of the result
+  const int m0 = mt * BM, n0 = nt * NC;
+  const unsigned lds = (unsigned)(uintptr_t)(__attribute__((address_space(3))) unsigned char *)s_ring;
+  // transfer t of wave w: rows 32 t + 8 w .. + 7, eight lanes a row; the lanes choose the chunk that belongs in their slot
+  const int tr = 8 * w + (lane >> 3), chunk = (lane & 7) ^ ((tr >> 1) & 7);
+  const lt_rsrc_t rx = lt_rsrc(a.x + m0 * a.ldx), rw0 = lt_rsrc(a.w[0] + n0 * a.ldw), rw1 = lt_rsrc(a.w[GATED ? 1 : 0] + n0 * a.ldw);
+  int vx[NX], vw[NW];
+#pragma unroll
+  for (int t = 0; t < NX; ++t) vx[t] = (min(m0 + 32 * t + tr, a.M - 1) - m0) * (int)a.ldx * 2 + 16 * chunk;
+#pragma unroll
+  for (int t = 0; t < NW; ++t) vw[t] = (min(n0 + 32 * (GATED ? t >> 1 : t) + tr, a.N - 1) - n0) * (int)a.ldw * 2 + 16 * chunk;
+  const int nk = (a.K + LT_K - 1) / LT_K;
+  auto dma = [&](int t, int kt, int slot) {
+    // (assembly: told that a load writes LDS, the compiler would wait for all of them in front of every barrier and LDS read;
+    // the waits stand by hand.  Columns past K, and slabs past the last, are out of the resource's range: zeros.)
+    const bool in = kt * LT_K + 8 * chunk < a.K;
+    const unsigned at = lds + (unsigned)(slot * SLAB + (t < NX ? t : t - NX) * 32 * LT_ROW + (t < NX ? 0 : BM * LT_ROW) + 8 * w * LT_ROW);
+    const int off = in ? (t < NX ? vx[t < NX ? t : 0] : vw[t < NX ? 0 : t - NX]) : LT_OUT;
+    const lt_rsrc_t rs = t < NX ? rx : (GATED && ((t - NX) & 1)) ? rw1 : rw0;
+    __asm__ volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, %3 offen lds"
+                     :: "s"(at), "v"(off), "s"(rs), "s"(kt * (LT_K * 2)) : "memory", "m0");
+  };
+  unsigned ax[4], aw[4];  // LDS address of the lane's fragment of step j in block 0 of the current slot
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    const unsigned c = (unsigned)(((4 * q + j) ^ ((fr >> 1) & 7)) * 16);
+    ax[j] = lds + (unsigned)((wm * WM * 32 + fr) * LT_ROW) + c;
+    aw[j] = lds + (unsigned)((BM + wn * WN * 32 + fr) * LT_ROW) + c;
+  }
+  typedef __attribute__((address_space(3))) const u32x4_t lds_u4;
+  auto read_x = [&](int j, int i) { return *(lds_u4 *)(uintptr_t)(ax[j] + (unsigned)(i * 32 * LT_ROW)); };
+  auto read_w = [&](int j, int i) { return *(lds_u4 *)(uintptr_t)(aw[j] + (unsigned)(i * 32 * LT_ROW)); };
+  f32x16_t acc[WM][WN];
+#pragma unroll
+  for (int i = 0; i < WM; ++i)
+#pragma unroll
+    for (int b = 0; b < WN; ++b)
+#pragma unroll
+      for (int e = 0; e < 16; ++e) acc[i][b][e] = 0.f;
+  u32x4_t fx[2][WM], fw[2][WN];
+#pragma unroll
+  for (int t = 0; t < NX + NW; ++t) dma(t, 0, 0);
+#pragma unroll
+  for (int t = 0; t < NX + NW; ++t) dma(t, 1, 1);
+  LT_VM0();
+  __syncthreads();
+#pragma unroll
+  for (int i = 0; i < WM; ++i) fx[0][i] = read_x(0, i);
+#pragma unroll
+  for (int i = 0; i < WN; ++i) fw[0][i] = read_w(0, i);
+  // slab kt in its slot.  The fragments of step j + 1 are read between the products of step j.  In front of step 3, whose fragments
+  // are the last of the slab, everybody has read the slab and slab kt + 1 has landed: behind that barrier its first fragments
+  // are read and slab kt + 2 is requested into this slot, one request behind a product.
+  int slot = 0;
+  for (int kt = 0; kt < nk; ++kt, slot ^= 1) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const int p = j & 1;
+      if (j == 3) {
+        LT_LGKM0();
+        LT_VM0();
+        __builtin_amdgcn_s_barrier();
+#pragma unroll
+        for (int i = 0; i < 4; ++i) { ax[i] ^= SLAB; aw[i] ^= SLAB; }  // (the ring starts on a multiple of its size)
+      }
+      __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+      for (int g = 0; g < NG; ++g) {
+        acc[g / WN][g % WN] = lin_mfma32<F16>(fw[p][g % WN], fx[p][g / WN], acc[g / WN][g % WN]);
+        __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+        for (int r = 0; r < WM + WN; ++r)
+          if (min(r, NG - 1) == g) {
+            if (r < WM) fx[p ^ 1][r] = read_x((j + 1) & 3, r);
+            else fw[p ^ 1][r - WM] = read_w((j + 1) & 3, r - WM);
+          }
+        if (j == 3) {
+#pragma unroll
+          for (int t = 0; t < NX + NW; ++t)
+            if (t * NG / (NX + NW) == g) dma(t, kt + 2, slot);
+        }
+        __builtin_amdgcn_sched_barrier(0);
+      }
+    }
+  }
+  // The sums leave through LDS, 32 rows of the wave at a time, so that a lane then has 8 adjacent columns of a row and the rest is
+  // one loop of whole lines.  Element e of a lane: column 8 (e / 4) + 4 q + e % 4 of W's block, row fr of x's.
+  LT_VM0();
+  __syncthreads();
+  constexpr int LDE = 32 * WN + 4;                       // floats between rows: 16 lanes that write 16 bytes each fall on all banks
+  constexpr int LPR = NC / 16, RPP = 64 / LPR;           // lanes of a row (8 columns each), rows of a pass
+  static_assert(4 * 32 * LDE * 4 <= 2 * SLAB, "the sums of four waves fit the ring");
+  float *buf = (float *)s_ring + w * 32 * LDE;
+  const int col = 8 * (lane % LPR), n = n0 + wn * (NC / 2) + col;
+  const int at = GATED ? (col >> 5) * 64 + (col & 31) : col;
+  const LinColumns<F16, GATED> c(a, n);
+#pragma unroll
+  for (int i = 0; i < WM; ++i) {
+#pragma unroll
+    for (int b = 0; b < WN; ++b)
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        *(f32x4_t *)(buf + fr * LDE + 32 * b + 8 * e + 4 * q) =
+            f32x4_t{acc[i][b][4 * e], acc[i][b][4 * e + 1], acc[i][b][4 * e + 2], acc[i][b][4 * e + 3]};
+    __builtin_amdgcn_wave_barrier();
+    for (int r = lane / LPR; r < 32; r += RPP) {
+      const int m = m0 + 32 * (wm * WM + i) + r;
+      if (m < a.M) c.store(a, m, buf + r * LDE + at, buf + r * LDE + at + 32);
+    }
+    __builtin_amdgcn_wave_barrier();
+  }
 }
 
 // ---- entry points -------------------------------------------------------------------------------------------------------------
@@ -132,9 +288,16 @@ static int lin_check(const char *who, const LinArgs &a, int dtype, bool gated) {
 
 template <bool F16, bool GATED>
 static int lin_launch(const LinArgs &a, hipStream_t s) {
-  const dim3 grid((a.N + LN_T - 1) / LN_T, (a.M + LN_T - 1) / LN_T);
-  hipLaunchKernelGGL(HIP_KERNEL_NAME(k_linear<F16, GATED>), grid, dim3(256), 0, s, a);
-  return moe_check_launch("k_linear");
+  LinArgs t = a;
+  t.whole = !(((uintptr_t)a.y | (uintptr_t)a.ldy * (a.y32 ? 4 : 2) | (uintptr_t)a.res | (a.res ? (uintptr_t)a.ldr * 2 : 0)) & 15);
+  if (a.M > 128) {
+    t.nm = (a.M + 255) / 256; t.nn = (a.N + (GATED ? 127 : 255)) / (GATED ? 128 : 256);
+    hipLaunchKernelGGL(HIP_KERNEL_NAME(k_linear_tile<F16, GATED, 4, 4>), dim3((t.nm * t.nn + 7) / 8 * 8), dim3(256), 0, s, t);
+  } else {
+    t.nm = (a.M + 127) / 128; t.nn = (a.N + (GATED ? 63 : 127)) / (GATED ? 64 : 128);
+    hipLaunchKernelGGL(HIP_KERNEL_NAME(k_linear_tile<F16, GATED, 2, 2>), dim3((t.nm * t.nn + 7) / 8 * 8), dim3(256), 0, s, t);
+  }
+  return moe_check_launch("k_linear_tile");
 }
 template <bool GATED>
 static int lin_run(const char *who, const LinArgs &a, int dtype, hipStream_t s) {
