@@ -12,11 +12,12 @@
 typedef __bf16 bf16x8_t __attribute__((ext_vector_type(8)));
 typedef float f32x4_t __attribute__((ext_vector_type(4)));
 typedef float f32x16_t __attribute__((ext_vector_type(16)));
+#define LT_OUT 0x7fffff00  // length of the buffer resources; a load from there on reads zeros
 typedef int lt_rsrc_t __attribute__((ext_vector_type(4)));
 // raw buffer resource over the 2 GiB from p on, as four scalars for the assembly below
 static __device__ __forceinline__ lt_rsrc_t lt_rsrc(const void *p) {
   const unsigned long long u = (unsigned long long)p;
-  return lt_rsrc_t{(int)(u32)u, (int)(u32)(u >> 32), 0x7fffff00, 0x00020000};
+  return lt_rsrc_t{(int)(u32)u, (int)(u32)(u >> 32), LT_OUT, 0x00020000};
 }
 
 struct LinArgs {
@@ -48,29 +49,41 @@ static __device__ __forceinline__ f32x4_t lin_mfma16(u32x4_t a, u32x4_t b, f32x4
 static __device__ __forceinline__ float lin_sigmoid(float v) {
   return __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(v * -1.44269504088896f));
 }
-static __device__ __forceinline__ void lin_act8(int act, float (&v)[8]) {
+template <int C>
+static __device__ __forceinline__ void lin_act(int act, float (&v)[C]) {
   switch (act) {
     case MOE_ACT_SILU:
 #pragma unroll
-      for (int i = 0; i < 8; ++i) v[i] = v[i] * lin_sigmoid(v[i]);
+      for (int i = 0; i < C; ++i) v[i] = v[i] * lin_sigmoid(v[i]);
       break;
     case MOE_ACT_GELU:
-      for (int i = 0; i < 8; ++i) v[i] = 0.5f * v[i] * erfcf(v[i] * -0.70710678118654752f);
+      for (int i = 0; i < C; ++i) v[i] = 0.5f * v[i] * erfcf(v[i] * -0.70710678118654752f);
       break;
     case MOE_ACT_GELU_TANH:  // (1 + tanh z) / 2 = 1 / (1 + e^-2z), z = sqrt(2 / pi) (v + 0.044715 v^3)
 #pragma unroll
-      for (int i = 0; i < 8; ++i) v[i] = v[i] * lin_sigmoid(1.5957691216057308f * v[i] * fmaf(0.044715f * v[i], v[i], 1.f));
+      for (int i = 0; i < C; ++i) v[i] = v[i] * lin_sigmoid(1.5957691216057308f * v[i] * fmaf(0.044715f * v[i], v[i], 1.f));
       break;
     case MOE_ACT_RELU:       // (a NaN stays one)
 #pragma unroll
-      for (int i = 0; i < 8; ++i) v[i] = v[i] <= 0.f ? 0.f : v[i];
+      for (int i = 0; i < C; ++i) v[i] = v[i] <= 0.f ? 0.f : v[i];
       break;
     case MOE_ACT_RELU2:
 #pragma unroll
-      for (int i = 0; i < 8; ++i) v[i] = v[i] <= 0.f ? 0.f : v[i] * v[i];
+      for (int i = 0; i < C; ++i) v[i] = v[i] <= 0.f ? 0.f : v[i] * v[i];
       break;
     default: break;
   }
+}
+
+// element (m, n): bias, activation, gate, residual and the one rounding
+template <bool F16, bool GATED>
+static __device__ __forceinline__ void lin_store(const LinArgs &a, int m, int n, float s0, float s1) {
+  float v[1] = {a.bias[0] ? s0 + lin_f32<F16>(a.bias[0][n]) : s0};
+  lin_act(a.act, v);
+  if constexpr (GATED) v[0] *= a.bias[1] ? s1 + lin_f32<F16>(a.bias[1][n]) : s1;
+  if (a.res) v[0] += lin_f32<F16>(a.res[m * a.ldr + n]);
+  if (a.y32) ((float *)a.y)[m * a.ldy + n] = v[0];
+  else ((uint16_t *)a.y)[m * a.ldy + n] = lin_bits<F16>(v[0]);
 }
 
 // Eight adjacent columns of the result from column n on (past N: left out): bias, activation, gate, residual and the one rounding
@@ -91,7 +104,7 @@ struct LinColumns {
     float v[8];
 #pragma unroll
     for (int i = 0; i < 8; ++i) v[i] = s0[i] + b0[i];
-    lin_act8(a.act, v);
+    lin_act(a.act, v);
     if constexpr (GATED) {
 #pragma unroll
       for (int i = 0; i < 8; ++i) v[i] *= s1[i] + b1[i];
@@ -116,15 +129,95 @@ struct LinColumns {
       }
       return;
     }
+    if (a.res) {
+      uint16_t r[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) r[i] = a.res[m * a.ldr + n + min(i, count - 1)];  // (all of them on their way at once)
+#pragma unroll
+      for (int i = 0; i < 8; ++i) v[i] += lin_f32<F16>(r[i]);
+    }
 #pragma unroll
     for (int i = 0; i < 8; ++i)
       if (i < count) {
-        if (a.res) v[i] += lin_f32<F16>(a.res[m * a.ldr + n + i]);
         if (a.y32) ((float *)a.y)[m * a.ldy + n + i] = v[i];
         else ((uint16_t *)a.y)[m * a.ldy + n + i] = lin_bits<F16>(v[i]);
       }
   }
 };
+
+// ---- few rows of x: the matrix streams past them --------------------------------------------------------------------------------
+// A workgroup of eight waves takes R = 16 / SH rows of W (gated: of both matrices), its waves the pieces of K in turn; their sums meet
+// in LDS.  Weights go from memory into the matrix core's operands: one v_mfma_f32_16x16x32 per 1 KiB.  With SH = 1 the 16 rows of
+// the operand are 16 rows of W; with few rows of x (M <= 16 / SH) the operand is R rows of W by SH pieces of K, row s R + r and column
+// s R + m hold piece s of both, and the products of unlike pieces are left unread: a smaller unit of work (more workgroups for a
+// short matrix) and longer runs of a row per load.
+// MB: blocks of 16 rows of x.
+#define LR_WAVES 8
+#define LR_U 4  // loads of a matrix in flight per wave, twice
+template <bool F16, bool GATED, int MB, int SH>
+__global__ __launch_bounds__(64 * LR_WAVES) void k_linear_rows(const LinArgs a) {
+  constexpr int NM = GATED ? 2 : 1, R = 16 / SH, STEP = 32 * SH * LR_U, SPAN = STEP * LR_WAVES;
+  __shared__ f32x4_t red[LR_WAVES][NM][MB][64];
+  const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int r = (lane & 15) % R, s = (lane & 15) / R, n0 = blockIdx.x * R;
+  const int k0 = 8 * ((lane >> 4) * SH + s);                    // the lane's columns inside 32 SH
+  const rsrc_t rx = make_rsrc(a.x, LT_OUT), rw0 = make_rsrc(a.w[0] + n0 * a.ldw, LT_OUT), rw1 = make_rsrc(a.w[GATED ? 1 : 0] + n0 * a.ldw, LT_OUT);
+  const int vw = (min(n0 + r, a.N - 1) - n0) * (int)a.ldw * 2;
+  int vx[MB];
+#pragma unroll
+  for (int b = 0; b < MB; ++b) vx[b] = min(16 * b + r, a.M - 1) * (int)a.ldx * 2;
+  f32x4_t acc[NM][MB] = {};
+  uint4 fw[2][NM][LR_U], fx[2][MB][LR_U];
+  auto load = [&](int p, int base) {
+#pragma unroll
+    for (int u = 0; u < LR_U; ++u) {
+      const int k = base + 32 * SH * u + k0;
+      const bool in = k < a.K;                                  // past the end: zeros on both sides
+      fw[p][0][u] = bload16(rw0, in ? vw + 2 * k : LT_OUT, 0);
+      if constexpr (GATED) fw[p][1][u] = bload16(rw1, in ? vw + 2 * k : LT_OUT, 0);
+#pragma unroll
+      for (int b = 0; b < MB; ++b) fx[p][b][u] = bload16(rx, in ? vx[b] + 2 * k : LT_OUT, 0);
+    }
+  };
+  auto use = [&](int p) {
+#pragma unroll
+    for (int u = 0; u < LR_U; ++u)
+#pragma unroll
+      for (int i = 0; i < NM; ++i)
+#pragma unroll
+        for (int b = 0; b < MB; ++b)
+          acc[i][b] = lin_mfma16<F16>(__builtin_bit_cast(u32x4_t, fw[p][i][u]), __builtin_bit_cast(u32x4_t, fx[p][b][u]), acc[i][b]);
+  };
+  load(0, w * STEP);
+  for (int base = w * STEP; base < a.K; base += 2 * SPAN) {
+    load(1, base + SPAN);
+    use(0);
+    load(0, base + 2 * SPAN);
+    use(1);
+  }
+#pragma unroll
+  for (int i = 0; i < NM; ++i)
+#pragma unroll
+    for (int b = 0; b < MB; ++b) red[w][i][b][lane] = acc[i][b];
+  __syncthreads();
+  // result (m, n): element n' % 4 of lane 16 (n' / 4) + m', n' = s R + n and m' = s R + m, over the pieces and the waves in order
+  for (int t = tid; t < R * a.M; t += 64 * LR_WAVES) {
+    const int n = t % R, m = t / R, b = m >> 4;
+    if (n0 + n >= a.N) continue;
+    float sum[NM];
+#pragma unroll
+    for (int i = 0; i < NM; ++i) {
+      sum[i] = 0.f;
+#pragma unroll
+      for (int p = 0; p < SH; ++p) {
+        const int row = p * R + n;
+#pragma unroll
+        for (int v = 0; v < LR_WAVES; ++v) sum[i] += ((const float *)&red[v][i][b][16 * (row >> 2) + p * R + (m & 15)])[row & 3];
+      }
+    }
+    lin_store<F16, GATED>(a, m, n0 + n, sum[0], sum[NM - 1]);
+  }
+}
 
 // ---- tile kernel --------------------------------------------------------------------------------------------------------------
 // Four waves (2 x 2), wave (wm, wn) on WM x WN blocks of 32 x 32: a tile of 64 WM rows of x by 64 WN rows of W.  A gated pair's W
@@ -132,7 +225,6 @@ struct LinColumns {
 // of a column.  K advances 64 at a time (a slab); slabs go global -> LDS directly, two of them in LDS.
 #define LT_K 64
 #define LT_ROW 128  // bytes of a row of a slab: 8 chunks of 16, chunk c of row r in slot c ^ ((r >> 1) & 7)
-#define LT_OUT 0x7fffff00
 template <bool F16>
 static __device__ __forceinline__ f32x16_t lin_mfma32(u32x4_t a, u32x4_t b, f32x16_t c) {
   if constexpr (F16) return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8_t, a), __builtin_bit_cast(f16x8_t, b), c, 0, 0, 0);
@@ -290,6 +382,18 @@ template <bool F16, bool GATED>
 static int lin_launch(const LinArgs &a, hipStream_t s) {
   LinArgs t = a;
   t.whole = !(((uintptr_t)a.y | (uintptr_t)a.ldy * (a.y32 ? 4 : 2) | (uintptr_t)a.res | (a.res ? (uintptr_t)a.ldr * 2 : 0)) & 15);
+  if (a.M <= 32) {
+    const bool two = a.M > 16;
+    const int sh = a.M <= 4 && a.N < 16 * 512 ? 4 : a.M <= 8 && a.N < 16 * 512 ? 2 : 1;
+    const dim3 grid((a.N + 16 / sh - 1) / (16 / sh));
+#define LR_LAUNCH(MB_, SH_) hipLaunchKernelGGL(HIP_KERNEL_NAME(k_linear_rows<F16, GATED, MB_, SH_>), grid, dim3(64 * LR_WAVES), 0, s, t)
+    if (two) LR_LAUNCH(2, 1);
+    else if (sh == 4) LR_LAUNCH(1, 4);
+    else if (sh == 2) LR_LAUNCH(1, 2);
+    else LR_LAUNCH(1, 1);
+#undef LR_LAUNCH
+    return moe_check_launch("k_linear_rows");
+  }
   if (a.M > 128) {
     t.nm = (a.M + 255) / 256; t.nn = (a.N + (GATED ? 127 : 255)) / (GATED ? 128 : 256);
     hipLaunchKernelGGL(HIP_KERNEL_NAME(k_linear_tile<F16, GATED, 4, 4>), dim3((t.nm * t.nn + 7) / 8 * 8), dim3(256), 0, s, t);
