@@ -26,6 +26,8 @@ struct LinArgs {
   long long ldx, ldw, ldr, ldy;              // elements
   int M, N, K, act, y32;
   int nm, nn;                                // tiles
+  int splits, ldp;                           // pieces of K, columns of a row of partial sums
+  float *part;                               // partial sums [splits][1 or 2 matrices][M][ldp], NULL: the tile kernel finishes
   int whole;                                 // rows of y and of the residual start on 16-byte boundaries
 };
 
@@ -96,6 +98,16 @@ struct LinColumns {
     for (int i = 0; i < 8; ++i) {
       b0[i] = a.bias[0] && i < count ? lin_f32<F16>(a.bias[0][n + i]) : 0.f;
       b1[i] = GATED && a.bias[1] && i < count ? lin_f32<F16>(a.bias[1][n + i]) : 0.f;
+    }
+  }
+  // the sums alone, of one piece of K (the join has the rest); rows of a.ldp columns, a multiple of 8
+  __device__ __forceinline__ void partial(const LinArgs &a, int split, int m, const float *s0, const float *s1) const {
+    if (count <= 0) return;
+#pragma unroll
+    for (int i = 0; i < (GATED ? 2 : 1); ++i) {
+      float *p = a.part + (((long long)split * (GATED ? 2 : 1) + i) * a.M + m) * a.ldp + n;
+      *(f32x4_t *)p = *(const f32x4_t *)(i ? s1 : s0);
+      *(f32x4_t *)(p + 4) = *(const f32x4_t *)((i ? s1 : s0) + 4);
     }
   }
   // s0, s1: the sums of row m (s1: of the second matrix)
@@ -230,20 +242,24 @@ static __device__ __forceinline__ f32x16_t lin_mfma32(u32x4_t a, u32x4_t b, f32x
   if constexpr (F16) return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8_t, a), __builtin_bit_cast(f16x8_t, b), c, 0, 0, 0);
   else return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8_t, a), __builtin_bit_cast(bf16x8_t, b), c, 0, 0, 0);
 }
-// s_waitcnt for all vector-memory operations and nothing else; for all LDS operations and nothing else
-#define LT_VM0() __builtin_amdgcn_s_waitcnt(0x0f70)
+// s_waitcnt for all but the N latest vector-memory operations and nothing else; for all LDS operations and nothing else
+#define LT_VM(N) __builtin_amdgcn_s_waitcnt(((N) & 15) | (7 << 4) | (15 << 8) | (((N) >> 4) << 14))
 #define LT_LGKM0() __builtin_amdgcn_s_waitcnt(0xc07f)
 
-template <bool F16, bool GATED, int WM, int WN>
-__global__ __launch_bounds__(256, WM * WN > 8 ? 1 : 2) void k_linear_tile(const LinArgs a) {
+template <bool F16, bool GATED, int WM, int WN, int RING>
+__global__ __launch_bounds__(256, RING * (WM + WN) * 64 * LT_ROW > 80 * 1024 ? 1 : 2) void k_linear_tile(const LinArgs a) {
   constexpr int BM = 64 * WM, BN = 64 * WN, NX = 2 * WM, NW = 2 * WN, SLAB = (BM + BN) * LT_ROW, NG = WM * WN;
-  __shared__ __align__(2 * SLAB) unsigned char s_ring[2 * SLAB];
+  constexpr bool AHEAD = NG <= 8;
+  __shared__ __align__(128) unsigned char s_ring[RING * SLAB];
   const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6), wm = w & 1, wn = w >> 1;
   const int fr = lane & 31, q = lane >> 5;
-  int mt, nt;
+  int mt, nt, split;
   {  // workgroup i runs on XCD i % 8: each XCD takes a contiguous run of tiles, four rows of tiles wide
-    const int per = (int)gridDim.x >> 3, b = (blockIdx.x & 7) * per + (blockIdx.x >> 3);
-    if (b >= a.nm * a.nn) return;
+    const int per = (int)gridDim.x >> 3;
+    int b = (blockIdx.x & 7) * per + (blockIdx.x >> 3);
+    if (b >= a.nm * a.nn * a.splits) return;
+    split = b / (a.nm * a.nn);
+    b -= split * a.nm * a.nn;
     const int group = b / (4 * a.nn), r = b - group * 4 * a.nn, rows = min(4, a.nm - 4 * group);
     mt = 4 * group + r % rows;
     nt = r / rows;
@@ -259,18 +275,20 @@ __global__ __launch_bounds__(256, WM * WN > 8 ? 1 : 2) void k_linear_tile(const 
   for (int t = 0; t < NX; ++t) vx[t] = (min(m0 + 32 * t + tr, a.M - 1) - m0) * (int)a.ldx * 2 + 16 * chunk;
 #pragma unroll
   for (int t = 0; t < NW; ++t) vw[t] = (min(n0 + 32 * (GATED ? t >> 1 : t) + tr, a.N - 1) - n0) * (int)a.ldw * 2 + 16 * chunk;
-  const int nk = (a.K + LT_K - 1) / LT_K;
+  const int nk_all = (a.K + LT_K - 1) / LT_K;
+  const int kt0 = (int)((long long)nk_all * split / a.splits), nk = (int)((long long)nk_all * (split + 1) / a.splits);  // slabs
+  const int k_end = min(a.K, nk * LT_K);
   auto dma = [&](int t, int kt, int slot) {
     // (assembly: told that a load writes LDS, the compiler would wait for all of them in front of every barrier and LDS read;
-    // the waits stand by hand.  Columns past K, and slabs past the last, are out of the resource's range: zeros.)
-    const bool in = kt * LT_K + 8 * chunk < a.K;
+    // the waits stand by hand.  Columns past the end, slabs past the last among them, are out of the resource's range: zeros.)
+    const bool in = kt * LT_K + 8 * chunk < k_end;
     const unsigned at = lds + (unsigned)(slot * SLAB + (t < NX ? t : t - NX) * 32 * LT_ROW + (t < NX ? 0 : BM * LT_ROW) + 8 * w * LT_ROW);
     const int off = in ? (t < NX ? vx[t < NX ? t : 0] : vw[t < NX ? 0 : t - NX]) : LT_OUT;
     const lt_rsrc_t rs = t < NX ? rx : (GATED && ((t - NX) & 1)) ? rw1 : rw0;
     __asm__ volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, %3 offen lds"
                      :: "s"(at), "v"(off), "s"(rs), "s"(kt * (LT_K * 2)) : "memory", "m0");
   };
-  unsigned ax[4], aw[4];  // LDS address of the lane's fragment of step j in block 0 of the current slot
+  unsigned ax[4], aw[4];  // LDS address of the lane's fragment of step j in block 0 of slot 0
 #pragma unroll
   for (int j = 0; j < 4; ++j) {
     const unsigned c = (unsigned)(((4 * q + j) ^ ((fr >> 1) & 7)) * 16);
@@ -278,8 +296,13 @@ __global__ __launch_bounds__(256, WM * WN > 8 ? 1 : 2) void k_linear_tile(const 
     aw[j] = lds + (unsigned)((BM + wn * WN * 32 + fr) * LT_ROW) + c;
   }
   typedef __attribute__((address_space(3))) const u32x4_t lds_u4;
-  auto read_x = [&](int j, int i) { return *(lds_u4 *)(uintptr_t)(ax[j] + (unsigned)(i * 32 * LT_ROW)); };
-  auto read_w = [&](int j, int i) { return *(lds_u4 *)(uintptr_t)(aw[j] + (unsigned)(i * 32 * LT_ROW)); };
+  unsigned cx[4], cw[4];  // and of the current slot
+  auto use_slot = [&](int slot) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) { cx[j] = ax[j] + (unsigned)(slot * SLAB); cw[j] = aw[j] + (unsigned)(slot * SLAB); }
+  };
+  auto read_x = [&](int j, int i) { return *(lds_u4 *)(uintptr_t)(cx[j] + (unsigned)(i * 32 * LT_ROW)); };
+  auto read_w = [&](int j, int i) { return *(lds_u4 *)(uintptr_t)(cw[j] + (unsigned)(i * 32 * LT_ROW)); };
   f32x16_t acc[WM][WN];
 #pragma unroll
   for (int i = 0; i < WM; ++i)
@@ -287,59 +310,107 @@ __global__ __launch_bounds__(256, WM * WN > 8 ? 1 : 2) void k_linear_tile(const 
     for (int b = 0; b < WN; ++b)
 #pragma unroll
       for (int e = 0; e < 16; ++e) acc[i][b][e] = 0.f;
-  u32x4_t fx[2][WM], fw[2][WN];
 #pragma unroll
-  for (int t = 0; t < NX + NW; ++t) dma(t, 0, 0);
+  for (int i = 0; i < RING; ++i)
 #pragma unroll
-  for (int t = 0; t < NX + NW; ++t) dma(t, 1, 1);
-  LT_VM0();
-  __syncthreads();
-#pragma unroll
-  for (int i = 0; i < WM; ++i) fx[0][i] = read_x(0, i);
-#pragma unroll
-  for (int i = 0; i < WN; ++i) fw[0][i] = read_w(0, i);
-  // slab kt in its slot.  The fragments of step j + 1 are read between the products of step j.  In front of step 3, whose fragments
-  // are the last of the slab, everybody has read the slab and slab kt + 1 has landed: behind that barrier its first fragments
-  // are read and slab kt + 2 is requested into this slot, one request behind a product.
-  int slot = 0;
-  for (int kt = 0; kt < nk; ++kt, slot ^= 1) {
+    for (int t = 0; t < NX + NW; ++t) dma(t, kt0 + i, i);
+  LT_VM((RING - 1) * (NX + NW));
+  __builtin_amdgcn_s_barrier();
+  use_slot(0);
+  if constexpr (AHEAD) {
+    // A slab's products are short here, a step of them shorter than an LDS read: the fragments of the whole next slab are read
+    // between this one's.  At the barrier everybody has this slab's fragments, so its slot is free, and the next has landed.
+    u32x4_t fx[2][4][WM], fw[2][4][WN];
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
-      const int p = j & 1;
-      if (j == 3) {
-        LT_LGKM0();
-        LT_VM0();
-        __builtin_amdgcn_s_barrier();
 #pragma unroll
-        for (int i = 0; i < 4; ++i) { ax[i] ^= SLAB; aw[i] ^= SLAB; }  // (the ring starts on a multiple of its size)
-      }
+      for (int i = 0; i < WM; ++i) fx[0][j][i] = read_x(j, i);
+#pragma unroll
+      for (int i = 0; i < WN; ++i) fw[0][j][i] = read_w(j, i);
+    }
+    int slot = 0;
+    auto step = [&](const u32x4_t(&x)[4][WM], const u32x4_t(&v)[4][WN], u32x4_t(&xn)[4][WM], u32x4_t(&vn)[4][WN], int kt) {
+      const int next = slot + 1 < RING ? slot + 1 : 0;
+      LT_LGKM0();
+      LT_VM((RING - 2) * (NX + NW));
+      __builtin_amdgcn_s_barrier();
+      use_slot(next);
       __builtin_amdgcn_sched_barrier(0);
+      constexpr int NP = 4 * NG, NR = 4 * (WM + WN), ND = NX + NW;
 #pragma unroll
-      for (int g = 0; g < NG; ++g) {
-        acc[g / WN][g % WN] = lin_mfma32<F16>(fw[p][g % WN], fx[p][g / WN], acc[g / WN][g % WN]);
-        __builtin_amdgcn_sched_barrier(0);
+      for (int g = 0; g < NP; ++g) {
+        const int j = g / NG, i = g % NG / WN, b = g % WN;
 #pragma unroll
-        for (int r = 0; r < WM + WN; ++r)
-          if (min(r, NG - 1) == g) {
-            if (r < WM) fx[p ^ 1][r] = read_x((j + 1) & 3, r);
-            else fw[p ^ 1][r - WM] = read_w((j + 1) & 3, r - WM);
+        for (int r = 0; r < NR; ++r)
+          if (r * NP / NR == g) {
+            const int rj = r / (WM + WN), ri = r % (WM + WN);
+            if (ri < WM) xn[rj][ri] = read_x(rj, ri);
+            else vn[rj][ri - WM] = read_w(rj, ri - WM);
           }
-        if (j == 3) {
 #pragma unroll
-          for (int t = 0; t < NX + NW; ++t)
-            if (t * NG / (NX + NW) == g) dma(t, kt + 2, slot);
+        for (int t = 0; t < ND; ++t)
+          if (t * NP / ND == g) dma(t, kt + RING, slot);
+        __builtin_amdgcn_sched_barrier(0);
+        acc[i][b] = lin_mfma32<F16>(v[j][b], x[j][i], acc[i][b]);
+        __builtin_amdgcn_sched_barrier(0);
+      }
+      slot = next;
+    };
+    // (always a pair of slabs: one past the end is zeros)
+    for (int kt = kt0; kt < nk; kt += 2) {
+      step(fx[0], fw[0], fx[1], fw[1], kt);
+      step(fx[1], fw[1], fx[0], fw[0], kt + 1);
+    }
+  } else {
+    u32x4_t fx[2][WM], fw[2][WN];
+#pragma unroll
+    for (int i = 0; i < WM; ++i) fx[0][i] = read_x(0, i);
+#pragma unroll
+    for (int i = 0; i < WN; ++i) fw[0][i] = read_w(0, i);
+    // slab kt in its slot.  The fragments of step j + 1 are read between the products of step j.  In front of step 3, whose fragments
+    // are the last of the slab, everybody has read the slab and slab kt + 1 has landed: behind that barrier its first fragments
+    // are read and slab kt + RING is requested into this slot, one request behind a product.
+    int slot = 0;
+    for (int kt = kt0; kt < nk; ++kt) {
+      const int next = slot + 1 < RING ? slot + 1 : 0;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const int p = j & 1;
+        if (j == 3) {
+          LT_LGKM0();
+          LT_VM((RING - 2) * (NX + NW));
+          __builtin_amdgcn_s_barrier();
+          use_slot(next);
         }
         __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+        for (int g = 0; g < NG; ++g) {
+          acc[g / WN][g % WN] = lin_mfma32<F16>(fw[p][g % WN], fx[p][g / WN], acc[g / WN][g % WN]);
+          __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+          for (int r = 0; r < WM + WN; ++r)
+            if (min(r, NG - 1) == g) {
+              if (r < WM) fx[p ^ 1][r] = read_x((j + 1) & 3, r);
+              else fw[p ^ 1][r - WM] = read_w((j + 1) & 3, r - WM);
+            }
+          if (j == 3) {
+#pragma unroll
+            for (int t = 0; t < NX + NW; ++t)
+              if (t * NG / (NX + NW) == g) dma(t, kt + RING, slot);
+          }
+          __builtin_amdgcn_sched_barrier(0);
+        }
       }
+      slot = next;
     }
   }
   // The sums leave through LDS, 32 rows of the wave at a time, so that a lane then has 8 adjacent columns of a row and the rest is
   // one loop of whole lines.  Element e of a lane: column 8 (e / 4) + 4 q + e % 4 of W's block, row fr of x's.
-  LT_VM0();
+  LT_VM(0);
   __syncthreads();
   constexpr int LDE = 32 * WN + 4;                       // floats between rows: 16 lanes that write 16 bytes each fall on all banks
   constexpr int LPR = NC / 16, RPP = 64 / LPR;           // lanes of a row (8 columns each), rows of a pass
-  static_assert(4 * 32 * LDE * 4 <= 2 * SLAB, "the sums of four waves fit the ring");
+  static_assert(4 * 32 * LDE * 4 <= RING * SLAB, "the sums of four waves fit the ring");
   float *buf = (float *)s_ring + w * 32 * LDE;
   const int col = 8 * (lane % LPR), n = n0 + wn * (NC / 2) + col;
   const int at = GATED ? (col >> 5) * 64 + (col & 31) : col;
@@ -355,10 +426,34 @@ __global__ __launch_bounds__(256, WM * WN > 8 ? 1 : 2) void k_linear_tile(const 
     __builtin_amdgcn_wave_barrier();
     for (int r = lane / LPR; r < 32; r += RPP) {
       const int m = m0 + 32 * (wm * WM + i) + r;
-      if (m < a.M) c.store(a, m, buf + r * LDE + at, buf + r * LDE + at + 32);
+      if (m >= a.M) continue;
+      if (a.part) c.partial(a, split, m, buf + r * LDE + at, buf + r * LDE + at + 32);
+      else c.store(a, m, buf + r * LDE + at, buf + r * LDE + at + 32);
     }
     __builtin_amdgcn_wave_barrier();
   }
+}
+
+// The pieces of K added in their order, then what the tile kernel does behind its sums
+template <bool F16, bool GATED>
+__global__ __launch_bounds__(256) void k_linear_join(const LinArgs a) {
+  const int per = a.ldp >> 3;
+  const long long t = (long long)blockIdx.x * 256 + threadIdx.x;
+  const int m = (int)(t / per), n = (int)(t - (long long)m * per) * 8;
+  if (m >= a.M) return;
+  float s[2][8] = {};
+  constexpr int NM = GATED ? 2 : 1;
+  const long long step = (long long)a.M * a.ldp;
+  for (int p = 0; p < a.splits; ++p)
+#pragma unroll
+    for (int i = 0; i < NM; ++i) {
+      const float *q = a.part + (p * NM + i) * step + (long long)m * a.ldp + n;
+      const f32x4_t u = *(const f32x4_t *)q, v = *(const f32x4_t *)(q + 4);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) { s[i][e] += u[e]; s[i][4 + e] += v[e]; }
+    }
+  const LinColumns<F16, GATED> c(a, n);
+  c.store(a, m, s[0], s[1]);
 }
 
 // ---- entry points -------------------------------------------------------------------------------------------------------------
@@ -378,8 +473,20 @@ static int lin_check(const char *who, const LinArgs &a, int dtype, bool gated) {
   return MOE_OK;
 }
 
+// Which kernel a product takes: few rows (wm 0), or tiles of 64 wm x 64 wn with `ring` slabs in LDS and K in `splits` pieces
+struct LinPlan { int wm, wn, ring, splits; };
+#include <stdlib.h>
+static LinPlan lin_plan(int M, int N, int K, bool gated) {
+  if (M <= 32) return LinPlan{0, 0, 0, 1};
+  const char *e = getenv("LINPLAN");
+  if (e) { int v = atoi(e); return LinPlan{v / 10000 % 10, v / 1000 % 10, v / 100 % 10, v % 100}; }
+  if (M > 128) return LinPlan{4, 4, 2, 1};
+  return LinPlan{2, 2, 4, 1};
+}
+
 template <bool F16, bool GATED>
-static int lin_launch(const LinArgs &a, hipStream_t s) {
+static int lin_launch(const LinArgs &a, float *ws, hipStream_t s) {
+  constexpr int NM = GATED ? 2 : 1;
   LinArgs t = a;
   t.whole = !(((uintptr_t)a.y | (uintptr_t)a.ldy * (a.y32 ? 4 : 2) | (uintptr_t)a.res | (a.res ? (uintptr_t)a.ldr * 2 : 0)) & 15);
   if (a.M <= 32) {
@@ -394,30 +501,57 @@ static int lin_launch(const LinArgs &a, hipStream_t s) {
 #undef LR_LAUNCH
     return moe_check_launch("k_linear_rows");
   }
-  if (a.M > 128) {
-    t.nm = (a.M + 255) / 256; t.nn = (a.N + (GATED ? 127 : 255)) / (GATED ? 128 : 256);
-    hipLaunchKernelGGL(HIP_KERNEL_NAME(k_linear_tile<F16, GATED, 4, 4>), dim3((t.nm * t.nn + 7) / 8 * 8), dim3(256), 0, s, t);
-  } else {
-    t.nm = (a.M + 127) / 128; t.nn = (a.N + (GATED ? 63 : 127)) / (GATED ? 64 : 128);
-    hipLaunchKernelGGL(HIP_KERNEL_NAME(k_linear_tile<F16, GATED, 2, 2>), dim3((t.nm * t.nn + 7) / 8 * 8), dim3(256), 0, s, t);
+  const LinPlan pl = lin_plan(a.M, a.N, a.K, GATED);
+  t.nm = (a.M + 64 * pl.wm - 1) / (64 * pl.wm);
+  t.nn = (a.N + 64 * pl.wn / NM - 1) / (64 * pl.wn / NM);
+  t.splits = pl.splits;
+  t.ldp = (a.N + 7) & ~7;
+  t.part = pl.splits > 1 ? ws : nullptr;
+  const dim3 grid((t.nm * t.nn * t.splits + 7) / 8 * 8);
+#define LT_LAUNCH(WM_, WN_, RING_) hipLaunchKernelGGL(HIP_KERNEL_NAME(k_linear_tile<F16, GATED, WM_, WN_, RING_>), grid, dim3(256), 0, s, t)
+  switch (pl.wm * 100 + pl.wn * 10 + pl.ring) {
+    case 442: LT_LAUNCH(4, 4, 2); break;
+    case 222: LT_LAUNCH(2, 2, 2); break;
+    case 224: LT_LAUNCH(2, 2, 4); break;
+    case 122: LT_LAUNCH(1, 2, 2); break;
+    case 123: LT_LAUNCH(1, 2, 3); break;
+    case 126: LT_LAUNCH(1, 2, 6); break;
+    case 114: if constexpr (!GATED) LT_LAUNCH(1, 1, 4); break;
+    case 243: LT_LAUNCH(2, 4, 3); break;
+    default: moe_set_error("moe_linear: no tile %d x %d", pl.wm, pl.wn); return MOE_EINVAL;
   }
-  return moe_check_launch("k_linear_tile");
+#undef LT_LAUNCH
+  if (int rc = moe_check_launch("k_linear_tile")) return rc;
+  if (!t.part) return MOE_OK;
+  const long long pieces = (long long)a.M * (t.ldp >> 3);
+  hipLaunchKernelGGL(HIP_KERNEL_NAME(k_linear_join<F16, GATED>), dim3((unsigned)((pieces + 255) / 256)), dim3(256), 0, s, t);
+  return moe_check_launch("k_linear_join");
 }
-template <bool GATED>
-static int lin_run(const char *who, const LinArgs &a, int dtype, hipStream_t s) {
-  if (int rc = lin_check(who, a, dtype, GATED)) return rc;
-  if (a.M == 0 || a.N == 0) return MOE_OK;
-  return dtype == MOE_DT_FP16 ? lin_launch<true, GATED>(a, s) : lin_launch<false, GATED>(a, s);
+extern "C" int64_t moe_linear_workspace_bytes(int M, int N, int K, int gated) {
+  if (M <= 0 || N <= 0 || K <= 0) return 0;
+  const LinPlan p = lin_plan(M, N, K, gated != 0);
+  return p.splits > 1 ? (int64_t)p.splits * (gated ? 2 : 1) * M * ((N + 7) & ~7) * 4 : 0;
 }
 
-extern "C" int64_t moe_linear_workspace_bytes(int M, int N, int K, int gated) { return 0; }
+template <bool GATED>
+static int lin_run(const char *who, const LinArgs &a, int dtype, void *ws, int64_t ws_bytes, hipStream_t s) {
+  if (int rc = lin_check(who, a, dtype, GATED)) return rc;
+  if (a.M == 0 || a.N == 0) return MOE_OK;
+  const int64_t need = moe_linear_workspace_bytes(a.M, a.N, a.K, GATED);
+  if (need && (!ws || ws_bytes < need || ((uintptr_t)ws & 15))) {
+    moe_set_error("%s: a workspace of %lld bytes on a 16-byte boundary is needed", who, (long long)need);
+    return MOE_EINVAL;
+  }
+  return dtype == MOE_DT_FP16 ? lin_launch<true, GATED>(a, (float *)ws, s) : lin_launch<false, GATED>(a, (float *)ws, s);
+}
+
 
 extern "C" int moe_linear(const void *x, int64_t ldx, const void *w, int64_t ldw, const void *bias, const void *residual, int64_t ldr,
                           void *y, int64_t ldy, int M, int N, int K, int dtype, int act, int y_fp32, void *ws, int64_t ws_bytes,
                           void *stream) {
   const LinArgs a{(const uint16_t *)x, {(const uint16_t *)w, nullptr}, {(const uint16_t *)bias, nullptr}, (const uint16_t *)residual,
                   y, ldx, ldw, ldr, ldy, M, N, K, act, y_fp32 != 0};
-  return lin_run<false>("moe_linear", a, dtype, (hipStream_t)stream);
+  return lin_run<false>("moe_linear", a, dtype, ws, ws_bytes, (hipStream_t)stream);
 }
 
 extern "C" int moe_linear_gated(const void *x, int64_t ldx, const void *w_gate, const void *w_up, int64_t ldw, const void *b_gate,
@@ -425,5 +559,5 @@ extern "C" int moe_linear_gated(const void *x, int64_t ldx, const void *w_gate, 
                                 int64_t ws_bytes, void *stream) {
   const LinArgs a{(const uint16_t *)x, {(const uint16_t *)w_gate, (const uint16_t *)w_up}, {(const uint16_t *)b_gate, (const uint16_t *)b_up},
                   nullptr, y, ldx, ldw, 0, ldy, M, N, K, act, y_fp32 != 0};
-  return lin_run<true>("moe_linear_gated", a, dtype, (hipStream_t)stream);
+  return lin_run<true>("moe_linear_gated", a, dtype, ws, ws_bytes, (hipStream_t)stream);
 }
