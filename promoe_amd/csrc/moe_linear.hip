@@ -250,7 +250,8 @@ template <bool F16, bool GATED, int WM, int WN, int RING>
 __global__ __launch_bounds__(256, RING * (WM + WN) * 64 * LT_ROW > 80 * 1024 ? 1 : 2) void k_linear_tile(const LinArgs a) {
   constexpr int BM = 64 * WM, BN = 64 * WN, NX = 2 * WM, NW = 2 * WN, SLAB = (BM + BN) * LT_ROW, NG = WM * WN;
   constexpr bool AHEAD = NG <= 8;
-  __shared__ __align__(128) unsigned char s_ring[RING * SLAB];
+  constexpr int LDS = AHEAD ? RING * SLAB : RING * SLAB / 2;
+  __shared__ __align__(128) unsigned char s_ring[LDS];
   const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6), wm = w & 1, wn = w >> 1;
   const int fr = lane & 31, q = lane >> 5;
   int mt, nt, split;
@@ -278,28 +279,28 @@ __global__ __launch_bounds__(256, RING * (WM + WN) * 64 * LT_ROW > 80 * 1024 ? 1
   const int nk_all = (a.K + LT_K - 1) / LT_K;
   const int kt0 = (int)((long long)nk_all * split / a.splits), nk = (int)((long long)nk_all * (split + 1) / a.splits);  // slabs
   const int k_end = min(a.K, nk * LT_K);
-  auto dma = [&](int t, int kt, int slot) {
+  auto dma = [&](int t, int kt, int place) {  // place: where in the ring the rows of x (t < NX), of W, begin
     // (assembly: told that a load writes LDS, the compiler would wait for all of them in front of every barrier and LDS read;
     // the waits stand by hand.  Columns past the end, slabs past the last among them, are out of the resource's range: zeros.)
     const bool in = kt * LT_K + 8 * chunk < k_end;
-    const unsigned at = lds + (unsigned)(slot * SLAB + (t < NX ? t : t - NX) * 32 * LT_ROW + (t < NX ? 0 : BM * LT_ROW) + 8 * w * LT_ROW);
+    const unsigned at = lds + (unsigned)(place + ((t < NX ? t : t - NX) * 32 + 8 * w) * LT_ROW);
     const int off = in ? (t < NX ? vx[t < NX ? t : 0] : vw[t < NX ? 0 : t - NX]) : LT_OUT;
     const lt_rsrc_t rs = t < NX ? rx : (GATED && ((t - NX) & 1)) ? rw1 : rw0;
     __asm__ volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, %3 offen lds"
                      :: "s"(at), "v"(off), "s"(rs), "s"(kt * (LT_K * 2)) : "memory", "m0");
   };
-  unsigned ax[4], aw[4];  // LDS address of the lane's fragment of step j in block 0 of slot 0
+  unsigned ax[4], aw[4];  // LDS address of the lane's fragment of step j in block 0, of rows that begin where the ring does
 #pragma unroll
   for (int j = 0; j < 4; ++j) {
     const unsigned c = (unsigned)(((4 * q + j) ^ ((fr >> 1) & 7)) * 16);
     ax[j] = lds + (unsigned)((wm * WM * 32 + fr) * LT_ROW) + c;
-    aw[j] = lds + (unsigned)((BM + wn * WN * 32 + fr) * LT_ROW) + c;
+    aw[j] = lds + (unsigned)((wn * WN * 32 + fr) * LT_ROW) + c;
   }
   typedef __attribute__((address_space(3))) const u32x4_t lds_u4;
-  unsigned cx[4], cw[4];  // and of the current slot
-  auto use_slot = [&](int slot) {
+  unsigned cx[4], cw[4];  // and of the current slab
+  auto use = [&](int place_x, int place_w) {
 #pragma unroll
-    for (int j = 0; j < 4; ++j) { cx[j] = ax[j] + (unsigned)(slot * SLAB); cw[j] = aw[j] + (unsigned)(slot * SLAB); }
+    for (int j = 0; j < 4; ++j) { cx[j] = ax[j] + (unsigned)place_x; cw[j] = aw[j] + (unsigned)place_w; }
   };
   auto read_x = [&](int j, int i) { return *(lds_u4 *)(uintptr_t)(cx[j] + (unsigned)(i * 32 * LT_ROW)); };
   auto read_w = [&](int j, int i) { return *(lds_u4 *)(uintptr_t)(cw[j] + (unsigned)(i * 32 * LT_ROW)); };
@@ -310,16 +311,16 @@ __global__ __launch_bounds__(256, RING * (WM + WN) * 64 * LT_ROW > 80 * 1024 ? 1
     for (int b = 0; b < WN; ++b)
 #pragma unroll
       for (int e = 0; e < 16; ++e) acc[i][b][e] = 0.f;
-#pragma unroll
-  for (int i = 0; i < RING; ++i)
-#pragma unroll
-    for (int t = 0; t < NX + NW; ++t) dma(t, kt0 + i, i);
-  LT_VM((RING - 1) * (NX + NW));
-  __builtin_amdgcn_s_barrier();
-  use_slot(0);
   if constexpr (AHEAD) {
     // A slab's products are short here, a step of them shorter than an LDS read: the fragments of the whole next slab are read
     // between this one's.  At the barrier everybody has this slab's fragments, so its slot is free, and the next has landed.
+#pragma unroll
+    for (int i = 0; i < RING; ++i)
+#pragma unroll
+      for (int t = 0; t < NX + NW; ++t) dma(t, kt0 + i, i * SLAB + (t < NX ? 0 : BM * LT_ROW));
+    LT_VM((RING - 1) * (NX + NW));
+    __builtin_amdgcn_s_barrier();
+    use(0, BM * LT_ROW);
     u32x4_t fx[2][4][WM], fw[2][4][WN];
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
@@ -334,7 +335,7 @@ __global__ __launch_bounds__(256, RING * (WM + WN) * 64 * LT_ROW > 80 * 1024 ? 1
       LT_LGKM0();
       LT_VM((RING - 2) * (NX + NW));
       __builtin_amdgcn_s_barrier();
-      use_slot(next);
+      use(next * SLAB, next * SLAB + BM * LT_ROW);
       __builtin_amdgcn_sched_barrier(0);
       constexpr int NP = 4 * NG, NR = 4 * (WM + WN), ND = NX + NW;
 #pragma unroll
@@ -349,7 +350,7 @@ __global__ __launch_bounds__(256, RING * (WM + WN) * 64 * LT_ROW > 80 * 1024 ? 1
           }
 #pragma unroll
         for (int t = 0; t < ND; ++t)
-          if (t * NP / ND == g) dma(t, kt + RING, slot);
+          if (t * NP / ND == g) dma(t, kt + RING, slot * SLAB + (t < NX ? 0 : BM * LT_ROW));
         __builtin_amdgcn_sched_barrier(0);
         acc[i][b] = lin_mfma32<F16>(v[j][b], x[j][i], acc[i][b]);
         __builtin_amdgcn_sched_barrier(0);
@@ -362,46 +363,60 @@ __global__ __launch_bounds__(256, RING * (WM + WN) * 64 * LT_ROW > 80 * 1024 ? 1
       step(fx[1], fw[1], fx[0], fw[0], kt + 1);
     }
   } else {
+    // One step's products cover an LDS read, so the fragments of step j + 1 are read between those of step j.  LDS has room for two
+    // slabs and a half: a ring of HALVES halves, x and W of a slab in turn (half h of the run in place h % HALVES).  In front of step
+    // 3, whose fragments are the last of slab kt, everybody has read the slab and slab kt + 1 has landed.  The transfers go out evenly, a
+    // quarter of a half per quarter of a step's products: 64 bytes per cycle and compute unit is all that the path takes, half of the
+    // time that the products of a slab need.  All 16 of a wave in step 3 stopped the products for as long again (59 % busy matrix cores).
+    static_assert(NX == NW, "halves of one size");
+    constexpr int HALF = BM * LT_ROW;
+    static_assert(RING == 5, "halves");
+    auto place = [&](int h) { return h % RING * HALF; };
     u32x4_t fx[2][WM], fw[2][WN];
+#pragma unroll
+    for (int h = 0; h < 3; ++h)
+#pragma unroll
+      for (int t = 0; t < NX; ++t) dma(t + (h & 1) * NX, kt0 + (h >> 1), place(h));
+#pragma unroll
+    for (int t = 0; t < NX / 2; ++t) dma(NX + t, kt0 + 1, place(3));
+    LT_VM(NX + NX / 2);
+    __builtin_amdgcn_s_barrier();
+    use(place(0), place(1));
 #pragma unroll
     for (int i = 0; i < WM; ++i) fx[0][i] = read_x(0, i);
 #pragma unroll
     for (int i = 0; i < WN; ++i) fw[0][i] = read_w(0, i);
-    // slab kt in its slot.  The fragments of step j + 1 are read between the products of step j.  In front of step 3, whose fragments
-    // are the last of the slab, everybody has read the slab and slab kt + 1 has landed: behind that barrier its first fragments
-    // are read and slab kt + RING is requested into this slot, one request behind a product.
-    int slot = 0;
+    int h = 0;  // place of slab kt's x half
     for (int kt = kt0; kt < nk; ++kt) {
-      const int next = slot + 1 < RING ? slot + 1 : 0;
+      auto ahead = [&](int n) { const int v = h + n; return (v >= RING ? v - RING : v) * HALF; };
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
         const int p = j & 1;
         if (j == 3) {
           LT_LGKM0();
-          LT_VM((RING - 2) * (NX + NW));
+          LT_VM(NX);  // (x of slab kt + 2 may be on its way)
           __builtin_amdgcn_s_barrier();
-          use_slot(next);
+          use(ahead(2), ahead(3));
         }
         __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
         for (int g = 0; g < NG; ++g) {
           acc[g / WN][g % WN] = lin_mfma32<F16>(fw[p][g % WN], fx[p][g / WN], acc[g / WN][g % WN]);
           __builtin_amdgcn_sched_barrier(0);
+          if (g < WM) fx[p ^ 1][g] = read_x((j + 1) & 3, g);
+          else if (g < WM + WN) fw[p ^ 1][g - WM] = read_w((j + 1) & 3, g - WM);
 #pragma unroll
-          for (int r = 0; r < WM + WN; ++r)
-            if (min(r, NG - 1) == g) {
-              if (r < WM) fx[p ^ 1][r] = read_x((j + 1) & 3, r);
-              else fw[p ^ 1][r - WM] = read_w((j + 1) & 3, r - WM);
+          for (int t = 0; t < NX / 2; ++t)
+            if (t * NG / (NX / 2) == g) {
+              if (j == 0) dma(NX + NX / 2 + t, kt + 1, ahead(3));  // W of the next slab, second half of its rows
+              if (j == 1) dma(t, kt + 2, ahead(4));                // x of the one behind it, where W of slab kt - 1 was
+              if (j == 2) dma(NX / 2 + t, kt + 2, ahead(4));
+              if (j == 3) dma(NX + t, kt + 2, ahead(0));           // W of it, first half, where x of slab kt was
             }
-          if (j == 3) {
-#pragma unroll
-            for (int t = 0; t < NX + NW; ++t)
-              if (t * NG / (NX + NW) == g) dma(t, kt + RING, slot);
-          }
           __builtin_amdgcn_sched_barrier(0);
         }
       }
-      slot = next;
+      h = h + 2 >= RING ? h + 2 - RING : h + 2;
     }
   }
   // The sums leave through LDS, 32 rows of the wave at a time, so that a lane then has 8 adjacent columns of a row and the rest is
@@ -410,7 +425,7 @@ __global__ __launch_bounds__(256, RING * (WM + WN) * 64 * LT_ROW > 80 * 1024 ? 1
   __syncthreads();
   constexpr int LDE = 32 * WN + 4;                       // floats between rows: 16 lanes that write 16 bytes each fall on all banks
   constexpr int LPR = NC / 16, RPP = 64 / LPR;           // lanes of a row (8 columns each), rows of a pass
-  static_assert(4 * 32 * LDE * 4 <= RING * SLAB, "the sums of four waves fit the ring");
+  static_assert(4 * 32 * LDE * 4 <= LDS, "the sums of four waves fit the ring");
   float *buf = (float *)s_ring + w * 32 * LDE;
   const int col = 8 * (lane % LPR), n = n0 + wn * (NC / 2) + col;
   const int at = GATED ? (col >> 5) * 64 + (col & 31) : col;
@@ -480,7 +495,7 @@ static LinPlan lin_plan(int M, int N, int K, bool gated) {
   if (M <= 32) return LinPlan{0, 0, 0, 1};
   const char *e = getenv("LINPLAN");
   if (e) { int v = atoi(e); return LinPlan{v / 10000 % 10, v / 1000 % 10, v / 100 % 10, v % 100}; }
-  if (M > 128) return LinPlan{4, 4, 2, 1};
+  if (M > 128) return LinPlan{4, 4, 5, 1};
   return LinPlan{2, 2, 4, 1};
 }
 
@@ -510,11 +525,8 @@ static int lin_launch(const LinArgs &a, float *ws, hipStream_t s) {
   const dim3 grid((t.nm * t.nn * t.splits + 7) / 8 * 8);
 #define LT_LAUNCH(WM_, WN_, RING_) hipLaunchKernelGGL(HIP_KERNEL_NAME(k_linear_tile<F16, GATED, WM_, WN_, RING_>), grid, dim3(256), 0, s, t)
   switch (pl.wm * 100 + pl.wn * 10 + pl.ring) {
-    case 442: LT_LAUNCH(4, 4, 2); break;
-    case 222: LT_LAUNCH(2, 2, 2); break;
+    case 445: LT_LAUNCH(4, 4, 5); break;
     case 224: LT_LAUNCH(2, 2, 4); break;
-    case 122: LT_LAUNCH(1, 2, 2); break;
-    case 123: LT_LAUNCH(1, 2, 3); break;
     case 126: LT_LAUNCH(1, 2, 6); break;
     case 114: if constexpr (!GATED) LT_LAUNCH(1, 1, 4); break;
     case 243: LT_LAUNCH(2, 4, 3); break;
