@@ -364,58 +364,60 @@ __global__ __launch_bounds__(256, RING * (WM + WN) * 64 * LT_ROW > 80 * 1024 ? 1
     }
   } else {
     // One step's products cover an LDS read, so the fragments of step j + 1 are read between those of step j.  LDS has room for two
-    // slabs and a half: a ring of HALVES halves, x and W of a slab in turn (half h of the run in place h % HALVES).  In front of step
-    // 3, whose fragments are the last of slab kt, everybody has read the slab and slab kt + 1 has landed.  The transfers go out evenly, a
-    // quarter of a half per quarter of a step's products: 64 bytes per cycle and compute unit is all that the path takes, half of the
-    // time that the products of a slab need.  All 16 of a wave in step 3 stopped the products for as long again (59 % busy matrix cores).
-    static_assert(NX == NW, "halves of one size");
+    // slabs and a half: a ring of five halves, x and W of a slab in turn (half h of the run in place h % 5).  The loop starts at step 3 of
+    // a slab kt, whose fragments are the last of it: in front of it everybody has read slab kt and slab kt + 1 has landed; in it and in
+    // step 0 of slab kt + 1 the wave's transfers of W of slab kt + 2 go out (where x of slab kt was), in steps 1 and 2 those of x of slab
+    // kt + 3.  Spread like that since 64 bytes per cycle and compute unit is all that the path takes, half of the time that the products
+    // of a slab need: all 16 of a wave in step 3 stopped the products for as long again (59 % busy matrix cores, now 74).
+    static_assert(RING == 5 && NX == NW && NG == 2 * (WM + WN), "halves of one size, and a read per two products");
     constexpr int HALF = BM * LT_ROW;
-    static_assert(RING == 5, "halves");
-    auto place = [&](int h) { return h % RING * HALF; };
-    u32x4_t fx[2][WM], fw[2][WN];
+    u32x4_t fx[2][WM] = {}, fw[2][WN] = {};  // (step 3 in front of the first slab: products of zeros)
 #pragma unroll
     for (int h = 0; h < 3; ++h)
 #pragma unroll
-      for (int t = 0; t < NX; ++t) dma(t + (h & 1) * NX, kt0 + (h >> 1), place(h));
+      for (int t = 0; t < NX; ++t) dma(t + (h & 1) * NX, kt0 + (h >> 1), h * HALF);
+    // fragment r of a step in the order of need: x's first block, W's, the rest of x's
+    auto read = [&](int r, int j, int p) {
+      if (r == 0) fx[p][0] = read_x(j, 0);
+      else if (r <= WN) fw[p][r - 1] = read_w(j, r - 1);
+      else fx[p][r - WN] = read_x(j, r - WN);
+    };
+    use(0, HALF);
+    int h = 3;  // place of W of slab kt + 2
+    for (int kt = kt0 - 1;; ++kt) {
+      LT_LGKM0();
+      LT_VM(NX);  // (x of slab kt + 2 may be on its way)
+      __builtin_amdgcn_s_barrier();
+      const int h1 = h + 1 < RING ? h + 1 : 0;  // place of x of slab kt + 3
 #pragma unroll
-    for (int t = 0; t < NX / 2; ++t) dma(NX + t, kt0 + 1, place(3));
-    LT_VM(NX + NX / 2);
-    __builtin_amdgcn_s_barrier();
-    use(place(0), place(1));
-#pragma unroll
-    for (int i = 0; i < WM; ++i) fx[0][i] = read_x(0, i);
-#pragma unroll
-    for (int i = 0; i < WN; ++i) fw[0][i] = read_w(0, i);
-    int h = 0;  // place of slab kt's x half
-    for (int kt = kt0; kt < nk; ++kt) {
-      auto ahead = [&](int n) { const int v = h + n; return (v >= RING ? v - RING : v) * HALF; };
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const int p = j & 1;
-        if (j == 3) {
-          LT_LGKM0();
-          LT_VM(NX);  // (x of slab kt + 2 may be on its way)
-          __builtin_amdgcn_s_barrier();
-          use(ahead(2), ahead(3));
-        }
+      for (int s = 0; s < 4; ++s) {
+        const int j = (s + 3) & 3, p = j & 1;
+        if (s == 1 && kt == nk - 1) break;
         __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
         for (int g = 0; g < NG; ++g) {
           acc[g / WN][g % WN] = lin_mfma32<F16>(fw[p][g % WN], fx[p][g / WN], acc[g / WN][g % WN]);
           __builtin_amdgcn_sched_barrier(0);
-          if (g < WM) fx[p ^ 1][g] = read_x((j + 1) & 3, g);
-          else if (g < WM + WN) fw[p ^ 1][g - WM] = read_w((j + 1) & 3, g - WM);
+          // (all four waves at once: one read per two products is half of what LDS gives; before the barrier they have to be over)
+          if (j == 2 ? g < WM + WN : g % 2 == 0) read(j == 2 ? g : g / 2, (j + 1) & 3, p ^ 1);
 #pragma unroll
           for (int t = 0; t < NX / 2; ++t)
-            if (t * NG / (NX / 2) == g) {
-              if (j == 0) dma(NX + NX / 2 + t, kt + 1, ahead(3));  // W of the next slab, second half of its rows
-              if (j == 1) dma(t, kt + 2, ahead(4));                // x of the one behind it, where W of slab kt - 1 was
-              if (j == 2) dma(NX / 2 + t, kt + 2, ahead(4));
-              if (j == 3) dma(NX + t, kt + 2, ahead(0));           // W of it, first half, where x of slab kt was
+            if (t * NG / (NX / 2) + 1 == g) {
+              if (j == 3) dma(NX + t, kt + 2, h * HALF);
+              if (j == 0) dma(NX + NX / 2 + t, kt + 2, h * HALF);
+              if (j == 1) dma(t, kt + 3, h1 * HALF);
+              if (j == 2) dma(NX / 2 + t, kt + 3, h1 * HALF);
             }
+          if (j == 2 && g == WM + WN + 2) {  // the next slab's addresses, behind this one's last read
+            const int px = (h + 4 < RING ? h + 4 : h + 4 - RING) * HALF, pw = h * HALF;
+            use(px, pw);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) __asm__ volatile("" : "+v"(cx[i]), "+v"(cw[i]));
+          }
           __builtin_amdgcn_sched_barrier(0);
         }
       }
+      if (kt == nk - 1) break;
       h = h + 2 >= RING ? h + 2 - RING : h + 2;
     }
   }
