@@ -27,6 +27,7 @@ struct LinArgs {
   int M, N, K, act, y32;
   int nm, nn;                                // tiles
   int splits, ldp;                           // pieces of K, columns of a row of partial sums
+  int slabs, extra;                          // slabs of a piece; the first `extra` pieces have one more
   float *part;                               // partial sums [splits][1 or 2 matrices][M][ldp], NULL: the tile kernel finishes
   int whole;                                 // rows of y and of the residual start on 16-byte boundaries
 };
@@ -51,6 +52,13 @@ static __device__ __forceinline__ f32x4_t lin_mfma16(u32x4_t a, u32x4_t b, f32x4
 static __device__ __forceinline__ float lin_sigmoid(float v) {
   return __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(v * -1.44269504088896f));
 }
+// erfc of x >= 0 by the rational approximation 7.1.26 of Abramowitz and Stegun's handbook, off by at most 1.5e-7 (erf in fp32 next
+// to one: 6e-8): a dozen operations without a branch, where the library's has three
+static __device__ __forceinline__ float lin_erfc(float x) {
+  const float t = __builtin_amdgcn_rcpf(fmaf(0.3275911f, x, 1.f));
+  const float p = fmaf(fmaf(fmaf(fmaf(1.061405429f, t, -1.453152027f), t, 1.421413741f), t, -0.284496736f), t, 0.254829592f);
+  return p * t * __builtin_amdgcn_exp2f(x * x * -1.44269504088896f);
+}
 template <int C>
 static __device__ __forceinline__ void lin_act(int act, float (&v)[C]) {
   switch (act) {
@@ -59,7 +67,11 @@ static __device__ __forceinline__ void lin_act(int act, float (&v)[C]) {
       for (int i = 0; i < C; ++i) v[i] = v[i] * lin_sigmoid(v[i]);
       break;
     case MOE_ACT_GELU:
-      for (int i = 0; i < C; ++i) v[i] = 0.5f * v[i] * erfcf(v[i] * -0.70710678118654752f);
+#pragma unroll
+      for (int i = 0; i < C; ++i) {
+        const float h = 0.5f * lin_erfc(fabsf(v[i]) * 0.70710678118654752f);
+        v[i] *= v[i] > 0.f ? 1.f - h : h;
+      }
       break;
     case MOE_ACT_GELU_TANH:  // (1 + tanh z) / 2 = 1 / (1 + e^-2z), z = sqrt(2 / pi) (v + 0.044715 v^3)
 #pragma unroll
@@ -88,6 +100,22 @@ static __device__ __forceinline__ void lin_store(const LinArgs &a, int m, int n,
   else ((uint16_t *)a.y)[m * a.ldy + n] = lin_bits<F16>(v[0]);
 }
 
+template <bool F16>
+static __device__ __forceinline__ void lin_add(float (&v)[8], const u32x4_t r) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    v[2 * i] += lin_f32<F16>((uint16_t)r[i]);
+    v[2 * i + 1] += lin_f32<F16>((uint16_t)(r[i] >> 16));
+  }
+}
+template <bool F16>
+static __device__ __forceinline__ u32x4_t lin_pack(const float (&v)[8]) {
+  u32x4_t o;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) o[i] = lin_bits<F16>(v[2 * i]) | (u32)lin_bits<F16>(v[2 * i + 1]) << 16;
+  return o;
+}
+
 // Eight adjacent columns of the result from column n on (past N: left out): bias, activation, gate, residual and the one rounding
 template <bool F16, bool GATED>
 struct LinColumns {
@@ -95,10 +123,18 @@ struct LinColumns {
   float b0[8], b1[8];
   __device__ __forceinline__ LinColumns(const LinArgs &a, int n_) : n(n_), count(min(8, a.N - n_)) {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      b0[i] = a.bias[0] && i < count ? lin_f32<F16>(a.bias[0][n + i]) : 0.f;
-      b1[i] = GATED && a.bias[1] && i < count ? lin_f32<F16>(a.bias[1][n + i]) : 0.f;
-    }
+    for (int i = 0; i < 8; ++i) b0[i] = b1[i] = 0.f;
+    if (a.bias[0])  // (no condition around a load: all of them are on their way at once)
+#pragma unroll
+      for (int i = 0; i < 8; ++i) b0[i] = lin_f32<F16>(a.bias[0][min(n + i, a.N - 1)]);
+    if (GATED && a.bias[1])
+#pragma unroll
+      for (int i = 0; i < 8; ++i) b1[i] = lin_f32<F16>(a.bias[1][min(n + i, a.N - 1)]);
+  }
+  // the residual of row m where its rows are whole (asked for a row ahead: its trip to memory is longer than a row's work)
+  __device__ __forceinline__ u32x4_t residual(const LinArgs &a, int m) const {
+    if (GATED || !a.res || !a.whole || count < 8 || m >= a.M) return u32x4_t{0, 0, 0, 0};
+    return *(const u32x4_t *)(a.res + m * a.ldr + n);
   }
   // the sums alone, of one piece of K (the join has the rest); rows of a.ldp columns, a multiple of 8
   __device__ __forceinline__ void partial(const LinArgs &a, int split, int m, const float *s0, const float *s1) const {
@@ -110,8 +146,19 @@ struct LinColumns {
       *(f32x4_t *)(p + 4) = *(const f32x4_t *)((i ? s1 : s0) + 4);
     }
   }
-  // s0, s1: the sums of row m (s1: of the second matrix)
-  __device__ __forceinline__ void store(const LinArgs &a, int m, const float *s0, const float *s1) const {
+  // bias, a known activation and gate on the sums s0 (s1: of the second matrix), in place
+  template <int ACT>
+  __device__ __forceinline__ void finish(float (&s0)[8], const float (&s1)[8]) const {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) s0[i] += b0[i];
+    lin_act(ACT, s0);
+    if constexpr (GATED) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) s0[i] *= s1[i] + b1[i];
+    }
+  }
+  // s0, s1: the sums of row m (s1: of the second matrix); r: its residual
+  __device__ __forceinline__ void store(const LinArgs &a, int m, const float *s0, const float *s1, const u32x4_t r) const {
     if (count <= 0) return;
     float v[8];
 #pragma unroll
@@ -122,31 +169,22 @@ struct LinColumns {
       for (int i = 0; i < 8; ++i) v[i] *= s1[i] + b1[i];
     }
     if (count == 8 && a.whole) {  // whole rows of 16-byte pieces
-      if (a.res) {
-        const u32x4_t r = *(const u32x4_t *)(a.res + m * a.ldr + n);
-        v[0] += lin_f32<F16>((uint16_t)r.x); v[1] += lin_f32<F16>((uint16_t)(r.x >> 16));
-        v[2] += lin_f32<F16>((uint16_t)r.y); v[3] += lin_f32<F16>((uint16_t)(r.y >> 16));
-        v[4] += lin_f32<F16>((uint16_t)r.z); v[5] += lin_f32<F16>((uint16_t)(r.z >> 16));
-        v[6] += lin_f32<F16>((uint16_t)r.w); v[7] += lin_f32<F16>((uint16_t)(r.w >> 16));
-      }
+      if (!GATED && a.res) lin_add<F16>(v, r);
       if (a.y32) {
         float *y = (float *)a.y + m * a.ldy + n;
         *(f32x4_t *)y = f32x4_t{v[0], v[1], v[2], v[3]};
         *(f32x4_t *)(y + 4) = f32x4_t{v[4], v[5], v[6], v[7]};
       } else {
-        u32x4_t r;
-        r.x = lin_bits<F16>(v[0]) | (u32)lin_bits<F16>(v[1]) << 16; r.y = lin_bits<F16>(v[2]) | (u32)lin_bits<F16>(v[3]) << 16;
-        r.z = lin_bits<F16>(v[4]) | (u32)lin_bits<F16>(v[5]) << 16; r.w = lin_bits<F16>(v[6]) | (u32)lin_bits<F16>(v[7]) << 16;
-        *(u32x4_t *)((uint16_t *)a.y + m * a.ldy + n) = r;
+        *(u32x4_t *)((uint16_t *)a.y + m * a.ldy + n) = lin_pack<F16>(v);
       }
       return;
     }
-    if (a.res) {
-      uint16_t r[8];
+    if (!GATED && a.res) {
+      uint16_t e[8];
 #pragma unroll
-      for (int i = 0; i < 8; ++i) r[i] = a.res[m * a.ldr + n + min(i, count - 1)];  // (all of them on their way at once)
+      for (int i = 0; i < 8; ++i) e[i] = a.res[m * a.ldr + n + min(i, count - 1)];
 #pragma unroll
-      for (int i = 0; i < 8; ++i) v[i] += lin_f32<F16>(r[i]);
+      for (int i = 0; i < 8; ++i) v[i] += lin_f32<F16>(e[i]);
     }
 #pragma unroll
     for (int i = 0; i < 8; ++i)
@@ -231,6 +269,15 @@ __global__ __launch_bounds__(64 * LR_WAVES) void k_linear_rows(const LinArgs a) 
   }
 }
 
+// f(0), f(1), .. f(N - 1) with numbers known to the compiler
+template <int N, int I = 0, class F>
+static __device__ __forceinline__ void lt_each(const F &f) {
+  if constexpr (I < N) {
+    f(std::integral_constant<int, I>());
+    lt_each<N, I + 1>(f);
+  }
+}
+
 // ---- tile kernel --------------------------------------------------------------------------------------------------------------
 // Four waves (2 x 2), wave (wm, wn) on WM x WN blocks of 32 x 32: a tile of 64 WM rows of x by 64 WN rows of W.  A gated pair's W
 // blocks alternate between the two matrices (block b: matrix b & 1, its columns 32 (b >> 1) ..), so that a lane holds both sums
@@ -249,9 +296,7 @@ static __device__ __forceinline__ f32x16_t lin_mfma32(u32x4_t a, u32x4_t b, f32x
 template <bool F16, bool GATED, int WM, int WN, int RING>
 __global__ __launch_bounds__(256, RING * (WM + WN) * 64 * LT_ROW > 80 * 1024 ? 1 : 2) void k_linear_tile(const LinArgs a) {
   constexpr int BM = 64 * WM, BN = 64 * WN, NX = 2 * WM, NW = 2 * WN, SLAB = (BM + BN) * LT_ROW, NG = WM * WN;
-  constexpr bool AHEAD = NG <= 8;
-  constexpr int LDS = AHEAD ? RING * SLAB : RING * SLAB / 2;
-  __shared__ __align__(128) unsigned char s_ring[LDS];
+  __shared__ __align__(128) unsigned char s_ring[RING * SLAB];
   const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6), wm = w & 1, wn = w >> 1;
   const int fr = lane & 31, q = lane >> 5;
   int mt, nt, split;
@@ -276,8 +321,7 @@ __global__ __launch_bounds__(256, RING * (WM + WN) * 64 * LT_ROW > 80 * 1024 ? 1
   for (int t = 0; t < NX; ++t) vx[t] = (min(m0 + 32 * t + tr, a.M - 1) - m0) * (int)a.ldx * 2 + 16 * chunk;
 #pragma unroll
   for (int t = 0; t < NW; ++t) vw[t] = (min(n0 + 32 * (GATED ? t >> 1 : t) + tr, a.N - 1) - n0) * (int)a.ldw * 2 + 16 * chunk;
-  const int nk_all = (a.K + LT_K - 1) / LT_K;
-  const int kt0 = (int)((long long)nk_all * split / a.splits), nk = (int)((long long)nk_all * (split + 1) / a.splits);  // slabs
+  const int kt0 = split * a.slabs + min(split, a.extra), nk = kt0 + a.slabs + (split < a.extra);
   const int k_end = min(a.K, nk * LT_K);
   auto dma = [&](int t, int kt, int place) {  // place: where in the ring the rows of x (t < NX), of W, begin
     // (assembly: told that a load writes LDS, the compiler would wait for all of them in front of every barrier and LDS read;
@@ -311,115 +355,55 @@ __global__ __launch_bounds__(256, RING * (WM + WN) * 64 * LT_ROW > 80 * 1024 ? 1
     for (int b = 0; b < WN; ++b)
 #pragma unroll
       for (int e = 0; e < 16; ++e) acc[i][b][e] = 0.f;
-  if constexpr (AHEAD) {
-    // A slab's products are short here, a step of them shorter than an LDS read: the fragments of the whole next slab are read
-    // between this one's.  At the barrier everybody has this slab's fragments, so its slot is free, and the next has landed.
+  // A slab's products are short here, a step of them shorter than an LDS read: the fragments of the whole next slab are read
+  // between this one's.  At the barrier everybody has this slab's fragments, so its slot is free, and the next has landed.
 #pragma unroll
-    for (int i = 0; i < RING; ++i)
+  for (int i = 0; i < RING; ++i)
 #pragma unroll
-      for (int t = 0; t < NX + NW; ++t) dma(t, kt0 + i, i * SLAB + (t < NX ? 0 : BM * LT_ROW));
-    LT_VM((RING - 1) * (NX + NW));
+    for (int t = 0; t < NX + NW; ++t) dma(t, kt0 + i, i * SLAB + (t < NX ? 0 : BM * LT_ROW));
+  LT_VM((RING - 1) * (NX + NW));
+  __builtin_amdgcn_s_barrier();
+  use(0, BM * LT_ROW);
+  u32x4_t fx[2][4][WM], fw[2][4][WN];
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+#pragma unroll
+    for (int i = 0; i < WM; ++i) fx[0][j][i] = read_x(j, i);
+#pragma unroll
+    for (int i = 0; i < WN; ++i) fw[0][j][i] = read_w(j, i);
+  }
+  int slot = 0;
+  auto step = [&](const u32x4_t(&x)[4][WM], const u32x4_t(&v)[4][WN], u32x4_t(&xn)[4][WM], u32x4_t(&vn)[4][WN], int kt) {
+    const int next = slot + 1 < RING ? slot + 1 : 0;
+    LT_LGKM0();
+    LT_VM((RING - 2) * (NX + NW));
     __builtin_amdgcn_s_barrier();
-    use(0, BM * LT_ROW);
-    u32x4_t fx[2][4][WM], fw[2][4][WN];
+    use(next * SLAB, next * SLAB + BM * LT_ROW);
+    __builtin_amdgcn_sched_barrier(0);
+    constexpr int NP = 4 * NG, NR = 4 * (WM + WN), ND = NX + NW;
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
+    for (int g = 0; g < NP; ++g) {
+      const int j = g / NG, i = g % NG / WN, b = g % WN;
 #pragma unroll
-      for (int i = 0; i < WM; ++i) fx[0][j][i] = read_x(j, i);
-#pragma unroll
-      for (int i = 0; i < WN; ++i) fw[0][j][i] = read_w(j, i);
-    }
-    int slot = 0;
-    auto step = [&](const u32x4_t(&x)[4][WM], const u32x4_t(&v)[4][WN], u32x4_t(&xn)[4][WM], u32x4_t(&vn)[4][WN], int kt) {
-      const int next = slot + 1 < RING ? slot + 1 : 0;
-      LT_LGKM0();
-      LT_VM((RING - 2) * (NX + NW));
-      __builtin_amdgcn_s_barrier();
-      use(next * SLAB, next * SLAB + BM * LT_ROW);
-      __builtin_amdgcn_sched_barrier(0);
-      constexpr int NP = 4 * NG, NR = 4 * (WM + WN), ND = NX + NW;
-#pragma unroll
-      for (int g = 0; g < NP; ++g) {
-        const int j = g / NG, i = g % NG / WN, b = g % WN;
-#pragma unroll
-        for (int r = 0; r < NR; ++r)
-          if (r * NP / NR == g) {
-            const int rj = r / (WM + WN), ri = r % (WM + WN);
-            if (ri < WM) xn[rj][ri] = read_x(rj, ri);
-            else vn[rj][ri - WM] = read_w(rj, ri - WM);
-          }
-#pragma unroll
-        for (int t = 0; t < ND; ++t)
-          if (t * NP / ND == g) dma(t, kt + RING, slot * SLAB + (t < NX ? 0 : BM * LT_ROW));
-        __builtin_amdgcn_sched_barrier(0);
-        acc[i][b] = lin_mfma32<F16>(v[j][b], x[j][i], acc[i][b]);
-        __builtin_amdgcn_sched_barrier(0);
-      }
-      slot = next;
-    };
-    // (always a pair of slabs: one past the end is zeros)
-    for (int kt = kt0; kt < nk; kt += 2) {
-      step(fx[0], fw[0], fx[1], fw[1], kt);
-      step(fx[1], fw[1], fx[0], fw[0], kt + 1);
-    }
-  } else {
-    // One step's products cover an LDS read, so the fragments of step j + 1 are read between those of step j.  LDS has room for two
-    // slabs and a half: a ring of five halves, x and W of a slab in turn (half h of the run in place h % 5).  The loop starts at step 3 of
-    // a slab kt, whose fragments are the last of it: in front of it everybody has read slab kt and slab kt + 1 has landed; in it and in
-    // step 0 of slab kt + 1 the wave's transfers of W of slab kt + 2 go out (where x of slab kt was), in steps 1 and 2 those of x of slab
-    // kt + 3.  Spread like that since 64 bytes per cycle and compute unit is all that the path takes, half of the time that the products
-    // of a slab need: all 16 of a wave in step 3 stopped the products for as long again (59 % busy matrix cores, now 74).
-    static_assert(RING == 5 && NX == NW && NG == 2 * (WM + WN), "halves of one size, and a read per two products");
-    constexpr int HALF = BM * LT_ROW;
-    u32x4_t fx[2][WM] = {}, fw[2][WN] = {};  // (step 3 in front of the first slab: products of zeros)
-#pragma unroll
-    for (int h = 0; h < 3; ++h)
-#pragma unroll
-      for (int t = 0; t < NX; ++t) dma(t + (h & 1) * NX, kt0 + (h >> 1), h * HALF);
-    // fragment r of a step in the order of need: x's first block, W's, the rest of x's
-    auto read = [&](int r, int j, int p) {
-      if (r == 0) fx[p][0] = read_x(j, 0);
-      else if (r <= WN) fw[p][r - 1] = read_w(j, r - 1);
-      else fx[p][r - WN] = read_x(j, r - WN);
-    };
-    use(0, HALF);
-    int h = 3;  // place of W of slab kt + 2
-    for (int kt = kt0 - 1;; ++kt) {
-      LT_LGKM0();
-      LT_VM(NX);  // (x of slab kt + 2 may be on its way)
-      __builtin_amdgcn_s_barrier();
-      const int h1 = h + 1 < RING ? h + 1 : 0;  // place of x of slab kt + 3
-#pragma unroll
-      for (int s = 0; s < 4; ++s) {
-        const int j = (s + 3) & 3, p = j & 1;
-        if (s == 1 && kt == nk - 1) break;
-        __builtin_amdgcn_sched_barrier(0);
-#pragma unroll
-        for (int g = 0; g < NG; ++g) {
-          acc[g / WN][g % WN] = lin_mfma32<F16>(fw[p][g % WN], fx[p][g / WN], acc[g / WN][g % WN]);
-          __builtin_amdgcn_sched_barrier(0);
-          // (all four waves at once: one read per two products is half of what LDS gives; before the barrier they have to be over)
-          if (j == 2 ? g < WM + WN : g % 2 == 0) read(j == 2 ? g : g / 2, (j + 1) & 3, p ^ 1);
-#pragma unroll
-          for (int t = 0; t < NX / 2; ++t)
-            if (t * NG / (NX / 2) + 1 == g) {
-              if (j == 3) dma(NX + t, kt + 2, h * HALF);
-              if (j == 0) dma(NX + NX / 2 + t, kt + 2, h * HALF);
-              if (j == 1) dma(t, kt + 3, h1 * HALF);
-              if (j == 2) dma(NX / 2 + t, kt + 3, h1 * HALF);
-            }
-          if (j == 2 && g == WM + WN + 2) {  // the next slab's addresses, behind this one's last read
-            const int px = (h + 4 < RING ? h + 4 : h + 4 - RING) * HALF, pw = h * HALF;
-            use(px, pw);
-#pragma unroll
-            for (int i = 0; i < 4; ++i) __asm__ volatile("" : "+v"(cx[i]), "+v"(cw[i]));
-          }
-          __builtin_amdgcn_sched_barrier(0);
+      for (int r = 0; r < NR; ++r)
+        if (r * NP / NR == g) {
+          const int rj = r / (WM + WN), ri = r % (WM + WN);
+          if (ri < WM) xn[rj][ri] = read_x(rj, ri);
+          else vn[rj][ri - WM] = read_w(rj, ri - WM);
         }
-      }
-      if (kt == nk - 1) break;
-      h = h + 2 >= RING ? h + 2 - RING : h + 2;
+#pragma unroll
+      for (int t = 0; t < ND; ++t)
+        if (t * NP / ND == g) dma(t, kt + RING, slot * SLAB + (t < NX ? 0 : BM * LT_ROW));
+      __builtin_amdgcn_sched_barrier(0);
+      acc[i][b] = lin_mfma32<F16>(v[j][b], x[j][i], acc[i][b]);
+      __builtin_amdgcn_sched_barrier(0);
     }
+    slot = next;
+  };
+  // (always a pair of slabs: one past the end is zeros)
+  for (int kt = kt0; kt < nk; kt += 2) {
+    step(fx[0], fw[0], fx[1], fw[1], kt);
+    step(fx[1], fw[1], fx[0], fw[0], kt + 1);
   }
   // The sums leave through LDS, 32 rows of the wave at a time, so that a lane then has 8 adjacent columns of a row and the rest is
   // one loop of whole lines.  Element e of a lane: column 8 (e / 4) + 4 q + e % 4 of W's block, row fr of x's.
@@ -427,28 +411,276 @@ __global__ __launch_bounds__(256, RING * (WM + WN) * 64 * LT_ROW > 80 * 1024 ? 1
   __syncthreads();
   constexpr int LDE = 32 * WN + 4;                       // floats between rows: 16 lanes that write 16 bytes each fall on all banks
   constexpr int LPR = NC / 16, RPP = 64 / LPR;           // lanes of a row (8 columns each), rows of a pass
-  static_assert(4 * 32 * LDE * 4 <= LDS, "the sums of four waves fit the ring");
+  static_assert(4 * 32 * LDE * 4 <= RING * SLAB, "the sums of four waves fit the ring");
   float *buf = (float *)s_ring + w * 32 * LDE;
   const int col = 8 * (lane % LPR), n = n0 + wn * (NC / 2) + col;
   const int at = GATED ? (col >> 5) * 64 + (col & 31) : col;
   const LinColumns<F16, GATED> c(a, n);
-#pragma unroll
+  // (one copy of the loop for all blocks: code that runs once a tile waits for its instructions, line by line)
+#pragma clang loop unroll(disable)
   for (int i = 0; i < WM; ++i) {
+    lt_each<WM>([&](auto i_) {
+      if (i == decltype(i_)::value) {
 #pragma unroll
-    for (int b = 0; b < WN; ++b)
+        for (int b = 0; b < WN; ++b)
 #pragma unroll
-      for (int e = 0; e < 4; ++e)
-        *(f32x4_t *)(buf + fr * LDE + 32 * b + 8 * e + 4 * q) =
-            f32x4_t{acc[i][b][4 * e], acc[i][b][4 * e + 1], acc[i][b][4 * e + 2], acc[i][b][4 * e + 3]};
+          for (int e = 0; e < 4; ++e) {
+            const f32x16_t &s = acc[decltype(i_)::value][b];
+            *(f32x4_t *)(buf + fr * LDE + 32 * b + 8 * e + 4 * q) = f32x4_t{s[4 * e], s[4 * e + 1], s[4 * e + 2], s[4 * e + 3]};
+          }
+        __asm__ volatile("; %0" :: "i"(decltype(i_)::value));  // (or the compiler makes one copy of them, over registers chosen by i)
+      }
+    });
     __builtin_amdgcn_wave_barrier();
+    const int first = m0 + 32 * (wm * WM + i) + lane / LPR;
+    u32x4_t res = c.residual(a, first);
+#pragma clang loop unroll(disable)
     for (int r = lane / LPR; r < 32; r += RPP) {
-      const int m = m0 + 32 * (wm * WM + i) + r;
-      if (m >= a.M) continue;
-      if (a.part) c.partial(a, split, m, buf + r * LDE + at, buf + r * LDE + at + 32);
-      else c.store(a, m, buf + r * LDE + at, buf + r * LDE + at + 32);
+      const int m = first - lane / LPR + r;
+      const u32x4_t ahead = c.residual(a, r + RPP < 32 ? m + RPP : a.M);
+      if (m < a.M) {
+        if (a.part) c.partial(a, split, m, buf + r * LDE + at, buf + r * LDE + at + 32);
+        else c.store(a, m, buf + r * LDE + at, buf + r * LDE + at + 32, res);
+      }
+      res = ahead;
     }
     __builtin_amdgcn_wave_barrier();
   }
+}
+
+// ---- wide tiles: 256 x 256, one workgroup per compute unit that goes from tile to tile -------------------------------------------------
+// The layout of k_linear_tile with WM = WN = 4.  One step's products (16) cover an LDS read, so the fragments of step j + 1 are read
+// between those of step j.  LDS has room for two slabs and a half: a ring of five halves, x and W of a slab in turn (half h of the run in
+// place h % 5).  The loop turns at a barrier in front of step 3 of slab g - 1, whose fragments are that slab's last: everybody has read
+// slab g - 1 then, and slab g has landed; in step 0 of slab g the wave's transfers of W of slab g + 1 go out (where x of slab g - 1 was),
+// in steps 1 and 2 those of x of slab g + 2 (where its W was).  Spread like that since 64 bytes per cycle and compute unit is all that
+// the path takes, half of the time that the products of a slab need: all 16 of a wave in step 3 stopped the products for as long again
+// (59 % busy matrix cores, spread 74).
+// The run of slabs goes on from tile to tile: the next tile's first slab and the half behind it land under the last products, and the
+// sums leave through the places of the last slab while nothing else needs them.
+template <bool F16, bool GATED>
+__global__ __launch_bounds__(256, 1) void k_linear_wide(const LinArgs a) {
+  constexpr int B = 256, NT = 8, HALF = B * LT_ROW, NC = GATED ? B / 2 : B;
+  __shared__ __align__(1024) unsigned char s_ring[5 * HALF];
+  const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6), wm = w & 1, wn = w >> 1;
+  const int fr = lane & 31, q = lane >> 5;
+  const unsigned lds = (unsigned)(uintptr_t)(__attribute__((address_space(3))) unsigned char *)s_ring;
+  // workgroup i runs on XCD i % 8: each XCD takes a contiguous run of tiles, four rows of tiles wide
+  const int tiles = a.nm * a.nn, stride = (int)gridDim.x >> 3;
+  const int per = (tiles * a.splits + 7) >> 3, last = min(tiles * a.splits, ((int)(blockIdx.x & 7) + 1) * per);
+  struct Tile { int m0, n0, split, kt0, kt1; };  // kt1 0: none
+  auto tile_of = [&](int v) {
+    if (v >= last) return Tile{0, 0, 0, 0, 0};
+    const int split = v / tiles, b = v - split * tiles, group = b / (4 * a.nn), r = b - group * 4 * a.nn, rows = min(4, a.nm - 4 * group);
+    const int nt = r / rows, mt = 4 * group + r - nt * rows, kt0 = split * a.slabs + min(split, a.extra);
+    // (scalars, whatever the divisions are made of)
+    return Tile{__builtin_amdgcn_readfirstlane(mt) * B, __builtin_amdgcn_readfirstlane(nt) * NC, __builtin_amdgcn_readfirstlane(split),
+                __builtin_amdgcn_readfirstlane(kt0), __builtin_amdgcn_readfirstlane(kt0 + a.slabs + (split < a.extra))};
+  };
+  int v = (int)(blockIdx.x & 7) * per + ((int)blockIdx.x >> 3);
+  if (v >= last) return;
+  Tile cur = tile_of(v), nxt = tile_of(v + stride);
+  // transfer t of wave w: rows 32 t + 8 w .. + 7, eight lanes a row; the lanes choose the chunk that belongs in their slot
+  const int tr = 8 * w + (lane >> 3), chunk = (lane & 7) ^ ((tr >> 1) & 7);
+  // x and W each have a cursor: the slab that their next transfers bring, of this tile or of the next (past the last tile: zeros).  A
+  // tile has at least two slabs.
+  int vx[NT], vw[NT], kx, kw, end_x, end_w;
+  lt_rsrc_t rx, rw0, rw1{};
+  auto start_x = [&](const Tile &t) {
+    kx = t.kt0; end_x = t.kt1;
+    rx = lt_rsrc(a.x + t.m0 * a.ldx);
+#pragma unroll
+    for (int i = 0; i < NT; ++i) vx[i] = (min(t.m0 + 32 * i + tr, a.M - 1) - t.m0) * (int)a.ldx * 2 + 16 * chunk;
+  };
+  auto start_w = [&](const Tile &t) {
+    kw = t.kt0; end_w = t.kt1;
+    rw0 = lt_rsrc(a.w[0] + t.n0 * a.ldw);
+    if constexpr (GATED) rw1 = lt_rsrc(a.w[1] + t.n0 * a.ldw);
+#pragma unroll
+    for (int i = 0; i < NT; ++i) vw[i] = (min(t.n0 + 32 * (GATED ? i >> 1 : i) + tr, a.N - 1) - t.n0) * (int)a.ldw * 2 + 16 * chunk;
+  };
+  // (assembly: see k_linear_tile)
+  auto send = [&](int off, const lt_rsrc_t rs, int kt, bool in, int to, auto t) {
+    __asm__ volatile("s_add_u32 m0, %0, %4\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, %3 offen lds"
+                     :: "s"(to), "v"(in ? off : LT_OUT), "s"(rs), "s"(kt * (LT_K * 2)), "i"(decltype(t)::value * 32 * LT_ROW)
+                     : "memory", "m0", "scc");
+  };
+  const int mine = (int)lds + 8 * w * LT_ROW;  // the wave's rows in a half
+  auto in_x = [&]() { return kx * LT_K + 8 * chunk < min(a.K, end_x * LT_K); };
+  auto in_w = [&]() { return kw * LT_K + 8 * chunk < min(a.K, end_w * LT_K); };
+  auto send_x = [&](auto t, int h, bool in) { send(vx[t], rx, kx, in, mine + h * HALF, t); };
+  auto send_w = [&](auto t, int h, bool in) { send(vw[t], GATED && (t & 1) ? rw1 : rw0, kw, in, mine + h * HALF, t); };
+  unsigned ax[4], aw[4], cx[4], cw[4];  // LDS address of the lane's fragment of step j in block 0: in place 0, and of the slab in use
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    const unsigned c = (unsigned)(((4 * q + j) ^ ((fr >> 1) & 7)) * 16);
+    ax[j] = lds + (unsigned)((wm * 128 + fr) * LT_ROW) + c;
+    aw[j] = lds + (unsigned)((wn * 128 + fr) * LT_ROW) + c;
+  }
+  auto use = [&](int hx, int hw) {
+    int px = hx * HALF, pw = hw * HALF;
+    __asm__ volatile("" : "+s"(px), "+s"(pw));  // (here, and not in front of the slab's first product)
+#pragma unroll
+    for (int j = 0; j < 4; ++j) { cx[j] = ax[j] + (unsigned)px; cw[j] = aw[j] + (unsigned)pw; }
+  };
+  typedef __attribute__((address_space(3))) u32x4_t lds_u4;
+  f32x16_t acc[4][4];
+  u32x4_t fx[2][4], fw[2][4];
+  // fragment r of a step in the order of need: x's first block, W's, the rest of x's
+  auto read = [&](int r, int j, int p) {
+    if (r == 0) fx[p][0] = *(lds_u4 *)(uintptr_t)cx[j];
+    else if (r <= 4) fw[p][r - 1] = *(lds_u4 *)(uintptr_t)(cw[j] + (unsigned)((r - 1) * 32 * LT_ROW));
+    else fx[p][r - 4] = *(lds_u4 *)(uintptr_t)(cx[j] + (unsigned)((r - 4) * 32 * LT_ROW));
+  };
+  start_x(cur);
+  start_w(cur);
+  lt_each<NT>([&](auto t) { send_x(t, 0, in_x()); });
+  ++kx;
+  lt_each<NT>([&](auto t) { send_w(t, 1, in_w()); });
+  ++kw;
+  lt_each<NT>([&](auto t) { send_x(t, 2, in_x()); });
+  ++kx;
+  use(0, 1);
+  int h = 3;  // place of W of the next slab
+  auto clear = [&]() {
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+#pragma unroll
+      for (int e = 0; e < 16; ++e) acc[i >> 2][i & 3][e] = 0.f;
+    }
+  };
+  // products of step j; between them the reads of the next step and the slab's transfers
+  auto step = [&](auto j_, auto transfer) {
+    constexpr int j = decltype(j_)::value, p = j & 1;
+    __builtin_amdgcn_sched_barrier(0);
+    lt_each<16>([&](auto g_) {
+      constexpr int g = decltype(g_)::value;
+      acc[g >> 2][g & 3] = lin_mfma32<F16>(fw[p][g & 3], fx[p][g >> 2], acc[g >> 2][g & 3]);
+      __builtin_amdgcn_sched_barrier(0);
+      // (all four waves at once: one read per two products is half of what LDS gives; before the barrier they have to be over)
+      if constexpr (j == 2) { if constexpr (g < 8) read(g, 3, p ^ 1); }
+      else if constexpr (g % 2 == 0) read(g / 2, (j + 1) & 3, p ^ 1);
+      transfer(g_);
+      if constexpr (j == 2 && g == 10) use(h >= 1 ? h - 1 : 4, h);  // the next slab's addresses, behind this one's last read
+      __builtin_amdgcn_sched_barrier(0);
+    });
+  };
+  clear();
+#pragma unroll
+  for (int i = 0; i < 4; ++i) fx[1][i] = fw[1][i] = u32x4_t{0, 0, 0, 0};  // (step 3 in front of the first slab: products of zeros)
+  int left = cur.kt1 - cur.kt0;  // slabs of the tile ahead
+  for (;;) {
+    LT_LGKM0();
+    LT_VM(NT);  // (x of the slab after next may be on its way)
+    __builtin_amdgcn_s_barrier();
+    step(std::integral_constant<int, 3>(), [](auto) {});
+    const int h1 = h + 1 < 5 ? h + 1 : 0;
+    if (left == 0) {
+      // 32 rows of the wave at a time through the kilobytes of the places h and h1 that its own transfers will fill, so that a lane then
+      // has 8 adjacent columns of a row and the rest works on whole lines.  Element e of a lane: column 8 (e / 4) + 4 q + e % 4 of W's
+      // block, row fr of x's; chunk c (four columns) of row r stands in place c ^ (r & 15) of the row's 512 bytes.
+      constexpr int LPR = NC / 16, RPP = 64 / LPR, NP = 32 / RPP;  // lanes of a row (8 columns each), rows of a pass, passes
+      const int lr = lane / LPR, col = 8 * (lane % LPR), at = GATED ? (col >> 5) * 16 + ((col & 31) >> 2) : col >> 2;
+      const unsigned put = (unsigned)(mine + (fr < 16 ? h : h1) * HALF + ((fr >> 1) & 7) * 32 * LT_ROW + (fr & 1) * 512 + (q ^ (fr & 15)) * 16);
+      const unsigned get0 = (unsigned)(mine + (lr >> 1) * 32 * LT_ROW + (lr & 1) * 512 + (at ^ lr) * 16);
+      const unsigned get[2] = {get0 + (unsigned)(h * HALF), get0 + (unsigned)(h1 * HALF)};
+      // pass p of a lane: row lr + RPP p; chunk k of its four (two: columns, gated the second two: of the second matrix)
+      auto fetch = [&](int p, float (&s0)[8], float (&s1)[8]) {
+#pragma unroll
+        for (int k = 0; k < (GATED ? 4 : 2); ++k) {
+          const int in_half = p % (16 / RPP), x = (RPP * in_half) ^ (k & 1) ^ (k >> 1) * 8;
+          const unsigned from = ((p < 16 / RPP ? get[0] : get[1]) ^ (unsigned)(16 * x)) + (unsigned)(in_half * (RPP / 2) * 32 * LT_ROW);
+          const f32x4_t f = __builtin_bit_cast(f32x4_t, *(lds_u4 *)(uintptr_t)from);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) (k >> 1 ? s1 : s0)[4 * (k & 1) + e] = f[e];
+        }
+      };
+      const int n = cur.n0 + wn * (NC / 2) + col, row0 = cur.m0 + wm * 128 + lr;
+      const LinColumns<F16, GATED> c(a, n);
+      // (one copy of the passes for all four blocks: code that runs once a tile waits for its instructions, line by line)
+      auto blocks = [&](auto rows) {
+#pragma clang loop unroll(disable)
+        for (int i = 0; i < 4; ++i) {
+          lt_each<4>([&](auto i_) {
+            if (i == decltype(i_)::value) {
+#pragma unroll
+              for (int b = 0; b < 4; ++b)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                  const f32x16_t &s = acc[decltype(i_)::value][b];
+                  *(lds_u4 *)(uintptr_t)(put ^ (unsigned)(16 * (8 * b + 2 * e))) =
+                      __builtin_bit_cast(u32x4_t, f32x4_t{s[4 * e], s[4 * e + 1], s[4 * e + 2], s[4 * e + 3]});
+                }
+              __asm__ volatile("; %0" :: "i"(decltype(i_)::value));  // (or the compiler makes one copy of the four, over registers chosen by i)
+            }
+          });
+          __builtin_amdgcn_wave_barrier();
+          rows(row0 + 32 * i);
+          __builtin_amdgcn_wave_barrier();
+        }
+      };
+      const bool inside = a.whole && !a.y32 && !a.part && cur.m0 + B <= a.M && cur.n0 + NC <= a.N;
+      // a tile inside the result: no conditions, addresses by addition, the activation chosen once
+      auto plain = [&](int m, auto act_) {
+        const uint16_t *pr = GATED || !a.res ? nullptr : a.res + m * a.ldr + n;
+        uint16_t *py = (uint16_t *)a.y + m * a.ldy + n;
+        u32x4_t res[NP];
+        if (!GATED && a.res)
+#pragma unroll
+          for (int p = 0; p < NP; ++p) res[p] = *(const u32x4_t *)(pr + p * RPP * a.ldr);
+#pragma unroll
+        for (int p = 0; p < NP; ++p) {
+          float s0[8], s1[8];
+          fetch(p, s0, s1);
+          c.template finish<decltype(act_)::value>(s0, s1);
+          if (!GATED && a.res) lin_add<F16>(s0, res[p]);
+          *(u32x4_t *)(py + p * RPP * a.ldy) = lin_pack<F16>(s0);
+        }
+      };
+      blocks([&](int m) {
+        switch (inside ? a.act : -1) {
+          case MOE_ACT_NONE: plain(m, std::integral_constant<int, MOE_ACT_NONE>()); break;
+          case MOE_ACT_SILU: plain(m, std::integral_constant<int, MOE_ACT_SILU>()); break;
+          case MOE_ACT_GELU: plain(m, std::integral_constant<int, MOE_ACT_GELU>()); break;
+          case MOE_ACT_GELU_TANH: plain(m, std::integral_constant<int, MOE_ACT_GELU_TANH>()); break;
+          case MOE_ACT_RELU: plain(m, std::integral_constant<int, MOE_ACT_RELU>()); break;
+          case MOE_ACT_RELU2: plain(m, std::integral_constant<int, MOE_ACT_RELU2>()); break;
+          default: {
+            u32x4_t res = c.residual(a, m);
+#pragma clang loop unroll(disable)
+            for (int p = 0; p < NP; ++p) {
+              const u32x4_t ahead = c.residual(a, p + 1 < NP ? m + (p + 1) * RPP : a.M);
+              float s0[8], s1[8];
+              fetch(p, s0, s1);
+              if (m + p * RPP < a.M) {
+                if (a.part) c.partial(a, cur.split, m + p * RPP, s0, s1);
+                else c.store(a, m + p * RPP, s0, s1, res);
+              }
+              res = ahead;
+            }
+          }
+        }
+      });
+      if (nxt.kt1 == 0) break;
+      v += stride;
+      cur = nxt;
+      nxt = tile_of(v + stride);
+      left = cur.kt1 - cur.kt0;
+      LT_LGKM0();  // (the wave's reads of its places are over)
+      clear();
+    }
+    if (kw == end_w && end_w) start_w(nxt);
+    if (kx == end_x && end_x) start_x(nxt);
+    const bool iw = in_w(), ix = in_x();
+    --left;
+    step(std::integral_constant<int, 0>(), [&](auto g) { if constexpr (g % 2 == 1) send_w(std::integral_constant<int, g / 2>(), h, iw); });
+    step(std::integral_constant<int, 1>(), [&](auto g) { if constexpr (g % 4 == 1) send_x(std::integral_constant<int, g / 4>(), h1, ix); });
+    step(std::integral_constant<int, 2>(), [&](auto g) { if constexpr (g % 4 == 1) send_x(std::integral_constant<int, 4 + g / 4>(), h1, ix); });
+    ++kw;
+    ++kx;
+    h = h1 + 1 < 5 ? h1 + 1 : 0;
+  }
+  LT_VM(0);  // nothing of this workgroup's is on its way into LDS when it ends
 }
 
 // The pieces of K added in their order, then what the tile kernel does behind its sums
@@ -470,7 +702,7 @@ __global__ __launch_bounds__(256) void k_linear_join(const LinArgs a) {
       for (int e = 0; e < 4; ++e) { s[i][e] += u[e]; s[i][4 + e] += v[e]; }
     }
   const LinColumns<F16, GATED> c(a, n);
-  c.store(a, m, s[0], s[1]);
+  c.store(a, m, s[0], s[1], c.residual(a, m));
 }
 
 // ---- entry points -------------------------------------------------------------------------------------------------------------
@@ -497,7 +729,7 @@ static LinPlan lin_plan(int M, int N, int K, bool gated) {
   if (M <= 32) return LinPlan{0, 0, 0, 1};
   const char *e = getenv("LINPLAN");
   if (e) { int v = atoi(e); return LinPlan{v / 10000 % 10, v / 1000 % 10, v / 100 % 10, v % 100}; }
-  if (M > 128) return LinPlan{4, 4, 5, 1};
+  if (M > 128 && K > LT_K) return LinPlan{4, 4, 5, 1};
   return LinPlan{2, 2, 4, 1};
 }
 
@@ -524,10 +756,14 @@ static int lin_launch(const LinArgs &a, float *ws, hipStream_t s) {
   t.splits = pl.splits;
   t.ldp = (a.N + 7) & ~7;
   t.part = pl.splits > 1 ? ws : nullptr;
+  t.slabs = (a.K + LT_K - 1) / LT_K / pl.splits;
+  t.extra = (a.K + LT_K - 1) / LT_K % pl.splits;
   const dim3 grid((t.nm * t.nn * t.splits + 7) / 8 * 8);
 #define LT_LAUNCH(WM_, WN_, RING_) hipLaunchKernelGGL(HIP_KERNEL_NAME(k_linear_tile<F16, GATED, WM_, WN_, RING_>), grid, dim3(256), 0, s, t)
   switch (pl.wm * 100 + pl.wn * 10 + pl.ring) {
-    case 445: LT_LAUNCH(4, 4, 5); break;
+    case 445:
+      hipLaunchKernelGGL(HIP_KERNEL_NAME(k_linear_wide<F16, GATED>), dim3(grid.x < 256 ? grid.x : 256), dim3(256), 0, s, t);
+      break;
     case 224: LT_LAUNCH(2, 2, 4); break;
     case 126: LT_LAUNCH(1, 2, 6); break;
     case 114: if constexpr (!GATED) LT_LAUNCH(1, 1, 4); break;
