@@ -449,21 +449,22 @@ __global__ __launch_bounds__(256, RING * (WM + WN) * 64 * LT_ROW > 80 * 1024 ? 1
 }
 
 // ---- wide tiles: 256 x 256, one workgroup per compute unit that goes from tile to tile -------------------------------------------------
-// The layout of k_linear_tile with WM = WN = 4.  One step's products (16) cover an LDS read, so the fragments of step j + 1 are read
-// between those of step j.  LDS has room for two slabs and a half: a ring of five halves, x and W of a slab in turn (half h of the run in
-// place h % 5).  The loop turns at a barrier in front of step 3 of slab g - 1, whose fragments are that slab's last: everybody has read
-// slab g - 1 then, and slab g has landed; in step 0 of slab g the wave's transfers of W of slab g + 1 go out (where x of slab g - 1 was),
-// in steps 1 and 2 those of x of slab g + 2 (where its W was).  Spread like that since 64 bytes per cycle and compute unit is all that
-// the path takes, half of the time that the products of a slab need: all 16 of a wave in step 3 stopped the products for as long again
-// (59 % busy matrix cores, spread 74).
-// The run of slabs goes on from tile to tile: the next tile's first slab and the half behind it land under the last products, and the
-// sums leave through the places of the last slab while nothing else needs them.
+// Four waves (2 x 2), each on 8 x 8 blocks of 16 x 16.  A slab (64 columns) is two steps of 64 products v_mfma_f32_16x16x32: a step covers
+// an LDS read many times, so the fragments of the next step are read between its products.  (At this size the card is at its power
+// limit, and what counts is the energy of a product: the 32 x 32 x 16 form reads and writes twice the sums per product of two values.)
+// LDS has room for two slabs and a half: a ring of five halves, x and W of a slab in turn (half h of the run in place h % 5).  The loop
+// turns at a barrier in front of step 1 of slab g - 1, whose fragments are that slab's last: everybody has read slab g - 1 then, and
+// slab g has landed.  In that step the wave's transfers of W of slab g + 1 go out (where x of slab g - 1 was), in step 0 of slab g those
+// of x of slab g + 2 (where its W was).  Evenly, since 64 bytes per cycle and compute unit is all that the path takes, half of the time
+// that the products of a slab need: all 16 of a wave at once stopped the products for as long again (59 % busy matrix cores, then 74).
+// The run of slabs goes on from tile to tile: the next tile's first slab and the W half behind it land under the last products, and the
+// sums leave through the one place that nothing else needs then.
 template <bool F16, bool GATED>
 __global__ __launch_bounds__(256, 1) void k_linear_wide(const LinArgs a) {
   constexpr int B = 256, NT = 8, HALF = B * LT_ROW, NC = GATED ? B / 2 : B;
   __shared__ __align__(1024) unsigned char s_ring[5 * HALF];
   const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6), wm = w & 1, wn = w >> 1;
-  const int fr = lane & 31, q = lane >> 5;
+  const int fr = lane & 15, q = lane >> 4;
   const unsigned lds = (unsigned)(uintptr_t)(__attribute__((address_space(3))) unsigned char *)s_ring;
   // workgroup i runs on XCD i % 8: each XCD takes a contiguous run of tiles, four rows of tiles wide
   const int tiles = a.nm * a.nn, stride = (int)gridDim.x >> 3;
@@ -510,10 +511,10 @@ __global__ __launch_bounds__(256, 1) void k_linear_wide(const LinArgs a) {
   auto in_w = [&]() { return kw * LT_K + 8 * chunk < min(a.K, end_w * LT_K); };
   auto send_x = [&](auto t, int h, bool in) { send(vx[t], rx, kx, in, mine + h * HALF, t); };
   auto send_w = [&](auto t, int h, bool in) { send(vw[t], GATED && (t & 1) ? rw1 : rw0, kw, in, mine + h * HALF, t); };
-  unsigned ax[4], aw[4], cx[4], cw[4];  // LDS address of the lane's fragment of step j in block 0: in place 0, and of the slab in use
+  unsigned ax[2], aw[2], cx[2], cw[2];  // LDS address of the lane's fragment of step j in block 0: in place 0, and of the slab in use
 #pragma unroll
-  for (int j = 0; j < 4; ++j) {
-    const unsigned c = (unsigned)(((4 * q + j) ^ ((fr >> 1) & 7)) * 16);
+  for (int j = 0; j < 2; ++j) {
+    const unsigned c = (unsigned)(((4 * j + q) ^ ((fr >> 1) & 7)) * 16);
     ax[j] = lds + (unsigned)((wm * 128 + fr) * LT_ROW) + c;
     aw[j] = lds + (unsigned)((wn * 128 + fr) * LT_ROW) + c;
   }
@@ -521,16 +522,16 @@ __global__ __launch_bounds__(256, 1) void k_linear_wide(const LinArgs a) {
     int px = hx * HALF, pw = hw * HALF;
     __asm__ volatile("" : "+s"(px), "+s"(pw));  // (here, and not in front of the slab's first product)
 #pragma unroll
-    for (int j = 0; j < 4; ++j) { cx[j] = ax[j] + (unsigned)px; cw[j] = aw[j] + (unsigned)pw; }
+    for (int j = 0; j < 2; ++j) { cx[j] = ax[j] + (unsigned)px; cw[j] = aw[j] + (unsigned)pw; }
   };
   typedef __attribute__((address_space(3))) u32x4_t lds_u4;
-  f32x16_t acc[4][4];
-  u32x4_t fx[2][4], fw[2][4];
+  f32x4_t acc[8][8];
+  u32x4_t fx[2][8], fw[2][8];
   // fragment r of a step in the order of need: x's first block, W's, the rest of x's
-  auto read = [&](int r, int j, int p) {
-    if (r == 0) fx[p][0] = *(lds_u4 *)(uintptr_t)cx[j];
-    else if (r <= 4) fw[p][r - 1] = *(lds_u4 *)(uintptr_t)(cw[j] + (unsigned)((r - 1) * 32 * LT_ROW));
-    else fx[p][r - 4] = *(lds_u4 *)(uintptr_t)(cx[j] + (unsigned)((r - 4) * 32 * LT_ROW));
+  auto read = [&](int r, int j) {
+    if (r == 0) fx[j][0] = *(lds_u4 *)(uintptr_t)cx[j];
+    else if (r <= 8) fw[j][r - 1] = *(lds_u4 *)(uintptr_t)(cw[j] + (unsigned)((r - 1) * 16 * LT_ROW));
+    else fx[j][r - 8] = *(lds_u4 *)(uintptr_t)(cx[j] + (unsigned)((r - 8) * 16 * LT_ROW));
   };
   start_x(cur);
   start_w(cur);
@@ -544,52 +545,51 @@ __global__ __launch_bounds__(256, 1) void k_linear_wide(const LinArgs a) {
   int h = 3;  // place of W of the next slab
   auto clear = [&]() {
 #pragma unroll
-    for (int i = 0; i < 16; ++i) {
-#pragma unroll
-      for (int e = 0; e < 16; ++e) acc[i >> 2][i & 3][e] = 0.f;
-    }
+    for (int i = 0; i < 64; ++i) acc[i >> 3][i & 7] = f32x4_t{0.f, 0.f, 0.f, 0.f};
   };
-  // products of step j; between them the reads of the next step and the slab's transfers
+  // products of step j; between them the reads of the other step and eight transfers
   auto step = [&](auto j_, auto transfer) {
-    constexpr int j = decltype(j_)::value, p = j & 1;
+    constexpr int j = decltype(j_)::value;
     __builtin_amdgcn_sched_barrier(0);
-    lt_each<16>([&](auto g_) {
+    lt_each<64>([&](auto g_) {
       constexpr int g = decltype(g_)::value;
-      acc[g >> 2][g & 3] = lin_mfma32<F16>(fw[p][g & 3], fx[p][g >> 2], acc[g >> 2][g & 3]);
+      acc[g >> 3][g & 7] = lin_mfma16<F16>(fw[j][g & 7], fx[j][g >> 3], acc[g >> 3][g & 7]);
       __builtin_amdgcn_sched_barrier(0);
-      // (all four waves at once: one read per two products is half of what LDS gives; before the barrier they have to be over)
-      if constexpr (j == 2) { if constexpr (g < 8) read(g, 3, p ^ 1); }
-      else if constexpr (g % 2 == 0) read(g / 2, (j + 1) & 3, p ^ 1);
-      transfer(g_);
-      if constexpr (j == 2 && g == 10) use(h >= 1 ? h - 1 : 4, h);  // the next slab's addresses, behind this one's last read
+      // (in front of the barrier the reads have to be over: those of step 1 come in the first half of step 0)
+      if constexpr (j == 0) { if constexpr (g % 2 == 0 && g < 32) read(g / 2, 1); }
+      else if constexpr (g % 4 == 0) read(g / 4, 0);
+      if constexpr (g % 8 == 3) transfer(std::integral_constant<int, g / 8>());
+      if constexpr (j == 0 && g == 36) use(h >= 1 ? h - 1 : 4, h);  // the next slab's addresses, behind this one's last read
       __builtin_amdgcn_sched_barrier(0);
     });
   };
   clear();
 #pragma unroll
-  for (int i = 0; i < 4; ++i) fx[1][i] = fw[1][i] = u32x4_t{0, 0, 0, 0};  // (step 3 in front of the first slab: products of zeros)
+  for (int i = 0; i < 8; ++i) fx[1][i] = fw[1][i] = u32x4_t{0, 0, 0, 0};  // (step 1 in front of the first slab: products of zeros)
   int left = cur.kt1 - cur.kt0;  // slabs of the tile ahead
   for (;;) {
+    if (kw == end_w && end_w) start_w(nxt);
+    const bool iw = in_w();
     LT_LGKM0();
     LT_VM(NT);  // (x of the slab after next may be on its way)
     __builtin_amdgcn_s_barrier();
-    step(std::integral_constant<int, 3>(), [](auto) {});
+    step(std::integral_constant<int, 1>(), [&](auto t) { send_w(t, h, iw); });
+    ++kw;
     const int h1 = h + 1 < 5 ? h + 1 : 0;
     if (left == 0) {
-      // 32 rows of the wave at a time through the kilobytes of the places h and h1 that its own transfers will fill, so that a lane then
-      // has 8 adjacent columns of a row and the rest works on whole lines.  Element e of a lane: column 8 (e / 4) + 4 q + e % 4 of W's
-      // block, row fr of x's; chunk c (four columns) of row r stands in place c ^ (r & 15) of the row's 512 bytes.
-      constexpr int LPR = NC / 16, RPP = 64 / LPR, NP = 32 / RPP;  // lanes of a row (8 columns each), rows of a pass, passes
+      // 16 rows of the wave at a time through the kilobytes of place h1 that its own transfers will fill, so that a lane then has 8
+      // adjacent columns of a row and the rest works on whole lines.  Element e of a lane: column 4 q + e of W's block, row fr of x's;
+      // chunk c (four columns) of row r stands in place c ^ r of the row's 512 bytes.
+      constexpr int LPR = NC / 16, RPP = 64 / LPR, NP = 16 / RPP;  // lanes of a row (8 columns each), rows of a pass, passes
       const int lr = lane / LPR, col = 8 * (lane % LPR), at = GATED ? (col >> 5) * 16 + ((col & 31) >> 2) : col >> 2;
-      const unsigned put = (unsigned)(mine + (fr < 16 ? h : h1) * HALF + ((fr >> 1) & 7) * 32 * LT_ROW + (fr & 1) * 512 + (q ^ (fr & 15)) * 16);
-      const unsigned get0 = (unsigned)(mine + (lr >> 1) * 32 * LT_ROW + (lr & 1) * 512 + (at ^ lr) * 16);
-      const unsigned get[2] = {get0 + (unsigned)(h * HALF), get0 + (unsigned)(h1 * HALF)};
+      const unsigned put = (unsigned)(mine + h1 * HALF + (fr >> 1) * 32 * LT_ROW + (fr & 1) * 512 + (q ^ fr) * 16);
+      const unsigned get = (unsigned)(mine + h1 * HALF + (lr >> 1) * 32 * LT_ROW + (lr & 1) * 512 + (at ^ lr) * 16);
       // pass p of a lane: row lr + RPP p; chunk k of its four (two: columns, gated the second two: of the second matrix)
       auto fetch = [&](int p, float (&s0)[8], float (&s1)[8]) {
 #pragma unroll
         for (int k = 0; k < (GATED ? 4 : 2); ++k) {
-          const int in_half = p % (16 / RPP), x = (RPP * in_half) ^ (k & 1) ^ (k >> 1) * 8;
-          const unsigned from = ((p < 16 / RPP ? get[0] : get[1]) ^ (unsigned)(16 * x)) + (unsigned)(in_half * (RPP / 2) * 32 * LT_ROW);
+          const int x = (RPP * p) ^ (k & 1) ^ (k >> 1) * 8;
+          const unsigned from = (get ^ (unsigned)(16 * x)) + (unsigned)(p * (RPP / 2) * 32 * LT_ROW);
           const f32x4_t f = __builtin_bit_cast(f32x4_t, *(lds_u4 *)(uintptr_t)from);
 #pragma unroll
           for (int e = 0; e < 4; ++e) (k >> 1 ? s1 : s0)[4 * (k & 1) + e] = f[e];
@@ -597,25 +597,20 @@ __global__ __launch_bounds__(256, 1) void k_linear_wide(const LinArgs a) {
       };
       const int n = cur.n0 + wn * (NC / 2) + col, row0 = cur.m0 + wm * 128 + lr;
       const LinColumns<F16, GATED> c(a, n);
-      // (one copy of the passes for all four blocks: code that runs once a tile waits for its instructions, line by line)
+      // (one copy of the passes for all eight blocks: code that runs once a tile waits for its instructions, line by line)
       auto blocks = [&](auto rows) {
 #pragma clang loop unroll(disable)
-        for (int i = 0; i < 4; ++i) {
-          lt_each<4>([&](auto i_) {
+        for (int i = 0; i < 8; ++i) {
+          lt_each<8>([&](auto i_) {
             if (i == decltype(i_)::value) {
 #pragma unroll
-              for (int b = 0; b < 4; ++b)
-#pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                  const f32x16_t &s = acc[decltype(i_)::value][b];
-                  *(lds_u4 *)(uintptr_t)(put ^ (unsigned)(16 * (8 * b + 2 * e))) =
-                      __builtin_bit_cast(u32x4_t, f32x4_t{s[4 * e], s[4 * e + 1], s[4 * e + 2], s[4 * e + 3]});
-                }
-              __asm__ volatile("; %0" :: "i"(decltype(i_)::value));  // (or the compiler makes one copy of the four, over registers chosen by i)
+              for (int b = 0; b < 8; ++b)
+                *(lds_u4 *)(uintptr_t)(put ^ (unsigned)(16 * 4 * b)) = __builtin_bit_cast(u32x4_t, acc[decltype(i_)::value][b]);
+              __asm__ volatile("; %0" :: "i"(decltype(i_)::value));  // (or the compiler makes one copy of the eight, over registers chosen by i)
             }
           });
           __builtin_amdgcn_wave_barrier();
-          rows(row0 + 32 * i);
+          rows(row0 + 16 * i);
           __builtin_amdgcn_wave_barrier();
         }
       };
@@ -628,14 +623,17 @@ __global__ __launch_bounds__(256, 1) void k_linear_wide(const LinArgs a) {
         if (!GATED && a.res)
 #pragma unroll
           for (int p = 0; p < NP; ++p) res[p] = *(const u32x4_t *)(pr + p * RPP * a.ldr);
+        float s0[2][8], s1[2][8];
+        fetch(0, s0[0], s1[0]);
 #pragma unroll
-        for (int p = 0; p < NP; ++p) {
-          float s0[8], s1[8];
-          fetch(p, s0, s1);
-          c.template finish<decltype(act_)::value>(s0, s1);
-          if (!GATED && a.res) lin_add<F16>(s0, res[p]);
-          *(u32x4_t *)(py + p * RPP * a.ldy) = lin_pack<F16>(s0);
+        for (int p = 0; p < NP; ++p) {  // (one pass read ahead and no more: the compiler counts on registers that the sums have)
+          __builtin_amdgcn_sched_barrier(0);
+          if (p + 1 < NP) fetch(p + 1, s0[(p + 1) & 1], s1[(p + 1) & 1]);
+          c.template finish<decltype(act_)::value>(s0[p & 1], s1[p & 1]);
+          if (!GATED && a.res) lin_add<F16>(s0[p & 1], res[p]);
+          *(u32x4_t *)(py + p * RPP * a.ldy) = lin_pack<F16>(s0[p & 1]);
         }
+        __builtin_amdgcn_sched_barrier(0);
       };
       blocks([&](int m) {
         switch (inside ? a.act : -1) {
@@ -646,15 +644,17 @@ __global__ __launch_bounds__(256, 1) void k_linear_wide(const LinArgs a) {
           case MOE_ACT_RELU: plain(m, std::integral_constant<int, MOE_ACT_RELU>()); break;
           case MOE_ACT_RELU2: plain(m, std::integral_constant<int, MOE_ACT_RELU2>()); break;
           default: {
-            u32x4_t res = c.residual(a, m);
+            LinColumns<F16, GATED> c1 = c;
+            __asm__ volatile("" : "+v"(c1.n), "+v"(c1.count));  // (what follows from them is not kept in registers over the blocks)
+            u32x4_t res = c1.residual(a, m);
 #pragma clang loop unroll(disable)
             for (int p = 0; p < NP; ++p) {
-              const u32x4_t ahead = c.residual(a, p + 1 < NP ? m + (p + 1) * RPP : a.M);
+              const u32x4_t ahead = c1.residual(a, p + 1 < NP ? m + (p + 1) * RPP : a.M);
               float s0[8], s1[8];
               fetch(p, s0, s1);
               if (m + p * RPP < a.M) {
-                if (a.part) c.partial(a, cur.split, m + p * RPP, s0, s1);
-                else c.store(a, m + p * RPP, s0, s1, res);
+                if (a.part) c1.partial(a, cur.split, m + p * RPP, s0, s1);
+                else c1.store(a, m + p * RPP, s0, s1, res);
               }
               res = ahead;
             }
@@ -669,14 +669,10 @@ __global__ __launch_bounds__(256, 1) void k_linear_wide(const LinArgs a) {
       LT_LGKM0();  // (the wave's reads of its places are over)
       clear();
     }
-    if (kw == end_w && end_w) start_w(nxt);
     if (kx == end_x && end_x) start_x(nxt);
-    const bool iw = in_w(), ix = in_x();
+    const bool ix = in_x();
     --left;
-    step(std::integral_constant<int, 0>(), [&](auto g) { if constexpr (g % 2 == 1) send_w(std::integral_constant<int, g / 2>(), h, iw); });
-    step(std::integral_constant<int, 1>(), [&](auto g) { if constexpr (g % 4 == 1) send_x(std::integral_constant<int, g / 4>(), h1, ix); });
-    step(std::integral_constant<int, 2>(), [&](auto g) { if constexpr (g % 4 == 1) send_x(std::integral_constant<int, 4 + g / 4>(), h1, ix); });
-    ++kw;
+    step(std::integral_constant<int, 0>(), [&](auto t) { send_x(t, h1, ix); });
     ++kx;
     h = h1 + 1 < 5 ? h1 + 1 : 0;
   }
