@@ -483,8 +483,8 @@ __global__ __launch_bounds__(256, 1) void k_linear_wide(const LinArgs a) {
   Tile cur = tile_of(v), nxt = tile_of(v + stride);
   // transfer t of wave w: rows 32 t + 8 w .. + 7, eight lanes a row; the lanes choose the chunk that belongs in their slot
   const int tr = 8 * w + (lane >> 3), chunk = (lane & 7) ^ ((tr >> 1) & 7);
-  // x and W each have a cursor: the slab that their next transfers bring, of this tile or of the next (past the last tile: zeros).  A
-  // tile has at least two slabs.
+  // x and W each have a cursor: the slab that their next transfers bring, of this tile or of the next.  A tile has at least two slabs.
+  // Columns past K, and everything past the last tile, are out of the resource's range: zeros.
   int vx[NT], vw[NT], kx, kw, end_x, end_w;
   lt_rsrc_t rx, rw0, rw1{};
   auto start_x = [&](const Tile &t) {
@@ -500,17 +500,29 @@ __global__ __launch_bounds__(256, 1) void k_linear_wide(const LinArgs a) {
 #pragma unroll
     for (int i = 0; i < NT; ++i) vw[i] = (min(t.n0 + 32 * (GATED ? i >> 1 : i) + tr, a.N - 1) - t.n0) * (int)a.ldw * 2 + 16 * chunk;
   };
+  // what a slab's transfers need beyond the slab before: the next tile's rows, or the lanes past K left out (a slab that ends past K is its
+  // tile's last)
+  auto leave_out = [&](int (&o)[NT], bool all, int k) {
+#pragma unroll
+    for (int i = 0; i < NT; ++i) o[i] = all || k * LT_K + 8 * chunk >= a.K ? LT_OUT : o[i];
+  };
+  auto turn_x = [&]() {
+    if (kx == end_x) { if (nxt.kt1) start_x(nxt); else { end_x = 0; leave_out(vx, true, 0); } }
+    if (kx * LT_K + LT_K > a.K) leave_out(vx, false, kx);
+  };
+  auto turn_w = [&]() {
+    if (kw == end_w) { if (nxt.kt1) start_w(nxt); else { end_w = 0; leave_out(vw, true, 0); } }
+    if (kw * LT_K + LT_K > a.K) leave_out(vw, false, kw);
+  };
   // (assembly: see k_linear_tile)
-  auto send = [&](int off, const lt_rsrc_t rs, int kt, bool in, int to, auto t) {
+  auto send = [&](int off, const lt_rsrc_t rs, int kt, int to, auto t) {
     __asm__ volatile("s_add_u32 m0, %0, %4\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, %3 offen lds"
-                     :: "s"(to), "v"(in ? off : LT_OUT), "s"(rs), "s"(kt * (LT_K * 2)), "i"(decltype(t)::value * 32 * LT_ROW)
+                     :: "s"(to), "v"(off), "s"(rs), "s"(kt * (LT_K * 2)), "i"(decltype(t)::value * 32 * LT_ROW)
                      : "memory", "m0", "scc");
   };
   const int mine = (int)lds + 8 * w * LT_ROW;  // the wave's rows in a half
-  auto in_x = [&]() { return kx * LT_K + 8 * chunk < min(a.K, end_x * LT_K); };
-  auto in_w = [&]() { return kw * LT_K + 8 * chunk < min(a.K, end_w * LT_K); };
-  auto send_x = [&](auto t, int h, bool in) { send(vx[t], rx, kx, in, mine + h * HALF, t); };
-  auto send_w = [&](auto t, int h, bool in) { send(vw[t], GATED && (t & 1) ? rw1 : rw0, kw, in, mine + h * HALF, t); };
+  auto send_x = [&](auto t, int h) { send(vx[t], rx, kx, mine + h * HALF, t); };
+  auto send_w = [&](auto t, int h) { send(vw[t], GATED && (t & 1) ? rw1 : rw0, kw, mine + h * HALF, t); };
   unsigned ax[2], aw[2], cx[2], cw[2];  // LDS address of the lane's fragment of step j in block 0: in place 0, and of the slab in use
 #pragma unroll
   for (int j = 0; j < 2; ++j) {
@@ -535,11 +547,12 @@ __global__ __launch_bounds__(256, 1) void k_linear_wide(const LinArgs a) {
   };
   start_x(cur);
   start_w(cur);
-  lt_each<NT>([&](auto t) { send_x(t, 0, in_x()); });
+  lt_each<NT>([&](auto t) { send_x(t, 0); });
   ++kx;
-  lt_each<NT>([&](auto t) { send_w(t, 1, in_w()); });
+  lt_each<NT>([&](auto t) { send_w(t, 1); });
   ++kw;
-  lt_each<NT>([&](auto t) { send_x(t, 2, in_x()); });
+  turn_x();
+  lt_each<NT>([&](auto t) { send_x(t, 2); });
   ++kx;
   use(0, 1);
   int h = 3;  // place of W of the next slab
@@ -568,12 +581,11 @@ __global__ __launch_bounds__(256, 1) void k_linear_wide(const LinArgs a) {
   for (int i = 0; i < 8; ++i) fx[1][i] = fw[1][i] = u32x4_t{0, 0, 0, 0};  // (step 1 in front of the first slab: products of zeros)
   int left = cur.kt1 - cur.kt0;  // slabs of the tile ahead
   for (;;) {
-    if (kw == end_w && end_w) start_w(nxt);
-    const bool iw = in_w();
+    turn_w();
     LT_LGKM0();
     LT_VM(NT);  // (x of the slab after next may be on its way)
     __builtin_amdgcn_s_barrier();
-    step(std::integral_constant<int, 1>(), [&](auto t) { send_w(t, h, iw); });
+    step(std::integral_constant<int, 1>(), [&](auto t) { send_w(t, h); });
     ++kw;
     const int h1 = h + 1 < 5 ? h + 1 : 0;
     if (left == 0) {
@@ -669,10 +681,9 @@ __global__ __launch_bounds__(256, 1) void k_linear_wide(const LinArgs a) {
       LT_LGKM0();  // (the wave's reads of its places are over)
       clear();
     }
-    if (kx == end_x && end_x) start_x(nxt);
-    const bool ix = in_x();
+    turn_x();
     --left;
-    step(std::integral_constant<int, 0>(), [&](auto t) { send_x(t, h1, ix); });
+    step(std::integral_constant<int, 0>(), [&](auto t) { send_x(t, h1); });
     ++kx;
     h = h1 + 1 < 5 ? h1 + 1 : 0;
   }
