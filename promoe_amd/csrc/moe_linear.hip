@@ -201,23 +201,20 @@ struct LinColumns {
 // the operand are 16 rows of W; with few rows of x (M <= 16 / SH) the operand is R rows of W by SH pieces of K, row s R + r and column
 // s R + m hold piece s of both, and the products of unlike pieces are left unread: a smaller unit of work (more workgroups for a
 // short matrix) and longer runs of a row per load.
-// MB: blocks of 16 rows of x.
 #define LR_WAVES 8
 #define LR_U 4  // loads of a matrix in flight per wave, twice
-template <bool F16, bool GATED, int MB, int SH>
+template <bool F16, bool GATED, int SH>
 __global__ __launch_bounds__(64 * LR_WAVES) void k_linear_rows(const LinArgs a) {
   constexpr int NM = GATED ? 2 : 1, R = 16 / SH, STEP = 32 * SH * LR_U, SPAN = STEP * LR_WAVES;
-  __shared__ f32x4_t red[LR_WAVES][NM][MB][64];
+  __shared__ f32x4_t red[LR_WAVES][NM][64];
   const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int r = (lane & 15) % R, s = (lane & 15) / R, n0 = blockIdx.x * R;
   const int k0 = 8 * ((lane >> 4) * SH + s);                    // the lane's columns inside 32 SH
   const rsrc_t rx = make_rsrc(a.x, LT_OUT), rw0 = make_rsrc(a.w[0] + n0 * a.ldw, LT_OUT), rw1 = make_rsrc(a.w[GATED ? 1 : 0] + n0 * a.ldw, LT_OUT);
   const int vw = (min(n0 + r, a.N - 1) - n0) * (int)a.ldw * 2;
-  int vx[MB];
-#pragma unroll
-  for (int b = 0; b < MB; ++b) vx[b] = min(16 * b + r, a.M - 1) * (int)a.ldx * 2;
-  f32x4_t acc[NM][MB] = {};
-  uint4 fw[2][NM][LR_U], fx[2][MB][LR_U];
+  const int vx = min(r, a.M - 1) * (int)a.ldx * 2;
+  f32x4_t acc[NM] = {};
+  uint4 fw[2][NM][LR_U], fx[2][LR_U];
   auto load = [&](int p, int base) {
 #pragma unroll
     for (int u = 0; u < LR_U; ++u) {
@@ -225,8 +222,7 @@ __global__ __launch_bounds__(64 * LR_WAVES) void k_linear_rows(const LinArgs a) 
       const bool in = k < a.K;                                  // past the end: zeros on both sides
       fw[p][0][u] = bload16(rw0, in ? vw + 2 * k : LT_OUT, 0);
       if constexpr (GATED) fw[p][1][u] = bload16(rw1, in ? vw + 2 * k : LT_OUT, 0);
-#pragma unroll
-      for (int b = 0; b < MB; ++b) fx[p][b][u] = bload16(rx, in ? vx[b] + 2 * k : LT_OUT, 0);
+      fx[p][u] = bload16(rx, in ? vx + 2 * k : LT_OUT, 0);
     }
   };
   auto use = [&](int p) {
@@ -234,9 +230,7 @@ __global__ __launch_bounds__(64 * LR_WAVES) void k_linear_rows(const LinArgs a) 
     for (int u = 0; u < LR_U; ++u)
 #pragma unroll
       for (int i = 0; i < NM; ++i)
-#pragma unroll
-        for (int b = 0; b < MB; ++b)
-          acc[i][b] = lin_mfma16<F16>(__builtin_bit_cast(u32x4_t, fw[p][i][u]), __builtin_bit_cast(u32x4_t, fx[p][b][u]), acc[i][b]);
+        acc[i] = lin_mfma16<F16>(__builtin_bit_cast(u32x4_t, fw[p][i][u]), __builtin_bit_cast(u32x4_t, fx[p][u]), acc[i]);
   };
   load(0, w * STEP);
   for (int base = w * STEP; base < a.K; base += 2 * SPAN) {
@@ -246,13 +240,11 @@ __global__ __launch_bounds__(64 * LR_WAVES) void k_linear_rows(const LinArgs a) 
     use(1);
   }
 #pragma unroll
-  for (int i = 0; i < NM; ++i)
-#pragma unroll
-    for (int b = 0; b < MB; ++b) red[w][i][b][lane] = acc[i][b];
+  for (int i = 0; i < NM; ++i) red[w][i][lane] = acc[i];
   __syncthreads();
   // result (m, n): element n' % 4 of lane 16 (n' / 4) + m', n' = s R + n and m' = s R + m, over the pieces and the waves in order
   for (int t = tid; t < R * a.M; t += 64 * LR_WAVES) {
-    const int n = t % R, m = t / R, b = m >> 4;
+    const int n = t % R, m = t / R;
     if (n0 + n >= a.N) continue;
     float sum[NM];
 #pragma unroll
@@ -262,7 +254,7 @@ __global__ __launch_bounds__(64 * LR_WAVES) void k_linear_rows(const LinArgs a) 
       for (int p = 0; p < SH; ++p) {
         const int row = p * R + n;
 #pragma unroll
-        for (int v = 0; v < LR_WAVES; ++v) sum[i] += ((const float *)&red[v][i][b][16 * (row >> 2) + p * R + (m & 15)])[row & 3];
+        for (int v = 0; v < LR_WAVES; ++v) sum[i] += ((const float *)&red[v][i][16 * (row >> 2) + p * R + m])[row & 3];
       }
     }
     lin_store<F16, GATED>(a, m, n0 + n, sum[0], sum[NM - 1]);
@@ -594,8 +586,8 @@ __global__ __launch_bounds__(256, 1) void k_linear_wide(const LinArgs a) {
       // chunk c (four columns) of row r stands in place c ^ r of the row's 512 bytes.
       constexpr int LPR = NC / 16, RPP = 64 / LPR, NP = 16 / RPP;  // lanes of a row (8 columns each), rows of a pass, passes
       const int lr = lane / LPR, col = 8 * (lane % LPR), at = GATED ? (col >> 5) * 16 + ((col & 31) >> 2) : col >> 2;
-      const unsigned put = (unsigned)(mine + h1 * HALF + (fr >> 1) * 32 * LT_ROW + (fr & 1) * 512 + (q ^ fr) * 16);
-      const unsigned get = (unsigned)(mine + h1 * HALF + (lr >> 1) * 32 * LT_ROW + (lr & 1) * 512 + (at ^ lr) * 16);
+      unsigned put = (unsigned)(mine + h1 * HALF + (fr >> 1) * 32 * LT_ROW + (fr & 1) * 512 + (q ^ fr) * 16);
+      unsigned get = (unsigned)(mine + h1 * HALF + (lr >> 1) * 32 * LT_ROW + (lr & 1) * 512 + (at ^ lr) * 16);
       // pass p of a lane: row lr + RPP p; chunk k of its four (two: columns, gated the second two: of the second matrix)
       auto fetch = [&](int p, float (&s0)[8], float (&s1)[8]) {
 #pragma unroll
@@ -613,6 +605,7 @@ __global__ __launch_bounds__(256, 1) void k_linear_wide(const LinArgs a) {
       auto blocks = [&](auto rows) {
 #pragma clang loop unroll(disable)
         for (int i = 0; i < 8; ++i) {
+          __asm__ volatile("" : "+v"(put), "+v"(get));  // (the addresses that follow from them are not kept over the blocks)
           lt_each<8>([&](auto i_) {
             if (i == decltype(i_)::value) {
 #pragma unroll
@@ -729,15 +722,42 @@ static int lin_check(const char *who, const LinArgs &a, int dtype, bool gated) {
   return MOE_OK;
 }
 
-// Which kernel a product takes: few rows (wm 0), or tiles of 64 wm x 64 wn with `ring` slabs in LDS and K in `splits` pieces
+// Which kernel a product takes: few rows (wm 0), or tiles of 64 wm x 64 wn with `ring` slabs in LDS (4 x 4: the wide kernel) and K in
+// `splits` pieces.  The plan of the least time after a model of one launch, us, fitted to 1900 measured times of 100 shapes (33 to 4096
+// rows; the chosen plan is 1.6 % slower than the best of all on average, 22 % at worst):
+//   rounds x (slabs x (c0 + c1 x share of the compute units in use) + f),  with pieces 2.5 + 0.33 a piece + 0.15 per MB of partial sums
+// c0, c1: a slab of a workgroup on an idle chip, and what the others' traffic adds; f: start and epilogue.  The narrow tiles are bound by
+// LDS (96 (wm + wn) bytes x rows read and written for 32 wm wn of products), the wide one by the matrix cores, at the power limit.
+// us, best other tile / chosen: 64 x 4096 x 4096 14.5 / 13.1 (64 x 64, 3 pieces), 512 x 4096 x 4096 28.7 / 25.0 (64 x 128), 1024 x 4096 x
+// 4096 49 / 38.1 (128 x 128), 300 x 2048 x 10944 33.7 / 31.6 (128 x 128, 4 pieces), 2048 x 4096 x 4096 101 / 67.7 (128 x 256).
+// Few rows, us, k_linear_rows / best tile: 3 x 2048 x 10944 13.4 / 14.8, 8 x 4096 x 4096 11.2 / 11.5, 16 x 4096 x 4096 10.7 / 11.6, 8 x 2048 x
+// 1408 4.9 / 7.4, 16 x 2048 x 1408 6.0 / 7.4; past 8 rows a long reduction is faster on tiles in pieces (every workgroup reads all of x,
+// which no longer passes unnoticed beside the weights): 12 x 2048 x 10944 23.0 / 15.5, 16 x 4096 x 14336 37.7 / 27.9, and past 16 the tiles
+// are in general: 24 x 4096 x 4096 13.3 / 12.0, 24 gated 14336 x 4096 69 / 51.
 struct LinPlan { int wm, wn, ring, splits; };
-#include <stdlib.h>
 static LinPlan lin_plan(int M, int N, int K, bool gated) {
-  if (M <= 32) return LinPlan{0, 0, 0, 1};
-  const char *e = getenv("LINPLAN");
-  if (e) { int v = atoi(e); return LinPlan{v / 10000 % 10, v / 1000 % 10, v / 100 % 10, v % 100}; }
-  if (M > 128 && K > LT_K) return LinPlan{4, 4, 5, 1};
-  return LinPlan{2, 2, 4, 1};
+  if (M <= 8 || (M <= 16 && K <= 4096)) return LinPlan{0, 0, 0, 1};
+  struct Tile { int wm, wn, ring, per_cu; float c0, c1, f; };
+  static const Tile tiles[] = {{1, 1, 4, 2, 0.173f, 0.135f, 0.f}, {1, 2, 6, 1, 0.269f, 0.139f, 1.46f}, {2, 2, 4, 1, 0.380f, 0.221f, 2.2f},
+                               {2, 4, 3, 1, 0.674f, 0.236f, 4.34f}, {4, 4, 5, 1, 1.146f, 0.f, 9.21f}};
+  static const int pieces[] = {1, 2, 3, 4, 5, 6, 8, 12, 16};
+  const long long slabs = (K + LT_K - 1) / LT_K;
+  LinPlan best{2, 2, 4, 1};
+  float least = 1e30f;
+  for (const Tile &t : tiles) {
+    if (gated && t.wn == 1) continue;  // (a pair needs both matrices' blocks in a wave)
+    const int cols = 64 * t.wn / (gated ? 2 : 1);
+    const long long n = ((long long)M + 64 * t.wm - 1) / (64 * t.wm) * (((long long)N + cols - 1) / cols);
+    for (int s : pieces) {
+      if (s > slabs || (s > 1 && n * s > 640) || (t.wm == 4 && slabs < 2 * s)) break;
+      const long long wgs = n * s, rounds = (wgs + 256 * t.per_cu - 1) / (256 * t.per_cu);
+      const float use = wgs >= 256 * t.per_cu ? (float)t.per_cu : (float)wgs / 256.f;
+      float us = (float)rounds * ((float)((slabs + s - 1) / s) * (t.c0 + t.c1 * use) + t.f);
+      if (s > 1) us += 2.5f + 0.33f * (float)s + 0.148e-6f * 8.f * (float)s * (gated ? 2.f : 1.f) * (float)M * (float)N;
+      if (us < least) { least = us; best = LinPlan{t.wm, t.wn, t.ring, s}; }
+    }
+  }
+  return best;
 }
 
 template <bool F16, bool GATED>
@@ -745,19 +765,18 @@ static int lin_launch(const LinArgs &a, float *ws, hipStream_t s) {
   constexpr int NM = GATED ? 2 : 1;
   LinArgs t = a;
   t.whole = !(((uintptr_t)a.y | (uintptr_t)a.ldy * (a.y32 ? 4 : 2) | (uintptr_t)a.res | (a.res ? (uintptr_t)a.ldr * 2 : 0)) & 15);
-  if (a.M <= 32) {
-    const bool two = a.M > 16;
-    const int sh = a.M <= 4 && a.N < 16 * 512 ? 4 : a.M <= 8 && a.N < 16 * 512 ? 2 : 1;
+  const LinPlan pl = lin_plan(a.M, a.N, a.K, GATED);
+  if (pl.wm == 0) {
+    // rows of x in the operand beside pieces of K: more workgroups where 16 rows of W each would be fewer than two per compute unit
+    const int sh = a.N >= 16 * 512 ? 1 : a.M <= 4 ? 4 : a.M <= 8 ? 2 : 1;
     const dim3 grid((a.N + 16 / sh - 1) / (16 / sh));
-#define LR_LAUNCH(MB_, SH_) hipLaunchKernelGGL(HIP_KERNEL_NAME(k_linear_rows<F16, GATED, MB_, SH_>), grid, dim3(64 * LR_WAVES), 0, s, t)
-    if (two) LR_LAUNCH(2, 1);
-    else if (sh == 4) LR_LAUNCH(1, 4);
-    else if (sh == 2) LR_LAUNCH(1, 2);
-    else LR_LAUNCH(1, 1);
+#define LR_LAUNCH(SH_) hipLaunchKernelGGL(HIP_KERNEL_NAME(k_linear_rows<F16, GATED, SH_>), grid, dim3(64 * LR_WAVES), 0, s, t)
+    if (sh == 4) LR_LAUNCH(4);
+    else if (sh == 2) LR_LAUNCH(2);
+    else LR_LAUNCH(1);
 #undef LR_LAUNCH
     return moe_check_launch("k_linear_rows");
   }
-  const LinPlan pl = lin_plan(a.M, a.N, a.K, GATED);
   t.nm = (a.M + 64 * pl.wm - 1) / (64 * pl.wm);
   t.nn = (a.N + 64 * pl.wn / NM - 1) / (64 * pl.wn / NM);
   t.splits = pl.splits;
