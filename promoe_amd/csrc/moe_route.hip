@@ -10,6 +10,7 @@
 // ordered behind everything.  Whatever the values are, k different experts of kept groups come out: the dispatch counts on it.
 #include <hip/hip_runtime.h>
 #include <stdint.h>
+#include <type_traits>
 
 #include "moe_common.h"
 #include "moe_kernels.h"
@@ -146,17 +147,247 @@ static __device__ __forceinline__ void group_topk_token(const GroupRule &q, cons
   }
 }
 
+// ---- four tokens by a wave, in 32 bits where that decides ---------------------------------------------------------------------------
+// 16 lanes a token: lane j holds experts j, j + 16, ... (V of them).  Scores, group values and the k + 1 largest c in 32 bits; a
+// token whose every decision (the groups kept, the order of those choices) stands by more than 32 bits can be wrong goes out with these
+// choices, and any other one again through group_topk_token: equal values, values next to a border (0.4 to 2 % of random tokens), rows of masks,
+// infinities.  Without a bias (and sums of two) the logits themselves are ordered, exactly.  Weights are in 64 bits either way.
+// What 32 bits can be wrong by: sigmoid s (1 - s) (|l| 2^-24 + 2^-23) for 2^x and 2^-23 for the reciprocal, together under 2^-22; softmax 2^-20 of the
+// row's largest probability (eight additions one after the other, 2^x, the quotient); the bias added 2^-24 of the sum.
+template <int N>
+static __device__ __forceinline__ float gr_ror(float x) {  // lane j: x of lane j - N within its 16
+  return __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, x), 0x120 + N, 0xf, 0xf, true));
+}
+static __device__ __forceinline__ float gr_max16(float x) {
+  x = fmaxf(x, gr_ror<8>(x)); x = fmaxf(x, gr_ror<4>(x)); x = fmaxf(x, gr_ror<2>(x));
+  return fmaxf(x, gr_ror<1>(x));
+}
+static __device__ __forceinline__ float gr_sum16(float x) {
+  x += gr_ror<8>(x); x += gr_ror<4>(x); x += gr_ror<2>(x);
+  return x + gr_ror<1>(x);
+}
+template <int N>
+static __device__ __forceinline__ double gr_ror(double x) {
+  const long long u = __builtin_bit_cast(long long, x);
+  const int lo = __builtin_amdgcn_update_dpp(0, (int)u, 0x120 + N, 0xf, 0xf, true);
+  const int hi = __builtin_amdgcn_update_dpp(0, (int)(u >> 32), 0x120 + N, 0xf, 0xf, true);
+  return __builtin_bit_cast(double, (long long)(unsigned)lo | (long long)hi << 32);
+}
+static __device__ __forceinline__ double gr_sum16(double x) {
+  x += gr_ror<8>(x); x += gr_ror<4>(x); x += gr_ror<2>(x);
+  return x + gr_ror<1>(x);
+}
+// e^x for x <= 0 to about 2^-41: 2^n times the Taylor polynomial of 2^f, |f| <= 1/2, of degree 10 (next term 2.2e-13)
+static __device__ __forceinline__ double gr_exp(double x) {
+  x = fmax(x, -800.0);  // (zero from there on)
+  const double y = x * 1.4426950408889634074, n = rint(y), z = (y - n) * 0.69314718055994530942;
+  double p = 1.0 / 3628800;
+  p = fma(p, z, 1.0 / 362880); p = fma(p, z, 1.0 / 40320); p = fma(p, z, 1.0 / 5040); p = fma(p, z, 1.0 / 720); p = fma(p, z, 1.0 / 120);
+  p = fma(p, z, 1.0 / 24); p = fma(p, z, 1.0 / 6); p = fma(p, z, 0.5); p = fma(p, z, 1.0); p = fma(p, z, 1.0);
+  return ldexp(p, (int)n);
+}
+
+#define GR_ROW 288  // floats of a token in LDS: 256 experts, one unused behind every 16
+struct GroupLds {
+  union {
+    float c[4][GR_ROW];
+    double exact[GR_MAXE];
+  };
+  float v[4][16];
+};
+// tokens t0 .. t0 + 3 (those below T).  s_idx, s_mask as in group_topk_token, of token 0.
+template <int V>
+static __device__ __forceinline__ void group_topk_quad(const GroupRule &q, const float *__restrict__ logits, const int ldl, const int t0,
+                                                       const int T, const float *__restrict__ bias, const int lane, GroupLds &m,
+                                                       int *__restrict__ idx, float *__restrict__ w, int *s_idx, unsigned long long (*s_mask)[4]) {
+  constexpr float INF = __builtin_inff();
+  const int tok = lane >> 4, j = lane & 15, t = min(t0 + tok, T - 1);
+  const float *row = logits + (size_t)t * ldl;
+  const bool by_logit = !bias && (!q.top2 || q.keep == q.G);
+  float l[V], c[V];
+#pragma unroll
+  for (int r = 0; r < V; ++r) l[r] = row[min(16 * r + j, q.E - 1)];
+#pragma unroll
+  for (int r = 0; r < V; ++r) l[r] = 16 * r + j < q.E ? fmaxf(l[r], -INF) : -INF;
+  float top = l[0];
+#pragma unroll
+  for (int r = 1; r < V; ++r) top = fmaxf(top, l[r]);
+  top = gr_max16(top);
+  bool sure = top > -INF && top < INF;
+  float unsure_abs = 9.3132257e-10f, unsure_rel = 0.f;  // values this close (2^-30; relative to both) may be in either order
+  if (by_logit) {
+#pragma unroll
+    for (int r = 0; r < V; ++r) c[r] = l[r];
+    if (q.sigmoid) sure = sure && top <= 15.f;  // (from about 34 on scores of different logits are equal in 64 bits)
+  } else {
+    if (q.sigmoid) {
+#pragma unroll
+      for (int r = 0; r < V; ++r) c[r] = __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(l[r] * -1.44269504088896f));
+      unsure_abs = 9.5367432e-7f;               // 2^-20
+    } else {
+      float s[V];
+#pragma unroll
+      for (int r = 0; r < V; ++r) s[r] = c[r] = __builtin_amdgcn_exp2f((l[r] - top) * 1.44269504088896f);
+#pragma unroll
+      for (int k = V / 2; k >= 1; k >>= 1)
+#pragma unroll
+        for (int r = 0; r < k; ++r) s[r] += s[r + k];
+      const float most = 1.f / gr_sum16(s[0]);
+#pragma unroll
+      for (int r = 0; r < V; ++r) c[r] *= most;
+      unsure_abs = 3.8146973e-6f * most;        // 2^-18
+    }
+    unsure_rel = 9.5367432e-7f;
+    if (bias) {
+#pragma unroll
+      for (int r = 0; r < V; ++r) c[r] += bias[min(16 * r + j, q.E - 1)];
+    }
+#pragma unroll
+    for (int r = 0; r < V; ++r) c[r] = 16 * r + j < q.E ? fmaxf(c[r], -INF) : -INF;  // (a NaN counts as -inf)
+  }
+  if (q.keep < q.G) {  // (at most 16 groups)
+    float *sc = m.c[tok], *sv = m.v[tok];
+    __builtin_amdgcn_wave_barrier();
+#pragma unroll
+    for (int r = 0; r < V; ++r) sc[17 * r + j] = c[r];
+    __builtin_amdgcn_wave_barrier();
+    int lanes = 16;    // of a group
+    while (lanes * q.G > 16) lanes >>= 1;
+    const int g = j / lanes, part = j - g * lanes;
+    float a = -INF, b = -INF;  // the two largest
+    for (int i = part; i < q.size; i += lanes) {
+      const int e = g * q.size + i;
+      const float x = g < q.G ? sc[e + (e >> 4)] : -INF;
+      b = fmaxf(b, fminf(a, x));
+      a = fmaxf(a, x);
+    }
+    for (int k = 1; k < lanes; k <<= 1) {
+      const float oa = __shfl_xor(a, k, 64), ob = __shfl_xor(b, k, 64);
+      b = fmaxf(fminf(a, oa), fmaxf(b, ob));
+      a = fmaxf(a, oa);
+    }
+    const float v = q.top2 ? a + b : a;
+    if (part == 0) sv[g] = v;
+    __builtin_amdgcn_wave_barrier();
+    int before = 0;
+    for (int k = 0; k < q.G; ++k) before += sv[k] > v;
+    const bool kept = g < q.G && before < q.keep;
+    const float least = -gr_max16(kept ? -v : -INF), most = gr_max16(g < q.G && !kept ? v : -INF);
+    // (a sum of two is off by twice as much; equal values, NaN and two infinities are not sure)
+    sure = sure && least - most > 2.f * unsure_abs + unsure_rel * (fabsf(least) + fabsf(most));
+    if (by_logit) sure = sure && least > (q.sigmoid ? -700.f : top - 700.f);
+    const unsigned bits = (unsigned)(__ballot(kept) >> (16 * tok)) & 0xffffu;
+    const unsigned over = (65536u + (unsigned)q.size - 1u) / (unsigned)q.size;  // e / size = e over >> 16 for e < 256
+#pragma unroll
+    for (int r = 0; r < V; ++r)
+      if (!((bits >> ((((unsigned)(16 * r + j) * over) >> 16) * lanes)) & 1u)) c[r] = -INF;
+  }
+  // k + 1 rounds of the largest value; lane i keeps choice i (two of them past 16 choices)
+  float last = INF, at_lane = c[0];
+  int r_lane = 0, mine[2] = {0, 0};
+#pragma unroll
+  for (int r = 1; r < V; ++r)
+    if (c[r] > at_lane) { at_lane = c[r]; r_lane = r; }
+  const bool more = q.k < q.keep * q.size;
+  for (int i = 0; i < q.k + more; ++i) {
+    const float best = gr_max16(at_lane);
+    const bool won = at_lane == best;
+    const unsigned who = (unsigned)(__ballot(won) >> (16 * tok)) & 0xffffu;
+    sure = sure && (i == q.k || (who & (who - 1u)) == 0u) &&
+           (i == 0 || (i == q.k && best == -INF) || last - best > unsure_abs + unsure_rel * (fabsf(last) + fabsf(best)));
+    if (i == q.k) break;
+    sure = sure && best > (by_logit ? (q.sigmoid ? -700.f : top - 700.f) : -INF);
+    last = best;
+    const int e = (int)gr_max16(won ? (float)(16 * r_lane + j) : -1.f);
+    if ((i & 15) == j) mine[i >> 4] = e;
+    float next = -INF;
+    int r_next = 0;
+#pragma unroll
+    for (int r = 0; r < V; ++r) {
+      c[r] = won && r == r_lane ? -INF : c[r];
+      if (c[r] > next) { next = c[r]; r_next = r; }
+    }
+    at_lane = next;
+    r_lane = r_next;
+  }
+  // weights, in 64 bits: lane i those of its choices
+  double den = 1.0;
+  if (!q.sigmoid) {
+    double s = 0.0;
+#pragma unroll
+    for (int r = 0; r < V; ++r) s += gr_exp((double)l[r] - (double)top);
+    den = gr_sum16(s);
+  }
+  double s[2], total = 0.0;
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    s[h] = 0.0;
+    if (h && q.k <= 16) break;
+    const double x = (double)fmaxf(row[mine[h]], -INF);
+    s[h] = q.sigmoid ? 1.0 / (1.0 + exp(-x)) : gr_exp(x - (double)top) / den;
+    total += j + 16 * h < q.k ? s[h] : 0.0;
+  }
+  if (q.renorm) total = gr_sum16(total);
+  const bool live = t0 + tok < T;
+  if (live && sure) {
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const int i = j + 16 * h;
+      if (i >= q.k) break;
+      const double x = q.renorm ? (total == 0.0 ? 0.0 : s[h] / total) : s[h];
+      idx[(size_t)t * q.k + i] = mine[h];
+      w[(size_t)t * q.k + i] = (float)(x * (double)q.scale);
+      if (s_idx) s_idx[t * q.k + i] = mine[h];
+    }
+  }
+  if (s_mask) {  // bit e of the token's mask: an or of its lanes' choices, 16 bits of experts at a time
+    if (live && sure) {
+      for (int r = j; r < 4; r += 16) s_mask[t][r] = 0ull;
+    }
+    __builtin_amdgcn_wave_barrier();
+    if (live && sure) {
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+        if (j + 16 * h < q.k) atomicOr(&s_mask[t][mine[h] >> 6], 1ull << (mine[h] & 63));
+    }
+  }
+  unsigned long long again = __ballot(live && !sure && j == 0);
+  __builtin_amdgcn_wave_barrier();
+  while (again) {
+    const int k = (int)__builtin_ctzll(again) >> 4, tk = t0 + k;
+    again &= again - 1ull;
+    group_topk_token<(V + 3) / 4>(q, logits + (size_t)tk * ldl, bias, lane, m.exact, idx + (size_t)tk * q.k, w + (size_t)tk * q.k,
+                                  s_idx ? s_idx + tk * q.k : nullptr, s_mask ? s_mask[tk] : nullptr);
+  }
+}
+// V 0: more groups than a token has lanes: 64-bit scores throughout, a token by a wave
+template <int V>
+static __device__ __forceinline__ void group_topk_four(const GroupRule &q, const float *__restrict__ logits, const int ldl, const int t0,
+                                                       const int T, const float *__restrict__ bias, const int lane, GroupLds &m,
+                                                       int *__restrict__ idx, float *__restrict__ w, int *s_idx, unsigned long long (*s_mask)[4]) {
+  if constexpr (V == 0) {
+    for (int t = t0; t < min(t0 + 4, T); ++t)
+      group_topk_token<4>(q, logits + (size_t)t * ldl, bias, lane, m.exact, idx + (size_t)t * q.k, w + (size_t)t * q.k,
+                          s_idx ? s_idx + t * q.k : nullptr, s_mask ? s_mask[t] : nullptr);
+  } else {
+    group_topk_quad<V>(q, logits, ldl, t0, T, bias, lane, m, idx, w, s_idx, s_mask);
+  }
+}
+// f(V) for the form that a rule takes
+template <class F>
+static void gr_form(const GroupRule &q, const F &f) {
+  if (q.keep < q.G && q.G > 16) f(std::integral_constant<int, 0>());
+  else if (q.E <= 64) f(std::integral_constant<int, 4>());
+  else if (q.E <= 128) f(std::integral_constant<int, 8>());
+  else f(std::integral_constant<int, 16>());
+}
+
+template <int V>
 __global__ __launch_bounds__(256) void k_group_topk(const GroupRule q, const float *__restrict__ logits, const int T, const int ldl,
                                                     const float *__restrict__ bias, int *__restrict__ idx, float *__restrict__ w) {
-  __shared__ double s_c[4][GR_MAXE];
-  const int lane = threadIdx.x & 63, wv = threadIdx.x >> 6, t = blockIdx.x * 4 + wv;
-  if (t >= T) return;
-  const float *row = logits + (size_t)t * ldl;
-  int *ir = idx + (size_t)t * q.k;
-  float *wr = w + (size_t)t * q.k;
-  if (q.E <= 64) group_topk_token<1>(q, row, bias, lane, s_c[wv], ir, wr, nullptr, nullptr);
-  else if (q.E <= 128) group_topk_token<2>(q, row, bias, lane, s_c[wv], ir, wr, nullptr, nullptr);
-  else group_topk_token<4>(q, row, bias, lane, s_c[wv], ir, wr, nullptr, nullptr);
+  __shared__ GroupLds s_m[4];
+  const int lane = threadIdx.x & 63, wv = threadIdx.x >> 6, t0 = 4 * (blockIdx.x * 4 + wv);
+  if (t0 < T) group_topk_four<V>(q, logits, ldl, t0, T, bias, lane, s_m[wv], idx, w, nullptr, nullptr);
 }
 
 // ---- with the stable dispatch of a decode batch in the same launch: one workgroup, a wave per token in turn --------------------
@@ -173,25 +404,18 @@ struct GroupDispatch {
   int host_seq_val;
 };
 
-template <int NW>
+template <int NW, int V>
 __global__ __launch_bounds__(64 * NW) void k_group_topk_dispatch(const GroupRule q, const float *__restrict__ logits, const int T,
                                                                  const int ldl, const float *__restrict__ bias, int *__restrict__ idx,
                                                                  float *__restrict__ w, const GroupDispatch d) {
   constexpr int NT = 64 * NW;
-  __shared__ double s_c[NW][GR_MAXE];
+  __shared__ GroupLds s_m[NW];
   __shared__ int s_idx[GR_MAXP];
   __shared__ unsigned long long s_mask[GR_MAXT][4];
   __shared__ int s_off[GR_MAXE];
   __shared__ int s_rows[4], s_used[4], s_tot;
   const int tid = threadIdx.x, lane = tid & 63, wv = tid >> 6, E = q.E, k = q.k;
-  for (int t = wv; t < T; t += NW) {
-    const float *row = logits + (size_t)t * ldl;
-    int *ir = idx + (size_t)t * k;
-    float *wr = w + (size_t)t * k;
-    if (E <= 64) group_topk_token<1>(q, row, bias, lane, s_c[wv], ir, wr, s_idx + t * k, s_mask[t]);
-    else if (E <= 128) group_topk_token<2>(q, row, bias, lane, s_c[wv], ir, wr, s_idx + t * k, s_mask[t]);
-    else group_topk_token<4>(q, row, bias, lane, s_c[wv], ir, wr, s_idx + t * k, s_mask[t]);
-  }
+  if (4 * wv < T) group_topk_four<V>(q, logits, ldl, 4 * wv, T, bias, lane, s_m[wv], idx, w, s_idx, s_mask);  // (T <= 4 NW)
   __syncthreads();
   // A token holds an expert at most once: the pairs of an expert in stable order are its tokens in order, so the place of
   // (t, e) is the offset of e plus the tokens before t whose mask has e.  Thread e owns expert e (E <= 256 <= threads).
@@ -276,7 +500,10 @@ extern "C" int moe_group_topk(const float *logits, int T, int E, int ldl, int k,
   if (T == 0) return MOE_OK;
   hipStream_t s = (hipStream_t)stream;
   moe_ktimer_begin(MOE_K_TOPK, s);
-  hipLaunchKernelGGL(k_group_topk, dim3((T + 3) / 4), dim3(256), 0, s, rule_of(*rule_host, E, k), logits, T, ldl, bias, idx, w);
+  const GroupRule q = rule_of(*rule_host, E, k);
+  gr_form(q, [&](auto v) {
+    hipLaunchKernelGGL(HIP_KERNEL_NAME(k_group_topk<decltype(v)::value>), dim3((T + 15) / 16), dim3(256), 0, s, q, logits, T, ldl, bias, idx, w);
+  });
   moe_ktimer_end(MOE_K_TOPK, s);
   return moe_check_launch("k_group_topk");
 }
@@ -298,9 +525,14 @@ extern "C" int moe_group_topk_dispatch(const float *logits, int T, int E, int ld
                         units_host_out, n_active_host_out, seq_host_out, seq_value};
   const GroupRule q = rule_of(*rule_host, E, k);
   moe_ktimer_begin(MOE_K_TOPK, s);
-  // (a wave per token: four waves for few tokens, whose barriers are cheaper; thread e also owns expert e)
-  if (T <= 4) hipLaunchKernelGGL(k_group_topk_dispatch<4>, dim3(1), dim3(256), 0, s, q, logits, T, ldl, bias, idx, w, d);
-  else hipLaunchKernelGGL(k_group_topk_dispatch<16>, dim3(1), dim3(1024), 0, s, q, logits, T, ldl, bias, idx, w, d);
+  // (four tokens a wave: four waves for up to 16 tokens, whose barriers are cheaper; thread e also owns expert e)
+  gr_form(q, [&](auto v) {
+    constexpr int V = decltype(v)::value;
+    if (T <= 16)
+      hipLaunchKernelGGL(HIP_KERNEL_NAME(k_group_topk_dispatch<4, V>), dim3(1), dim3(256), 0, s, q, logits, T, ldl, bias, idx, w, d);
+    else
+      hipLaunchKernelGGL(HIP_KERNEL_NAME(k_group_topk_dispatch<16, V>), dim3(1), dim3(1024), 0, s, q, logits, T, ldl, bias, idx, w, d);
+  });
   moe_ktimer_end(MOE_K_TOPK, s);
   return moe_check_launch("k_group_topk_dispatch");
 }

@@ -71,61 +71,69 @@ class RouteRule(L.RouteRule):
         super().__init__(L.SCORES[scores], n_group, topk_group, L.GROUP_VALUES[group_value], int(bool(renorm)), scale)
 
 
-def _operands(what: str, *tensors):
-    """Tensors of a call (None among them): on one GPU, and none that a gradient is expected of."""
-    dev = tensors[0].device
-    if dev.type != "cuda":
-        raise L.MoeError("%s: tensors of a GPU are needed, not of %s" % (what, dev))
-    for t in tensors:
-        if t is None:
-            continue
-        if t.device != dev:
-            raise L.MoeError("%s: tensors of %s and of %s" % (what, dev, t.device))
-        if t.requires_grad and torch.is_grad_enabled():
-            raise L.MoeError("%s has no gradient: call it under torch.no_grad() or with detached tensors" % what)
-    return dev
+# the current stream's handle without a Stream object around it, where this torch offers that (a third of a small call's time)
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (lambda index: torch.cuda.current_stream(index).cuda_stream)
+
+
+def _operands(what: str, first: torch.Tensor, *others) -> int:
+    """Index of the GPU that all tensors of a call (None among them) are on; none may be one that a gradient is expected of."""
+    index = first.get_device()
+    if index < 0:
+        raise L.MoeError("%s: tensors of a GPU are needed, not of %s" % (what, first.device))
+    grad = torch.is_grad_enabled()
+    if grad and first.requires_grad:
+        raise L.MoeError("%s has no gradient: call it under torch.no_grad() or with detached tensors" % what)
+    for t in others:
+        if t is not None:
+            if t.get_device() != index:
+                raise L.MoeError("%s: tensors of %s and of %s" % (what, first.device, t.device))
+            if grad and t.requires_grad:
+                raise L.MoeError("%s has no gradient: call it under torch.no_grad() or with detached tensors" % what)
+    return index
 
 
 def _route_args(what, logits, k, rule, bias):
-    """(device, T, E, row stride) of a routing call."""
+    """(GPU, T, E, row stride) of a routing call."""
     if logits.dim() != 2 or logits.dtype != torch.float32 or (logits.shape[1] > 1 and logits.stride(1) != 1):
         raise L.MoeError("%s: logits must be fp32 [T, E] with the experts of a row side by side" % what)
     if not isinstance(rule, L.RouteRule):
         raise L.MoeError("%s: rule must be a RouteRule" % what)
-    dev = _operands(what, logits, bias)
+    index = _operands(what, logits, bias)
     T, E = logits.shape
     if bias is not None and (bias.dtype != torch.float32 or bias.shape != (E,) or not bias.is_contiguous()):
         raise L.MoeError("%s: bias must be fp32 [%d], contiguous" % (what, E))
-    return dev, T, E, logits.stride(0) if T > 1 else E
+    if not 0 < k <= E:
+        raise L.MoeError("%s: %d of %d experts" % (what, k, E))
+    return index, T, E, logits.stride(0) if T > 1 else E
 
 
 def group_topk(logits: torch.Tensor, k: int, rule: RouteRule, bias: torch.Tensor | None = None):
     """Routing with groups of experts and a selection bias (moe_group_topk): logits fp32 [T, E] (rows may be further apart: a
     slice in front of a shared expert's gate column) -> (idx [T, k] int32, w [T, k] fp32).  The bias [E] takes part in the
-    choice, not in the weights."""
-    dev, T, E, ldl = _route_args("group_topk", logits, k, rule, bias)
-    if dev.index != torch.cuda.current_device():
-        with torch.cuda.device(dev):
+    choice, not in the weights.  Serving only: tensors that a gradient is expected of are refused."""
+    index, T, E, ldl = _route_args("group_topk", logits, k, rule, bias)
+    if index != torch.cuda.current_device():
+        with torch.cuda.device(index):
             return group_topk(logits, k, rule, bias)
-    idx = torch.empty(T, k, dtype=torch.int32, device=dev)
-    w = torch.empty(T, k, dtype=torch.float32, device=dev)
-    check(lib.moe_group_topk(logits.data_ptr(), T, E, ldl, k, byref(rule), ptr(bias), idx.data_ptr(), w.data_ptr(), cur_stream()),
-          "moe_group_topk")
+    idx = torch.empty((T, k), dtype=torch.int32, device=logits.device)
+    w = torch.empty_like(idx, dtype=torch.float32)
+    check(lib.moe_group_topk(logits.data_ptr(), T, E, ldl, k, byref(rule), ptr(bias), idx.data_ptr(), w.data_ptr(),
+                             _raw_stream(index)), "moe_group_topk")
     return idx, w
 
 
 def group_topk_dispatch(logits: torch.Tensor, k: int, rule: RouteRule, bias: torch.Tensor | None = None):
     """group_topk and the stable dispatch in one launch for T <= 64 and T*k <= 512.  Returns (idx, w, Dispatch)."""
-    dev, T, E, ldl = _route_args("group_topk_dispatch", logits, k, rule, bias)
-    if dev.index != torch.cuda.current_device():
-        with torch.cuda.device(dev):
+    index, T, E, ldl = _route_args("group_topk_dispatch", logits, k, rule, bias)
+    if not 0 < T <= 64 or T * k > 512:
+        raise L.MoeError("group_topk_dispatch: %d tokens with %d choices each (group_topk and dispatch take any)" % (T, k))
+    if index != torch.cuda.current_device():
+        with torch.cuda.device(index):
             return group_topk_dispatch(logits, k, rule, bias)
-    idx = torch.empty(T, k, dtype=torch.int32, device=dev)
-    w = torch.empty(T, k, dtype=torch.float32, device=dev)
-    d = Dispatch(T, k, E, min(E, T * k), dev)
+    d, (idx, w) = Dispatch.packed(T, k, E, logits.device)
     check(lib.moe_group_topk_dispatch(logits.data_ptr(), T, E, ldl, k, byref(rule), ptr(bias), ptr(idx), ptr(w), ptr(d.counts),
                                       ptr(d.offsets), ptr(d.sorted_pair), ptr(d.pos_of_pair), ptr(d.sorted_tok), ptr(d.units),
-                                      ptr(d.n_active), ptr(d.active_ids), d.max_units, 0, 0, 0, 0, cur_stream()),
+                                      ptr(d.n_active), ptr(d.active_ids), d.max_units, 0, 0, 0, 0, _raw_stream(index)),
           "moe_group_topk_dispatch")
     return idx, w, d
 
@@ -147,9 +155,21 @@ class Dispatch:
         self.active_ids = torch.empty(max(max_units, 1), dtype=torch.int64, device=device)
         self.err = torch.zeros(1, **i32)
 
+    @classmethod
+    def packed(cls, T: int, k: int, E: int, device):
+        """The buffers of a launch that raises no error word, and its idx and w, as parts of one allocation."""
+        d = cls.__new__(cls)
+        P = T * k
+        U = min(E, P)
+        d.T, d.k, d.E, d.max_units, d.err = T, k, E, U, None
+        units, ids, idx, w, d.counts, d.offsets, d.sorted_pair, d.pos_of_pair, d.sorted_tok, d.n_active = torch.empty(
+            6 * U + 5 * P + 2 * E + 2, dtype=torch.int32, device=device).split_with_sizes([4 * U, 2 * U, P, P, E, E + 1, P, P, P, 1])
+        d.active_ids, d.units = ids.view(torch.int64), units.view(U, 4)
+        return d, (idx.view(T, k), w.view(torch.float32).view(T, k))
+
     def check(self):
         """Raises if the multi-workgroup dispatch kernel reported a time-out (synchronises)."""
-        if int(self.err.item()):
+        if self.err is not None and int(self.err.item()):
             raise L.MoeError("moe_dispatch_ws: a workgroup did not get the others' counts in time")
 
 
@@ -482,57 +502,63 @@ def combine(part_r, part_s, topk_w, pos_of_pair, shared_gate_logit, T: int, H: i
     return out
 
 
-def _rows(what: str, t: torch.Tensor, cols: int) -> int:
-    """Elements between the rows of a [R, cols] matrix whose rows are whole."""
-    if t.dim() != 2 or t.shape[1] != cols or (cols > 1 and t.stride(1) != 1):
-        raise L.MoeError("%s: a matrix of whole rows of %d columns is needed, not %s with strides %s"
-                         % (what, cols, tuple(t.shape), t.stride()))
-    return t.stride(0) if t.shape[0] > 1 else cols
+def _rows(what: str, t: torch.Tensor, rows: int, cols: int) -> int:
+    """Elements between the rows of a [rows, cols] matrix whose rows are whole."""
+    if t.shape != (rows, cols) or (cols > 1 and t.stride(1) != 1):
+        raise L.MoeError("%s: a matrix [%d, %d] of whole rows is needed, not %s with strides %s"
+                         % (what, rows, cols, tuple(t.shape), t.stride()))
+    return t.stride(0) if rows > 1 else (cols + 7) // 8 * 8
 
 
 def _product(what, x, mats, biases, act, residual, out, out_dtype):
-    dt = L.DTYPES.get(x.dtype)
-    if dt is None or act not in L.ACTS:
+    dtype = x.dtype
+    code = L.DTYPES.get(dtype)
+    if code is None or act not in L.ACTS:
         raise L.MoeError("%s: bf16 or fp16 operands and one of the activations %s" % (what, sorted(L.ACTS)))
-    dev = _operands(what, x, *mats, *biases, residual, out)
-    if dev.index != torch.cuda.current_device():
-        with torch.cuda.device(dev):
+    index = _operands(what, x, *mats, *biases, residual, out)
+    if index != torch.cuda.current_device():
+        with torch.cuda.device(index):
             return _product(what, x, mats, biases, act, residual, out, out_dtype)
-    if x.dim() != 2 or mats[0].dim() != 2:
+    w = mats[0]
+    if x.dim() != 2 or w.dim() != 2:
         raise L.MoeError("%s: x must be [M, K] and a matrix [N, K]" % what)
     M, K = x.shape
-    N = mats[0].shape[0]
-    ldx, ldw = _rows(what, x, K), _rows(what, mats[0], K)
+    N = w.shape[0]
+    ldx, ldw = _rows(what, x, M, K), _rows(what, w, N, K)
     for m in mats:
-        if m.dtype != x.dtype or m.shape != (N, K) or _rows(what, m, K) != ldw:
-            raise L.MoeError("%s: matrices of one shape, row stride and type (%s)" % (what, x.dtype))
+        if m.dtype != dtype or (m is not w and _rows(what, m, N, K) != ldw):
+            raise L.MoeError("%s: matrices of one row stride and of x's type, %s" % (what, dtype))
     for b in biases:
-        if b is not None and (b.dtype != x.dtype or b.shape != (N,) or not b.is_contiguous()):
-            raise L.MoeError("%s: a bias must be %s [%d], contiguous" % (what, x.dtype, N))
+        if b is not None and (b.dtype != dtype or b.shape != (N,) or not b.is_contiguous()):
+            raise L.MoeError("%s: a bias must be %s [%d], contiguous" % (what, dtype, N))
     ldr = 0
     if residual is not None:
-        if residual.dtype != x.dtype or residual.dim() != 2 or residual.shape[0] != M:
-            raise L.MoeError("%s: the residual must be %s [%d, %d]" % (what, x.dtype, M, N))
-        ldr = _rows(what, residual, N)
+        if residual.dtype != dtype:
+            raise L.MoeError("%s: the residual must be %s" % (what, dtype))
+        ldr = _rows(what, residual, M, N)
     if out is None:
-        out = torch.empty(M, N, dtype=out_dtype or x.dtype, device=dev)
-    elif out.dim() != 2 or out.shape[0] != M or (out_dtype is not None and out.dtype != out_dtype):
-        raise L.MoeError("%s: out must be [%d, %d] of the type asked for" % (what, M, N))
-    if out.dtype != x.dtype and out.dtype != torch.float32:
-        raise L.MoeError("%s: results are %s or fp32" % (what, x.dtype))
-    ldy = _rows(what, out, N)
-    ws = None
-    n_ws = lib.moe_linear_workspace_bytes(M, N, K, len(mats) - 1)
-    if n_ws:
-        ws = torch.empty(n_ws, dtype=torch.uint8, device=dev)
-    y32 = out.dtype == torch.float32
-    if len(mats) == 1:
-        check(lib.moe_linear(x.data_ptr(), ldx, mats[0].data_ptr(), ldw, ptr(biases[0]), ptr(residual), ldr, out.data_ptr(), ldy,
-                             M, N, K, dt, L.ACTS[act], y32, ptr(ws), n_ws, cur_stream()), "moe_linear")
+        out = torch.empty((M, N), dtype=out_dtype or dtype, device=x.device)
+        ldy = N
     else:
-        check(lib.moe_linear_gated(x.data_ptr(), ldx, mats[0].data_ptr(), mats[1].data_ptr(), ldw, ptr(biases[0]), ptr(biases[1]),
-                                   out.data_ptr(), ldy, M, N, K, dt, L.ACTS[act], y32, ptr(ws), n_ws, cur_stream()),
-              "moe_linear_gated")
+        ldy = _rows(what, out, M, N)
+        if out_dtype is not None and out.dtype != out_dtype:
+            raise L.MoeError("%s: out is %s, asked for was %s" % (what, out.dtype, out_dtype))
+    y32 = out.dtype == torch.float32
+    if not y32 and out.dtype != dtype:
+        raise L.MoeError("%s: results are %s or fp32" % (what, dtype))
+    ws_ptr, gated = 0, len(mats) == 2
+    n_ws = lib.moe_linear_workspace_bytes(M, N, K, gated)
+    if n_ws:
+        ws = torch.empty(n_ws, dtype=torch.uint8, device=x.device)
+        ws_ptr = ws.data_ptr()
+    if gated:
+        rc = lib.moe_linear_gated(x.data_ptr(), ldx, w.data_ptr(), mats[1].data_ptr(), ldw, ptr(biases[0]), ptr(biases[1]),
+                                  out.data_ptr(), ldy, M, N, K, code, L.ACTS[act], y32, ws_ptr, n_ws, _raw_stream(index))
+    else:
+        rc = lib.moe_linear(x.data_ptr(), ldx, w.data_ptr(), ldw, ptr(biases[0]), ptr(residual), ldr, out.data_ptr(), ldy, M, N, K,
+                            code, L.ACTS[act], y32, ws_ptr, n_ws, _raw_stream(index))
+    if rc:
+        check(rc, what)
     return out
 
 
