@@ -14,9 +14,12 @@ Qwen2-MoE (softmax -> top-k, optional renormalisation, sigmoid-gated shared expe
 (softmax -> top-k -> renormalise, which is the softmax over the selected logits) and the DeepSeek
 family (DeepSeek-MoE / DeepSeek-V2-Lite: softmax -> greedy top-k without renormalisation, a plain
 shared expert `shared_experts` of n_shared_experts * I columns; the reference's metas for it are
-utils/common_metas.py:17-41 and 69-94).  In the DeepSeek models the first decoder layers are dense:
+utils/common_metas.py:17-41 and 69-94).  Routers with groups of experts (DeepSeek-V2: a group is worth its best expert)
+and routers with sigmoid scores and a selection bias (`e_score_correction_bias`; a group is worth its two best) become the
+engine's routing rule of the layer (ops.RouteRule).  In the DeepSeek models the first decoder layers are dense:
 MoE layers are numbered from 0 in model order, so decoder layer i is engine layer
-i - first_k_dense_replace (the reference subtracts the same 1, common_metas.py:19-23).
+i - first_k_dense_replace (the reference subtracts the same 1, common_metas.py:19-23).  With `fuse_dense` the
+dense gated layers run as two launches each (ops.linear_gated, ops.linear).
 """
 from __future__ import annotations
 
@@ -27,6 +30,7 @@ import torch
 
 from . import _lib as L
 from . import layout as LY
+from . import ops
 from . import quant
 from .engine import ModuleMeta, PrefetchMngr, PinnedBuffer
 
@@ -47,11 +51,64 @@ def _route_mode(block) -> int:
     gate = block.gate
     if hasattr(gate, "topk_method"):                         # DeepSeek router
         if gate.topk_method != "greedy":
-            raise NotImplementedError("DeepSeek routing method %r (only 'greedy' top-k is supported)" % gate.topk_method)
+            raise NotImplementedError("DeepSeek routing method %r (only 'greedy' and 'group_limited_greedy' top-k are supported)"
+                                      % gate.topk_method)
         return L.ROUTE_SOFTMAX_TOPK
     if hasattr(gate, "norm_topk_prob"):                      # Qwen2-MoE router
         return L.ROUTE_SOFTMAX_TOPK_RENORM if gate.norm_topk_prob else L.ROUTE_SOFTMAX_TOPK
     return L.ROUTE_TOPK_SOFTMAX                              # Mixtral: renormalised top-k of the softmax
+
+
+def _route_rule(block):
+    """(rule, selection bias or None) of a router with groups of experts or sigmoid scores and a selection bias; (None, None)
+    for the routers of _route_mode."""
+    gate = block.gate
+
+    def find(*names):
+        for o in (gate, block):
+            for n in names:
+                if getattr(o, n, None) is not None:
+                    return getattr(o, n)
+        raise NotImplementedError("a router of class %s without %s" % (type(gate).__name__, " or ".join(names)))
+
+    bias = getattr(gate, "e_score_correction_bias", None)
+    if bias is not None:                                     # scores are sigmoids, the bias balances the choice
+        return ops.RouteRule("sigmoid", int(find("n_group", "num_group")), int(find("topk_group")), "top2",
+                             bool(find("norm_topk_prob")), float(find("routed_scaling_factor"))), bias
+    if getattr(gate, "topk_method", None) == "group_limited_greedy":
+        return ops.RouteRule("softmax", int(find("num_group", "n_group")), int(find("topk_group")), "max", False,
+                             float(find("routed_scaling_factor"))), None
+    return None, None
+
+
+_HIDDEN_ACTS = {"silu": "silu", "swish": "silu", "gelu": "gelu", "gelu_new": "gelu_tanh", "gelu_pytorch_tanh": "gelu_tanh",
+                "relu": "relu", "relu2": "relu2"}
+
+
+def find_dense_mlps(model):
+    """[(qualified name, module, activation)] of the dense gated feed-forward layers (gate_proj, up_proj, down_proj) that are no part
+    of a sparse block and whose shapes and activation the fused products take."""
+    inside = {id(m) for _, blk in find_moe_blocks(model) for m in blk.modules()}
+    out = []
+    for name, mod in model.named_modules():
+        parts = [getattr(mod, n, None) for n in ("gate_proj", "up_proj", "down_proj")]
+        if id(mod) in inside or not all(isinstance(p, torch.nn.Linear) for p in parts):
+            continue
+        act = _HIDDEN_ACTS.get(getattr(getattr(mod, "config", None), "hidden_act", None))
+        g, u, d = parts
+        if act and g.weight.shape == u.weight.shape and d.weight.shape == g.weight.shape[::-1] and d.in_features % 8 == 0 \
+                and g.in_features % 8 == 0:
+            out.append((name, mod, act))
+    return out
+
+
+def _fused_mlp_forward(act):
+    def forward(self, x):
+        # (detached, as the engine's own blocks are: nothing here has a gradient)
+        w = [None if t is None else t.detach() for p in (self.gate_proj, self.up_proj, self.down_proj) for t in (p.weight, p.bias)]
+        h = ops.linear_gated(x.detach().reshape(-1, x.shape[-1]), w[0], w[2], w[1], w[3], act=act)
+        return ops.linear(h, w[4], w[5]).reshape(*x.shape[:-1], w[4].shape[0])
+    return forward
 
 
 def _shared_expert(block):
@@ -73,14 +130,15 @@ def _expert_image(gate_w, up_w, down_w, H, I, fmt):
 
 
 def inject_model(model, device="cuda:0", fmt: str = "bf16", max_tokens: int = 4096, drop_expert_params: bool = True,
-                 **cfg) -> PrefetchMngr:
+                 fuse_dense: bool = False, **cfg) -> PrefetchMngr:
     """Move the model's dense parts to `device` in bf16, keep its experts in pinned host memory behind the
     slot cache, and route every sparse block through the engine.  Returns the engine (also kept as
     `model._prefetch_mngr`, the attribute the reference attaches, utils/__init__.py:66-70).
     On return torch's current stream is the engine's compute stream: run the model on it.
 
     fmt "bf16" keeps the experts' weights as they are (rounded to bf16); "int4" quantises them to
-    int4-g128 on the way in.  cfg: engine configuration keys (cache_rate, cache_policy, ...).
+    int4-g128 on the way in.  fuse_dense: the dense gated layers (find_dense_mlps) run as two fused launches instead of the
+    module's own operations; their intermediate rows are rounded once instead of three times.  cfg: engine configuration keys (cache_rate, cache_policy, ...).
     The shapes must fit the kernels: H and I multiples of 128 (bf16) / 128 and 16 (int4)."""
     if fmt not in ("bf16", "int4"):
         raise ValueError("fmt must be 'bf16' or 'int4'")
@@ -111,7 +169,8 @@ def inject_model(model, device="cuda:0", fmt: str = "bf16", max_tokens: int = 40
             raise ValueError("block %s differs in shape from the first block" % name)
         # DeepSeek scales the routed experts' sum by a constant; it goes into their down projections (multiplied in
         # fp32, before the one rounding to bf16 / the quantisation of the image)
-        scale = float(getattr(blk.gate, "routed_scaling_factor", 1.0) or 1.0)
+        # (a layer with a routing rule has it in its weights)
+        scale = 1.0 if _route_rule(blk)[0] is not None else float(getattr(blk.gate, "routed_scaling_factor", 1.0) or 1.0)
         for e in range(E):
             img = _expert_image(gu[e, :I], gu[e, I:], dn[e] if scale == 1.0 else dn[e].detach().float() * scale, H, I, fmt)
             base = (l * E + e) * total
@@ -125,6 +184,8 @@ def inject_model(model, device="cuda:0", fmt: str = "bf16", max_tokens: int = 40
             if sh is not None:
                 for lin in (sh.gate_proj, sh.up_proj, sh.down_proj):
                     lin.weight = torch.nn.Parameter(torch.empty(0), requires_grad=False)
+    # (a selection bias keeps its 32 bits)
+    rules = [(r, None if b is None else b.detach().float().to(device)) for r, b in (_route_rule(blk) for _, blk in blocks)]
     model.to(device=device, dtype=torch.bfloat16)
     torch.cuda.set_device(device)
     # a stream of torch's own is handed over as it is; from the legacy default stream (handle 0) the
@@ -155,8 +216,9 @@ def inject_model(model, device="cuda:0", fmt: str = "bf16", max_tokens: int = 40
         if sg is not None:
             gw = torch.cat([gw, sg.weight.detach().to(torch.bfloat16).reshape(1, H)])
         sh = None if shared_imgs[l] is None else torch.from_numpy(np.ascontiguousarray(shared_imgs[l])).to(device)
-        pm.set_layer(l, H, I, I_sh, top_k, _route_mode(blk), gw.contiguous(), None, sh, shared_gated=sg is not None,
-                     fmt=L.FMT_BF16 if fmt == "bf16" else L.FMT_INT4_G128)
+        pm.set_layer(l, H, I, I_sh, top_k, L.ROUTE_SOFTMAX_TOPK if rules[l][0] is not None else _route_mode(blk), gw.contiguous(), None,
+                     sh, shared_gated=sg is not None, fmt=L.FMT_BF16 if fmt == "bf16" else L.FMT_INT4_G128, rule=rules[l][0],
+                     select_bias=rules[l][1])
     pm.forward_prepare(max_tokens)
     pm.launch_thread()
 
@@ -173,5 +235,8 @@ def inject_model(model, device="cuda:0", fmt: str = "bf16", max_tokens: int = 40
     for l, (name, blk) in enumerate(blocks):
         blk._layer_id = l                                   # the reference's metadata attribute (utils/__init__.py:25-31)
         blk.forward = types.MethodType(make_forward(l), blk)
+    if fuse_dense:
+        for _, mod, act in find_dense_mlps(model):
+            mod.forward = types.MethodType(_fused_mlp_forward(act), mod)
     model._prefetch_mngr = pm
     return pm
