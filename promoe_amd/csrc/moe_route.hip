@@ -23,6 +23,8 @@
 struct GroupRule {
   int E, k, G, size, keep, sigmoid, top2, renorm;
   float scale;
+  // four tokens by a wave: 2^shift lanes of a token's 16 share a group (all groups kept: a lane is one), `per` experts a lane
+  int shift, per;
 };
 
 static __device__ __forceinline__ double gr_shfl_xor(double x, int m) { return __shfl_xor(x, m, 64); }
@@ -54,7 +56,10 @@ static __device__ __forceinline__ void group_topk_token(const GroupRule &q, cons
   }
   if (q.sigmoid) {
 #pragma unroll
-    for (int r = 0; r < NR; ++r) s[r] = 1.0 / (1.0 + exp(-(double)l[r]));
+    for (int r = 0; r < NR; ++r) {
+      s[r] = 1.0 / (1.0 + exp(-(double)l[r]));
+      __builtin_amdgcn_sched_barrier(0);  // (one after the other: in 64 registers)
+    }
   } else {
     float m = l[0];
 #pragma unroll
@@ -65,10 +70,14 @@ static __device__ __forceinline__ void group_topk_token(const GroupRule &q, cons
     for (int r = 0; r < NR; ++r) {
       s[r] = lane + 64 * r < q.E ? exp((double)l[r] - (double)m) : 0.0;
       sum += s[r];
+      __builtin_amdgcn_sched_barrier(0);
     }
     sum = gr_wave_sum(sum);
 #pragma unroll
-    for (int r = 0; r < NR; ++r) s[r] = s[r] / sum;
+    for (int r = 0; r < NR; ++r) {
+      s[r] = s[r] / sum;
+      __builtin_amdgcn_sched_barrier(0);
+    }
     if (m == -__builtin_inff()) {  // a row that its mask leaves nothing of: scores of zero
 #pragma unroll
       for (int r = 0; r < NR; ++r) s[r] = 0.0;
@@ -148,12 +157,17 @@ static __device__ __forceinline__ void group_topk_token(const GroupRule &q, cons
 }
 
 // ---- four tokens by a wave, in 32 bits where that decides ---------------------------------------------------------------------------
-// 16 lanes a token: lane j holds experts j, j + 16, ... (V of them).  Scores, group values and the k + 1 largest c in 32 bits; a
+// 16 lanes a token, a lane has a run of at most V experts of one group.  Scores, group values and the k + 1 largest c in 32 bits; a
 // token whose every decision (the groups kept, the order of those choices) stands by more than 32 bits can be wrong goes out with these
-// choices, and any other one again through group_topk_token: equal values, values next to a border (0.4 to 2 % of random tokens), rows of masks,
-// infinities.  Without a bias (and sums of two) the logits themselves are ordered, exactly.  Weights are in 64 bits either way.
+// choices, and any other one again through group_topk_token: equal values, values next to a border (under 2 % of random tokens), rows of
+// masks, infinities.  Without a bias (and sums of two) the logits themselves are ordered.  Weights are in 64 bits either way.
 // What 32 bits can be wrong by: sigmoid s (1 - s) (|l| 2^-24 + 2^-23) for 2^x and 2^-23 for the reciprocal, together under 2^-22; softmax 2^-20 of the
-// row's largest probability (eight additions one after the other, 2^x, the quotient); the bias added 2^-24 of the sum.
+// row's largest probability (nine additions one after the other, 2^x, the quotient); the bias added 2^-24 of the sum; the place in the
+// lane's run, which the ordered value carries in its last bits, V 2^-23 of it.
+// Bound by the vector unit: 32768 tokens over 256 experts in 8 groups, a bias and sums of two take 28 us (36 MB: 7 us at a copy's rate), 1200
+// operations a wave of four.  A wave per token in 64 bits takes 67; experts dealt out one by one (16 r + lane), their indexes beside the
+// values and the groups' values through LDS 36 (1900 operations); no fours in order 30; 82 registers instead of 64, which cost the exact
+// form some in scratch, two waves fewer a SIMD and 2 us.
 template <int N>
 static __device__ __forceinline__ float gr_ror(float x) {  // lane j: x of lane j - N within its 16
   return __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, x), 0x120 + N, 0xf, 0xf, true));
@@ -187,13 +201,30 @@ static __device__ __forceinline__ double gr_exp(double x) {
   return ldexp(p, (int)n);
 }
 
-#define GR_ROW 288  // floats of a token in LDS: 256 experts, one unused behind every 16
-struct GroupLds {
-  union {
-    float c[4][GR_ROW];
-    double exact[GR_MAXE];
-  };
-  float v[4][16];
+// a / b for b in the middle of the range: reciprocal and two of Newton's steps, the quotient corrected once
+static __device__ __forceinline__ double gr_div(double a, double b) {
+  double r = __builtin_amdgcn_rcp(b);
+  r = fma(fma(-b, r, 1.0), r, r);
+  r = fma(fma(-b, r, 1.0), r, r);
+  const double x = a * r;
+  return fma(fma(-b, x, a), r, x);
+}
+// floats as integers of the same order, and back
+static __device__ __forceinline__ int gr_key(float x) {
+  const int b = __builtin_bit_cast(int, x);
+  return b ^ ((b >> 31) & 0x7fffffff);
+}
+static __device__ __forceinline__ float gr_value(int k) { return __builtin_bit_cast(float, k ^ ((k >> 31) & 0x7fffffff)); }
+template <int N>
+static __device__ __forceinline__ int gr_ror_i(int x) { return __builtin_amdgcn_update_dpp(0, x, 0x120 + N, 0xf, 0xf, true); }
+static __device__ __forceinline__ int gr_max16_i(int x) {
+  x = max(x, gr_ror_i<8>(x)); x = max(x, gr_ror_i<4>(x)); x = max(x, gr_ror_i<2>(x));
+  return max(x, gr_ror_i<1>(x));
+}
+
+union GroupLds {
+  float v[4][16];          // the groups' values of four tokens
+  double exact[GR_MAXE];
 };
 // tokens t0 .. t0 + 3 (those below T).  s_idx, s_mask as in group_topk_token, of token 0.
 template <int V>
@@ -201,14 +232,32 @@ static __device__ __forceinline__ void group_topk_quad(const GroupRule &q, const
                                                        const int T, const float *__restrict__ bias, const int lane, GroupLds &m,
                                                        int *__restrict__ idx, float *__restrict__ w, int *s_idx, unsigned long long (*s_mask)[4]) {
   constexpr float INF = __builtin_inff();
+  constexpr int NONE = (int)0x80000000;
   const int tok = lane >> 4, j = lane & 15, t = min(t0 + tok, T - 1);
-  const float *row = logits + (size_t)t * ldl;
   const bool by_logit = !bias && (!q.top2 || q.keep == q.G);
+  // lane j's run of experts: in group j >> shift, part j & .. of it
+  const int g = j >> q.shift, per = q.per, size = q.keep < q.G ? q.size : per, G = q.keep < q.G ? q.G : 16;
+  const int part0 = (j - (g << q.shift)) * per, start = g * size + part0;
+  const int count = g < G ? max(0, min(min(per, size - part0), q.E - start)) : 0;
+  // (sixteen bytes from any float on; what a run does not hold is masked, and zeros behind the last row)
+  const long long end = ((long long)(T - 1 - t0) * ldl + q.E) * 4;
+  const rsrc_t rl = make_rsrc(logits + (size_t)t0 * ldl, (int)(end < 0x7fffff00ll ? end : 0x7fffff00ll)), rb = make_rsrc(bias, bias ? q.E * 4 : 0);
+  const int at = ((t - t0) * ldl + start) * 4;
   float l[V], c[V];
 #pragma unroll
-  for (int r = 0; r < V; ++r) l[r] = row[min(16 * r + j, q.E - 1)];
+  for (int r = 0; r < V; r += 4) {
+    const float4 x = __builtin_bit_cast(float4, bload16(rl, r < count ? at + 4 * r : 0, 0));
+    l[r] = x.x; l[r + 1] = x.y; l[r + 2] = x.z; l[r + 3] = x.w;
+  }
+  if (bias) {
 #pragma unroll
-  for (int r = 0; r < V; ++r) l[r] = 16 * r + j < q.E ? fmaxf(l[r], -INF) : -INF;
+    for (int r = 0; r < V; r += 4) {
+      const float4 x = __builtin_bit_cast(float4, bload16(rb, r < count ? (start + r) * 4 : 0, 0));
+      c[r] = x.x; c[r + 1] = x.y; c[r + 2] = x.z; c[r + 3] = x.w;
+    }
+  }
+#pragma unroll
+  for (int r = 0; r < V; ++r) l[r] = r < count ? fmaxf(l[r], -INF) : -INF;
   float top = l[0];
 #pragma unroll
   for (int r = 1; r < V; ++r) top = fmaxf(top, l[r]);
@@ -220,95 +269,99 @@ static __device__ __forceinline__ void group_topk_quad(const GroupRule &q, const
     for (int r = 0; r < V; ++r) c[r] = l[r];
     if (q.sigmoid) sure = sure && top <= 15.f;  // (from about 34 on scores of different logits are equal in 64 bits)
   } else {
+    float s[V];
     if (q.sigmoid) {
 #pragma unroll
-      for (int r = 0; r < V; ++r) c[r] = __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(l[r] * -1.44269504088896f));
+      for (int r = 0; r < V; ++r) s[r] = __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(l[r] * -1.44269504088896f));
       unsure_abs = 9.5367432e-7f;               // 2^-20
     } else {
-      float s[V];
+      float sum[V];
 #pragma unroll
-      for (int r = 0; r < V; ++r) s[r] = c[r] = __builtin_amdgcn_exp2f((l[r] - top) * 1.44269504088896f);
+      for (int r = 0; r < V; ++r) sum[r] = s[r] = __builtin_amdgcn_exp2f((l[r] - top) * 1.44269504088896f);
 #pragma unroll
       for (int k = V / 2; k >= 1; k >>= 1)
 #pragma unroll
-        for (int r = 0; r < k; ++r) s[r] += s[r + k];
-      const float most = 1.f / gr_sum16(s[0]);
+        for (int r = 0; r < k; ++r) sum[r] += sum[r + k];
+      const float most = 1.f / gr_sum16(sum[0]);
 #pragma unroll
-      for (int r = 0; r < V; ++r) c[r] *= most;
+      for (int r = 0; r < V; ++r) s[r] *= most;
       unsure_abs = 3.8146973e-6f * most;        // 2^-18
     }
     unsure_rel = 9.5367432e-7f;
-    if (bias) {
 #pragma unroll
-      for (int r = 0; r < V; ++r) c[r] += bias[min(16 * r + j, q.E - 1)];
-    }
-#pragma unroll
-    for (int r = 0; r < V; ++r) c[r] = 16 * r + j < q.E ? fmaxf(c[r], -INF) : -INF;  // (a NaN counts as -inf)
+    for (int r = 0; r < V; ++r) c[r] = r < count ? fmaxf(bias ? s[r] + c[r] : s[r], -INF) : -INF;  // (a NaN counts as -inf)
   }
-  if (q.keep < q.G) {  // (at most 16 groups)
-    float *sc = m.c[tok], *sv = m.v[tok];
-    __builtin_amdgcn_wave_barrier();
+  bool mine_kept = true;
+  if (q.keep < q.G) {
+    float a = c[0], b = -INF;  // the two largest of the lane, of the group
 #pragma unroll
-    for (int r = 0; r < V; ++r) sc[17 * r + j] = c[r];
-    __builtin_amdgcn_wave_barrier();
-    int lanes = 16;    // of a group
-    while (lanes * q.G > 16) lanes >>= 1;
-    const int g = j / lanes, part = j - g * lanes;
-    float a = -INF, b = -INF;  // the two largest
-    for (int i = part; i < q.size; i += lanes) {
-      const int e = g * q.size + i;
-      const float x = g < q.G ? sc[e + (e >> 4)] : -INF;
-      b = fmaxf(b, fminf(a, x));
-      a = fmaxf(a, x);
+    for (int r = 1; r < V; ++r) {
+      if (q.top2) b = fmaxf(b, fminf(a, c[r]));
+      a = fmaxf(a, c[r]);
     }
-    for (int k = 1; k < lanes; k <<= 1) {
+    for (int k = 1; k < 1 << q.shift; k <<= 1) {
       const float oa = __shfl_xor(a, k, 64), ob = __shfl_xor(b, k, 64);
       b = fmaxf(fminf(a, oa), fmaxf(b, ob));
       a = fmaxf(a, oa);
     }
     const float v = q.top2 ? a + b : a;
-    if (part == 0) sv[g] = v;
+    float *sv = m.v[tok];
+    __builtin_amdgcn_wave_barrier();
+    if (part0 == 0) sv[g] = v;
     __builtin_amdgcn_wave_barrier();
     int before = 0;
-    for (int k = 0; k < q.G; ++k) before += sv[k] > v;
-    const bool kept = g < q.G && before < q.keep;
-    const float least = -gr_max16(kept ? -v : -INF), most = gr_max16(g < q.G && !kept ? v : -INF);
+    for (int k = 0; k < G; ++k) before += sv[k] > v;
+    mine_kept = g < G && before < q.keep;
+    const float least = -gr_max16(mine_kept ? -v : -INF), most = gr_max16(g < G && !mine_kept ? v : -INF);
     // (a sum of two is off by twice as much; equal values, NaN and two infinities are not sure)
     sure = sure && least - most > 2.f * unsure_abs + unsure_rel * (fabsf(least) + fabsf(most));
     if (by_logit) sure = sure && least > (q.sigmoid ? -700.f : top - 700.f);
-    const unsigned bits = (unsigned)(__ballot(kept) >> (16 * tok)) & 0xffffu;
-    const unsigned over = (65536u + (unsigned)q.size - 1u) / (unsigned)q.size;  // e / size = e over >> 16 for e < 256
-#pragma unroll
-    for (int r = 0; r < V; ++r)
-      if (!((bits >> ((((unsigned)(16 * r + j) * over) >> 16) * lanes)) & 1u)) c[r] = -INF;
   }
-  // k + 1 rounds of the largest value; lane i keeps choice i (two of them past 16 choices)
-  float last = INF, at_lane = c[0];
-  int r_lane = 0, mine[2] = {0, 0};
+  // k + 1 rounds of the largest value; lane i keeps choice i (two of them past 16 choices).  The place in the run in the last bits.
+  int key[V], at_lane = NONE;
 #pragma unroll
-  for (int r = 1; r < V; ++r)
-    if (c[r] > at_lane) { at_lane = c[r]; r_lane = r; }
+  for (int r = 0; r < V; ++r) {
+    const int x = (gr_key(c[r]) & -V) | r;
+    key[r] = mine_kept & (c[r] > -1e38f) ? x : NONE;
+  }
+  // (fours in descending order: a round takes the first of one away)
+#pragma unroll
+  for (int r = 0; r < V; r += 4) {
+    auto order = [&](int x, int y) {
+      const int hi = max(key[r + x], key[r + y]);
+      key[r + y] = min(key[r + x], key[r + y]);
+      key[r + x] = hi;
+    };
+    order(0, 1); order(2, 3); order(0, 2); order(1, 3); order(1, 2);
+    at_lane = max(at_lane, key[r]);
+  }
+  unsure_rel += (float)V * 1.3e-7f;
+  const float floor = by_logit ? (q.sigmoid ? -700.f : top - 700.f) : -1e37f;
   const bool more = q.k < q.keep * q.size;
+  float last = INF;
+  int mine[2] = {0, 0};
   for (int i = 0; i < q.k + more; ++i) {
-    const float best = gr_max16(at_lane);
-    const bool won = at_lane == best;
-    const unsigned who = (unsigned)(__ballot(won) >> (16 * tok)) & 0xffffu;
-    sure = sure && (i == q.k || (who & (who - 1u)) == 0u) &&
-           (i == 0 || (i == q.k && best == -INF) || last - best > unsure_abs + unsure_rel * (fabsf(last) + fabsf(best)));
+    const int best = gr_max16_i(at_lane);
+    const unsigned who = (unsigned)(__ballot(at_lane == best) >> (16 * tok)) & 0xffffu;
+    const float value = gr_value(best);
+    // (a last round that finds none, and the first, have no border)
+    sure &= (i == 0) | ((i == q.k) & (best == NONE)) | (last - value > unsure_abs + unsure_rel * (fabsf(last) + fabsf(value)));
     if (i == q.k) break;
-    sure = sure && best > (by_logit ? (q.sigmoid ? -700.f : top - 700.f) : -INF);
-    last = best;
-    const int e = (int)gr_max16(won ? (float)(16 * r_lane + j) : -1.f);
-    if ((i & 15) == j) mine[i >> 4] = e;
-    float next = -INF;
-    int r_next = 0;
+    sure &= (best != NONE) & (value > floor) & ((who & (who - 1u)) == 0u);
+    last = value;
+    const int jw = __builtin_ctz(who | 0x10000u), gw = jw >> q.shift;
+    const int e = gw * size + (jw - (gw << q.shift)) * per + (best & (V - 1));
+    if ((i & 15) == j) mine[i >> 4] = sure ? e : 0;
+    at_lane = NONE;
 #pragma unroll
-    for (int r = 0; r < V; ++r) {
-      c[r] = won && r == r_lane ? -INF : c[r];
-      if (c[r] > next) { next = c[r]; r_next = r; }
+    for (int r = 0; r < V; r += 4) {
+      const bool gone = key[r] == best;
+      key[r] = gone ? key[r + 1] : key[r];
+      key[r + 1] = gone ? key[r + 2] : key[r + 1];
+      key[r + 2] = gone ? key[r + 3] : key[r + 2];
+      key[r + 3] = gone ? NONE : key[r + 3];
+      at_lane = max(at_lane, key[r]);
     }
-    at_lane = next;
-    r_lane = r_next;
   }
   // weights, in 64 bits: lane i those of its choices
   double den = 1.0;
@@ -323,8 +376,8 @@ static __device__ __forceinline__ void group_topk_quad(const GroupRule &q, const
   for (int h = 0; h < 2; ++h) {
     s[h] = 0.0;
     if (h && q.k <= 16) break;
-    const double x = (double)fmaxf(row[mine[h]], -INF);
-    s[h] = q.sigmoid ? 1.0 / (1.0 + exp(-x)) : gr_exp(x - (double)top) / den;
+    const double x = (double)fmaxf(logits[(size_t)t * ldl + mine[h]], -INF), p = gr_exp(q.sigmoid ? -fabs(x) : x - (double)top);
+    s[h] = q.sigmoid ? gr_div(x < 0.0 ? p : 1.0, 1.0 + p) : gr_div(p, den);
     total += j + 16 * h < q.k ? s[h] : 0.0;
   }
   if (q.renorm) total = gr_sum16(total);
@@ -340,10 +393,8 @@ static __device__ __forceinline__ void group_topk_quad(const GroupRule &q, const
       if (s_idx) s_idx[t * q.k + i] = mine[h];
     }
   }
-  if (s_mask) {  // bit e of the token's mask: an or of its lanes' choices, 16 bits of experts at a time
-    if (live && sure) {
-      for (int r = j; r < 4; r += 16) s_mask[t][r] = 0ull;
-    }
+  if (s_mask) {  // bit e of the token's mask
+    if (live && sure && j < 4) s_mask[t][j] = 0ull;
     __builtin_amdgcn_wave_barrier();
     if (live && sure) {
 #pragma unroll
@@ -356,8 +407,8 @@ static __device__ __forceinline__ void group_topk_quad(const GroupRule &q, const
   while (again) {
     const int k = (int)__builtin_ctzll(again) >> 4, tk = t0 + k;
     again &= again - 1ull;
-    group_topk_token<(V + 3) / 4>(q, logits + (size_t)tk * ldl, bias, lane, m.exact, idx + (size_t)tk * q.k, w + (size_t)tk * q.k,
-                                  s_idx ? s_idx + tk * q.k : nullptr, s_mask ? s_mask[tk] : nullptr);
+    group_topk_token<4>(q, logits + (size_t)tk * ldl, bias, lane, m.exact, idx + (size_t)tk * q.k, w + (size_t)tk * q.k,
+                        s_idx ? s_idx + tk * q.k : nullptr, s_mask ? s_mask[tk] : nullptr);
   }
 }
 // V 0: more groups than a token has lanes: 64-bit scores throughout, a token by a wave
@@ -376,17 +427,18 @@ static __device__ __forceinline__ void group_topk_four(const GroupRule &q, const
 // f(V) for the form that a rule takes
 template <class F>
 static void gr_form(const GroupRule &q, const F &f) {
-  if (q.keep < q.G && q.G > 16) f(std::integral_constant<int, 0>());
-  else if (q.E <= 64) f(std::integral_constant<int, 4>());
-  else if (q.E <= 128) f(std::integral_constant<int, 8>());
-  else f(std::integral_constant<int, 16>());
+  if (q.per == 0) f(std::integral_constant<int, 0>());
+  else if (q.per <= 4) f(std::integral_constant<int, 4>());
+  else if (q.per <= 8) f(std::integral_constant<int, 8>());
+  else if (q.per <= 16) f(std::integral_constant<int, 16>());
+  else f(std::integral_constant<int, 32>());
 }
 
 template <int V>
-__global__ __launch_bounds__(256) void k_group_topk(const GroupRule q, const float *__restrict__ logits, const int T, const int ldl,
+__global__ __launch_bounds__(256, V == 32 ? 4 : 8) void k_group_topk(const GroupRule q, const float *__restrict__ logits, const int T, const int ldl,
                                                     const float *__restrict__ bias, int *__restrict__ idx, float *__restrict__ w) {
   __shared__ GroupLds s_m[4];
-  const int lane = threadIdx.x & 63, wv = threadIdx.x >> 6, t0 = 4 * (blockIdx.x * 4 + wv);
+  const int lane = threadIdx.x & 63, wv = threadIdx.x >> 6, t0 = __builtin_amdgcn_readfirstlane(4 * (blockIdx.x * 4 + wv));
   if (t0 < T) group_topk_four<V>(q, logits, ldl, t0, T, bias, lane, s_m[wv], idx, w, nullptr, nullptr);
 }
 
@@ -414,7 +466,7 @@ __global__ __launch_bounds__(64 * NW) void k_group_topk_dispatch(const GroupRule
   __shared__ unsigned long long s_mask[GR_MAXT][4];
   __shared__ int s_off[GR_MAXE];
   __shared__ int s_rows[4], s_used[4], s_tot;
-  const int tid = threadIdx.x, lane = tid & 63, wv = tid >> 6, E = q.E, k = q.k;
+  const int tid = threadIdx.x, lane = tid & 63, wv = __builtin_amdgcn_readfirstlane(tid >> 6), E = q.E, k = q.k;
   if (4 * wv < T) group_topk_four<V>(q, logits, ldl, 4 * wv, T, bias, lane, s_m[wv], idx, w, s_idx, s_mask);  // (T <= 4 NW)
   __syncthreads();
   // A token holds an expert at most once: the pairs of an expert in stable order are its tokens in order, so the place of
@@ -485,9 +537,16 @@ static int rule_check(const char *who, const moe_route_rule *r, int E, int k) {
   }
   return MOE_OK;
 }
-static GroupRule rule_of(const moe_route_rule &r, int E, int k) {
-  return GroupRule{E, k, r.n_group, E / r.n_group, r.topk_group, r.scores == MOE_SCORES_SIGMOID, r.group_value == MOE_GROUP_TOP2,
-                   r.renorm != 0, r.scale};
+static GroupRule rule_of(const moe_route_rule &r, int E, int k, int ldl) {
+  GroupRule q{E, k, r.n_group, E / r.n_group, r.topk_group, r.scores == MOE_SCORES_SIGMOID, r.group_value == MOE_GROUP_TOP2,
+              r.renorm != 0, r.scale, 0, 0};
+  if (ldl > 1 << 26) return q;  // (four rows have to be in reach of 31 bits)
+  if (q.keep == q.G) q.per = (E + 15) / 16;
+  else if (q.G <= 16) {
+    while ((q.G << (q.shift + 1)) <= 16) ++q.shift;
+    q.per = (q.size + (1 << q.shift) - 1) >> q.shift;
+  }
+  return q;
 }
 
 extern "C" int moe_group_topk(const float *logits, int T, int E, int ldl, int k, const moe_route_rule *rule_host, const float *bias,
@@ -500,7 +559,7 @@ extern "C" int moe_group_topk(const float *logits, int T, int E, int ldl, int k,
   if (T == 0) return MOE_OK;
   hipStream_t s = (hipStream_t)stream;
   moe_ktimer_begin(MOE_K_TOPK, s);
-  const GroupRule q = rule_of(*rule_host, E, k);
+  const GroupRule q = rule_of(*rule_host, E, k, ldl);
   gr_form(q, [&](auto v) {
     hipLaunchKernelGGL(HIP_KERNEL_NAME(k_group_topk<decltype(v)::value>), dim3((T + 15) / 16), dim3(256), 0, s, q, logits, T, ldl, bias, idx, w);
   });
@@ -523,7 +582,7 @@ extern "C" int moe_group_topk_dispatch(const float *logits, int T, int E, int ld
   hipStream_t s = (hipStream_t)stream;
   const GroupDispatch d{counts, offsets, sorted_pair, pos_of_pair, sorted_tok, units, n_active, (long long *)active_ids, max_units,
                         units_host_out, n_active_host_out, seq_host_out, seq_value};
-  const GroupRule q = rule_of(*rule_host, E, k);
+  const GroupRule q = rule_of(*rule_host, E, k, ldl);
   moe_ktimer_begin(MOE_K_TOPK, s);
   // (four tokens a wave: four waves for up to 16 tokens, whose barriers are cheaper; thread e also owns expert e)
   gr_form(q, [&](auto v) {
