@@ -476,8 +476,8 @@ int moe_combine_windows(const float *part_r, const float *part_s, const float *t
  * x [M, K], W [N, K], biases [N], residual [M, N] all bf16 or all fp16 (dtype); y [M, N] of that type or fp32 (y_fp32).
  * Sums, biases, activation, product and residual in fp32, one rounding at the end.  Rows are ldx, ldw, ldr and ldy elements apart
  * (both matrices of a pair ldw).  K, ldx and ldw multiples of 8, ldx and ldw below 2^21, x and the matrices on 16-byte boundaries; M
- * and N are any, 0 included.  bias, b_gate, b_up and residual may be NULL; residual may be y itself (same rows and type), y must not
- * overlap anything else.
+ * and N from 0 to 2^26.  bias, b_gate, b_up and residual may be NULL; residual may be y itself (same rows and type); a y that
+ * overlaps anything else is refused (rows side by side in one buffer, the same distance apart, do not overlap).
  * ws: moe_linear_workspace_bytes(M, N, K, gated) of device memory, not shared by calls that overlap, with no contents to keep; a
  * smaller one or NULL is refused where that number is not 0. */
 #define MOE_DT_BF16 0

@@ -706,11 +706,22 @@ __global__ __launch_bounds__(256) void k_linear_join(const LinArgs a) {
 }
 
 // ---- entry points -------------------------------------------------------------------------------------------------------------
+// Does the result share a byte with p's `rows` rows of `len` bytes, `ld` bytes apart?  (Rows side by side in one buffer do not; rows of
+// different distances whose ranges meet are taken to.)
+static bool lin_shares(const LinArgs &a, const void *p, long long rows, long long ld, long long len) {
+  if (!p) return false;
+  const long long e = a.y32 ? 4 : 2, ldy = a.ldy * e, ny = a.N * e;
+  const intptr_t y = (intptr_t)a.y, q = (intptr_t)p;
+  if (y + (a.M - 1) * ldy + ny <= q || q + (rows - 1) * ld + len <= y) return false;
+  if (ldy != ld) return true;
+  const long long d = ((y - q) % ld + ld) % ld;
+  return d < len || d + ny > ld;
+}
 static int lin_check(const char *who, const LinArgs &a, int dtype, bool gated) {
   const bool empty = a.M == 0 || a.N == 0;
   if (a.M < 0 || a.N < 0 || a.K <= 0 || a.K % 8 || (dtype != MOE_DT_BF16 && dtype != MOE_DT_FP16) || a.act < MOE_ACT_NONE ||
       a.act > MOE_ACT_RELU2 || a.ldx < a.K || a.ldx % 8 || a.ldw < a.K || a.ldw % 8 || a.ldy < a.N || (a.res && a.ldr < a.N) ||
-      a.ldx >= 1 << 21 || a.ldw >= 1 << 21) {
+      a.ldx >= 1 << 21 || a.ldw >= 1 << 21 || a.M > 1 << 26 || a.N > 1 << 26) {
     moe_set_error("%s: bad shape (M=%d N=%d K=%d dtype=%d act=%d, rows %lld %lld %lld %lld elements apart)", who, a.M, a.N, a.K, dtype,
                   a.act, a.ldx, a.ldw, a.res ? a.ldr : 0, a.ldy);
     return MOE_EINVAL;
@@ -719,17 +730,25 @@ static int lin_check(const char *who, const LinArgs &a, int dtype, bool gated) {
     moe_set_error("%s: operands must be present, x and the matrices on 16-byte boundaries", who);
     return MOE_EINVAL;
   }
+  const bool in_place = a.res == a.y && !a.y32 && (a.ldr == a.ldy || a.M == 1);
+  if (!empty && (lin_shares(a, a.x, a.M, a.ldx * 2, a.K * 2ll) || lin_shares(a, a.w[0], a.N, a.ldw * 2, a.K * 2ll) ||
+                 lin_shares(a, a.w[1], a.N, a.ldw * 2, a.K * 2ll) || lin_shares(a, a.bias[0], 1, a.N * 2ll, a.N * 2ll) ||
+                 lin_shares(a, a.bias[1], 1, a.N * 2ll, a.N * 2ll) || (!in_place && lin_shares(a, a.res, a.M, a.ldr * 2, a.N * 2ll)))) {
+    moe_set_error("%s: the result overlaps an operand (only a residual may be the result itself)", who);
+    return MOE_EINVAL;
+  }
   return MOE_OK;
 }
 
 // Which kernel a product takes: few rows (wm 0), or tiles of 64 wm x 64 wn with `ring` slabs in LDS (4 x 4: the wide kernel) and K in
-// `splits` pieces.  The plan of the least time after a model of one launch, us, fitted to 1900 measured times of 100 shapes (33 to 4096
+// `splits` pieces.  The plan of the least time after a model of one launch, us, fitted to 2550 measured times of 100 shapes (33 to 4096
 // rows; the chosen plan is 1.6 % slower than the best of all on average, 22 % at worst):
 //   rounds x (slabs x (c0 + c1 x share of the compute units in use) + f),  with pieces 2.5 + 0.33 a piece + 0.15 per MB of partial sums
 // c0, c1: a slab of a workgroup on an idle chip, and what the others' traffic adds; f: start and epilogue.  The narrow tiles are bound by
 // LDS (96 (wm + wn) bytes x rows read and written for 32 wm wn of products), the wide one by the matrix cores, at the power limit.
-// us, best other tile / chosen: 64 x 4096 x 4096 14.5 / 13.1 (64 x 64, 3 pieces), 512 x 4096 x 4096 28.7 / 25.0 (64 x 128), 1024 x 4096 x
-// 4096 49 / 38.1 (128 x 128), 300 x 2048 x 10944 33.7 / 31.6 (128 x 128, 4 pieces), 2048 x 4096 x 4096 101 / 67.7 (128 x 256).
+// us, best other tile / chosen: 64 x 4096 x 4096 14.7 / 12.9 (64 x 64, 3 pieces), 512 x 4096 x 4096 28.6 / 25.0 (64 x 128), 1024 x 4096 x
+// 4096 48.2 / 38.1 (128 x 128), 384 x 2048 x 10944 37.8 / 34.5 (128 x 128, 5 pieces), 2048 x 4096 x 4096 79.3 / 67.7 (128 x 256), 1536 x 2048 x
+// 10944 90.9 / 77.2 (256 x 256, 5 pieces); gated 128 x 14336 x 4096 70.2 / 56.8 (128 x 128), 2048 x 10944 x 2048 206 / 160 (256 x 256).
 // Few rows, us, k_linear_rows / best tile: 3 x 2048 x 10944 13.4 / 14.8, 8 x 4096 x 4096 11.2 / 11.5, 16 x 4096 x 4096 10.7 / 11.6, 8 x 2048 x
 // 1408 4.9 / 7.4, 16 x 2048 x 1408 6.0 / 7.4; past 8 rows a long reduction is faster on tiles in pieces (every workgroup reads all of x,
 // which no longer passes unnoticed beside the weights): 12 x 2048 x 10944 23.0 / 15.5, 16 x 4096 x 14336 37.7 / 27.9, and past 16 the tiles
@@ -779,6 +798,10 @@ static int lin_launch(const LinArgs &a, float *ws, hipStream_t s) {
   }
   t.nm = (a.M + 64 * pl.wm - 1) / (64 * pl.wm);
   t.nn = (a.N + 64 * pl.wn / NM - 1) / (64 * pl.wn / NM);
+  if ((long long)t.nm * t.nn * pl.splits >= 1 << 24) {  // (a grid has fewer than 2^32 threads)
+    moe_set_error("moe_linear: %d x %d results are too many for one launch", a.M, a.N);
+    return MOE_EINVAL;
+  }
   t.splits = pl.splits;
   t.ldp = (a.N + 7) & ~7;
   t.part = pl.splits > 1 ? ws : nullptr;

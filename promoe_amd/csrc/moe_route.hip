@@ -552,7 +552,7 @@ static GroupRule rule_of(const moe_route_rule &r, int E, int k, int ldl) {
 extern "C" int moe_group_topk(const float *logits, int T, int E, int ldl, int k, const moe_route_rule *rule_host, const float *bias,
                               int *idx, float *w, void *stream) {
   if (int rc = rule_check("moe_group_topk", rule_host, E, k)) return rc;
-  if (T < 0 || ldl < E || (T > 0 && (!logits || !idx || !w))) {
+  if (T < 0 || T > 1 << 27 || ldl < E || (T > 0 && (!logits || !idx || !w))) {
     moe_set_error("moe_group_topk: bad argument (T=%d E=%d ldl=%d)", T, E, ldl);
     return MOE_EINVAL;
   }

@@ -567,7 +567,7 @@ def linear(x: torch.Tensor, w: torch.Tensor, bias: torch.Tensor | None = None, a
     """act(x w^T + bias) + residual in one pass (moe_linear): x [M, K], w [N, K], bias [N] and residual [M, N] all bf16 or all
     fp16; act one of none, silu, gelu, gelu_tanh, relu, relu2.  Sums and epilogue in fp32, rounded once to the type of x (or left
     in fp32: out_dtype).  K and the row strides of x and w are multiples of 8; rows of x, w, residual and out may be further apart
-    than they are long.  out may be the residual itself (added in place)."""
+    than they are long.  out may be the residual itself (added in place) and overlaps nothing else."""
     return _product("linear", x, (w,), (bias,), act, residual, out, out_dtype)
 
 

@@ -129,6 +129,17 @@ def test_sizes_of_dense_layers(cuda, M, N, K, gated):
     run(cuda, M, N, K, torch.bfloat16, "silu" if gated else "none", False, not gated, gated)
 
 
+# Every tile on sizes that end inside it, with K whole and in pieces, and more tiles than workgroups of the widest one.
+@pytest.mark.parametrize("M,N,K,gated", [(130, 2049, 4104, False), (510, 4093, 4104, False), (450, 4099, 2056, False), (260, 2049, 10952, False), (512, 4099, 1032, False),
+                                         (1030, 1023, 8200, False), (1000, 4099, 1032, False), (768, 2050, 10952, False), (2000, 4097, 520, False),
+                                         (1300, 2050, 10952, False), (4090, 8203, 1032, False), (100, 320, 1544, True), (1000, 1409, 520, True),
+                                         (512, 2051, 4104, True), (1300, 1021, 10952, True), (4090, 4101, 1032, True)])
+def test_every_tile_on_ragged_sizes(cuda, M, N, K, gated):
+    f16 = N % 2 == 0
+    run(cuda, M, N, K, torch.float16 if f16 else torch.bfloat16, "gelu" if gated else "relu2", True, not gated, gated, gap=8,
+        out_dtype=torch.float32 if f16 and gated else None)
+
+
 @pytest.mark.parametrize("M,N,K", [(1, 64, 512), (30, 80, 264), (300, 300, 512)])
 def test_residual_in_place_and_aligned_only_to_its_type(cuda, M, N, K):
     """out is the residual; rows of an odd number of elements from an odd offset on."""
@@ -212,3 +223,19 @@ def test_empty_other_stream_graph_and_refusals(cuda):
         ops.linear(x, w)
     with torch.no_grad():
         ops.linear(x, w)
+
+
+def test_a_result_beside_its_operand_in_one_buffer(cuda):
+    """x and y as columns of one matrix; y over x is refused."""
+    from promoe_amd import _lib as L
+    from promoe_amd import ops
+    print("case linear_beside", flush=True)
+    gen = torch.Generator(device=cuda).manual_seed(9)
+    for M in (1, 5, 70):
+        buf = torch.randn(M, 192, device=cuda, generator=gen).to(torch.bfloat16)
+        w = rows((64, 128), 0.1, torch.bfloat16, gen, cuda)
+        y, e = expect(buf[:, :128], [w], [None], "none", None)
+        check(ops.linear(buf[:, :128], w, out=buf[:, 128:]), y, e)
+        for out in (buf[:, 127:191], buf[:, :64]):
+            with pytest.raises(L.MoeError, match="overlaps"):
+                ops.linear(buf[:, :128], w, out=out)
