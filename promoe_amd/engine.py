@@ -313,17 +313,19 @@ class PrefetchMngr:
                   shared_gated=False, fmt: int = L.FMT_INT4_G128, rule=None, select_bias=None):
         """rule (ops.RouteRule): the layer's router has groups of experts, sigmoid scores or a selection bias (select_bias, fp32
         [num_expert] on the device); route_mode is not used then."""
+        n = gate_w.shape[0] - int(shared_gated)
+        if select_bias is not None:
+            if rule is None or select_bias.dtype != torch.float32 or select_bias.shape != (n,) or select_bias.device != gate_w.device:
+                raise L.MoeError("set_layer: select_bias goes with a rule and must be fp32 [%d] on %s" % (n, gate_w.device))
+            select_bias = select_bias.contiguous()
+        if rule is not None:                                 # (refused before the layer is described: no layer without its rule)
+            check(lib.moe_group_topk(None, 0, n, n, top_k, C.byref(rule), None, None, None, None), "set_layer")
         d = L.LayerDesc(H, I, I_sh, top_k, route_mode, fmt, int(shared_gated), L.ptr(gate_w), L.ptr(gate_bias),
                         L.ptr(shared))
         self._keep.append((gate_w, gate_bias, shared))
         check(lib.moe_set_layer(self._h, layer_id, C.byref(d)), "set_layer")
         if rule is not None:
-            if select_bias is not None:
-                n = gate_w.shape[0] - int(shared_gated)
-                if select_bias.dtype != torch.float32 or select_bias.shape != (n,) or select_bias.device != gate_w.device:
-                    raise L.MoeError("set_layer: select_bias must be fp32 [%d] on %s" % (n, gate_w.device))
-                select_bias = select_bias.contiguous()
-                self._keep.append(select_bias)
+            self._keep.append(select_bias)
             check(lib.moe_set_layer_routing(self._h, layer_id, C.byref(rule), L.ptr(select_bias)), "set_layer")
 
     def forward_prepare(self, max_tokens: int):

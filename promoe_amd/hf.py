@@ -73,29 +73,47 @@ def _route_rule(block):
 
     bias = getattr(gate, "e_score_correction_bias", None)
     if bias is not None:                                     # scores are sigmoids, the bias balances the choice
+        kind = getattr(gate, "scoring_func", None) or getattr(gate, "score_function", None) or "sigmoid"
+        if kind != "sigmoid":
+            raise NotImplementedError("a selection bias on scores of kind %r (only 'sigmoid' is supported)" % (kind,))
         return ops.RouteRule("sigmoid", int(find("n_group", "num_group")), int(find("topk_group")), "top2",
                              bool(find("norm_topk_prob")), float(find("routed_scaling_factor"))), bias
     if getattr(gate, "topk_method", None) == "group_limited_greedy":
+        if getattr(gate, "norm_topk_prob", False):           # (transformers' own router does not divide by the sum; others do)
+            raise NotImplementedError("norm_topk_prob with 'group_limited_greedy'")
         return ops.RouteRule("softmax", int(find("num_group", "n_group")), int(find("topk_group")), "max", False,
                              float(find("routed_scaling_factor"))), None
     return None, None
 
 
-_HIDDEN_ACTS = {"silu": "silu", "swish": "silu", "gelu": "gelu", "gelu_new": "gelu_tanh", "gelu_pytorch_tanh": "gelu_tanh",
-                "relu": "relu", "relu2": "relu2"}
+def _activation_of(fn):
+    """The name under which ops.linear_gated has a module's activation, from its values; None for any other."""
+    x = torch.tensor([-3.0, -1.5, -0.4, 0.3, 1.25, 2.5], dtype=torch.float64)
+    known = {"silu": torch.nn.functional.silu(x), "gelu": torch.nn.functional.gelu(x),
+             "gelu_tanh": torch.nn.functional.gelu(x, approximate="tanh"), "relu": x.relu(), "relu2": x.relu() ** 2}
+    try:
+        with torch.no_grad():
+            y = fn(x.clone())
+        return next((n for n, v in known.items() if torch.allclose(y, v, rtol=0, atol=1e-6)), None)
+    except Exception:                                        # (one with parameters of another type or device, say)
+        return None
 
 
 def find_dense_mlps(model):
-    """[(qualified name, module, activation)] of the dense gated feed-forward layers (gate_proj, up_proj, down_proj) that are no part
-    of a sparse block and whose shapes and activation the fused products take."""
+    """[(qualified name, module, activation)] of the dense gated feed-forward layers (gate_proj, up_proj, down_proj and act_fn, nothing
+    else) that are no part of a sparse block and whose shapes and activation the fused products take.  Layers whose products are
+    not plain ones (subclasses of Linear: quantised or with adapters; hooks; a forward put in place of the class's) are left."""
     inside = {id(m) for _, blk in find_moe_blocks(model) for m in blk.modules()}
     out = []
     for name, mod in model.named_modules():
         parts = [getattr(mod, n, None) for n in ("gate_proj", "up_proj", "down_proj")]
-        if id(mod) in inside or not all(isinstance(p, torch.nn.Linear) for p in parts):
+        if id(mod) in inside or not all(type(p) is torch.nn.Linear for p in parts):
             continue
-        act = _HIDDEN_ACTS.get(getattr(getattr(mod, "config", None), "hidden_act", None))
+        if any("forward" in vars(m) or m._forward_hooks or m._forward_pre_hooks for m in parts) or "forward" in vars(mod) \
+                or set(dict(mod.named_children())) - {"gate_proj", "up_proj", "down_proj", "act_fn"}:
+            continue
         g, u, d = parts
+        act = _activation_of(getattr(mod, "act_fn", None))
         if act and g.weight.shape == u.weight.shape and d.weight.shape == g.weight.shape[::-1] and d.in_features % 8 == 0 \
                 and g.in_features % 8 == 0:
             out.append((name, mod, act))
