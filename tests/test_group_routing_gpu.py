@@ -221,3 +221,37 @@ def test_layer_forward_with_groups(cuda, kind, cache_rate):
     assert np.abs(y - ref).max() / np.abs(ref).max() <= 2e-2
     pm.drain()
     pm.close()
+
+
+@pytest.mark.parametrize("ldl", [1 << 26, (1 << 26) + 4])
+def test_rows_far_apart(cuda, ldl):
+    """Rows at both sides of the distance that four of them may have, far enough for offsets past 2^31: as rows side by side."""
+    from promoe_amd import ops
+    print(f"case group_topk_far ldl={ldl}", flush=True)
+    c = RULES[5]
+    _, _, ld, bd = _data(c, 37, 3, cuda)
+    far = torch.empty(36 * ldl + c[0], device=cuda).as_strided((37, c[0]), (ldl, 1))
+    far.copy_(ld)
+    for f in (ops.group_topk, ops.group_topk_dispatch):
+        a, b = f(ld, c[1], _rule(c), bd), f(far, c[1], _rule(c), bd)
+        assert torch.equal(a[0], b[0]) and torch.equal(a[1], b[1])
+
+
+def test_logits_and_bias_on_any_float(cuda):
+    """Views that start at any float, in the middle of larger buffers, and end with them."""
+    from promoe_amd import ops
+    print("case group_topk_any_float", flush=True)
+    for c in (RULES[5], RULES[2], RULES[0]):
+        lg, bias, _, _ = _data(c, 13, 21, cuda)
+        ridx, rw = _ref(lg, c, bias)
+        for off in range(4):
+            for gap in (0, 1, 2, 5):
+                row = c[0] + gap
+                buf = torch.full((off + 12 * row + c[0],), float("nan"), device=cuda)
+                v = buf[off:].as_strided((13, c[0]), (row, 1), off)
+                v.copy_(torch.from_numpy(lg))
+                b = torch.full((off + c[0],), float("nan"), device=cuda)[off:]
+                b.copy_(torch.from_numpy(bias))
+                idx, w = ops.group_topk(v, c[1], _rule(c), b)
+                assert np.array_equal(idx.cpu().numpy(), ridx)
+                _close(w.cpu().numpy(), rw)

@@ -239,3 +239,28 @@ def test_a_result_beside_its_operand_in_one_buffer(cuda):
         for out in (buf[:, 127:191], buf[:, :64]):
             with pytest.raises(L.MoeError, match="overlaps"):
                 ops.linear(buf[:, :128], w, out=out)
+
+
+@pytest.mark.parametrize("M,N,K,gated", [(5, 1100, 512, False), (450, 1100, 264, False), (1000, 1409, 520, True), (2000, 1030, 8200, False)])
+def test_rows_far_apart(cuda, M, N, K, gated):
+    """Rows 4 MiB apart, so that offsets pass 2^31 elements and 2^32 bytes: the same bits as from rows side by side."""
+    from promoe_amd import ops
+    print(f"case linear_far M={M} N={N} K={K} gated={gated}", flush=True)
+    gen = torch.Generator(device=cuda).manual_seed(M)
+    ld = (1 << 21) - 8
+
+    def far(t):
+        v = torch.empty((t.shape[0] - 1) * ld + t.shape[1], dtype=t.dtype, device=cuda).as_strided(t.shape, (ld, 1))
+        v.copy_(t)
+        return v
+
+    x, w, u = (rows(s, 0.1, torch.bfloat16, gen, cuda).contiguous() for s in ((M, K), (N, K), (N, K)))
+    res = rows((M, N), 1.0, torch.bfloat16, gen, cuda).contiguous()
+    out = torch.empty((M - 1) * ld + N, dtype=torch.bfloat16, device=cuda).as_strided((M, N), (ld, 1))
+    if gated:
+        want = ops.linear_gated(x, w, u)
+        ops.linear_gated(far(x), far(w), far(u), out=out)
+    else:
+        want = ops.linear(x, w, residual=res)
+        ops.linear(far(x), far(w), residual=far(res), out=out)
+    assert torch.equal(out, want)
