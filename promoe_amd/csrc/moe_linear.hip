@@ -3,6 +3,7 @@
 // fp32 sums, which are rounded once, to the type of y.
 #include <hip/hip_runtime.h>
 #include <stdint.h>
+#include <algorithm>
 #include <type_traits>
 
 #include "moe_common.h"
@@ -29,7 +30,6 @@ struct LinArgs {
   int splits, ldp;                           // pieces of K, columns of a row of partial sums
   int slabs, extra;                          // slabs of a piece; the first `extra` pieces have one more
   float *part;                               // partial sums [splits][1 or 2 matrices][M][ldp], NULL: the tile kernel finishes
-  int whole;                                 // rows of y and of the residual start on 16-byte boundaries
 };
 
 template <bool F16>
@@ -116,6 +116,10 @@ static __device__ __forceinline__ u32x4_t lin_pack(const float (&v)[8]) {
   return o;
 }
 
+// Sixteen bytes of a result or residual, whose rows may start at any element: the hardware splits an access that crosses a line (us, the
+// elements one by one / together: 379 x 1409 x 2048 12.9 / 10.7, 1000 x 1409 x 2048 18.6 / 15.7, of 1408 columns 15.4)
+typedef u32x4_t u32x4_any __attribute__((aligned(2)));
+typedef f32x4_t f32x4_any __attribute__((aligned(4)));
 // Eight adjacent columns of the result from column n on (past N: left out): bias, activation, gate, residual and the one rounding
 template <bool F16, bool GATED>
 struct LinColumns {
@@ -131,10 +135,10 @@ struct LinColumns {
 #pragma unroll
       for (int i = 0; i < 8; ++i) b1[i] = lin_f32<F16>(a.bias[1][min(n + i, a.N - 1)]);
   }
-  // the residual of row m where its rows are whole (asked for a row ahead: its trip to memory is longer than a row's work)
+  // the residual of row m where all eight are there (asked for a row ahead: its trip to memory is longer than a row's work)
   __device__ __forceinline__ u32x4_t residual(const LinArgs &a, int m) const {
-    if (GATED || !a.res || !a.whole || count < 8 || m >= a.M) return u32x4_t{0, 0, 0, 0};
-    return *(const u32x4_t *)(a.res + m * a.ldr + n);
+    if (GATED || !a.res || count < 8 || m >= a.M) return u32x4_t{0, 0, 0, 0};
+    return *(const u32x4_any *)(a.res + m * a.ldr + n);
   }
   // the sums alone, of one piece of K (the join has the rest); rows of a.ldp columns, a multiple of 8
   __device__ __forceinline__ void partial(const LinArgs &a, int split, int m, const float *s0, const float *s1) const {
@@ -168,14 +172,14 @@ struct LinColumns {
 #pragma unroll
       for (int i = 0; i < 8; ++i) v[i] *= s1[i] + b1[i];
     }
-    if (count == 8 && a.whole) {  // whole rows of 16-byte pieces
+    if (count == 8) {
       if (!GATED && a.res) lin_add<F16>(v, r);
       if (a.y32) {
         float *y = (float *)a.y + m * a.ldy + n;
-        *(f32x4_t *)y = f32x4_t{v[0], v[1], v[2], v[3]};
-        *(f32x4_t *)(y + 4) = f32x4_t{v[4], v[5], v[6], v[7]};
+        *(f32x4_any *)y = f32x4_t{v[0], v[1], v[2], v[3]};
+        *(f32x4_any *)(y + 4) = f32x4_t{v[4], v[5], v[6], v[7]};
       } else {
-        *(u32x4_t *)((uint16_t *)a.y + m * a.ldy + n) = lin_pack<F16>(v);
+        *(u32x4_any *)((uint16_t *)a.y + m * a.ldy + n) = lin_pack<F16>(v);
       }
       return;
     }
@@ -619,7 +623,7 @@ __global__ __launch_bounds__(256, 1) void k_linear_wide(const LinArgs a) {
           __builtin_amdgcn_wave_barrier();
         }
       };
-      const bool inside = a.whole && !a.y32 && !a.part && cur.m0 + B <= a.M && cur.n0 + NC <= a.N;
+      const bool inside = !a.y32 && !a.part && cur.m0 + B <= a.M && cur.n0 + NC <= a.N;
       // a tile inside the result: no conditions, addresses by addition, the activation chosen once
       auto plain = [&](int m, auto act_) {
         const uint16_t *pr = GATED || !a.res ? nullptr : a.res + m * a.ldr + n;
@@ -627,7 +631,7 @@ __global__ __launch_bounds__(256, 1) void k_linear_wide(const LinArgs a) {
         u32x4_t res[NP];
         if (!GATED && a.res)
 #pragma unroll
-          for (int p = 0; p < NP; ++p) res[p] = *(const u32x4_t *)(pr + p * RPP * a.ldr);
+          for (int p = 0; p < NP; ++p) res[p] = *(const u32x4_any *)(pr + p * RPP * a.ldr);
         float s0[2][8], s1[2][8];
         fetch(0, s0[0], s1[0]);
 #pragma unroll
@@ -636,7 +640,7 @@ __global__ __launch_bounds__(256, 1) void k_linear_wide(const LinArgs a) {
           if (p + 1 < NP) fetch(p + 1, s0[(p + 1) & 1], s1[(p + 1) & 1]);
           c.template finish<decltype(act_)::value>(s0[p & 1], s1[p & 1]);
           if (!GATED && a.res) lin_add<F16>(s0[p & 1], res[p]);
-          *(u32x4_t *)(py + p * RPP * a.ldy) = lin_pack<F16>(s0[p & 1]);
+          *(u32x4_any *)(py + p * RPP * a.ldy) = lin_pack<F16>(s0[p & 1]);
         }
         __builtin_amdgcn_sched_barrier(0);
       };
@@ -753,37 +757,63 @@ static int lin_check(const char *who, const LinArgs &a, int dtype, bool gated) {
 // 1408 4.9 / 7.4, 16 x 2048 x 1408 6.0 / 7.4; past 8 rows a long reduction is faster on tiles in pieces (every workgroup reads all of x,
 // which no longer passes unnoticed beside the weights): 12 x 2048 x 10944 23.0 / 15.5, 16 x 4096 x 14336 37.7 / 27.9, and past 16 the tiles
 // are in general: 24 x 4096 x 4096 13.3 / 12.0, 24 gated 14336 x 4096 69 / 51.
-struct LinPlan { int wm, wn, ring, splits; };
+struct LinTile { int wm, wn, ring, per_cu; float c0, c1, f; };
+static const LinTile LIN_TILES[] = {{1, 1, 4, 2, 0.173f, 0.135f, 0.f}, {1, 2, 6, 1, 0.269f, 0.139f, 1.46f}, {2, 2, 4, 1, 0.380f, 0.221f, 2.2f},
+                                    {2, 4, 3, 1, 0.674f, 0.236f, 4.34f}, {4, 4, 5, 1, 1.146f, 0.f, 9.21f}};
+static float lin_us(const LinTile &t, int M, int N, int K, bool gated, long long n, int s) {
+  const long long slabs = (K + LT_K - 1) / LT_K, wgs = n * s, rounds = (wgs + 256 * t.per_cu - 1) / (256 * t.per_cu);
+  const float use = wgs >= 256 * t.per_cu ? (float)t.per_cu : (float)wgs / 256.f;
+  const float us = (float)rounds * ((float)((slabs + s - 1) / s) * (t.c0 + t.c1 * use) + t.f);
+  return s == 1 ? us : us + 2.5f + 0.33f * (float)s + 0.148e-6f * 8.f * (float)s * (gated ? 2.f : 1.f) * (float)M * (float)N;
+}
+struct LinPlan { int wm, wn, ring, splits; float us; };
 static LinPlan lin_plan(int M, int N, int K, bool gated) {
-  if (M <= 8 || (M <= 16 && K <= 4096)) return LinPlan{0, 0, 0, 1};
-  struct Tile { int wm, wn, ring, per_cu; float c0, c1, f; };
-  static const Tile tiles[] = {{1, 1, 4, 2, 0.173f, 0.135f, 0.f}, {1, 2, 6, 1, 0.269f, 0.139f, 1.46f}, {2, 2, 4, 1, 0.380f, 0.221f, 2.2f},
-                               {2, 4, 3, 1, 0.674f, 0.236f, 4.34f}, {4, 4, 5, 1, 1.146f, 0.f, 9.21f}};
+  if (M <= 8 || (M <= 16 && K <= 4096)) return LinPlan{0, 0, 0, 1, 2.5f + 0.6e-6f * (gated ? 2.f : 1.f) * (float)N * (float)K};
   static const int pieces[] = {1, 2, 3, 4, 5, 6, 8, 12, 16};
   const long long slabs = (K + LT_K - 1) / LT_K;
-  LinPlan best{2, 2, 4, 1};
-  float least = 1e30f;
-  for (const Tile &t : tiles) {
+  LinPlan best{2, 2, 4, 1, 1e30f};
+  for (const LinTile &t : LIN_TILES) {
     if (gated && t.wn == 1) continue;  // (a pair needs both matrices' blocks in a wave)
     const int cols = 64 * t.wn / (gated ? 2 : 1);
     const long long n = ((long long)M + 64 * t.wm - 1) / (64 * t.wm) * (((long long)N + cols - 1) / cols);
     for (int s : pieces) {
       if (s > slabs || (s > 1 && n * s > 640) || (t.wm == 4 && slabs < 2 * s)) break;
-      const long long wgs = n * s, rounds = (wgs + 256 * t.per_cu - 1) / (256 * t.per_cu);
-      const float use = wgs >= 256 * t.per_cu ? (float)t.per_cu : (float)wgs / 256.f;
-      float us = (float)rounds * ((float)((slabs + s - 1) / s) * (t.c0 + t.c1 * use) + t.f);
-      if (s > 1) us += 2.5f + 0.33f * (float)s + 0.148e-6f * 8.f * (float)s * (gated ? 2.f : 1.f) * (float)M * (float)N;
-      if (us < least) { least = us; best = LinPlan{t.wm, t.wn, t.ring, s}; }
+      const float us = lin_us(t, M, N, K, gated, n, s);
+      if (us < best.us) best = LinPlan{t.wm, t.wn, t.ring, s, us};
     }
   }
   return best;
+}
+// Where a product is cut in two launches: the large tiles that fill the chip whole rounds through, and the columns (or rows) behind them
+// on tiles of their own, instead of a last round of a few (3 us: the second launch).  us, one launch / two: 4097 x 4096 x 4096 174 / 117,
+// 1184 x 13760 x 2112 111 / 85, gated 768 x 10944 x 2048 97 / 71, 1300 x 10944 x 2048 137 / 125, 768 x 14336 x 4096 183 / 167.
+struct LinCut { int M, N; };  // size of the first part
+static LinCut lin_cut(int M, int N, int K, bool gated) {
+  LinCut cut{M, N};
+  const int half = gated ? 2 : 1;
+  if (((long long)M + 127) / 128 * (((long long)N + 256 / half - 1) / (256 / half)) <= 256) return cut;
+  float least = lin_plan(M, N, K, gated).us;
+  for (const LinTile &t : LIN_TILES) {
+    if (t.wn != 4) continue;
+    const int cols = 256 / half, rows = 64 * t.wm;
+    const long long nm = ((long long)M + rows - 1) / rows, nn = ((long long)N + cols - 1) / cols, full = nm * nn / 256 * 256;
+    if (full == 0 || full == nm * nn || (t.wm == 4 && K <= LT_K)) continue;
+    auto consider = [&](long long am, long long an) {
+      if (am < 1 || an < 1 || am > nm || an > nn || (am == nm && an == nn)) return;
+      const int m = am == nm ? M : (int)am * rows, n = an == nn ? N : (int)an * cols;
+      const float us = 3.f + lin_us(t, m, n, K, gated, am * an, 1) + lin_plan(m < M ? M - m : M, n < N ? N - n : N, K, gated).us;
+      if (us < least) { least = us; cut = LinCut{m, n}; }
+    };
+    consider(nm, full / nm);
+    consider(full / nn, nn);
+  }
+  return cut;
 }
 
 template <bool F16, bool GATED>
 static int lin_launch(const LinArgs &a, float *ws, hipStream_t s) {
   constexpr int NM = GATED ? 2 : 1;
   LinArgs t = a;
-  t.whole = !(((uintptr_t)a.y | (uintptr_t)a.ldy * (a.y32 ? 4 : 2) | (uintptr_t)a.res | (a.res ? (uintptr_t)a.ldr * 2 : 0)) & 15);
   const LinPlan pl = lin_plan(a.M, a.N, a.K, GATED);
   if (pl.wm == 0) {
     // rows of x in the operand beside pieces of K: more workgroups where 16 rows of W each would be fewer than two per compute unit
@@ -828,8 +858,13 @@ static int lin_launch(const LinArgs &a, float *ws, hipStream_t s) {
 }
 extern "C" int64_t moe_linear_workspace_bytes(int M, int N, int K, int gated) {
   if (M <= 0 || N <= 0 || K <= 0) return 0;
-  const LinPlan p = lin_plan(M, N, K, gated != 0);
-  return p.splits > 1 ? (int64_t)p.splits * (gated ? 2 : 1) * M * ((N + 7) & ~7) * 4 : 0;
+  auto bytes = [&](int m, int n) -> int64_t {
+    const LinPlan p = lin_plan(m, n, K, gated != 0);
+    return p.splits > 1 ? (int64_t)p.splits * (gated ? 2 : 1) * m * ((n + 7) & ~7) * 4 : 0;
+  };
+  const LinCut c = lin_cut(M, N, K, gated != 0);
+  if (c.M == M && c.N == N) return bytes(M, N);
+  return std::max(bytes(c.M, c.N), bytes(c.M < M ? M - c.M : M, c.N < N ? N - c.N : N));
 }
 
 template <bool GATED>
@@ -841,7 +876,27 @@ static int lin_run(const char *who, const LinArgs &a, int dtype, void *ws, int64
     moe_set_error("%s: a workspace of %lld bytes on a 16-byte boundary is needed", who, (long long)need);
     return MOE_EINVAL;
   }
-  return dtype == MOE_DT_FP16 ? lin_launch<true, GATED>(a, (float *)ws, s) : lin_launch<false, GATED>(a, (float *)ws, s);
+  auto launch = [&](const LinArgs &p) {
+    return dtype == MOE_DT_FP16 ? lin_launch<true, GATED>(p, (float *)ws, s) : lin_launch<false, GATED>(p, (float *)ws, s);
+  };
+  const LinCut c = lin_cut(a.M, a.N, a.K, GATED);
+  if (c.M == a.M && c.N == a.N) return launch(a);
+  LinArgs p = a;
+  p.M = c.M;
+  p.N = c.N;
+  if (int rc = launch(p)) return rc;
+  p = a;
+  const long long m = c.M < a.M ? c.M : 0, n = c.N < a.N ? c.N : 0;
+  p.M -= (int)m;
+  p.N -= (int)n;
+  p.x += m * a.ldx;
+  for (int i = 0; i < (GATED ? 2 : 1); ++i) {
+    p.w[i] += n * a.ldw;
+    if (p.bias[i]) p.bias[i] += n;
+  }
+  if (p.res) p.res += m * a.ldr + n;
+  p.y = (char *)a.y + (m * a.ldy + n) * (a.y32 ? 4 : 2);
+  return launch(p);
 }
 
 

@@ -129,6 +129,14 @@ def test_sizes_of_dense_layers(cuda, M, N, K, gated):
     run(cuda, M, N, K, torch.bfloat16, "silu" if gated else "none", False, not gated, gated)
 
 
+@pytest.mark.parametrize("M,N,K,gated", [(1184, 13754, 2112, False), (768, 10944, 2056, True), (4104, 4090, 2056, False), (4120, 2041, 1032, True),
+                                         (4090, 8203, 1032, False)])
+def test_products_cut_in_two_launches(cuda, M, N, K, gated):
+    """Whole rounds of the widest tile, and the columns or rows behind them."""
+    run(cuda, M, N, K, torch.bfloat16 if N % 2 else torch.float16, "silu" if gated else "none", True, not gated, gated, gap=8 * (N % 2))
+    run(cuda, M, N, K, torch.bfloat16, "none", False, False, gated, out_dtype=torch.float32)
+
+
 # Every tile on sizes that end inside it, with K whole and in pieces, and more tiles than workgroups of the widest one.
 @pytest.mark.parametrize("M,N,K,gated", [(130, 2049, 4104, False), (510, 4093, 4104, False), (450, 4099, 2056, False), (260, 2049, 10952, False), (512, 4099, 1032, False),
                                          (1030, 1023, 8200, False), (1000, 4099, 1032, False), (768, 2050, 10952, False), (2000, 4097, 520, False),
