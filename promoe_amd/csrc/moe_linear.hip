@@ -205,6 +205,8 @@ struct LinColumns {
 // the operand are 16 rows of W; with few rows of x (M <= 16 / SH) the operand is R rows of W by SH pieces of K, row s R + r and column
 // s R + m hold piece s of both, and the products of unlike pieces are left unread: a smaller unit of work (more workgroups for a
 // short matrix) and longer runs of a row per load.
+// Bound by HBM: 1 x 2048 x 10944 (45 MB) 10.5 us, 4.3 TB/s; gated 1 x 10944 x 2048 (90 MB) 20.4 us, 4.4 TB/s (a large copy: 5.2).  Twice the
+// loads in flight, 16 waves or non-temporal loads are no faster.
 #define LR_WAVES 8
 #define LR_U 4  // loads of a matrix in flight per wave, twice
 template <bool F16, bool GATED, int SH>
@@ -277,7 +279,9 @@ static __device__ __forceinline__ void lt_each(const F &f) {
 // ---- tile kernel --------------------------------------------------------------------------------------------------------------
 // Four waves (2 x 2), wave (wm, wn) on WM x WN blocks of 32 x 32: a tile of 64 WM rows of x by 64 WN rows of W.  A gated pair's W
 // blocks alternate between the two matrices (block b: matrix b & 1, its columns 32 (b >> 1) ..), so that a lane holds both sums
-// of a column.  K advances 64 at a time (a slab); slabs go global -> LDS directly, two of them in LDS.
+// of a column.  K advances 64 at a time (a slab); slabs go global -> LDS directly, RING of them in LDS.
+// Bound by LDS, 192 (WM + WN) cycles a slab for 128 WM WN of products, and by few workgroups: 24 x 4096 x 4096 12.7 us and 4 for the
+// join, 512 x 4096 x 4096 25.0 (687 TFLOP/s), gated 251 x 2560 x 3584 19.1 (482), 1024 x 4096 x 4096 38.1 (902).
 #define LT_K 64
 #define LT_ROW 128  // bytes of a row of a slab: 8 chunks of 16, chunk c of row r in slot c ^ ((r >> 1) & 7)
 template <bool F16>
@@ -455,6 +459,8 @@ __global__ __launch_bounds__(256, RING * (WM + WN) * 64 * LT_ROW > 80 * 1024 ? 1
 // that the products of a slab need: all 16 of a wave at once stopped the products for as long again (59 % busy matrix cores, then 74).
 // The run of slabs goes on from tile to tile: the next tile's first slab and the W half behind it land under the last products, and the
 // sums leave through the one place that nothing else needs then.
+// Bound by power: 4096 x 4096 x 14336 331 us (1455 TFLOP/s, 73 % busy matrix cores at 1.75 to 1.9 GHz; the library's product 305 - 315), gated 4096 x
+// 14336 x 4096 664 us (1449; the library's of both matrices, no gate, 622 - 640).
 template <bool F16, bool GATED>
 __global__ __launch_bounds__(256, 1) void k_linear_wide(const LinArgs a) {
   constexpr int B = 256, NT = 8, HALF = B * LT_ROW, NC = GATED ? B / 2 : B;
@@ -749,7 +755,7 @@ static int lin_check(const char *who, const LinArgs &a, int dtype, bool gated) {
 // rows; the chosen plan is 1.6 % slower than the best of all on average, 22 % at worst):
 //   rounds x (slabs x (c0 + c1 x share of the compute units in use) + f),  with pieces 2.5 + 0.33 a piece + 0.15 per MB of partial sums
 // c0, c1: a slab of a workgroup on an idle chip, and what the others' traffic adds; f: start and epilogue.  The narrow tiles are bound by
-// LDS (96 (wm + wn) bytes x rows read and written for 32 wm wn of products), the wide one by the matrix cores, at the power limit.
+// LDS (192 (wm + wn) cycles a slab for 128 wm wn of products), the wide one by the matrix cores, at the power limit.
 // us, best other tile / chosen: 64 x 4096 x 4096 14.7 / 12.9 (64 x 64, 3 pieces), 512 x 4096 x 4096 28.6 / 25.0 (64 x 128), 1024 x 4096 x
 // 4096 48.2 / 38.1 (128 x 128), 384 x 2048 x 10944 37.8 / 34.5 (128 x 128, 5 pieces), 2048 x 4096 x 4096 79.3 / 67.7 (128 x 256), 1536 x 2048 x
 // 10944 90.9 / 77.2 (256 x 256, 5 pieces); gated 128 x 14336 x 4096 70.2 / 56.8 (128 x 128), 2048 x 10944 x 2048 206 / 160 (256 x 256).

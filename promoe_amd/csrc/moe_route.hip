@@ -442,7 +442,8 @@ __global__ __launch_bounds__(256, V == 32 ? 4 : 8) void k_group_topk(const Group
   if (t0 < T) group_topk_four<V>(q, logits, ldl, t0, T, bias, lane, s_m[wv], idx, w, nullptr, nullptr);
 }
 
-// ---- with the stable dispatch of a decode batch in the same launch: one workgroup, a wave per token in turn --------------------
+// ---- with the stable dispatch of a decode batch in the same launch: one workgroup, a wave per four tokens -----------------------
+// Latency: 1 token of 64 experts 4.7 us, 33 of 256 10.6 us.
 #define GR_MAXT 64
 #define GR_MAXP 512
 struct GroupDispatch {
