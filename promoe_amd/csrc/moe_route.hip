@@ -167,7 +167,8 @@ static __device__ __forceinline__ void group_topk_token(const GroupRule &q, cons
 // Bound by the vector unit: 32768 tokens over 256 experts in 8 groups, a bias and sums of two take 28 us (36 MB: 7 us at a copy's rate), 1200
 // operations a wave of four.  A wave per token in 64 bits takes 67; experts dealt out one by one (16 r + lane), their indexes beside the
 // values and the groups' values through LDS 36 (1900 operations); no fours in order 30; 82 registers instead of 64, which cost the exact
-// form some in scratch, two waves fewer a SIMD and 2 us.
+// form some in scratch, two waves fewer a SIMD and 2 us; waves that go on to
+// further tokens, whose logits are on their way meanwhile, four a SIMD, 40.
 template <int N>
 static __device__ __forceinline__ float gr_ror(float x) {  // lane j: x of lane j - N within its 16
   return __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, x), 0x120 + N, 0xf, 0xf, true));
