@@ -751,26 +751,26 @@ static int lin_check(const char *who, const LinArgs &a, int dtype, bool gated) {
 }
 
 // Which kernel a product takes: few rows (wm 0), or tiles of 64 wm x 64 wn with `ring` slabs in LDS (4 x 4: the wide kernel) and K in
-// `splits` pieces.  The plan of the least time after a model of one launch, us, fitted to 2550 measured times of 100 shapes (33 to 4096
-// rows; the chosen plan is 1.6 % slower than the best of all on average, 22 % at worst):
-//   rounds x (slabs x (c0 + c1 x share of the compute units in use) + f),  with pieces 2.5 + 0.33 a piece + 0.15 per MB of partial sums
+// `splits` pieces.  The plan of the least time after a model of one launch, us, fitted to 8758 measured times of 160 shapes (24 to 4096
+// rows; matrices from memory and from the last cache; the chosen plan is 0.9 % slower than the best of all on average, 19 % at worst):
+//   rounds x (slabs x (c0 + c1 x share of the compute units in use) + f),  with pieces 1.6 + 0.43 a piece + 0.15 per MB of partial sums
 // c0, c1: a slab of a workgroup on an idle chip, and what the others' traffic adds; f: start and epilogue.  The narrow tiles are bound by
 // LDS (192 (wm + wn) cycles a slab for 128 wm wn of products), the wide one by the matrix cores, at the power limit.
-// us, best other tile / chosen: 64 x 4096 x 4096 14.7 / 12.9 (64 x 64, 3 pieces), 512 x 4096 x 4096 28.6 / 25.0 (64 x 128), 1024 x 4096 x
-// 4096 48.2 / 38.1 (128 x 128), 384 x 2048 x 10944 37.8 / 34.5 (128 x 128, 5 pieces), 2048 x 4096 x 4096 79.3 / 67.7 (128 x 256), 1536 x 2048 x
-// 10944 90.9 / 77.2 (256 x 256, 5 pieces); gated 128 x 14336 x 4096 70.2 / 56.8 (128 x 128), 2048 x 10944 x 2048 206 / 160 (256 x 256).
+// us with matrices from memory, best other tile / chosen: 64 x 4096 x 4096 16.4 / 13.9 (64 x 64, 4 pieces), 512 x 4096 x 4096 32.8 / 31.6 (64 x 128), 1024 x 4096 x
+// 4096 48.3 / 44.1 (128 x 128), 384 x 2048 x 10944 38.1 / 35.0 (128 x 128, 5 pieces), 2048 x 4096 x 4096 78.8 / 67.9 (128 x 256), 1536 x 2048 x
+// 10944 90.4 / 81.5 (256 x 256, 5 pieces); gated 128 x 14336 x 4096 66.1 / 57.4 (128 x 128), 2048 x 10944 x 2048 205 / 166 (256 x 256).
 // Few rows, us, k_linear_rows / best tile: 3 x 2048 x 10944 13.4 / 14.8, 8 x 4096 x 4096 11.2 / 11.5, 16 x 4096 x 4096 10.7 / 11.6, 8 x 2048 x
 // 1408 4.9 / 7.4, 16 x 2048 x 1408 6.0 / 7.4; past 8 rows a long reduction is faster on tiles in pieces (every workgroup reads all of x,
 // which no longer passes unnoticed beside the weights): 12 x 2048 x 10944 23.0 / 15.5, 16 x 4096 x 14336 37.7 / 27.9, and past 16 the tiles
 // are in general: 24 x 4096 x 4096 13.3 / 12.0, 24 gated 14336 x 4096 69 / 51.
 struct LinTile { int wm, wn, ring, per_cu; float c0, c1, f; };
-static const LinTile LIN_TILES[] = {{1, 1, 4, 2, 0.173f, 0.135f, 0.f}, {1, 2, 6, 1, 0.269f, 0.139f, 1.46f}, {2, 2, 4, 1, 0.380f, 0.221f, 2.2f},
-                                    {2, 4, 3, 1, 0.674f, 0.236f, 4.34f}, {4, 4, 5, 1, 1.146f, 0.f, 9.21f}};
+static const LinTile LIN_TILES[] = {{1, 1, 4, 2, 0.173f, 0.129f, 0.13f}, {1, 2, 6, 1, 0.233f, 0.139f, 1.38f}, {2, 2, 4, 1, 0.380f, 0.245f, 2.27f},
+                                    {2, 4, 3, 1, 0.636f, 0.221f, 4.34f}, {4, 4, 5, 1, 1.176f, 0.f, 9.52f}};
 static float lin_us(const LinTile &t, int M, int N, int K, bool gated, long long n, int s) {
   const long long slabs = (K + LT_K - 1) / LT_K, wgs = n * s, rounds = (wgs + 256 * t.per_cu - 1) / (256 * t.per_cu);
-  const float use = wgs >= 256 * t.per_cu ? (float)t.per_cu : (float)wgs / 256.f;
+  const float use = wgs > 256 ? (float)t.per_cu : (float)wgs / 256.f;  // (one compute unit with two workgroups is what a launch waits for)
   const float us = (float)rounds * ((float)((slabs + s - 1) / s) * (t.c0 + t.c1 * use) + t.f);
-  return s == 1 ? us : us + 2.5f + 0.33f * (float)s + 0.148e-6f * 8.f * (float)s * (gated ? 2.f : 1.f) * (float)M * (float)N;
+  return s == 1 ? us : us + 1.6f + 0.43f * (float)s + 0.151e-6f * 8.f * (float)s * (gated ? 2.f : 1.f) * (float)M * (float)N;
 }
 struct LinPlan { int wm, wn, ring, splits; float us; };
 static LinPlan lin_plan(int M, int N, int K, bool gated) {
