@@ -280,8 +280,9 @@ static __device__ __forceinline__ void lt_each(const F &f) {
 // Four waves (2 x 2), wave (wm, wn) on WM x WN blocks of 32 x 32: a tile of 64 WM rows of x by 64 WN rows of W.  A gated pair's W
 // blocks alternate between the two matrices (block b: matrix b & 1, its columns 32 (b >> 1) ..), so that a lane holds both sums
 // of a column.  K advances 64 at a time (a slab); slabs go global -> LDS directly, RING of them in LDS.
-// Bound by LDS, 192 (WM + WN) cycles a slab for 128 WM WN of products, and by few workgroups: 24 x 4096 x 4096 12.7 us and 4 for the
-// join, 512 x 4096 x 4096 25.0 (687 TFLOP/s), gated 251 x 2560 x 3584 19.1 (482), 1024 x 4096 x 4096 38.1 (902).
+// Bound by LDS, 192 (WM + WN) cycles a slab for 128 WM WN of products, and by few workgroups: 24 x 4096 x 4096 9.9 us and 3.8 for the
+// join; with matrices from the last cache 512 x 4096 x 4096 25.0 (687 TFLOP/s), gated 251 x 2560 x 3584 19.1 (482), 1024 x 4096 x 4096 38.1 (902);
+// from memory 31.6, 28.6 and 44.1.
 #define LT_K 64
 #define LT_ROW 128  // bytes of a row of a slab: 8 chunks of 16, chunk c of row r in slot c ^ ((r >> 1) & 7)
 template <bool F16>

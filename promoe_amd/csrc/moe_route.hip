@@ -444,7 +444,7 @@ __global__ __launch_bounds__(256, V == 32 ? 4 : 8) void k_group_topk(const Group
 }
 
 // ---- with the stable dispatch of a decode batch in the same launch: one workgroup, a wave per four tokens -----------------------
-// Latency: 1 token of 64 experts 4.7 us, 33 of 256 10.6 us.
+// Latency: 1 token of 64 experts 4.8 us, 33 of 256 10.9 us.
 #define GR_MAXT 64
 #define GR_MAXP 512
 struct GroupDispatch {
