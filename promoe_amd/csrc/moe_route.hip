@@ -314,7 +314,10 @@ static __device__ __forceinline__ void group_topk_quad(const GroupRule &q, const
     for (int k = 0; k < G; ++k) before += sv[k] > v;
     mine_kept = g < G && before < q.keep;
     const float least = -gr_max16(mine_kept ? -v : -INF), most = gr_max16(g < G && !mine_kept ? v : -INF);
-    // (a sum of two is off by twice as much; equal values, NaN and two infinities are not sure)
+    // (more groups than stay where those at the border are equal: each has fewer than `keep` in front of it)
+    const unsigned heads = (unsigned)(__ballot(mine_kept && part0 == 0) >> (16 * tok)) & 0xffffu;
+    sure = sure && __popc(heads) == q.keep;
+    // (a sum of two is off by twice as much; NaN and two infinities are not sure)
     sure = sure && least - most > 2.f * unsure_abs + unsure_rel * (fabsf(least) + fabsf(most));
     if (by_logit) sure = sure && least > (q.sigmoid ? -700.f : top - 700.f);
   }

@@ -1,0 +1,55 @@
+"""Which groups stay where their values are hard to tell apart: group_topk and its dispatch against the definition in 64 bits (whole
+numbers equal, weights off by their one rounding to fp32)."""
+import numpy as np
+import pytest
+import torch
+
+from oracle import route_oracle as R
+
+pytestmark = pytest.mark.gpu
+
+
+def _many(lg, k, kind, bias, G, keep, renorm=False):
+    """The oracle's route for groups worth their two largest, all rows at once: (idx, w)."""
+    s = R.scores(lg, kind)
+    T, E = s.shape
+    c = s + bias.astype(np.float64)
+    g = np.sort(c.reshape(T, G, E // G), axis=2)
+    order = np.argsort(-(g[:, :, -1] + g[:, :, -2]), axis=1, kind="stable")[:, :keep]
+    kept = np.zeros((T, G), bool)
+    np.put_along_axis(kept, order, True, axis=1)
+    idx = np.argsort(-np.where(np.repeat(kept, E // G, axis=1), c, -np.inf), axis=1, kind="stable")[:, :k]
+    w = np.take_along_axis(s, idx, axis=1)
+    return idx.astype(np.int32), w / w.sum(axis=1, keepdims=True) if renorm else w
+
+
+def _check(lg, k, kind, bias, G, keep, dev):
+    from promoe_amd import ops
+    rule = ops.RouteRule(kind, G, keep, "top2")
+    ld, bd = torch.from_numpy(lg).to(dev), torch.from_numpy(bias).to(dev)
+    ridx, rw = _many(lg, k, kind, bias, G, keep)
+    for a, b in zip(_many(lg[:6], k, kind, bias, G, keep), R.route(lg[:6], k, kind, bias, G, keep, "top2")):
+        assert np.array_equal(a, b)
+    n = min(len(lg), 64, 512 // k)
+    for idx, w in (ops.group_topk(ld, k, rule, bd), ops.group_topk_dispatch(ld[:n], k, rule, bd)[:2]):
+        idx, w = idx.cpu().numpy(), w.cpu().numpy().astype(np.float64)
+        bad = (idx != ridx[: len(idx)]).any(axis=1)
+        assert not bad.any(), "%d of %d rows" % (bad.sum(), len(idx))
+        assert (np.abs(w - rw[: len(w)]) <= 2.0 ** -24 * 1.001 * rw[: len(w)] + 2.0 ** -149).all()
+
+
+@pytest.mark.parametrize("kind", ["sigmoid", "softmax"])
+@pytest.mark.parametrize("E,k,G,keep", [(16, 1, 8, 1), (16, 2, 8, 4), (24, 3, 3, 1), (60, 4, 6, 3), (256, 8, 8, 4), (32, 4, 16, 5),
+                                        (128, 2, 64, 7)])
+def test_groups_of_equal_value(cuda, E, k, G, keep, kind):
+    """Sums that are equal although what they are made of is not (3 + 2, 4 + 1), at the border between the groups that stay and the
+    others: the lower group stays, and one expert more or less would be chosen with the other."""
+    print(f"case group_equal {E} {k} {G} {keep} {kind}", flush=True)
+    for seed in range(24):
+        rng = np.random.default_rng(seed)
+        bias = (rng.integers(-8, 9, E) * 0.5).astype(np.float32)
+        # (scores of zero, one half and one; softmax: all the same, or one expert's alone)
+        lg = rng.choice(np.array([0.0, 200.0, -200.0], np.float32), (65, E))
+        if kind == "softmax":
+            lg[::2] = 0.0
+        _check(lg, k, kind, bias, G, keep, cuda)
