@@ -162,8 +162,9 @@ static __device__ __forceinline__ void group_topk_token(const GroupRule &q, cons
 // choices, and any other one again through group_topk_token: equal values, values next to a border (under 2 % of random tokens), rows of
 // masks, infinities.  Without a bias (and sums of two) the logits themselves are ordered.  Weights are in 64 bits either way.
 // What 32 bits can be wrong by: sigmoid s (1 - s) (|l| 2^-24 + 2^-23) for 2^x and 2^-23 for the reciprocal, together under 2^-22; softmax 2^-20 of the
-// row's largest probability (nine additions one after the other, 2^x, the quotient); the bias added 2^-24 of the sum; the place in the
-// lane's run, which the ordered value carries in its last bits, V 2^-23 of it.
+// row's largest probability (nine additions one after the other, 2^x, the quotient); the bias added 2^-24 of the sum c; a group's
+// value as a sum a + b of two such c 2^-24 (|a| + |b| + |a + b|), whatever cancels in it; the place in the lane's run, which the
+// ordered value carries in its last bits, V 2^-23 of it.
 // Bound by the vector unit: 32768 tokens over 256 experts in 8 groups, a bias and sums of two take 28 us (36 MB: 7 us at a copy's rate), 1200
 // operations a wave of four.  A wave per token in 64 bits takes 67; experts dealt out one by one (16 r + lane), their indexes beside the
 // values and the groups' values through LDS 36 (1900 operations); no fours in order 30; 82 registers instead of 64, which cost the exact
@@ -317,8 +318,10 @@ static __device__ __forceinline__ void group_topk_quad(const GroupRule &q, const
     // (more groups than stay where those at the border are equal: each has fewer than `keep` in front of it)
     const unsigned heads = (unsigned)(__ballot(mine_kept && part0 == 0) >> (16 * tok)) & 0xffffu;
     sure = sure && __popc(heads) == q.keep;
-    // (a sum of two is off by twice as much; NaN and two infinities are not sure)
-    sure = sure && least - most > 2.f * unsure_abs + unsure_rel * (fabsf(least) + fabsf(most));
+    // (a sum of two is off by twice as much, and with a bias by a part of what it is the sum of, which can be far more than the sum:
+    // 1000.4 - 999.8; NaN and two infinities are not sure)
+    const float size_of = q.top2 && bias ? gr_max16(g < G ? fabsf(a) + fabsf(b) : 0.f) : fabsf(least) + fabsf(most);
+    sure = sure && least - most > 2.f * unsure_abs + unsure_rel * size_of;
     if (by_logit) sure = sure && least > (q.sigmoid ? -700.f : top - 700.f);
   }
   // k + 1 rounds of the largest value; lane i keeps choice i (two of them past 16 choices).  The place in the run in the last bits.

@@ -53,3 +53,32 @@ def test_groups_of_equal_value(cuda, E, k, G, keep, kind):
         if kind == "softmax":
             lg[::2] = 0.0
         _check(lg, k, kind, bias, G, keep, cuda)
+
+
+@pytest.mark.parametrize("kind", ["sigmoid", "softmax"])
+@pytest.mark.parametrize("size", [2, 4, 32])
+def test_biases_of_both_signs(cuda, size, kind):
+    """A group's two largest are one of a large positive and one of a large negative bias (the others are behind both), so that
+    its value is what 32 bits have lost of them."""
+    T, G, keep = 65536, 8, 4
+    for big in (1.0, 16.0, 64.0, 256.0, 1e3, 1e4, 1e5, 1e6):
+        print(f"case group_cancel size={size} {kind} bias={big}", flush=True)
+        rng = np.random.default_rng(size)
+        lg = rng.normal(0, 1.2, (T, G * size)).astype(np.float32)
+        sign = np.full((G, size), -3.0)
+        sign[:, :2] = (1.0, -1.0)
+        bias = (sign * big + rng.normal(0, 0.05, (G, size))).astype(np.float32).reshape(-1)
+        _check(lg, 4, kind, bias, G, keep, cuda)
+
+
+def test_infinite_biases(cuda):
+    """-inf takes an expert out of the choice (of its group's value too), one +inf puts a group in front, two of them are equal
+    groups: the lower one."""
+    print("case group_infinite", flush=True)
+    rng = np.random.default_rng(4)
+    lg = rng.normal(0, 1.2, (300, 64)).astype(np.float32)
+    for at, v in (((3, 17, 40), -np.inf), ((9,), np.inf), ((9, 33), np.inf), ((9, 33, 50), np.inf)):
+        bias = rng.normal(0, 0.05, 64).astype(np.float32)
+        bias[list(at)] = v
+        for keep in (1, 2, 5):
+            _check(lg, 4, "sigmoid", bias, 8, keep, cuda)
