@@ -98,6 +98,8 @@ def _route_args(what, logits, k, rule, bias):
         raise L.MoeError("%s: logits must be fp32 [T, E] with the experts of a row side by side" % what)
     if not isinstance(rule, L.RouteRule):
         raise L.MoeError("%s: rule must be a RouteRule" % what)
+    if logits.shape[0] > 1 and logits.stride(0) >= 1 << 31:
+        raise L.MoeError("%s: rows of logits %d floats apart (fewer than 2^31 are needed)" % (what, logits.stride(0)))
     index = _operands(what, logits, bias)
     T, E = logits.shape
     if bias is not None and (bias.dtype != torch.float32 or bias.shape != (E,) or not bias.is_contiguous()):
