@@ -78,6 +78,11 @@ def _route_rule(block):
             raise NotImplementedError("a selection bias on scores of kind %r (only 'sigmoid' is supported)" % (kind,))
         return ops.RouteRule("sigmoid", int(find("n_group", "num_group")), int(find("topk_group")), "top2",
                              bool(find("norm_topk_prob")), float(find("routed_scaling_factor"))), bias
+    if isinstance(block, torch.nn.Module):                   # (on the block or deeper in the gate: routers of other forms, some on softmax)
+        other = [n for n in block.state_dict() if n.rsplit(".", 1)[-1] == "e_score_correction_bias"]
+        if other:
+            raise NotImplementedError("a block of class %s with a selection bias at %s (only one on the gate itself is supported)"
+                                      % (type(block).__name__, other[0]))
     if getattr(gate, "topk_method", None) == "group_limited_greedy":
         if getattr(gate, "norm_topk_prob", False):           # (transformers' own router does not divide by the sum; others do)
             raise NotImplementedError("norm_topk_prob with 'group_limited_greedy'")
