@@ -168,6 +168,9 @@ def inject_model(model, device="cuda:0", fmt: str = "bf16", max_tokens: int = 40
     blocks = find_moe_blocks(model)
     if not blocks:
         raise ValueError("the model has no sparse MoE block with fused expert tensors")
+    # (every router is read before the first weight moves: a model that is refused stays as it was)
+    rules = [_route_rule(blk) for _, blk in blocks]
+    modes = [L.ROUTE_SOFTMAX_TOPK if r is not None else _route_mode(blk) for (r, _), (_, blk) in zip(rules, blocks)]
     b0 = blocks[0][1]
     E, two_i, H = b0.experts.gate_up_proj.shape
     I = two_i // 2
@@ -193,7 +196,7 @@ def inject_model(model, device="cuda:0", fmt: str = "bf16", max_tokens: int = 40
         # DeepSeek scales the routed experts' sum by a constant; it goes into their down projections (multiplied in
         # fp32, before the one rounding to bf16 / the quantisation of the image)
         # (a layer with a routing rule has it in its weights)
-        scale = 1.0 if _route_rule(blk)[0] is not None else float(getattr(blk.gate, "routed_scaling_factor", 1.0) or 1.0)
+        scale = 1.0 if rules[l][0] is not None else float(getattr(blk.gate, "routed_scaling_factor", 1.0) or 1.0)
         for e in range(E):
             img = _expert_image(gu[e, :I], gu[e, I:], dn[e] if scale == 1.0 else dn[e].detach().float() * scale, H, I, fmt)
             base = (l * E + e) * total
@@ -208,7 +211,7 @@ def inject_model(model, device="cuda:0", fmt: str = "bf16", max_tokens: int = 40
                 for lin in (sh.gate_proj, sh.up_proj, sh.down_proj):
                     lin.weight = torch.nn.Parameter(torch.empty(0), requires_grad=False)
     # (a selection bias keeps its 32 bits)
-    rules = [(r, None if b is None else b.detach().float().to(device)) for r, b in (_route_rule(blk) for _, blk in blocks)]
+    rules = [(r, None if b is None else b.detach().float().to(device)) for r, b in rules]
     model.to(device=device, dtype=torch.bfloat16)
     torch.cuda.set_device(device)
     # a stream of torch's own is handed over as it is; from the legacy default stream (handle 0) the
@@ -239,9 +242,8 @@ def inject_model(model, device="cuda:0", fmt: str = "bf16", max_tokens: int = 40
         if sg is not None:
             gw = torch.cat([gw, sg.weight.detach().to(torch.bfloat16).reshape(1, H)])
         sh = None if shared_imgs[l] is None else torch.from_numpy(np.ascontiguousarray(shared_imgs[l])).to(device)
-        pm.set_layer(l, H, I, I_sh, top_k, L.ROUTE_SOFTMAX_TOPK if rules[l][0] is not None else _route_mode(blk), gw.contiguous(), None,
-                     sh, shared_gated=sg is not None, fmt=L.FMT_BF16 if fmt == "bf16" else L.FMT_INT4_G128, rule=rules[l][0],
-                     select_bias=rules[l][1])
+        pm.set_layer(l, H, I, I_sh, top_k, modes[l], gw.contiguous(), None, sh, shared_gated=sg is not None,
+                     fmt=L.FMT_BF16 if fmt == "bf16" else L.FMT_INT4_G128, rule=rules[l][0], select_bias=rules[l][1])
     pm.forward_prepare(max_tokens)
     pm.launch_thread()
 

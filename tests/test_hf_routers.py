@@ -100,3 +100,20 @@ def test_stock_blocks_are_described_as_they_are(name, more):
             y = b(x[None])
             y = (y[0] if isinstance(y, tuple) else y).reshape(40, 64)
             assert float((_described(b, x) - y).abs().max()) <= 1e-4 * float(y.abs().max())
+
+
+@pytest.mark.parametrize("case", ["bias on the block", "unknown method"])
+def test_a_refused_model_stays_as_it_was(case):
+    """The first block could be injected, the last one not: nothing of the model has moved or been dropped when the refusal comes."""
+    from promoe_amd import hf
+    model, blocks = _blocks("DeepseekV2")
+    if case == "unknown method":
+        blocks[-1].gate.topk_method = "other"
+    else:
+        blocks[-1].register_buffer("e_score_correction_bias", torch.zeros(16))
+    before = {n: t.clone() for n, t in model.state_dict().items()}
+    with pytest.raises(NotImplementedError):
+        hf.inject_model(model, device="cpu")
+    after = model.state_dict()
+    assert list(after) == list(before) and all(torch.equal(after[n], t) and after[n].dtype == t.dtype for n, t in before.items())
+    assert not any("forward" in vars(b) for b in blocks)
