@@ -54,6 +54,10 @@ def _route_mode(block) -> int:
             raise NotImplementedError("DeepSeek routing method %r (only 'greedy' and 'group_limited_greedy' top-k are supported)"
                                       % gate.topk_method)
         return L.ROUTE_SOFTMAX_TOPK
+    groups, keep = (next((getattr(o, n) for o in (gate, block) for n in names if getattr(o, n, None) is not None), 1)
+                    for names in (("num_group", "n_group"), ("topk_group",)))
+    if keep < groups:                                        # (what a group is worth is not to be told from a name)
+        raise NotImplementedError("a router of class %s that keeps %d of %d groups of experts" % (type(gate).__name__, keep, groups))
     if hasattr(gate, "norm_topk_prob"):                      # Qwen2-MoE router
         return L.ROUTE_SOFTMAX_TOPK_RENORM if gate.norm_topk_prob else L.ROUTE_SOFTMAX_TOPK
     return L.ROUTE_TOPK_SOFTMAX                              # Mixtral: renormalised top-k of the softmax

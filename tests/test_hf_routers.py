@@ -117,3 +117,15 @@ def test_a_refused_model_stays_as_it_was(case):
     after = model.state_dict()
     assert list(after) == list(before) and all(torch.equal(after[n], t) and after[n].dtype == t.dtype for n, t in before.items())
     assert not any("forward" in vars(b) for b in blocks)
+
+
+def test_groups_whose_value_is_unknown_are_refused():
+    from promoe_amd import hf
+    for name, more in (("Mistral4", dict(norm_topk_prob=True)), ("Mistral4", dict(norm_topk_prob=False))):
+        model, blocks = _blocks(name, **more)
+        for b in blocks:
+            assert hf._route_rule(b) == (None, None)
+            with pytest.raises(NotImplementedError, match="2 of 4 groups"):
+                hf._route_mode(b)
+        model, blocks = _blocks(name, n_group=1, topk_group=1, **more)
+        assert hf._route_mode(blocks[0]) == int(more["norm_topk_prob"])
