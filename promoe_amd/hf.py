@@ -47,6 +47,14 @@ def find_moe_blocks(model):
     return out
 
 
+def _check_parts(name, block):
+    """Refuses a block with weights that the engine's layer has no place for."""
+    known = {"gate", "experts", "shared_expert", "shared_experts", "shared_expert_gate"}
+    more = [n for n, m in block.named_children() if n not in known and m.state_dict()]
+    if more:
+        raise NotImplementedError("block %s of class %s has weights of its own in %s" % (name, type(block).__name__, ", ".join(more)))
+
+
 def _route_mode(block) -> int:
     gate = block.gate
     if hasattr(gate, "topk_method"):                         # DeepSeek router
@@ -173,6 +181,8 @@ def inject_model(model, device="cuda:0", fmt: str = "bf16", max_tokens: int = 40
     if not blocks:
         raise ValueError("the model has no sparse MoE block with fused expert tensors")
     # (every router is read before the first weight moves: a model that is refused stays as it was)
+    for name, blk in blocks:
+        _check_parts(name, blk)
     rules = [_route_rule(blk) for _, blk in blocks]
     modes = [L.ROUTE_SOFTMAX_TOPK if r is not None else _route_mode(blk) for (r, _), (_, blk) in zip(rules, blocks)]
     b0 = blocks[0][1]

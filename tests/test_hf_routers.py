@@ -129,3 +129,17 @@ def test_groups_whose_value_is_unknown_are_refused():
                 hf._route_mode(b)
         model, blocks = _blocks(name, n_group=1, topk_group=1, **more)
         assert hf._route_mode(blocks[0]) == int(more["norm_topk_prob"])
+
+
+@pytest.mark.parametrize("name,part", [("AXK1", "post_mlp_layernorm"), ("DeepseekV2", "norm")])
+def test_a_block_with_further_weights_is_refused(name, part):
+    """A norm behind the experts, say: the injected forward would leave it out."""
+    from promoe_amd import hf
+    model, blocks = _blocks(name)
+    if name == "DeepseekV2":
+        blocks[-1].act = nn.SiLU()                               # (a part without weights is none)
+        hf._check_parts("mlp", blocks[-1])
+        blocks[-1].norm = nn.LayerNorm(64)
+    with pytest.raises(NotImplementedError, match=part):
+        hf.inject_model(model, device="cpu")
+    assert blocks[0].experts.gate_up_proj.numel()
