@@ -105,13 +105,15 @@ def _route_rule(block):
 
 def _activation_of(fn):
     """The name under which ops.linear_gated has a module's activation, from its values; None for any other."""
-    x = torch.tensor([-3.0, -1.5, -0.4, 0.3, 1.25, 2.5], dtype=torch.float64)
+    # (all over the range, not only where activations bend: clipped ones are others)
+    far = torch.tensor([15.0, 20.0, 30.0, 50.0, 1e2, 1e3, 1e4, 1e5, 1e10, 1e30], dtype=torch.float64)
+    x = torch.cat([torch.linspace(-12.0, 12.0, 193, dtype=torch.float64), far, -far])
     known = {"silu": torch.nn.functional.silu(x), "gelu": torch.nn.functional.gelu(x),
              "gelu_tanh": torch.nn.functional.gelu(x, approximate="tanh"), "relu": x.relu(), "relu2": x.relu() ** 2}
     try:
         with torch.no_grad():
             y = fn(x.clone())
-        return next((n for n, v in known.items() if torch.allclose(y, v, rtol=0, atol=1e-6)), None)
+        return next((n for n, v in known.items() if torch.allclose(y, v, rtol=1e-6, atol=1e-6)), None)
     except Exception:                                        # (one with parameters of another type or device, say)
         return None
 
