@@ -118,10 +118,53 @@ def _activation_of(fn):
         return None
 
 
+class _StandIn(torch.nn.Module):
+    """In place of a Linear of the same sizes: column j of the result is the sum of columns j, j + n_out, .. of x, each with a factor."""
+
+    def __init__(self, n_in, n_out, seed, device):
+        super().__init__()
+        gen = torch.Generator().manual_seed(seed)
+        self.in_features, self.out_features, self.rows = n_in, n_out, -(-n_in // n_out)
+        self.factor = (1.0 + torch.rand(max(n_in, n_out), dtype=torch.float64, generator=gen)).to(device)
+        self.factor[1::2] *= -1.0
+        self.weight, self.bias = torch.empty(0, dtype=torch.float64, device=device), None  # (what asks for more of it than its type fails)
+
+    def forward(self, x):
+        if self.out_features > self.in_features:
+            at = torch.arange(self.out_features, device=x.device) % self.in_features
+            return x[..., at] * self.factor
+        x = torch.nn.functional.pad(x * self.factor, (0, self.rows * self.out_features - self.in_features))
+        return x.unflatten(-1, (self.rows, self.out_features)).sum(-2)
+
+
+def _is_gated_mlp(mod) -> bool:
+    """Does the class's forward compute down(act(gate(x)) * up(x)) and nothing else?  It is run in 64 bits on rows of small and large
+    values, over stand-ins for the three products: a factor, a clip or a selection among the columns shows."""
+    names = ("gate_proj", "up_proj", "down_proj")
+    device = mod.gate_proj.weight.device
+    probe = type(mod).__new__(type(mod))
+    probe.__dict__.update(mod.__dict__)
+    probe.__dict__["_modules"] = dict(mod._modules)
+    for i, n in enumerate(names):
+        p = getattr(mod, n)
+        probe._modules[n] = _StandIn(p.in_features, p.out_features, i, device)
+    gen = torch.Generator().manual_seed(7)
+    scale = torch.tensor([1e-2, 1.0, 5.0, 30.0, 1e3, 1e5], dtype=torch.float64)[:, None]
+    x = (torch.randn(6, mod.gate_proj.in_features, dtype=torch.float64, generator=gen) * scale).reshape(2, 3, -1).to(device)
+    try:
+        with torch.no_grad():
+            y = type(mod).forward(probe, x.clone())
+            ref = probe.down_proj(mod.act_fn(probe.gate_proj(x)) * probe.up_proj(x))
+        return y.shape == ref.shape and bool(((y - ref).abs() <= 1e-6 * ref.abs().amax(-1, keepdim=True)).all())
+    except Exception:                                        # (a forward that needs the weights themselves, or other arguments)
+        return False
+
+
 def find_dense_mlps(model):
     """[(qualified name, module, activation)] of the dense gated feed-forward layers (gate_proj, up_proj, down_proj and act_fn, nothing
-    else) that are no part of a sparse block and whose shapes and activation the fused products take.  Layers whose products are
-    not plain ones (subclasses of Linear: quantised or with adapters; hooks; a forward put in place of the class's) are left."""
+    else) that are no part of a sparse block and whose shapes, activation and forward are those of the fused products.  Layers whose
+    products are not plain ones (subclasses of Linear: quantised or with adapters; hooks; a forward put in place of the class's) are
+    left."""
     inside = {id(m) for _, blk in find_moe_blocks(model) for m in blk.modules()}
     out = []
     for name, mod in model.named_modules():
@@ -134,7 +177,7 @@ def find_dense_mlps(model):
         g, u, d = parts
         act = _activation_of(getattr(mod, "act_fn", None))
         if act and g.weight.shape == u.weight.shape and d.weight.shape == g.weight.shape[::-1] and d.in_features % 8 == 0 \
-                and g.in_features % 8 == 0:
+                and g.in_features % 8 == 0 and _is_gated_mlp(mod):
             out.append((name, mod, act))
     return out
 

@@ -35,3 +35,39 @@ def test_activations_of_transformers(monkeypatch):
     known = {"silu": "silu", "swish": "silu", "gelu": "gelu", "gelu_new": "gelu_tanh", "gelu_pytorch_tanh": "gelu_tanh", "relu": "relu", "relu2": "relu2"}
     known = {n: a for n, a in known.items() if n in acts}
     assert _found(monkeypatch, **{n: Mlp(act=acts[n]) for n in known}) == known
+
+
+def _mlp(forward, **attrs):
+    m = type("M", (Mlp,), {"forward": forward})()
+    for n, v in attrs.items():
+        setattr(m, n, v)
+    return m
+
+
+def test_a_forward_of_another_form_is_left(monkeypatch):
+    """Factors, clips and selections that are plain attributes of the module or constants of its class."""
+    others = dict(
+        factor=_mlp(lambda s, x: s.down_proj(s.act_fn(s.gate_proj(x) * s.m) * s.up_proj(x)), m=1.01),
+        out_factor=_mlp(lambda s, x: s.down_proj(s.act_fn(s.gate_proj(x)) * s.up_proj(x)) * s.m, m=nn.Parameter(torch.tensor(0.5))),
+        clip_gate=_mlp(lambda s, x: s.down_proj(s.act_fn(s.gate_proj(x).clamp(max=s.limit)) * s.up_proj(x)), limit=10.0),
+        clip_up=_mlp(lambda s, x: s.down_proj(s.act_fn(s.gate_proj(x)) * s.up_proj(x).clamp(-7, 7))),
+        up_plus_one=_mlp(lambda s, x: s.down_proj(s.act_fn(s.gate_proj(x)) * (s.up_proj(x) + 1))),
+        swapped=_mlp(lambda s, x: s.down_proj(s.act_fn(s.up_proj(x)) * s.gate_proj(x))),
+        added=_mlp(lambda s, x: x + s.down_proj(s.act_fn(s.gate_proj(x)) * s.up_proj(x))),
+        sparse=_mlp(lambda s, x: s.down_proj(s.act_fn(F.relu(s.gate_proj(x) - s.gate_proj(x).std(-1, keepdim=True))) * s.up_proj(x))),
+        last_column=_mlp(lambda s, x: s.down_proj(torch.cat([(h := s.act_fn(s.gate_proj(x)) * s.up_proj(x))[..., :-1], 0 * h[..., -1:]], -1))),
+        more_arguments=_mlp(lambda s, x, y: s.down_proj(s.act_fn(s.gate_proj(x)) * s.up_proj(x)) + y),
+        pair=_mlp(lambda s, x: (s.down_proj(s.act_fn(s.gate_proj(x)) * s.up_proj(x)), None)),
+        by_weight=_mlp(lambda s, x: s.down_proj(s.act_fn(F.linear(x, s.gate_proj.weight)) * s.up_proj(x))),
+    )
+    assert _found(monkeypatch, **others) == {}
+    same = dict(up_first=_mlp(lambda s, x: s.down_proj(s.up_proj(x) * s.act_fn(s.gate_proj(x)))),
+                typed=_mlp(lambda s, x: s.down_proj(s.act_fn(s.gate_proj(x.to(s.gate_proj.weight.dtype))) * s.up_proj(x))),
+                rows=_mlp(lambda s, x: s.down_proj(s.act_fn(s.gate_proj(x.reshape(-1, x.shape[-1]))) * s.up_proj(x.reshape(-1, x.shape[-1]))).view(x.shape)),
+                narrow=Mlp(H=64, I=24), bf16=Mlp().to(torch.bfloat16), short=Mlp(I=40))
+    assert _found(monkeypatch, **same) == {n: "silu" for n in same}
+    # (nothing of the module has changed)
+    m = Mlp()
+    before = {n: t.clone() for n, t in m.state_dict().items()}
+    _found(monkeypatch, m=m)
+    assert type(m.gate_proj) is nn.Linear and all(torch.equal(m.state_dict()[n], t) for n, t in before.items())
