@@ -160,6 +160,11 @@ def _is_gated_mlp(mod) -> bool:
         return False
 
 
+def _is_plain(m) -> bool:
+    """Would calling the module (or function) run its class's forward and nothing else?"""
+    return not isinstance(m, torch.nn.Module) or not (m._forward_hooks or m._forward_pre_hooks or "forward" in vars(m))
+
+
 def find_dense_mlps(model):
     """[(qualified name, module, activation)] of the dense gated feed-forward layers (gate_proj, up_proj, down_proj and act_fn, nothing
     else) that are no part of a sparse block and whose shapes, activation and forward are those of the fused products.  Layers whose
@@ -171,7 +176,7 @@ def find_dense_mlps(model):
         parts = [getattr(mod, n, None) for n in ("gate_proj", "up_proj", "down_proj")]
         if id(mod) in inside or not all(type(p) is torch.nn.Linear for p in parts):
             continue
-        if any("forward" in vars(m) or m._forward_hooks or m._forward_pre_hooks for m in parts) or "forward" in vars(mod) \
+        if not all(_is_plain(m) for m in (*parts, getattr(mod, "act_fn", None))) or "forward" in vars(mod) \
                 or set(dict(mod.named_children())) - {"gate_proj", "up_proj", "down_proj", "act_fn"}:
             continue
         g, u, d = parts

@@ -71,3 +71,12 @@ def test_a_forward_of_another_form_is_left(monkeypatch):
     before = {n: t.clone() for n, t in m.state_dict().items()}
     _found(monkeypatch, m=m)
     assert type(m.gate_proj) is nn.Linear and all(torch.equal(m.state_dict()[n], t) for n, t in before.items())
+
+
+def test_a_hook_on_the_activation_is_left(monkeypatch):
+    hooked, early, replaced = Mlp(), Mlp(), Mlp()
+    hooked.act_fn.register_forward_hook(lambda m, a, y: 2 * y)
+    seen = []
+    early.act_fn.register_forward_pre_hook(lambda m, a: seen.append(a[0].shape))
+    replaced.act_fn.forward = lambda x: F.silu(x)
+    assert _found(monkeypatch, hooked=hooked, early=early, replaced=replaced, fine=Mlp(), function=Mlp(act=F.silu)) == {"fine": "silu", "function": "silu"}
