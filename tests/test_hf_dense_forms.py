@@ -74,7 +74,7 @@ def test_a_forward_of_another_form_is_left(monkeypatch):
 
 
 def test_a_hook_on_the_activation_is_left(monkeypatch):
-    hooked, early, replaced = Mlp(), Mlp(), Mlp()
+    hooked, early, replaced = (Mlp(act=nn.SiLU()) for _ in range(3))  # (an activation of its own each)
     hooked.act_fn.register_forward_hook(lambda m, a, y: 2 * y)
     seen = []
     early.act_fn.register_forward_pre_hook(lambda m, a: seen.append(a[0].shape))
