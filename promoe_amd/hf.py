@@ -187,8 +187,12 @@ def find_dense_mlps(model):
     return out
 
 
-def _fused_mlp_forward(act):
+def _fused_mlp_forward(act, act_fn):
     def forward(self, x):
+        # (what has been put on or in place of a part since, an adapter or a hook say, has its effect: the class's own forward)
+        if self.act_fn is not act_fn or not _is_plain(act_fn) or \
+                not all(type(p) is torch.nn.Linear and _is_plain(p) for p in (self.gate_proj, self.up_proj, self.down_proj)):
+            return type(self).forward(self, x)
         # (detached, as the engine's own blocks are: nothing here has a gradient)
         w = [None if t is None else t.detach() for p in (self.gate_proj, self.up_proj, self.down_proj) for t in (p.weight, p.bias)]
         h = ops.linear_gated(x.detach().reshape(-1, x.shape[-1]), w[0], w[2], w[1], w[3], act=act)
@@ -326,6 +330,6 @@ def inject_model(model, device="cuda:0", fmt: str = "bf16", max_tokens: int = 40
         blk.forward = types.MethodType(make_forward(l), blk)
     if fuse_dense:
         for _, mod, act in find_dense_mlps(model):
-            mod.forward = types.MethodType(_fused_mlp_forward(act), mod)
+            mod.forward = types.MethodType(_fused_mlp_forward(act, mod.act_fn), mod)
     model._prefetch_mngr = pm
     return pm

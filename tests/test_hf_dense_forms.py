@@ -80,3 +80,62 @@ def test_a_hook_on_the_activation_is_left(monkeypatch):
     early.act_fn.register_forward_pre_hook(lambda m, a: seen.append(a[0].shape))
     replaced.act_fn.forward = lambda x: F.silu(x)
     assert _found(monkeypatch, hooked=hooked, early=early, replaced=replaced, fine=Mlp(), function=Mlp(act=F.silu)) == {"fine": "silu", "function": "silu"}
+
+
+def test_what_is_changed_after_the_injection_has_its_effect(monkeypatch):
+    """Hooks, replaced parts and forwards put on a fused layer later: the class's own forward runs, and the fused products again when
+    they are gone."""
+    import types
+
+    from promoe_amd import hf
+    calls = []
+
+    def gated(x, wg, wu, bg, bu, act):
+        calls.append("gated")
+        return F.silu(F.linear(x, wg, bg)) * F.linear(x, wu, bu)
+    monkeypatch.setattr(hf.ops, "linear_gated", gated)
+    monkeypatch.setattr(hf.ops, "linear", F.linear)
+    torch.manual_seed(2)
+    mlp, x = Mlp(act=nn.SiLU()), torch.randn(2, 5, 32)
+    plain = mlp(x).detach()
+    mlp.forward = types.MethodType(hf._fused_mlp_forward("silu", mlp.act_fn), mlp)
+
+    def fused():
+        calls.clear()
+        y = mlp(x)
+        return y.detach(), bool(calls)
+
+    def unchanged():
+        y, f = fused()
+        return f and torch.allclose(y, plain, atol=1e-6)
+    assert unchanged()
+    for part in ("gate_proj", "up_proj", "down_proj", "act_fn"):
+        handle = getattr(mlp, part).register_forward_hook(lambda m, a, y: 2 * y)
+        y, f = fused()
+        assert not f and torch.allclose(y, 2 * plain, atol=1e-5) == (part != "gate_proj")
+        handle.remove()
+        assert unchanged()
+    handle = mlp.up_proj.register_forward_pre_hook(lambda m, a: (a[0] * 2,))
+    y, f = fused()
+    assert not f and torch.allclose(y, 2 * plain, atol=1e-5)
+    handle.remove()
+
+    class Adapter(nn.Linear):
+        def forward(self, v):
+            return 3 * super().forward(v)
+    own = mlp.down_proj
+    mlp.down_proj = Adapter(64, 32, bias=False)
+    mlp.down_proj.weight = own.weight
+    y, f = fused()
+    assert not f and torch.allclose(y, 3 * plain, atol=1e-5)
+    mlp.down_proj = own
+    act = mlp.act_fn
+    mlp.act_fn = nn.ReLU()
+    y, f = fused()
+    assert not f and torch.allclose(y, Mlp.forward(mlp, x), atol=1e-6)
+    mlp.act_fn = act
+    assert unchanged()
+    # (other weights in the same parts are no other form)
+    mlp.down_proj.weight = nn.Parameter(2 * own.weight.detach())
+    y, f = fused()
+    assert f and torch.allclose(y, 2 * plain, atol=1e-5)
