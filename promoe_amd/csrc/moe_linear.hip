@@ -52,15 +52,25 @@ static __device__ __forceinline__ f32x4_t lin_mfma16(u32x4_t a, u32x4_t b, f32x4
 static __device__ __forceinline__ float lin_sigmoid(float v) {
   return __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(v * -1.44269504088896f));
 }
+// x y + the float of bits C, which stands in the instruction: from the compiler's hands constants go to scalar registers, and k_linear_wide,
+// which has none left, moves others out of their way (gated 4096 x 14336 x 4096: 8 us of 663)
+template <u32 C>
+static __device__ __forceinline__ float lin_fma_k(float x, float y) {
+  float r;
+  __asm__("v_fmaak_f32 %0, %1, %2, %3" : "=v"(r) : "v"(x), "v"(y), "n"(C));
+  return r;
+}
 // erfc(a / sqrt 2) / 2 for a >= 0 as 2^-(a q(a) + 1): q, of degree 9, is fitted to -log2(erfc(a / sqrt 2)) / a over [0, 11] in the maximum
 // norm (a linear programme), weighted so that v times the fit's error is 1.6e-8 at most, or 4e-3 of the tail; from there on it
 // grows, so that nothing is left before the range of fp32 ends.  gelu comes out 3.4e-8 off on average over [-7, 7], with an erf correctly
 // rounded to fp32 4.2e-8.  Twelve operations, one of them 2^x, without a branch, where the library's erf has three.
 static __device__ __forceinline__ float lin_half_erfc(float a) {
   float q = 5.36956876e-09f;
-  q = fmaf(q, a, -2.32354601e-07f); q = fmaf(q, a, 4.06335677e-06f); q = fmaf(q, a, -3.57522085e-05f); q = fmaf(q, a, 1.39703061e-04f);
-  q = fmaf(q, a, 2.88132411e-04f); q = fmaf(q, a, -7.29801325e-03f); q = fmaf(q, a, 5.26819479e-02f); q = fmaf(q, a, 4.59138335e-01f);
-  q = fmaf(q, a, 1.15111462f);
+#define LIN_STEP(C) q = lin_fma_k<__builtin_bit_cast(u32, C)>(q, a)
+  LIN_STEP(-2.32354601e-07f); LIN_STEP(4.06335677e-06f); LIN_STEP(-3.57522085e-05f);
+  LIN_STEP(1.39703061e-04f); LIN_STEP(2.88132411e-04f); LIN_STEP(-7.29801325e-03f);
+  LIN_STEP(5.26819479e-02f); LIN_STEP(4.59138335e-01f); LIN_STEP(1.15111462f);
+#undef LIN_STEP
   return __builtin_amdgcn_exp2f(fmaf(-a, q, -1.f));
 }
 template <int C>
