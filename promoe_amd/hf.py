@@ -182,7 +182,8 @@ def find_dense_mlps(model):
         g, u, d = parts
         act = _activation_of(getattr(mod, "act_fn", None))
         if act and g.weight.shape == u.weight.shape and d.weight.shape == g.weight.shape[::-1] and d.in_features % 8 == 0 \
-                and g.in_features % 8 == 0 and _is_gated_mlp(mod):
+                and g.in_features % 8 == 0 and all(p.weight.is_contiguous() and p.weight.data_ptr() % 16 == 0 for p in parts) \
+                and _is_gated_mlp(mod):
             out.append((name, mod, act))
     return out
 
@@ -193,9 +194,15 @@ def _fused_mlp_forward(act, act_fn):
         if self.act_fn is not act_fn or not _is_plain(act_fn) or \
                 not all(type(p) is torch.nn.Linear and _is_plain(p) for p in (self.gate_proj, self.up_proj, self.down_proj)):
             return type(self).forward(self, x)
+        if x.dtype != self.gate_proj.weight.dtype:           # (autocast brings the types together in the class's own products)
+            return type(self).forward(self, x)
+        rows = x.detach().reshape(-1, x.shape[-1])
+        apart, step = rows.stride()
+        if step != 1 or apart % 8 or not rows.shape[1] <= apart < 1 << 21 or rows.data_ptr() % 16:
+            rows = rows.clone(memory_format=torch.contiguous_format)
         # (detached, as the engine's own blocks are: nothing here has a gradient)
         w = [None if t is None else t.detach() for p in (self.gate_proj, self.up_proj, self.down_proj) for t in (p.weight, p.bias)]
-        h = ops.linear_gated(x.detach().reshape(-1, x.shape[-1]), w[0], w[2], w[1], w[3], act=act)
+        h = ops.linear_gated(rows, w[0], w[2], w[1], w[3], act=act)
         return ops.linear(h, w[4], w[5]).reshape(*x.shape[:-1], w[4].shape[0])
     return forward
 
