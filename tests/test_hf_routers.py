@@ -143,3 +143,16 @@ def test_a_block_with_further_weights_is_refused(name, part):
     with pytest.raises(NotImplementedError, match=part):
         hf.inject_model(model, device="cpu")
     assert blocks[0].experts.gate_up_proj.numel()
+
+
+def test_biases_below_every_score():
+    """Every c below zero: the experts of other groups are still out (not compared as zeros)."""
+    model, blocks = _blocks("DeepseekV3")
+    torch.manual_seed(2)
+    x = torch.randn(40, 64)
+    with torch.no_grad():
+        for b in blocks:
+            b.gate.e_score_correction_bias.add_(-3.0)
+            y = b(x[None])
+            y = (y[0] if isinstance(y, tuple) else y).reshape(40, 64)
+            assert float((_described(b, x) - y).abs().max()) <= 1e-4 * float(y.abs().max())
