@@ -105,10 +105,11 @@ int moe_topk(const float *logits, int T, int E, int ldl, int k, int mode, int *i
              void *stream);
 
 /* k1b for routers with groups of experts, sigmoid scores or a selection bias (E <= 256, k <= 32, n_group <= 64 groups of
- * E / n_group consecutive experts each).  Scores s: softmax over E, or sigmoid.  The experts are ordered by c = s + bias (bias
- * [E] fp32 or NULL).  A group is worth its largest c, or the sum of its two largest; the topk_group groups worth most are
- * kept, and the k largest c in them are chosen, descending.  w = s of the choice, / their sum if renorm, * scale.  Ties: the
- * lower group, the lower expert.  Scores and comparisons are in 64 bits, w is rounded once.
+ * E / n_group consecutive experts each; where more than 16 groups are not all kept, and for rows more than 2^26 floats apart, a
+ * slower form).  Scores s: softmax over E, or sigmoid.  The experts are ordered by c = s + bias (bias [E] fp32 or NULL).  A
+ * group is worth its largest c, or the sum of its two largest; the topk_group groups worth most are kept, and the k largest c
+ * in them are chosen, descending.  w = s of the choice, / their sum if renorm, * scale.  Ties: the lower group, the lower
+ * expert.  Scores and comparisons are in 64 bits, w is rounded once.
  * A NaN logit counts as -inf; a row of nothing else has weights 0 under softmax.  A c that is NaN (a NaN bias, +inf under
  * softmax, whose scores and weights are NaN) is ordered behind the others.  k different experts come out in every case.
  * No reference counterpart (its routers are torch's). */
@@ -474,7 +475,8 @@ int moe_combine_windows(const float *part_r, const float *part_s, const float *t
  *   moe_linear        y = act(x W^T + bias) + residual
  *   moe_linear_gated  y = act(x Wg^T + b_gate) * (x Wu^T + b_up)
  * x [M, K], W [N, K], biases [N], residual [M, N] all bf16 or all fp16 (dtype); y [M, N] of that type or fp32 (y_fp32).
- * Sums, biases, activation, product and residual in fp32, one rounding at the end.  Rows are ldx, ldw, ldr and ldy elements apart
+ * Sums, biases, activation, product and residual in fp32 (exponentials and reciprocals those of the hardware, to 1 ulp), one rounding
+ * at the end.  Rows are ldx, ldw, ldr and ldy elements apart
  * (both matrices of a pair ldw).  K, ldx and ldw multiples of 8, ldx and ldw below 2^21, x and the matrices on 16-byte boundaries; M
  * and N from 0 to 2^26.  bias, b_gate, b_up and residual may be NULL; residual may be y itself (same rows and type); a y that
  * overlaps anything else is refused (rows side by side in one buffer, the same distance apart, do not overlap).

@@ -294,8 +294,8 @@ static __device__ __forceinline__ void lt_each(const F &f) {
 // Four waves (2 x 2), wave (wm, wn) on WM x WN blocks of 32 x 32: a tile of 64 WM rows of x by 64 WN rows of W.  A gated pair's W
 // blocks alternate between the two matrices (block b: matrix b & 1, its columns 32 (b >> 1) ..), so that a lane holds both sums
 // of a column.  K advances 64 at a time (a slab); slabs go global -> LDS directly, RING of them in LDS.
-// Bound by LDS, 192 (WM + WN) cycles a slab for 128 WM WN of products, and by few workgroups: 24 x 4096 x 4096 9.9 us and 3.8 for the
-// join; with matrices from the last cache 512 x 4096 x 4096 25.0 (687 TFLOP/s), gated 251 x 2560 x 3584 19.1 (482), 1024 x 4096 x 4096 38.1 (902);
+// A slab costs 192 (WM + WN) cycles of LDS for 128 WM WN of products; with few workgroups about half of the time is that, the rest the
+// launch's start, the ring's fill, a barrier a slab and the epilogue: 24 x 4096 x 4096 9.9 us and 3.8 for the join; with matrices from the last cache 512 x 4096 x 4096 25.0 (687 TFLOP/s), gated 251 x 2560 x 3584 19.1 (482), 1024 x 4096 x 4096 38.1 (902);
 // from memory 31.6, 28.6 and 44.1.
 #define LT_K 64
 #define LT_ROW 128  // bytes of a row of a slab: 8 chunks of 16, chunk c of row r in slot c ^ ((r >> 1) & 7)
@@ -474,8 +474,9 @@ __global__ __launch_bounds__(256, RING * (WM + WN) * 64 * LT_ROW > 80 * 1024 ? 1
 // that the products of a slab need: all 16 of a wave at once stopped the products for as long again (59 % busy matrix cores, then 74).
 // The run of slabs goes on from tile to tile: the next tile's first slab and the W half behind it land under the last products, and the
 // sums leave through the one place that nothing else needs then.
-// Bound by power: 4096 x 4096 x 14336 331 us (1455 TFLOP/s, 73 % busy matrix cores at 1.75 to 1.9 GHz; the library's product 305 - 315), gated 4096 x
-// 14336 x 4096 664 us (1449; the library's of both matrices, no gate, 622 - 640).
+// Bound by power: 4096 x 4096 x 14336 328 to 350 us on different cards (1370 to 1470 TFLOP/s, 73 % busy matrix cores at 1.75 to 1.9 GHz; the
+// library's product 305 - 315), gated 4096 x 14336 x 4096 657 to 707 us (the library's of both matrices, no gate, 622 - 640); the first launches
+// after a pause up to 408 and 730.
 template <bool F16, bool GATED>
 __global__ __launch_bounds__(256, 1) void k_linear_wide(const LinArgs a) {
   constexpr int B = 256, NT = 8, HALF = B * LT_ROW, NC = GATED ? B / 2 : B;

@@ -15,8 +15,8 @@ Qwen2-MoE (softmax -> top-k, optional renormalisation, sigmoid-gated shared expe
 family (DeepSeek-MoE / DeepSeek-V2-Lite: softmax -> greedy top-k without renormalisation, a plain
 shared expert `shared_experts` of n_shared_experts * I columns; the reference's metas for it are
 utils/common_metas.py:17-41 and 69-94).  Routers with groups of experts (DeepSeek-V2: a group is worth its best expert)
-and routers with sigmoid scores and a selection bias (`e_score_correction_bias`; a group is worth its two best) become the
-engine's routing rule of the layer (ops.RouteRule).  In the DeepSeek models the first decoder layers are dense:
+and routers with sigmoid scores and a selection bias (`gate.e_score_correction_bias`; a group is worth its two best) become the
+engine's routing rule of the layer (ops.RouteRule); routers and blocks that look like these and are not are refused.  In the DeepSeek models the first decoder layers are dense:
 MoE layers are numbered from 0 in model order, so decoder layer i is engine layer
 i - first_k_dense_replace (the reference subtracts the same 1, common_metas.py:19-23).  With `fuse_dense` the
 dense gated layers run as two launches each (ops.linear_gated, ops.linear).
@@ -234,7 +234,9 @@ def inject_model(model, device="cuda:0", fmt: str = "bf16", max_tokens: int = 40
 
     fmt "bf16" keeps the experts' weights as they are (rounded to bf16); "int4" quantises them to
     int4-g128 on the way in.  fuse_dense: the dense gated layers (find_dense_mlps) run as two fused launches instead of the
-    module's own operations; their intermediate rows are rounded once instead of three times.  cfg: engine configuration keys (cache_rate, cache_policy, ...).
+    module's own operations; their intermediate rows are rounded once instead of three times.  Neither they nor the sparse blocks have a
+    gradient.  cfg: engine configuration keys (cache_rate, cache_policy, ...).  NotImplementedError: a router or a block that the engine's
+    layer cannot stand for (nothing of the model has moved then).
     The shapes must fit the kernels: H and I multiples of 128 (bf16) / 128 and 16 (int4)."""
     if fmt not in ("bf16", "int4"):
         raise ValueError("fmt must be 'bf16' or 'int4'")
