@@ -379,15 +379,19 @@ static __device__ __forceinline__ void group_topk_quad(const GroupRule &q, const
     den = gr_sum16(s);
   }
   double s[2], total = 0.0;
+  bool tiny = false;
 #pragma unroll
   for (int h = 0; h < 2; ++h) {
     s[h] = 0.0;
     if (h && q.k <= 16) break;
-    const double x = (double)fmaxf(logits[(size_t)t * ldl + mine[h]], -INF), p = gr_exp(q.sigmoid ? -fabs(x) : x - (double)top);
+    const double x = (double)fmaxf(logits[(size_t)t * ldl + mine[h]], -INF), d = q.sigmoid ? -fabs(x) : x - (double)top, p = gr_exp(d);
+    // (scores of few bits, and sigmoids that the exact form has as zero: the bias has chosen them, and in a sum of nothing else they count)
+    tiny |= j + 16 * h < q.k && d < -700.0 && d > -750.0;
     s[h] = q.sigmoid ? gr_div(x < 0.0 ? p : 1.0, 1.0 + p) : gr_div(p, den);
     total += j + 16 * h < q.k ? s[h] : 0.0;
   }
   if (q.renorm) total = gr_sum16(total);
+  sure = sure && ((unsigned)(__ballot(tiny) >> (16 * tok)) & 0xffffu) == 0u;
   const bool live = t0 + tok < T;
   if (live && sure) {
 #pragma unroll

@@ -82,3 +82,35 @@ def test_infinite_biases(cuda):
         bias[list(at)] = v
         for keep in (1, 2, 5):
             _check(lg, 4, "sigmoid", bias, 8, keep, cuda)
+
+
+@pytest.mark.parametrize("kind", ["sigmoid", "softmax"])
+def test_scores_at_the_end_of_the_range(cuda, kind):
+    """The bias chooses experts whose scores are the smallest that 64 bits hold, or nothing: renormalised, they are what counts.  The
+    form for few tokens a wave (rows 2^26 + 4 floats apart take it throughout) has the same bits; sigmoids past e^709 are zero, and so
+    are weights of nothing else."""
+    from promoe_amd import ops
+    print(f"case group_tiny {kind}", flush=True)
+    E, k, T, ldl = 64, 4, 24, (1 << 26) + 4
+    rng = np.random.default_rng(6)
+    lg = rng.uniform(-760, -690, (T, E)).astype(np.float32)
+    lg[:4] = rng.uniform(-745, -711, (4, E)).astype(np.float32)
+    if kind == "softmax":
+        lg[:, 0] = 0.0
+    bias = np.full(E, -8.0, np.float32)
+    bias[[5, 17, 30, 41]] = (4.0, 2.0, 8.0, 6.0)                     # far apart: 32 bits are certain of these
+    far = torch.empty((T - 1) * ldl + E, device=cuda).as_strided((T, E), (ldl, 1))
+    far.copy_(torch.from_numpy(lg))
+    bd = torch.from_numpy(bias).to(cuda)
+    for G, keep, gv in ((1, 1, "max"), (8, 4, "max")):
+        rule = ops.RouteRule(kind, G, keep, gv, True, 1.0)
+        idx, w = ops.group_topk(far.contiguous(), k, rule, bd)
+        i2, w2 = ops.group_topk(far, k, rule, bd)
+        assert (idx.cpu() == torch.tensor([30, 41, 5, 17], dtype=torch.int32)).all() and torch.equal(idx, i2)
+        assert torch.equal(w, w2), int((w != w2).any(1).sum())
+        i3, w3, _ = ops.group_topk_dispatch(far.contiguous(), k, rule, bd)
+        assert torch.equal(idx, i3) and torch.equal(w, w3)
+        if kind == "sigmoid":
+            assert (w[:4] == 0).all()
+            ref = R.route(lg, k, kind, bias, G, keep, gv, True, 1.0)[1]
+            assert np.array_equal(w.cpu().numpy() == 0, ref.astype(np.float32) == 0)
