@@ -98,15 +98,16 @@ def _route_args(what, logits, k, rule, bias):
         raise L.MoeError("%s: logits must be fp32 [T, E] with the experts of a row side by side" % what)
     if not isinstance(rule, L.RouteRule):
         raise L.MoeError("%s: rule must be a RouteRule" % what)
-    if logits.shape[0] > 1 and logits.stride(0) >= 1 << 31:
-        raise L.MoeError("%s: rows of logits %d floats apart (fewer than 2^31 are needed)" % (what, logits.stride(0)))
-    index = _operands(what, logits, bias)
     T, E = logits.shape
+    ldl = logits.stride(0) if T > 1 else E
+    if ldl >= 1 << 31:
+        raise L.MoeError("%s: rows of logits %d floats apart (fewer than 2^31 are needed)" % (what, ldl))
+    index = _operands(what, logits, bias)
     if bias is not None and (bias.dtype != torch.float32 or bias.shape != (E,) or not bias.is_contiguous()):
         raise L.MoeError("%s: bias must be fp32 [%d], contiguous" % (what, E))
     if not 0 < k <= E:
         raise L.MoeError("%s: %d of %d experts" % (what, k, E))
-    return index, T, E, logits.stride(0) if T > 1 else E
+    return index, T, E, ldl
 
 
 def group_topk(logits: torch.Tensor, k: int, rule: RouteRule, bias: torch.Tensor | None = None):
