@@ -165,7 +165,7 @@ static __device__ __forceinline__ void group_topk_token(const GroupRule &q, cons
 // row's largest probability (nine additions one after the other, 2^x, the quotient); the bias added 2^-24 of the sum c; a group's
 // value as a sum a + b of two such c 2^-24 (|a| + |b| + |a + b|), whatever cancels in it; the place in the lane's run, which the
 // ordered value carries in its last bits, V 2^-23 of it.
-// Bound by the vector unit: 32768 tokens over 256 experts in 8 groups, a bias and sums of two take 26.5 to 29 us (36 MB: 7 us at a copy's rate), 1200
+// Bound by the vector unit: 32768 tokens over 256 experts in 8 groups, a bias and sums of two take 26.5 to 29 us (36 MB: 7 us at a copy's rate), 1230
 // operations a wave of four.  A wave per token in 64 bits takes 67; experts dealt out one by one (16 r + lane), their indexes beside the
 // values and the groups' values through LDS 36 (1900 operations); no fours in order 30; 82 registers instead of 64, which cost the exact
 // form some in scratch, two waves fewer a SIMD and 2 us; waves that go on to
