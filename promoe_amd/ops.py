@@ -111,8 +111,8 @@ def _route_args(what, logits, k, rule, bias):
 
 
 def group_topk(logits: torch.Tensor, k: int, rule: RouteRule, bias: torch.Tensor | None = None):
-    """Routing with groups of experts and a selection bias (moe_group_topk): logits fp32 [T, E] (rows may be further apart: a
-    slice in front of a shared expert's gate column) -> (idx [T, k] int32, w [T, k] fp32).  The bias [E] takes part in the
+    """Routing with groups of experts and a selection bias (moe_group_topk): logits fp32 [T, E] (rows may be further apart, up to 2^31
+    floats: a slice in front of a shared expert's gate column) -> (idx [T, k] int32, w [T, k] fp32).  The bias [E] takes part in the
     choice, not in the weights.  Serving only: tensors that a gradient is expected of are refused."""
     index, T, E, ldl = _route_args("group_topk", logits, k, rule, bias)
     if index != torch.cuda.current_device():
