@@ -134,6 +134,7 @@ typedef struct moe_unit {
 
 /* k2: stable dispatch of the P = T*k (token,slot) pairs (pair p = t*k + j).
  * counts[E], offsets[E+1], sorted_pair[P], pos_of_pair[P], sorted_tok[P] (= p / k),
+ * (a pair whose idx is none of the E experts has pos_of_pair -1 and no place; moe_combine takes none such)
  * units[max_units] (active experts ascending id, rest m = 0), n_active[1],
  * active_ids[max_units] int64 (the `unique expert ids` list the reference's module
  * hands to report_experts, utils/__init__.py:84-88). */
@@ -484,6 +485,7 @@ int moe_combine_windows(const float *part_r, const float *part_s, const float *t
  * smaller one or NULL is refused where that number is not 0. */
 #define MOE_DT_BF16 0
 #define MOE_DT_FP16 1
+#define MOE_DT_FP32 2 /* where an entry says so */
 #define MOE_ACT_NONE 0
 #define MOE_ACT_SILU 1      /* v / (1 + e^-v) */
 #define MOE_ACT_GELU 2      /* v (1 + erf(v / sqrt 2)) / 2 */
@@ -497,6 +499,53 @@ int moe_linear(const void *x, int64_t ldx, const void *w, int64_t ldw, const voi
 int moe_linear_gated(const void *x, int64_t ldx, const void *w_gate, const void *w_up, int64_t ldw, const void *b_gate,
                      const void *b_up, void *y, int64_t ldy, int M, int N, int K, int dtype, int act, int y_fp32, void *ws,
                      int64_t ws_bytes, void *stream);
+
+/* Rows of the tokens in the order of their experts and back, by the places that a dispatch gives (pos_of_pair[t*k + j]: the place of
+ * choice j of token t, -1 for a choice of no expert; total: one int on the device, the pairs with a place, offsets[E]).
+ *   moe_sort_rows         y[p,:] = x[t,:] for the places p of token t; rows from total to T*k are zero
+ *   moe_unsort_rows       y[t,:] = sum_j w[t,j] x[pos(t,j),:] (w NULL: 1, the gradient of moe_sort_rows), in order of the choices
+ *   moe_unsort_rows_grad  dx[p,:] = w[t,j] dy[t,:] (rows from total on zero) and dw[t,j] = <dy[t,:], x[p,:]> (0 without a place); dx or
+ *                         dw may be NULL
+ * Rows of H elements of one type (dtype; w and dw fp32), ld elements apart, any alignment (rows on 16-byte boundaries go faster); sums and
+ * products in fp32, rounded once.  T below 2^26, T*k below 2^31, H below 2^24 (2^22 off those boundaries).  A result over what is read is
+ * refused.  No reference counterpart (its modules index with torch). */
+int moe_sort_rows(const void *x, int64_t ldx, void *y, int64_t ldy, const int *pos_of_pair, const int *total, int T, int k, int H,
+                  int dtype, void *stream);
+int moe_unsort_rows(const void *x, int64_t ldx, void *y, int64_t ldy, const int *pos_of_pair, const float *w, int T, int k, int H,
+                    int dtype, void *stream);
+int moe_unsort_rows_grad(const void *dy, int64_t lddy, const void *x, int64_t ldx, const int *pos_of_pair, const float *w, const int *total,
+                         void *dx, int64_t lddx, float *dw, int T, int k, int H, int dtype, void *stream);
+
+/* Matrices in microscaled 4-bit floating point: a code per value (two to a byte, the even column in the low half: sign, two bits of
+ * exponent, one of mantissa, i.e. 0, 0.5, 1, 1.5, 2, 3, 4, 6) and a byte per 32 columns, value = code * 2^(byte - 127); byte 255: NaN.
+ * Rows of K/2 bytes of codes ldc apart (16-byte boundaries) and of K/32 bytes of scales lds apart (4-byte boundaries; the bytes up to the
+ * next such boundary behind a row's scales are read and not used).  next_c, next_s: bytes between the matrices of consecutive
+ * experts. */
+typedef struct moe_mx4 {
+  const void *codes, *scales;
+  int64_t ldc, lds, next_c, next_s;
+} moe_mx4;
+/* M rows of K values (K % 32 == 0, rows ld elements apart on 16-byte boundaries, dtype any of three) to codes and scales and back.  The
+ * scale of a block is 2^(floor(log2 of its largest magnitude) - 2), at least 2^-127; codes are rounded to the nearest, ties to the even
+ * code, 6 beyond 6.  A block with a NaN or an infinity becomes NaN.  Back: rounded to dtype, which fp32 and bf16 do not need (beyond
+ * their range codes become infinite). */
+int moe_mx4_quantize(const void *x, int64_t ldx, int dtype, int64_t M, int K, void *codes, int64_t ldc, void *scales, int64_t lds,
+                     void *stream);
+int moe_mx4_dequantize(const void *codes, int64_t ldc, const void *scales, int64_t lds, int64_t M, int K, void *y, int64_t ldy, int dtype,
+                       void *stream);
+/* moe_linear and moe_linear_gated (w_up not NULL) with matrices in that form (descriptions on the host); x either 16-bit rows (ldx
+ * elements apart; the products are those of the values as they are) or rows in the same form (xq, x NULL).  bias, residual and y (unless
+ * y_fp32) have the type dtype, and so has a 16-bit x.  K % 32 == 0; rows less than 4 MiB apart; sums in fp32, one rounding.  The other rules
+ * as for moe_linear.
+ * moe_mx4_experts: the same for every expert e of a dispatch: rows offsets[e] .. + counts[e] of y are the product of those rows of x, or,
+ * with sorted_tok, of the rows sorted_tok[..] of x (x_rows of them), with matrix e; bias [E, N].  Rows behind the last pair are left as
+ * they were.  E <= 1024. */
+int moe_mx4_linear(const void *x, int64_t ldx, const moe_mx4 *xq_host, const moe_mx4 *w_host, const moe_mx4 *w_up_host, const void *bias,
+                   const void *bias_up, const void *residual, int64_t ldr, void *y, int64_t ldy, int M, int N, int K, int dtype, int act,
+                   int y_fp32, void *ws, int64_t ws_bytes, void *stream);
+int moe_mx4_experts(const void *x, int64_t ldx, const moe_mx4 *xq_host, const moe_mx4 *w_host, const moe_mx4 *w_up_host, const void *bias,
+                    const void *bias_up, void *y, int64_t ldy, const int *counts, const int *offsets, const moe_unit *units, int max_units,
+                    const int *sorted_tok, int x_rows, int P, int E, int N, int K, int dtype, int act, int y_fp32, void *stream);
 
 /* Per-kernel timing with HIP events recorded on the launch stream around every kernel
  * the launchers below start (no reference counterpart; used by the benchmark to report

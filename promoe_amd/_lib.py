@@ -23,6 +23,7 @@ lib = C.CDLL(LIB_PATH)
 MOE_OK, MOE_EINVAL, MOE_EHIP, MOE_ESTATE, MOE_ENOMEM, MOE_ENOTRESIDENT = 0, -1, -2, -3, -4, -5
 ROUTE_SOFTMAX_TOPK, ROUTE_SOFTMAX_TOPK_RENORM, ROUTE_TOPK_SOFTMAX = 0, 1, 2
 DTYPES = {torch.bfloat16: 0, torch.float16: 1}
+ROW_DTYPES = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}
 ACTS = {"none": 0, "silu": 1, "gelu": 2, "gelu_tanh": 3, "relu": 4, "relu2": 5}
 SCORES = {"softmax": 0, "sigmoid": 1}
 GROUP_VALUES = {"max": 0, "top2": 1}
@@ -41,6 +42,10 @@ class RouteRule(C.Structure):
                 ("scale", C.c_float)]
 
 
+class Mx4Desc(C.Structure):
+    _fields_ = [("codes", vp), ("scales", vp), ("ldc", i64), ("lds", i64), ("next_c", i64), ("next_s", i64)]
+
+
 class MoeError(RuntimeError):
     pass
 
@@ -57,6 +62,13 @@ _sig("moe_int4_layout_make", [i32, i32, C.POINTER(Int4Layout)])
 _sig("moe_linear_workspace_bytes", [i32, i32, i32, i32], i64)
 _sig("moe_linear", [vp, i64, vp, i64, vp, vp, i64, vp, i64, i32, i32, i32, i32, i32, i32, vp, i64, vp])
 _sig("moe_linear_gated", [vp, i64, vp, vp, i64, vp, vp, vp, i64, i32, i32, i32, i32, i32, i32, vp, i64, vp])
+_sig("moe_sort_rows", [vp, i64, vp, i64, vp, vp, i32, i32, i32, i32, vp])
+_sig("moe_unsort_rows", [vp, i64, vp, i64, vp, vp, i32, i32, i32, i32, vp])
+_sig("moe_unsort_rows_grad", [vp, i64, vp, i64, vp, vp, vp, vp, i64, vp, i32, i32, i32, i32, vp])
+_sig("moe_mx4_quantize", [vp, i64, i32, i64, i32, vp, i64, vp, i64, vp])
+_sig("moe_mx4_dequantize", [vp, i64, vp, i64, i64, i32, vp, i64, i32, vp])
+_sig("moe_mx4_linear", [vp, i64, vp, vp, vp, vp, vp, vp, i64, vp, i64, i32, i32, i32, i32, i32, i32, vp, i64, vp])
+_sig("moe_mx4_experts", [vp, i64, vp, vp, vp, vp, vp, vp, i64, vp, vp, vp, i32, vp, i32, i32, i32, i32, i32, i32, i32, i32, vp])
 _sig("moe_group_topk", [vp, i32, i32, i32, i32, vp, vp, vp, vp, vp])
 _sig("moe_group_topk_dispatch", [vp, i32, i32, i32, i32, vp] + [vp] * 11 + [i32, vp, vp, vp, i32, vp])
 _sig("moe_gate_logits", [vp, vp, vp, vp, i32, i32, i32, i32, vp])

@@ -218,6 +218,8 @@ __global__ __launch_bounds__(DISP_THREADS) void k_dispatch(
       sorted_pair[pos] = p;
       pos_of_pair[p] = pos;
       sorted_tok[pos] = p / k;
+    } else if (p < P) {
+      pos_of_pair[p] = -1;  // (a pair of no expert: it has no place)
     }
     __syncthreads();
   }
@@ -369,6 +371,8 @@ __global__ __launch_bounds__(DISP_THREADS) void k_dispatch_multi(const DispTopk 
     sorted_pair[pos] = p;
     pos_of_pair[p] = pos;
     sorted_tok[pos] = p / k;
+  } else if (tid < np) {
+    pos_of_pair[p] = -1;
   }
   // the last workgroup through the barrier clears it for the next launch
   if (tid == 0) {

@@ -1,0 +1,461 @@
+// Microscaled 4-bit floating point (gfx950): rows quantised and back, and the products of dense layers and of experts with weights
+// in that form.  A value is a code (sign, two bits of exponent, one of mantissa: 0, 0.5, 1, 1.5, 2, 3, 4, 6) times the power of two of
+// its block of 32 columns, 2^(byte - 127); byte 255 makes the block NaN.
+//   y = act(x W^T + b) + residual,   y = act(x Wg^T + bg) * (x Wu^T + bu)
+// x in the same form: both operands go into the scaled matrix products as they are.  x in bf16 or fp16: the weights become bf16 in
+// registers, exactly; an fp16 value is the sum of two bf16 (11 bits of mantissa), so that nothing of it is lost either.
+#include <hip/hip_runtime.h>
+#include <stdint.h>
+
+#include "moe_common.h"
+#include "moe_kernels.h"
+#include "moe_device.h"
+#include "moe_linear.h"
+
+typedef uint16_t u16x2_t __attribute__((ext_vector_type(2)));
+typedef int i32x8_t __attribute__((ext_vector_type(8)));
+typedef float f32x2_t __attribute__((ext_vector_type(2)));
+typedef _Float16 f16x2_t __attribute__((ext_vector_type(2)));
+
+// ---- rows into codes and back ---------------------------------------------------------------------------------------------------
+struct QuantArgs {
+  const void *x;              // the rows that are read: values, or codes
+  void *y;                    // the rows that are written: codes, or values
+  uint8_t *scales;
+  long long ldx, ldc, lds;    // elements between rows of values, bytes between rows of codes and of scales
+  long long n;                // pieces of 8 values
+  u32 per, magic, shift;      // pieces of a row; i / per = (mulhi(i, magic) + i) >> shift for i < 2^31
+};
+struct Place { long long x, c, s; };
+template <bool FLAT>  // FLAT: the rows lie end to end
+static __device__ __forceinline__ Place place_of(const QuantArgs &a, long long i) {
+  if constexpr (FLAT) return Place{8 * i, 4 * i, i >> 2};
+  const u32 row = (__umulhi((u32)i, a.magic) + (u32)i) >> a.shift, col = (u32)i - row * a.per;
+  return Place{row * a.ldx + 8 * (long long)col, row * a.ldc + 4 * (long long)col, row * a.lds + (col >> 2)};
+}
+// the largest of the four lanes of a block
+static __device__ __forceinline__ u32 quad_max(u32 v) {
+  v = max(v, (u32)__builtin_amdgcn_update_dpp(0, (int)v, 0xb1, 0xf, 0xf, true));  // quad_perm 1 0 3 2
+  return max(v, (u32)__builtin_amdgcn_update_dpp(0, (int)v, 0x4e, 0xf, 0xf, true));  // quad_perm 2 3 0 1
+}
+// Exponent byte of the scale of a block from the bits of its largest magnitude as fp32: floor(log2) - 2, at least 0; 255 (NaN) where a
+// value is none or infinite
+static __device__ __forceinline__ u32 scale_byte(u32 top) {
+  const u32 e = top >> 23;
+  return e == 255 ? 255u : e > 2 ? e - 2 : 0u;
+}
+// Four lanes a block, eight values each: one 16-byte load (two of fp32) and four bytes of codes, side by side over the lanes.  The
+// hardware's conversion divides by the scale, rounds to the nearest (ties to the even code) and goes no further than 6.
+#define QT_U 4  // pieces of a lane, all of them on their way at once
+template <int DT, bool FLAT>
+__global__ __launch_bounds__(256) void k_mx4_quantize(const QuantArgs a) {
+  const long long first = (long long)blockIdx.x * (256 * QT_U) + threadIdx.x;
+  u32x4_t v[QT_U][DT == MOE_DT_FP32 ? 2 : 1];
+#pragma unroll
+  for (int u = 0; u < QT_U; ++u) {
+    const long long i = min(first + 256 * u, a.n - 1);  // (no condition around a load)
+    const char *p = (const char *)a.x + place_of<FLAT>(a, i).x * (DT == MOE_DT_FP32 ? 4 : 2);
+    v[u][0] = *(const u32x4_t *)p;
+    if constexpr (DT == MOE_DT_FP32) v[u][1] = *(const u32x4_t *)(p + 16);
+  }
+#pragma unroll
+  for (int u = 0; u < QT_U; ++u) {
+    const long long i = first + 256 * u;
+    if (i >= a.n) break;
+    u32 top = 0;
+    if constexpr (DT == MOE_DT_FP32) {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) top = max(top, v[u][e >> 2][e & 3] & 0x7fffffffu);
+    } else {  // (magnitudes compare as whole numbers, two at a time)
+      u16x2_t m{0, 0};
+#pragma unroll
+      for (int e = 0; e < 4; ++e) m = __builtin_elementwise_max(m, __builtin_bit_cast(u16x2_t, v[u][0][e] & 0x7fff7fffu));
+      top = max(m[0], m[1]);
+    }
+    top = quad_max(top);
+    if constexpr (DT == MOE_DT_BF16) top <<= 16;
+    if constexpr (DT == MOE_DT_FP16) top = __float_as_uint(half_bits_to_f32((uint16_t)top));
+    const u32 byte = scale_byte(top);
+    const float s = __uint_as_float(byte << 23);        // (the conversion takes the exponent field alone: 0 is 2^-127)
+    u32 c = 0;
+    lt_each<4>([&](auto j_) {
+      constexpr int J = decltype(j_)::value;
+      if constexpr (DT == MOE_DT_FP32) {
+        const u32 p = v[u][DT == MOE_DT_FP32 ? J / 2 : 0][2 * (J & 1)], q = v[u][DT == MOE_DT_FP32 ? J / 2 : 0][2 * (J & 1) + 1];
+        c = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(c, __uint_as_float(p), __uint_as_float(q), s, J);
+      } else {
+        const u32 p = v[u][0][J];                       // (a value of its own: bit_cast of a vector's element takes the first one)
+        if constexpr (DT == MOE_DT_BF16) c = __builtin_amdgcn_cvt_scalef32_pk_fp4_bf16(c, __builtin_bit_cast(bf16x2_t, p), s, J);
+        else c = __builtin_amdgcn_cvt_scalef32_pk_fp4_f16(c, __builtin_bit_cast(f16x2_t, p), s, J);
+      }
+    });
+    const Place at = place_of<FLAT>(a, i);
+    *(u32 *)((char *)a.y + at.c) = c;
+    if ((threadIdx.x & 3) == 0) a.scales[at.s] = (uint8_t)byte;
+  }
+}
+template <int DT, bool FLAT>
+__global__ __launch_bounds__(256) void k_mx4_dequantize(const QuantArgs a) {
+  const long long first = (long long)blockIdx.x * (256 * QT_U) + threadIdx.x;
+  u32 c[QT_U], b[QT_U];
+#pragma unroll
+  for (int u = 0; u < QT_U; ++u) {
+    const Place at = place_of<FLAT>(a, min(first + 256 * u, a.n - 1));
+    c[u] = *(const u32 *)((const char *)a.x + at.c);
+    b[u] = a.scales[at.s];
+  }
+#pragma unroll
+  for (int u = 0; u < QT_U; ++u) {
+    const long long i = first + 256 * u;
+    if (i >= a.n) break;
+    const float s = __uint_as_float(b[u] << 23);
+    char *p = (char *)a.y + place_of<FLAT>(a, i).x * (DT == MOE_DT_FP32 ? 4 : 2);
+    f32x2_t f[4];
+    f[0] = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(c[u], s, 0);
+    f[1] = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(c[u], s, 1);
+    f[2] = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(c[u], s, 2);
+    f[3] = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(c[u], s, 3);
+    if constexpr (DT == MOE_DT_FP32) {
+      *(f32x4_t *)p = f32x4_t{f[0][0], f[0][1], f[1][0], f[1][1]};
+      *(f32x4_t *)(p + 16) = f32x4_t{f[2][0], f[2][1], f[3][0], f[3][1]};
+    } else {
+      const float v[8] = {f[0][0], f[0][1], f[1][0], f[1][1], f[2][0], f[2][1], f[3][0], f[3][1]};
+      *(u32x4_t *)p = lin_pack<DT == MOE_DT_FP16>(v);
+    }
+  }
+}
+
+// ---- products -------------------------------------------------------------------------------------------------------------------
+struct MxArgs {
+  const void *x;
+  const uint8_t *xs;                         // scales of x, NULL: x has 16 bits
+  const uint8_t *w[2], *ws[2];               // codes and scales of the matrices; [1]: the second one of a gated pair
+  const uint16_t *bias[2], *res;
+  void *y;
+  long long ldx, ldxs, ldw, ldws, ew, ews;   // bytes between rows; ew, ews: between the matrices of consecutive experts
+  long long ldr, ldy;                        // elements
+  int M, N, K, act, y32;                     // M: rows of y
+  int nm, nn, splits, ldp, slabs, extra;     // as in the products of 16-bit matrices
+  float *part;
+  // products by expert
+  const int *counts, *offsets, *tok;         // rows of each expert, its first; tok: the row of x of each row of y (NULL: the same)
+  const moe_unit *units;
+  int E;
+};
+enum { X_MX4 = 0, X_BF16 = 1, X_FP16 = 2 };   // what x is
+static __device__ __forceinline__ f32x4_t mx_mfma16(u32x4_t a, u32x4_t b, f32x4_t c, u32 sa, u32 sb) {
+  const i32x8_t a8{(int)a[0], (int)a[1], (int)a[2], (int)a[3], 0, 0, 0, 0}, b8{(int)b[0], (int)b[1], (int)b[2], (int)b[3], 0, 0, 0, 0};
+  return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(a8, b8, c, 4, 4, 0, (int)sa, 0, (int)sb);
+}
+// eight codes as bf16, exactly
+static __device__ __forceinline__ u32x4_t mx_bf16(u32 c, float s) {
+  return u32x4_t{__builtin_bit_cast(u32, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(c, s, 0)),
+                 __builtin_bit_cast(u32, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(c, s, 1)),
+                 __builtin_bit_cast(u32, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(c, s, 2)),
+                 __builtin_bit_cast(u32, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(c, s, 3))};
+}
+// eight fp16 values as the sums of two bf16: the first to the nearest, the second what is left (at most 4 bits)
+static __device__ __forceinline__ void mx_split(u32x4_t x, u32x4_t &hi, u32x4_t &lo) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const float a = half_bits_to_f32((uint16_t)x[i]), b = half_bits_to_f32((uint16_t)(x[i] >> 16));
+    const u32 h = lin_bits<false>(a) | (u32)lin_bits<false>(b) << 16;
+    const float c = a - bf16lo(h), d = b - bf16hi(h);   // (of an infinite value NaN: the second part is 0 then)
+    hi[i] = h;
+    lo[i] = (c == c ? lin_bits<false>(c) : 0u) | (u32)(d == d ? lin_bits<false>(d) : 0u) << 16;
+  }
+}
+
+// ---- few rows of x: the matrix streams past them --------------------------------------------------------------------------------
+// A workgroup of eight waves takes R = 16 / SH rows of W (gated: of both matrices), its waves the pieces of K in turn; their sums meet
+// in LDS.  A lane's load is one block, 32 columns of a row: with SH = 1 the 16 rows of the operand are 16 rows of W, with few rows of x
+// (at most 16 / SH) R rows of W by SH pieces of K: row s R + r and column s R + m hold piece s of both, and the products of unlike
+// pieces are left unread.  By expert the second dimension of the grid is a unit of the dispatch; more than 16 rows go in turn.
+#define MR_WAVES 8
+#define MR_U 2  // loads of a matrix in flight per wave, twice
+template <int X, bool F16, bool GATED, int SH>
+__global__ __launch_bounds__(64 * MR_WAVES) void k_mx4_rows(const MxArgs a) {
+  constexpr int NM = GATED ? 2 : 1, R = 16 / SH, STEP = 4 * SH * MR_U, SPAN = STEP * MR_WAVES, NX = X == X_MX4 ? 1 : 4;
+  __shared__ f32x4_t red[MR_WAVES][NM][64];
+  const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int r = (lane & 15) % R, s = (lane & 15) / R, n0 = blockIdx.x * R, blocks = a.K >> 5;
+  int e = 0, first = 0, rows = a.M;
+  if (a.units) {
+    const moe_unit u = a.units[blockIdx.y];
+    e = __builtin_amdgcn_readfirstlane(u.expert); first = __builtin_amdgcn_readfirstlane(u.row0); rows = __builtin_amdgcn_readfirstlane(u.m);
+    if ((unsigned)e >= (unsigned)a.E) return;
+  }
+  MxArgs o = a;                                                  // what the epilogue goes by
+  if (o.bias[0]) o.bias[0] += (long long)e * a.N;
+  if (GATED && o.bias[1]) o.bias[1] += (long long)e * a.N;
+  const int k0 = (lane >> 4) * SH + s;                           // the lane's block among 4 SH
+  rsrc_t rw[NM], rs[NM];
+#pragma unroll
+  for (int i = 0; i < NM; ++i) {
+    rw[i] = make_rsrc(a.w[i] + e * a.ew + n0 * a.ldw, LT_OUT);
+    rs[i] = make_rsrc(a.ws[i] + e * a.ews + n0 * a.ldws, LT_OUT);
+  }
+  const int row = min(n0 + r, a.N - 1) - n0, vw = row * (int)a.ldw, vs = row * (int)a.ldws;
+  for (int m0 = 0; m0 < rows; m0 += R) {
+    const int m = first + m0 + min(r, rows - 1 - m0);
+    const long long xrow = a.tok ? a.tok[m] : m, x0 = a.tok ? 0 : first + m0;  // (rows side by side from the block's first on)
+    const rsrc_t rx = make_rsrc((const char *)a.x + x0 * a.ldx, LT_OUT), rxs = make_rsrc(X == X_MX4 ? a.xs + x0 * a.ldxs : (const uint8_t *)a.x, LT_OUT);
+    const int vx = (int)((xrow - x0) * a.ldx), vxs = (int)((xrow - x0) * a.ldxs);
+    f32x4_t acc[NM] = {};
+    uint4 fw[2][NM][MR_U], fx[2][MR_U][NX];
+    u32 sw[2][NM][MR_U], sx[2][MR_U];
+    auto load = [&](int p, int base) {
+#pragma unroll
+      for (int u = 0; u < MR_U; ++u) {
+        const int k = base + 4 * SH * u + k0;
+        const bool in = k < blocks;                              // past the end: zeros on both sides
+#pragma unroll
+        for (int i = 0; i < NM; ++i) {
+          fw[p][i][u] = bload16(rw[i], in ? vw + 16 * k : LT_OUT, 0);
+          sw[p][i][u] = bload1(rs[i], in ? vs + k : LT_OUT, 0);
+        }
+        if constexpr (X == X_MX4) {
+          fx[p][u][0] = bload16(rx, in ? vx + 16 * k : LT_OUT, 0);
+          sx[p][u] = bload1(rxs, in ? vxs + k : LT_OUT, 0);
+        } else {
+#pragma unroll
+          for (int j = 0; j < 4; ++j) fx[p][u][j] = bload16(rx, in ? vx + 64 * k + 16 * j : LT_OUT, 0);
+        }
+      }
+    };
+    auto use = [&](int p) {
+#pragma unroll
+      for (int u = 0; u < MR_U; ++u) {
+        if constexpr (X == X_MX4) {
+#pragma unroll
+          for (int i = 0; i < NM; ++i)
+            acc[i] = mx_mfma16(__builtin_bit_cast(u32x4_t, fw[p][i][u]), __builtin_bit_cast(u32x4_t, fx[p][u][0]), acc[i], sw[p][i][u], sx[p][u]);
+        } else {
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            u32x4_t x = __builtin_bit_cast(u32x4_t, fx[p][u][j]), lo;
+            if constexpr (X == X_FP16) mx_split(x, x, lo);
+#pragma unroll
+            for (int i = 0; i < NM; ++i) {
+              const u32x4_t v = mx_bf16(__builtin_bit_cast(u32x4_t, fw[p][i][u])[j], __uint_as_float(sw[p][i][u] << 23));
+              acc[i] = lin_mfma16<false>(v, x, acc[i]);
+              if constexpr (X == X_FP16) acc[i] = lin_mfma16<false>(v, lo, acc[i]);
+            }
+          }
+        }
+      }
+    };
+    load(0, w * STEP);
+    for (int base = w * STEP; base < blocks; base += 2 * SPAN) {
+      load(1, base + SPAN);
+      use(0);
+      load(0, base + 2 * SPAN);
+      use(1);
+    }
+#pragma unroll
+    for (int i = 0; i < NM; ++i) red[w][i][lane] = acc[i];
+    __syncthreads();
+    // result (m, n): element n' % 4 of lane 16 (n' / 4) + m', n' = s R + n and m' = s R + m, over the pieces and the waves in order
+    const int cnt = min(R, rows - m0);
+    for (int t = tid; t < R * cnt; t += 64 * MR_WAVES) {
+      const int n = t % R, i_m = t / R;
+      if (n0 + n >= a.N) continue;
+      float sum[NM];
+#pragma unroll
+      for (int i = 0; i < NM; ++i) {
+        sum[i] = 0.f;
+#pragma unroll
+        for (int p = 0; p < SH; ++p) {
+          const int at = p * R + n;
+#pragma unroll
+          for (int v = 0; v < MR_WAVES; ++v) sum[i] += ((const float *)&red[v][i][16 * (at >> 2) + p * R + i_m])[at & 3];
+        }
+      }
+      lin_store<F16, GATED>(o, first + m0 + i_m, n0 + n, sum[0], sum[NM - 1]);
+    }
+    __syncthreads();
+  }
+}
+
+// ---- entry points -------------------------------------------------------------------------------------------------------------
+static bool mx_aligned(const void *codes, int64_t ldc, const void *scales, int64_t lds) {
+  return !(((uintptr_t)codes | (uintptr_t)ldc) & 15) && !(((uintptr_t)scales | (uintptr_t)lds) & 3);
+}
+static bool mx_meet(const void *a, int64_t na, int64_t la, int64_t len_a, const void *b, int64_t nb, int64_t lb, int64_t len_b) {
+  const char *p = (const char *)a, *q = (const char *)b;
+  return p && q && na > 0 && nb > 0 && len_a > 0 && len_b > 0 && p < q + (nb - 1) * lb + len_b && q < p + (na - 1) * la + len_a;
+}
+static int quant_check(const char *who, const void *v, int64_t ldv, int dtype, int64_t M, int K, const void *codes, int64_t ldc,
+                       const void *scales, int64_t lds) {
+  if (M < 0 || K < 0 || K % 32 || dtype < MOE_DT_BF16 || dtype > MOE_DT_FP32 || ldv < K || ldc < K / 2 || lds < K / 32 || M >= 1ll << 40 ||
+      ldv >= 1ll << 40 || ldc >= 1ll << 40 || lds >= 1ll << 40) {
+    moe_set_error("%s: bad shape (M=%lld K=%d dtype=%d, rows %lld, %lld and %lld apart)", who, (long long)M, K, dtype, (long long)ldv,
+                  (long long)ldc, (long long)lds);
+    return MOE_EINVAL;
+  }
+  if (!M || !K) return MOE_OK;
+  const int size = dtype == MOE_DT_FP32 ? 4 : 2;
+  if (!v || !codes || !scales || ((uintptr_t)v & 15) || ldv * size % 16 || !mx_aligned(codes, ldc, scales, 0)) {
+    moe_set_error("%s: rows of values and of codes must be present and on 16-byte boundaries, scales on 4-byte ones", who);
+    return MOE_EINVAL;
+  }
+  const int64_t n = M * (K / 8);
+  if (n / 1024 >= 1 << 24 || (n >= 1ll << 31 && !(ldv == K && ldc == K / 2 && lds == K / 32))) {
+    moe_set_error("%s: %lld x %d values are too many for one launch", who, (long long)M, K);
+    return MOE_EINVAL;
+  }
+  if (mx_meet(v, M, ldv * size, (int64_t)K * size, codes, M, ldc, K / 2) || mx_meet(v, M, ldv * size, (int64_t)K * size, scales, M, lds, K / 32) ||
+      mx_meet(codes, M, ldc, K / 2, scales, M, lds, K / 32)) {
+    moe_set_error("%s: values, codes and scales overlap", who);
+    return MOE_EINVAL;
+  }
+  return MOE_OK;
+}
+static QuantArgs quant_args(const void *x, void *y, void *scales, int64_t ldv, int64_t ldc, int64_t lds, int64_t M, int K, bool *flat) {
+  QuantArgs a{x, y, (uint8_t *)scales, ldv, ldc, lds, M * (K / 8), (u32)K / 8, 0, 0};
+  *flat = M == 1 || (ldv == K && ldc == K / 2 && lds == K / 32);
+  while ((1ull << a.shift) < a.per) ++a.shift;
+  a.magic = (u32)((((1ull << a.shift) - a.per) << 32) / a.per + 1);
+  return a;
+}
+#define QUANT_LAUNCH(KERNEL)                                                                                                     \
+  const dim3 grid((unsigned)((a.n + 256 * QT_U - 1) / (256 * QT_U)));                                                            \
+  hipStream_t s = (hipStream_t)stream;                                                                                           \
+  switch (dtype * 2 + (flat ? 1 : 0)) {                                                                                          \
+    case 0: hipLaunchKernelGGL(HIP_KERNEL_NAME(KERNEL<MOE_DT_BF16, false>), grid, dim3(256), 0, s, a); break;                    \
+    case 1: hipLaunchKernelGGL(HIP_KERNEL_NAME(KERNEL<MOE_DT_BF16, true>), grid, dim3(256), 0, s, a); break;                     \
+    case 2: hipLaunchKernelGGL(HIP_KERNEL_NAME(KERNEL<MOE_DT_FP16, false>), grid, dim3(256), 0, s, a); break;                    \
+    case 3: hipLaunchKernelGGL(HIP_KERNEL_NAME(KERNEL<MOE_DT_FP16, true>), grid, dim3(256), 0, s, a); break;                     \
+    case 4: hipLaunchKernelGGL(HIP_KERNEL_NAME(KERNEL<MOE_DT_FP32, false>), grid, dim3(256), 0, s, a); break;                    \
+    default: hipLaunchKernelGGL(HIP_KERNEL_NAME(KERNEL<MOE_DT_FP32, true>), grid, dim3(256), 0, s, a); break;                    \
+  }
+extern "C" int moe_mx4_quantize(const void *x, int64_t ldx, int dtype, int64_t M, int K, void *codes, int64_t ldc, void *scales,
+                                int64_t lds, void *stream) {
+  if (int rc = quant_check("moe_mx4_quantize", x, ldx, dtype, M, K, codes, ldc, scales, lds)) return rc;
+  if (!M || !K) return MOE_OK;
+  bool flat;
+  const QuantArgs a = quant_args(x, codes, scales, ldx, ldc, lds, M, K, &flat);
+  QUANT_LAUNCH(k_mx4_quantize)
+  return moe_check_launch("k_mx4_quantize");
+}
+extern "C" int moe_mx4_dequantize(const void *codes, int64_t ldc, const void *scales, int64_t lds, int64_t M, int K, void *y, int64_t ldy,
+                                  int dtype, void *stream) {
+  if (int rc = quant_check("moe_mx4_dequantize", y, ldy, dtype, M, K, codes, ldc, scales, lds)) return rc;
+  if (!M || !K) return MOE_OK;
+  bool flat;
+  const QuantArgs a = quant_args(codes, y, (void *)scales, ldy, ldc, lds, M, K, &flat);
+  QUANT_LAUNCH(k_mx4_dequantize)
+  return moe_check_launch("k_mx4_dequantize");
+}
+
+// What the products of both kinds check; xrows: rows of x, experts: matrices
+static int mx_check(const char *who, const MxArgs &a, int xkind, int64_t xrows, int experts, int dtype, bool gated) {
+  const int64_t xlen = xkind == X_MX4 ? a.K / 2 : a.K * 2ll, wlen = a.K / 2, slen = a.K / 32;
+  const bool empty = a.M == 0 || a.N == 0;
+  if (a.M < 0 || a.N < 0 || a.K <= 0 || a.K % 32 || (dtype != MOE_DT_BF16 && dtype != MOE_DT_FP16) || a.act < MOE_ACT_NONE ||
+      a.act > MOE_ACT_RELU2 || a.ldx < xlen || a.ldx % 16 || a.ldx >= 1 << 22 || a.ldw < wlen || a.ldw % 16 || a.ldw >= 1 << 22 ||
+      (xkind == X_MX4 && (a.ldxs < slen || a.ldxs % 4 || a.ldxs >= 1 << 22)) || a.ldws < slen || a.ldws % 4 || a.ldws >= 1 << 22 ||
+      a.ew < 0 || a.ews < 0 || a.ew % 16 || a.ews % 4 || a.ldy < a.N || (a.res && a.ldr < a.N) || a.M > 1 << 26 || a.N > 1 << 26) {
+    moe_set_error("%s: bad shape (M=%d N=%d K=%d dtype=%d act=%d, rows %lld %lld %lld %lld %lld %lld apart)", who, a.M, a.N, a.K, dtype,
+                  a.act, a.ldx, a.ldxs, a.ldw, a.ldws, a.res ? a.ldr : 0, a.ldy);
+    return MOE_EINVAL;
+  }
+  if (empty) return MOE_OK;
+  uintptr_t low = (uintptr_t)a.x, low4 = (uintptr_t)a.xs;
+  bool there = a.x && a.y && (xkind != X_MX4 || a.xs);
+  for (int i = 0; i < (gated ? 2 : 1); ++i) {
+    there = there && a.w[i] && a.ws[i];
+    low |= (uintptr_t)a.w[i];
+    low4 |= (uintptr_t)a.ws[i];
+  }
+  if (!there || (low & 15) || (low4 & 3)) {
+    moe_set_error("%s: operands must be present, x and codes on 16-byte boundaries, scales on 4-byte ones", who);
+    return MOE_EINVAL;
+  }
+  const int64_t e = a.y32 ? 4 : 2, ylen = a.N * e, yld = a.ldy * e;
+  auto meets = [&](const void *p, int64_t rows, int64_t ld, int64_t len) { return mx_meet(a.y, a.M, yld, ylen, p, rows, ld, len); };
+  bool shares = meets(a.x, xrows, a.ldx, xlen) || (xkind == X_MX4 && meets(a.xs, xrows, a.ldxs, slen));
+  for (int i = 0; i < (gated ? 2 : 1); ++i) {
+    shares = shares || meets(a.w[i], 1, 0, (experts - 1) * a.ew + (a.N - 1) * a.ldw + wlen) ||
+             meets(a.ws[i], 1, 0, (experts - 1) * a.ews + (a.N - 1) * a.ldws + slen) || meets(a.bias[i], 1, 0, 2ll * experts * a.N);
+  }
+  const bool in_place = a.res == a.y && !a.y32 && (a.ldr == a.ldy || a.M == 1);
+  if (shares || (!in_place && meets(a.res, a.M, a.ldr * 2, a.N * 2ll))) {
+    moe_set_error("%s: the result overlaps an operand (only a residual may be the result itself)", who);
+    return MOE_EINVAL;
+  }
+  return MOE_OK;
+}
+template <int X, bool F16, bool GATED>
+static int mx_launch(const MxArgs &a, int units, hipStream_t s) {
+  const dim3 grid((a.N + 15) / 16, units);
+  hipLaunchKernelGGL(HIP_KERNEL_NAME(k_mx4_rows<X, F16, GATED, 1>), grid, dim3(64 * MR_WAVES), 0, s, a);
+  return moe_check_launch("k_mx4_rows");
+}
+static int mx_run(const MxArgs &a, int xkind, int dtype, bool gated, int units, hipStream_t s) {
+  const bool f16 = dtype == MOE_DT_FP16;
+  switch ((xkind == X_MX4 ? 0 : 4) + (f16 ? 2 : 0) + (gated ? 1 : 0)) {
+    case 0: return mx_launch<X_MX4, false, false>(a, units, s);
+    case 1: return mx_launch<X_MX4, false, true>(a, units, s);
+    case 2: return mx_launch<X_MX4, true, false>(a, units, s);
+    case 3: return mx_launch<X_MX4, true, true>(a, units, s);
+    case 4: return mx_launch<X_BF16, false, false>(a, units, s);
+    case 5: return mx_launch<X_BF16, false, true>(a, units, s);
+    case 6: return mx_launch<X_FP16, true, false>(a, units, s);
+    default: return mx_launch<X_FP16, true, true>(a, units, s);
+  }
+}
+static MxArgs mx_args(const void *x, int64_t ldx, const moe_mx4 *xq, const moe_mx4 *w, const moe_mx4 *w_up, const void *bias,
+                      const void *bias_up, const void *residual, int64_t ldr, void *y, int64_t ldy, int M, int N, int K, int act, int y_fp32) {
+  MxArgs a{};
+  a.x = xq ? xq->codes : x;
+  a.xs = xq ? (const uint8_t *)xq->scales : nullptr;
+  a.ldx = xq ? xq->ldc : ldx < 1ll << 40 ? ldx * 2 : ldx;
+  a.ldxs = xq ? xq->lds : 0;
+  a.w[0] = (const uint8_t *)w->codes; a.ws[0] = (const uint8_t *)w->scales;
+  if (w_up) { a.w[1] = (const uint8_t *)w_up->codes; a.ws[1] = (const uint8_t *)w_up->scales; }
+  a.ldw = w->ldc; a.ldws = w->lds; a.ew = w->next_c; a.ews = w->next_s;
+  a.bias[0] = (const uint16_t *)bias; a.bias[1] = (const uint16_t *)bias_up; a.res = (const uint16_t *)residual;
+  a.y = y; a.ldr = ldr; a.ldy = ldy; a.M = M; a.N = N; a.K = K; a.act = act; a.y32 = y_fp32 != 0;
+  return a;
+}
+// the descriptions themselves
+static int mx_described(const char *who, const void *x, const moe_mx4 *xq, const moe_mx4 *w, const moe_mx4 *w_up) {
+  if (!w || (x && xq) || (w_up && (w_up->ldc != w->ldc || w_up->lds != w->lds || w_up->next_c != w->next_c || w_up->next_s != w->next_s))) {
+    moe_set_error("%s: one x, a matrix, and for a pair a second one laid out like the first", who);
+    return MOE_EINVAL;
+  }
+  return MOE_OK;
+}
+
+extern "C" int moe_mx4_linear(const void *x, int64_t ldx, const moe_mx4 *xq, const moe_mx4 *w, const moe_mx4 *w_up, const void *bias,
+                              const void *bias_up, const void *residual, int64_t ldr, void *y, int64_t ldy, int M, int N, int K, int dtype,
+                              int act, int y_fp32, void *ws, int64_t ws_bytes, void *stream) {
+  if (int rc = mx_described("moe_mx4_linear", x, xq, w, w_up)) return rc;
+  const MxArgs a = mx_args(x, ldx, xq, w, w_up, bias, bias_up, residual, ldr, y, ldy, M, N, K, act, y_fp32);
+  const int xkind = xq ? X_MX4 : dtype == MOE_DT_FP16 ? X_FP16 : X_BF16;
+  if (int rc = mx_check("moe_mx4_linear", a, xkind, M, 1, dtype, w_up != nullptr)) return rc;
+  if (!M || !N) return MOE_OK;
+  return mx_run(a, xkind, dtype, w_up != nullptr, 1, (hipStream_t)stream);
+}
+
+extern "C" int moe_mx4_experts(const void *x, int64_t ldx, const moe_mx4 *xq, const moe_mx4 *w, const moe_mx4 *w_up, const void *bias,
+                               const void *bias_up, void *y, int64_t ldy, const int *counts, const int *offsets, const moe_unit *units,
+                               int max_units, const int *sorted_tok, int x_rows, int P, int E, int N, int K, int dtype, int act, int y_fp32,
+                               void *stream) {
+  if (int rc = mx_described("moe_mx4_experts", x, xq, w, w_up)) return rc;
+  MxArgs a = mx_args(x, ldx, xq, w, w_up, bias, bias_up, nullptr, 0, y, ldy, P, N, K, act, y_fp32);
+  a.counts = counts; a.offsets = offsets; a.units = units; a.tok = sorted_tok; a.E = E;
+  const int xkind = xq ? X_MX4 : dtype == MOE_DT_FP16 ? X_FP16 : X_BF16;
+  if (E < 1 || E > 1024 || max_units < 0 || x_rows < 0 || (!sorted_tok && x_rows < P) || (P && N && (!counts || !offsets || !units))) {
+    moe_set_error("moe_mx4_experts: bad argument (E=%d P=%d max_units=%d rows of x %d)", E, P, max_units, x_rows);
+    return MOE_EINVAL;
+  }
+  if (int rc = mx_check("moe_mx4_experts", a, xkind, x_rows, E, dtype, w_up != nullptr)) return rc;
+  if (sorted_tok && x_rows * a.ldx >= 1ll << 31) {
+    moe_set_error("moe_mx4_experts: %d rows of tokens %lld bytes apart (less than 2 GiB are needed)", x_rows, a.ldx);
+    return MOE_EINVAL;
+  }
+  if (!P || !N || !max_units) return MOE_OK;
+  return mx_run(a, xkind, dtype, w_up != nullptr, max_units, (hipStream_t)stream);
+}

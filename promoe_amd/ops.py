@@ -580,3 +580,306 @@ def linear_gated(x: torch.Tensor, w_gate: torch.Tensor, w_up: torch.Tensor, b_ga
     """act(x w_gate^T + b_gate) * (x w_up^T + b_up) in one pass (moe_linear_gated): the first half of a gated dense layer.  Types,
     strides and activations as in linear."""
     return _product("linear_gated", x, (w_gate, w_up), (b_gate, b_up), act, None, out, out_dtype)
+
+
+class Mx4:
+    """Rows [..., K] of values in microscaled 4-bit floating point: codes uint8 [..., K / 2], two to a byte with the even column in the
+    low half (sign, two bits of exponent, one of mantissa: 0, 0.5, 1, 1.5, 2, 3, 4, 6), and scales uint8 [..., K / 32], a byte e per 32
+    columns that stands for 2^(e - 127); 255 makes the block NaN.  One matrix [N, K] or one per expert [E, N, K], K a multiple of 32.
+    The tensors are kept as they are where the kernels can read them so: rows of codes on 16-byte and of scales on 4-byte boundaries, with
+    the bytes up to the next one in the same storage.  Others are copied here, once (new tensors of quantize_mx4 never are)."""
+
+    __slots__ = ("codes", "scales", "shape", "desc")
+
+    def __init__(self, codes: torch.Tensor, scales: torch.Tensor):
+        if codes.dtype != torch.uint8 or scales.dtype != torch.uint8 or codes.dim() not in (2, 3) or codes.dim() != scales.dim():
+            raise L.MoeError("Mx4: codes and scales must be uint8 [N, K / 2] and [N, K / 32], or [E, N, ..] each")
+        K = 2 * codes.shape[-1]
+        if K == 0 or K % 32 or scales.shape != (*codes.shape[:-1], K // 32) or scales.device != codes.device:
+            raise L.MoeError("Mx4: codes %s and scales %s (K a multiple of 32, a scale per 32 columns, one device)"
+                             % (tuple(codes.shape), tuple(scales.shape)))
+        if codes.numel():
+            apart = [(n, st) for n, st in zip(codes.shape[:-1], codes.stride()) if n > 1]
+            if codes.stride(-1) != 1 or codes.data_ptr() % 16 or any(st % 16 for _, st in apart) or \
+                    (codes.shape[-2] > 1 and codes.stride(-2) < K // 2):
+                codes = codes.clone(memory_format=torch.contiguous_format)
+            blocks, tail = K // 32, (K // 32 + 3) // 4 * 4
+            apart = [(n, st) for n, st in zip(scales.shape[:-1], scales.stride()) if n > 1]
+            last = scales.storage_offset() + sum((n - 1) * st for n, st in apart) + tail
+            if (scales.stride(-1) != 1 and blocks > 1) or scales.data_ptr() % 4 or any(st % 4 for _, st in apart) or \
+                    (scales.shape[-2] > 1 and scales.stride(-2) < blocks) or last > scales.untyped_storage().nbytes():
+                wide = torch.zeros(*scales.shape[:-1], tail, dtype=torch.uint8, device=scales.device)
+                wide[..., :blocks] = scales
+                scales = wide[..., :blocks]
+        self._set(codes, scales)
+
+    def _set(self, codes, scales):
+        # (of one row the distance to the next is whatever the tensor says: the kernels get one that holds the row)
+        K2, blocks = codes.shape[-1], scales.shape[-1]
+        n = codes.shape[-2]
+        ldc, lds = (codes.stride(-2), scales.stride(-2)) if n > 1 else (K2, (blocks + 3) // 4 * 4)
+        next_c, next_s = (codes.stride(0), scales.stride(0)) if codes.dim() == 3 and codes.shape[0] > 1 else (0, 0)
+        self.codes, self.scales, self.shape = codes, scales, (*codes.shape[:-1], 2 * K2)
+        self.desc = L.Mx4Desc(codes.data_ptr(), scales.data_ptr(), ldc, lds, next_c, next_s)
+        return self
+
+    def __repr__(self):
+        return "Mx4(%s, %s)" % (list(self.shape), self.codes.device)
+
+
+def quantize_mx4(x: torch.Tensor) -> Mx4:
+    """Rows [..., K] of bf16, fp16 or fp32 to microscaled 4-bit floating point (moe_mx4_quantize): the scale of 32 columns is
+    2^(floor(log2 of their largest magnitude) - 2), at least 2^-127, codes go to the nearest (ties to the even code, 6 beyond 6); a block
+    with a NaN or an infinity becomes NaN.  K is a multiple of 32; x [N, K] may have its rows further apart (16-byte boundaries), x [E, N, K]
+    is contiguous."""
+    code = L.ROW_DTYPES.get(x.dtype)
+    if code is None or x.dim() not in (2, 3) or x.shape[-1] == 0 or x.shape[-1] % 32:
+        raise L.MoeError("quantize_mx4: bf16, fp16 or fp32 [N, K] or [E, N, K] with K a multiple of 32 are needed, not %s %s"
+                         % (x.dtype, tuple(x.shape)))
+    index = _operands("quantize_mx4", x)
+    if index != torch.cuda.current_device():
+        with torch.cuda.device(index):
+            return quantize_mx4(x)
+    K = x.shape[-1]
+    M = x.numel() // K
+    if x.dim() == 2:
+        ldx = _rows("quantize_mx4", x, M, K)
+    elif x.is_contiguous():
+        ldx = K
+    else:
+        raise L.MoeError("quantize_mx4: [E, N, K] must be contiguous")
+    blocks = K // 32
+    lds = (blocks + 3) // 4 * 4
+    codes = torch.empty((*x.shape[:-1], K // 2), dtype=torch.uint8, device=x.device)
+    scales = torch.empty((*x.shape[:-1], lds), dtype=torch.uint8, device=x.device)
+    rc = lib.moe_mx4_quantize(x.data_ptr(), ldx, code, M, K, codes.data_ptr(), K // 2, scales.data_ptr(), lds, _raw_stream(index))
+    if rc:
+        check(rc, "quantize_mx4")
+    return Mx4.__new__(Mx4)._set(codes, scales if lds == blocks else scales[..., :blocks])
+
+
+def dequantize_mx4(q: Mx4, dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
+    """The values of q as a new tensor (moe_mx4_dequantize).  Exact in bf16 and fp32 but for scales above 2^125, whose largest codes are
+    past their range; rounded in fp16."""
+    code = L.ROW_DTYPES.get(dtype)
+    if code is None or not isinstance(q, Mx4):
+        raise L.MoeError("dequantize_mx4: an Mx4 into bf16, fp16 or fp32")
+    index = _operands("dequantize_mx4", q.codes, q.scales)
+    if index != torch.cuda.current_device():
+        with torch.cuda.device(index):
+            return dequantize_mx4(q, dtype)
+    N, K = q.shape[-2:]
+    y = torch.empty(q.shape, dtype=dtype, device=q.codes.device)
+    d, size = q.desc, y.element_size()
+    parts = [(0, y.numel() // K)]
+    if len(q.shape) == 3 and q.shape[0] > 1 and N and not (d.next_c == N * d.ldc and d.next_s == N * d.lds):
+        parts = [(e, N) for e in range(q.shape[0])]       # (matrices that are not end to end go one by one)
+    for e, rows in parts:
+        check(lib.moe_mx4_dequantize((d.codes or 0) + e * d.next_c, d.ldc, (d.scales or 0) + e * d.next_s, d.lds, rows, K,
+                                     y.data_ptr() + e * N * K * size, K, code, _raw_stream(index)), "dequantize_mx4")
+    return y
+
+
+def _product_mx4(what, x, mats, biases, act, residual, out, out_dtype, d=None, of_tokens=False):
+    w = mats[0]
+    quantised = isinstance(x, Mx4)
+    if not all(isinstance(m, Mx4) for m in mats) or len(w.shape) != (2 if d is None else 3) or any(m.shape != w.shape for m in mats):
+        raise L.MoeError("%s: weights must be Mx4 %s, both of a pair of one shape" % (what, "[N, K]" if d is None else "[E, N, K]"))
+    if quantised:
+        dtype = next((t for t in (out_dtype, None if out is None else out.dtype) if t in L.DTYPES), None)
+        if dtype is None:
+            dtype = next((t.dtype for t in (*biases, residual) if t is not None), torch.bfloat16)
+    else:
+        dtype = x.dtype
+    code = L.DTYPES.get(dtype)
+    if code is None or act not in L.ACTS:
+        raise L.MoeError("%s: an x of bf16, fp16 or Mx4 and one of the activations %s" % (what, sorted(L.ACTS)))
+    parts = [t for m in mats for t in (m.codes, m.scales)]
+    first = x.codes if quantised else x
+    index = _operands(what, first, *parts, *((x.scales,) if quantised else ()), *biases, residual, out,
+                      *((d.counts, d.offsets, d.units, d.sorted_tok) if d is not None else ()))
+    if index != torch.cuda.current_device():
+        with torch.cuda.device(index):
+            return _product_mx4(what, x, mats, biases, act, residual, out, out_dtype, d, of_tokens)
+    if len(x.shape) != 2:
+        raise L.MoeError("%s: x must be [M, K]" % what)
+    rows, K = x.shape
+    N = w.shape[-2]
+    if w.shape[-1] != K:
+        raise L.MoeError("%s: rows of %d columns and weights of %d" % (what, K, w.shape[-1]))
+    M = rows
+    if d is not None:
+        M = d.T * d.k
+        if rows != (d.T if of_tokens else M) or w.shape[0] != d.E:
+            raise L.MoeError("%s: %d rows and %d matrices for %d tokens, %d choices each, of %d experts"
+                             % (what, rows, w.shape[0], d.T, d.k, d.E))
+    ldx = 0 if quantised else _rows(what, x, rows, K)
+    wd = w.desc
+    for m in mats[1:]:
+        md = m.desc
+        if (md.ldc, md.lds, md.next_c, md.next_s) != (wd.ldc, wd.lds, wd.next_c, wd.next_s):
+            raise L.MoeError("%s: both matrices of a pair must have the same strides" % what)
+    for b in biases:
+        if b is not None and (b.dtype != dtype or b.shape != w.shape[:-1] or not b.is_contiguous()):
+            raise L.MoeError("%s: a bias must be %s %s, contiguous" % (what, dtype, list(w.shape[:-1])))
+    ldr = 0
+    if residual is not None:
+        if residual.dtype != dtype:
+            raise L.MoeError("%s: the residual must be %s" % (what, dtype))
+        ldr = _rows(what, residual, M, N)
+    if out is None:
+        out = torch.empty((M, N), dtype=out_dtype or dtype, device=first.device)
+        ldy = N
+    else:
+        ldy = _rows(what, out, M, N)
+        if out_dtype is not None and out.dtype != out_dtype:
+            raise L.MoeError("%s: out is %s, asked for was %s" % (what, out.dtype, out_dtype))
+    y32 = out.dtype == torch.float32
+    if not y32 and out.dtype != dtype:
+        raise L.MoeError("%s: results are %s or fp32" % (what, dtype))
+    xp, xq = (0, byref(x.desc)) if quantised else (x.data_ptr(), None)
+    up, b_up = (byref(mats[1].desc), ptr(biases[1])) if len(mats) == 2 else (None, 0)
+    if d is None:
+        rc = lib.moe_mx4_linear(xp, ldx, xq, byref(wd), up, ptr(biases[0]), b_up, ptr(residual), ldr, out.data_ptr(), ldy, M, N, K, code,
+                                L.ACTS[act], y32, 0, 0, _raw_stream(index))
+    else:
+        rc = lib.moe_mx4_experts(xp, ldx, xq, byref(wd), up, ptr(biases[0]), b_up, out.data_ptr(), ldy, d.counts.data_ptr(),
+                                 d.offsets.data_ptr(), d.units.data_ptr(), d.max_units, d.sorted_tok.data_ptr() if of_tokens else 0, rows,
+                                 M, d.E, N, K, code, L.ACTS[act], y32, _raw_stream(index))
+    if rc:
+        check(rc, what)
+    return out
+
+
+def linear_mx4(x, w: Mx4, bias: torch.Tensor | None = None, act: str = "none", residual: torch.Tensor | None = None,
+               out: torch.Tensor | None = None, out_dtype: torch.dtype | None = None):
+    """act(x w^T + bias) + residual in one pass (moe_mx4_linear), w [N, K] an Mx4.  x [M, K] either bf16 or fp16, whose values take part
+    as they are, or an Mx4 (quantize_mx4), then both operands go to the matrix cores in 4 bits.  bias, residual and the result are of
+    x's type, or for an Mx4 all bf16 or all fp16 (the result: out_dtype, else theirs, else bf16); out_dtype fp32 leaves the sums in 32
+    bits.  Activations, strides and the rest as in linear, K a multiple of 32."""
+    return _product_mx4("linear_mx4", x, (w,), (bias,), act, residual, out, out_dtype)
+
+
+def linear_gated_mx4(x, w_gate: Mx4, w_up: Mx4, b_gate: torch.Tensor | None = None, b_up: torch.Tensor | None = None, act: str = "silu",
+                     out: torch.Tensor | None = None, out_dtype: torch.dtype | None = None):
+    """act(x w_gate^T + b_gate) * (x w_up^T + b_up) in one pass; types as in linear_mx4, both matrices with the same strides."""
+    return _product_mx4("linear_gated_mx4", x, (w_gate, w_up), (b_gate, b_up), act, None, out, out_dtype)
+
+
+def experts_linear_mx4(x, w: Mx4, d: Dispatch, bias: torch.Tensor | None = None, act: str = "none", of_tokens: bool = False,
+                       out: torch.Tensor | None = None, out_dtype: torch.dtype | None = None):
+    """act(x w[e]^T + bias[e]) for the rows of every expert e of a dispatch in one call (moe_mx4_experts): w [E, N, K], bias [E, N].
+    x [T*k, K] has its rows in the dispatch's order (sort_tokens, or what the first half of the experts left), or, with of_tokens, a row
+    for each token.  The result [T*k, N] is in the dispatch's order; rows behind the last pair are left as they were.  Types as in
+    linear_mx4."""
+    return _product_mx4("experts_linear_mx4", x, (w,), (bias,), act, None, out, out_dtype, d, of_tokens)
+
+
+def experts_gated_mx4(x, w_gate: Mx4, w_up: Mx4, d: Dispatch, b_gate: torch.Tensor | None = None, b_up: torch.Tensor | None = None,
+                      act: str = "silu", of_tokens: bool = False, out: torch.Tensor | None = None,
+                      out_dtype: torch.dtype | None = None):
+    """act(x w_gate[e]^T + b_gate[e]) * (x w_up[e]^T + b_up[e]): the first half of every expert, arguments as in experts_linear_mx4."""
+    return _product_mx4("experts_gated_mx4", x, (w_gate, w_up), (b_gate, b_up), act, None, out, out_dtype, d, of_tokens)
+
+
+def _sort(x, d, out=None):
+    T, k, H = d.T, d.k, x.shape[1]
+    ldx = _rows("sort_tokens", x, T, H)
+    y = torch.empty(T * k, H, dtype=x.dtype, device=x.device) if out is None else out
+    index = x.get_device()
+    rc = lib.moe_sort_rows(x.data_ptr(), ldx, y.data_ptr(), _rows("sort_tokens", y, T * k, H), d.pos_of_pair.data_ptr(),
+                           d.offsets.data_ptr() + 4 * d.E, T, k, H, L.ROW_DTYPES[x.dtype], _raw_stream(index))
+    if rc:
+        check(rc, "sort_tokens")
+    return y
+
+
+def _unsort(x, d, w, out=None):
+    T, k, H = d.T, d.k, x.shape[1]
+    ldx = _rows("unsort_tokens", x, T * k, H)
+    y = torch.empty(T, H, dtype=x.dtype, device=x.device) if out is None else out
+    rc = lib.moe_unsort_rows(x.data_ptr(), ldx, y.data_ptr(), _rows("unsort_tokens", y, T, H), d.pos_of_pair.data_ptr(), ptr(w), T, k, H,
+                             L.ROW_DTYPES[x.dtype], _raw_stream(x.get_device()))
+    if rc:
+        check(rc, "unsort_tokens")
+    return y
+
+
+def _whole_rows(t):
+    """A gradient as autograd hands it over (an expanded one, say) with rows that the kernels can read."""
+    return t if t.dim() == 2 and (t.stride(1) == 1 or t.shape[1] <= 1) and t.stride(0) >= t.shape[1] else t.contiguous()
+
+
+class _SortTokens(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, d):
+        ctx.d = d
+        return _sort(x, d)
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dy):
+        with torch.cuda.device(dy.device):
+            return _unsort(_whole_rows(dy), ctx.d, None), None
+
+
+class _UnsortTokens(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, w, d):
+        ctx.d = d
+        ctx.save_for_backward(x, w)
+        return _unsort(x, d, w)
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dy):
+        d, (x, w), dy = ctx.d, ctx.saved_tensors, _whole_rows(dy)
+        need_x, need_w = ctx.needs_input_grad[0], w is not None and ctx.needs_input_grad[1]
+        with torch.cuda.device(dy.device):
+            if w is None:
+                return _sort(dy, d), None, None
+            T, k, H = d.T, d.k, x.shape[1]
+            dx = torch.empty(x.shape, dtype=x.dtype, device=x.device) if need_x else None
+            dw = torch.empty(T, k, dtype=torch.float32, device=x.device) if need_w else None
+            check(lib.moe_unsort_rows_grad(dy.data_ptr(), _rows("unsort_tokens", dy, T, H), x.data_ptr(), _rows("unsort_tokens", x, T * k, H),
+                                           d.pos_of_pair.data_ptr(), w.data_ptr(), d.offsets.data_ptr() + 4 * d.E, ptr(dx), H, ptr(dw),
+                                           T, k, H, L.ROW_DTYPES[x.dtype], _raw_stream(x.get_device())), "unsort_tokens")
+        return dx, dw, None
+
+
+def _move_args(what, x, d, rows, w):
+    if x.dim() != 2 or x.dtype not in L.ROW_DTYPES or x.shape[0] != rows:
+        raise L.MoeError("%s: bf16, fp16 or fp32 [%d, H] is needed, not %s %s" % (what, rows, x.dtype, tuple(x.shape)))
+    if w is not None and (w.dtype != torch.float32 or w.shape != (d.T, d.k) or not w.is_contiguous()):
+        raise L.MoeError("%s: weights must be fp32 [%d, %d], contiguous" % (what, d.T, d.k))
+    index = x.get_device()
+    if index < 0 or any(t is not None and t.get_device() != index for t in (w, d.pos_of_pair, d.offsets)):
+        raise L.MoeError("%s: x, weights and dispatch must be on one GPU" % what)
+    _rows(what, x, rows, x.shape[1])
+    return index
+
+
+def sort_tokens(x: torch.Tensor, d: Dispatch) -> torch.Tensor:
+    """The tokens' rows x [T, H] in the order of their experts: [T*k, H], a token's row once for each of its choices (moe_sort_rows).
+    Choices of no expert (idx outside 0 .. E - 1) have no row; the rows behind the last one are zero.  Any alignment and row stride, bf16,
+    fp16 or fp32.  With a gradient (each token the sum of its rows', in fp32): d has to keep its contents until the backward pass."""
+    index = _move_args("sort_tokens", x, d, d.T, None)
+    if index != torch.cuda.current_device():
+        with torch.cuda.device(index):
+            return sort_tokens(x, d)
+    if torch.is_grad_enabled() and x.requires_grad:
+        return _SortTokens.apply(x, d)
+    return _sort(x, d)
+
+
+def unsort_tokens(x: torch.Tensor, d: Dispatch, w: torch.Tensor | None = None) -> torch.Tensor:
+    """The experts' rows x [T*k, H] back to their tokens: y[t] = sum over the choices of w[t, j] x[row of (t, j)] (moe_unsort_rows; w fp32
+    [T, k], or 1), in fp32 and in the order of the choices, rounded once to x's type.  Choices of no expert add nothing, whatever lies
+    behind the last row.  With gradients of x and w: d has to keep its contents until the backward pass."""
+    index = _move_args("unsort_tokens", x, d, d.T * d.k, w)
+    if index != torch.cuda.current_device():
+        with torch.cuda.device(index):
+            return unsort_tokens(x, d, w)
+    if torch.is_grad_enabled() and (x.requires_grad or (w is not None and w.requires_grad)):
+        return _UnsortTokens.apply(x, w, d)
+    return _unsort(x, d, w)
