@@ -539,7 +539,7 @@ int moe_mx4_dequantize(const void *codes, int64_t ldc, const void *scales, int64
  * as for moe_linear.
  * moe_mx4_experts: the same for every expert e of a dispatch: rows offsets[e] .. + counts[e] of y are the product of those rows of x, or,
  * with sorted_tok, of the rows sorted_tok[..] of x (x_rows of them), with matrix e; bias [E, N].  Rows behind the last pair are left as
- * they were.  E <= 1024. */
+ * they were.  E <= 1024, max_units >= min(E, P). */
 int moe_mx4_linear(const void *x, int64_t ldx, const moe_mx4 *xq_host, const moe_mx4 *w_host, const moe_mx4 *w_up_host, const void *bias,
                    const void *bias_up, const void *residual, int64_t ldr, void *y, int64_t ldy, int M, int N, int K, int dtype, int act,
                    int y_fp32, void *ws, int64_t ws_bytes, void *stream);

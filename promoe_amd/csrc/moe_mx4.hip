@@ -277,6 +277,297 @@ __global__ __launch_bounds__(64 * MR_WAVES) void k_mx4_rows(const MxArgs a) {
   }
 }
 
+// ---- tiles ----------------------------------------------------------------------------------------------------------------------
+// Where a workgroup works.  Dense: tile (mt, nt) of rows and columns and a piece of K.  By expert: the tiles of an expert's rows by nt; the
+// counts of all experts are added up by every wave, the host does not know them.
+struct MxTile { int m0, m_end, n0, e, split; };  // rows m0 .. m_end - 1 of y at most
+template <int BM, int NC>
+static __device__ __forceinline__ bool mx_tile_of(const MxArgs &a, int v, MxTile &t) {
+  const int lane = threadIdx.x & 63;
+  int nm = a.nm, r, first = 0, rows = a.M, e = 0;
+  if (!a.units) {
+    const int tiles = nm * a.nn;
+    if (v >= tiles * a.splits) return false;
+    t.split = v / tiles;
+    r = v - t.split * tiles;
+  } else {
+    // lane l has the experts per l .. per l + per - 1
+    const int per = (a.E + 63) >> 6;
+    int mine = 0;
+    for (int i = 0; i < per; ++i) {
+      const int x = per * lane + i;
+      mine += x < a.E ? (a.counts[x] + BM - 1) / BM : 0;
+    }
+    int upto = mine;
+#pragma unroll
+    for (int d = 1; d < 64; d <<= 1) {
+      const int o = __shfl_up(upto, d, 64);
+      if (lane >= d) upto += o;
+    }
+    const int mt_all = __builtin_amdgcn_readlane(upto, 63);
+    if (v >= mt_all * a.nn) return false;
+    // (tiles come expert by expert: v / nn is one of its tiles' rows, whichever)
+    const int at = v / a.nn;
+    const unsigned long long over = __ballot(upto > at);
+    const int l = (int)__builtin_ctzll(over);
+    int before = __builtin_amdgcn_readlane(upto - mine, l);
+    e = per * l;
+    int count = 0;
+    for (;; ++e) {
+      count = a.counts[e];
+      nm = (count + BM - 1) / BM;
+      if (before + nm > at || e == a.E - 1) break;
+      before += nm;
+    }
+    r = v - before * a.nn;
+    first = a.offsets[e];
+    rows = count;
+    t.split = 0;
+  }
+  // four rows of tiles wide
+  const int group = r / (4 * a.nn), in = r - group * 4 * a.nn, wide = min(4, nm - 4 * group);
+  const int nt = in / wide, mt = 4 * group + in - nt * wide;
+  t.m0 = __builtin_amdgcn_readfirstlane(first + mt * BM);
+  t.m_end = __builtin_amdgcn_readfirstlane(first + rows);
+  t.n0 = __builtin_amdgcn_readfirstlane(nt * NC);
+  t.e = __builtin_amdgcn_readfirstlane(e);
+  t.split = __builtin_amdgcn_readfirstlane(t.split);
+  return true;
+}
+// workgroup i runs on XCD i % 8: each XCD takes a contiguous run of tiles
+static __device__ __forceinline__ int mx_run_of() {
+  const int per = (int)gridDim.x >> 3;
+  return ((int)blockIdx.x & 7) * per + ((int)blockIdx.x >> 3);
+}
+// what the epilogue of a tile goes by
+static __device__ __forceinline__ MxArgs mx_out(const MxArgs &a, const MxTile &t) {
+  MxArgs o = a;
+  if (o.bias[0]) o.bias[0] += (long long)t.e * a.N;
+  if (o.bias[1]) o.bias[1] += (long long)t.e * a.N;
+  o.M = t.m_end;
+  return o;
+}
+// The end of a tile of 2 x 2 waves with WM x WN blocks of 32 x 32 each (a gated pair's W blocks alternate between the matrices): the sums of
+// rows from m0 and columns from n0 on, through the LDS that `ring` is.
+template <bool F16, bool GATED, int WM, int WN>
+static __device__ __forceinline__ void mx_tile_out(const MxArgs &a, const f32x16_t (&acc)[WM][WN], unsigned char *ring, int m0, int n0, int split) {
+  constexpr int NC = GATED ? 32 * WN : 64 * WN;
+  const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6), wm = w & 1, wn = w >> 1;
+  const int fr = lane & 31, q = lane >> 5;
+  // The sums leave through LDS, 32 rows of the wave at a time, so that a lane then has 8 adjacent columns of a row and the rest is
+  // one loop of whole lines.  Element e of a lane: column 8 (e / 4) + 4 q + e % 4 of W's block, row fr of x's.
+  LT_VM(0);
+  __syncthreads();
+  constexpr int LDE = 32 * WN + 4;                       // floats between rows: 16 lanes that write 16 bytes each fall on all banks
+  constexpr int LPR = NC / 16, RPP = 64 / LPR;           // lanes of a row (8 columns each), rows of a pass
+  float *buf = (float *)ring + w * 32 * LDE;
+  const int col = 8 * (lane % LPR), n = n0 + wn * (NC / 2) + col;
+  const int at = GATED ? (col >> 5) * 64 + (col & 31) : col;
+  const LinColumns<F16, GATED> c(a, n);
+  // (one copy of the loop for all blocks: code that runs once a tile waits for its instructions, line by line)
+#pragma clang loop unroll(disable)
+  for (int i = 0; i < WM; ++i) {
+    lt_each<WM>([&](auto i_) {
+      if (i == decltype(i_)::value) {
+#pragma unroll
+        for (int b = 0; b < WN; ++b)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const f32x16_t &s = acc[decltype(i_)::value][b];
+            *(f32x4_t *)(buf + fr * LDE + 32 * b + 8 * e + 4 * q) = f32x4_t{s[4 * e], s[4 * e + 1], s[4 * e + 2], s[4 * e + 3]};
+          }
+        __asm__ volatile("; %0" :: "i"(decltype(i_)::value));  // (or the compiler makes one copy of them, over registers chosen by i)
+      }
+    });
+    __builtin_amdgcn_wave_barrier();
+    const int first = m0 + 32 * (wm * WM + i) + lane / LPR;
+    u32x4_t res = c.residual(a, first);
+#pragma clang loop unroll(disable)
+    for (int r = lane / LPR; r < 32; r += RPP) {
+      const int m = first - lane / LPR + r;
+      const u32x4_t ahead = c.residual(a, r + RPP < 32 ? m + RPP : a.M);
+      if (m < a.M) {
+        if (a.part) c.partial(a, split, m, buf + r * LDE + at, buf + r * LDE + at + 32);
+        else c.store(a, m, buf + r * LDE + at, buf + r * LDE + at + 32, res);
+      }
+      res = ahead;
+    }
+    __builtin_amdgcn_wave_barrier();
+  }
+}
+
+// The pieces of K added in their order, then what a tile kernel does behind its sums: eight columns a thread of 256
+template <bool F16, bool GATED>
+__global__ __launch_bounds__(256) void k_mx4_join(const MxArgs a) {
+  const int per = a.ldp >> 3;
+  const long long t = (long long)blockIdx.x * 256 + threadIdx.x;
+  const int m = (int)(t / per), n = (int)(t - (long long)m * per) * 8;
+  if (m >= a.M) return;
+  float s[2][8] = {};
+  constexpr int NM = GATED ? 2 : 1;
+  const long long step = (long long)a.M * a.ldp;
+  for (int p = 0; p < a.splits; ++p)
+#pragma unroll
+    for (int i = 0; i < NM; ++i) {
+      const float *q = a.part + (p * NM + i) * step + (long long)m * a.ldp + n;
+      const f32x4_t u = *(const f32x4_t *)q, v = *(const f32x4_t *)(q + 4);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) { s[i][e] += u[e]; s[i][4 + e] += v[e]; }
+    }
+  const LinColumns<F16, GATED> c(a, n);
+  c.store(a, m, s[0], s[1], c.residual(a, m));
+}
+
+// x in 4 bits.  Four waves (2 x 2), wave (wm, wn) on WM x WN blocks of 32 x 32: a tile of 64 WM rows of x by 64 WN rows of W.  A gated
+// pair's W blocks alternate between the two matrices (block b: matrix b & 1, its columns 32 (b >> 1) ..), so that a lane holds both sums
+// of a column.  K advances 256 at a time (a slab: 128 bytes of codes and 8 of scales a row); slabs go global -> LDS directly, RING of them
+// in LDS.  A lane's operand of a product is one block of 32 columns: half q of the wave takes the blocks 4 q .. 4 q + 3 of a slab, so that
+// the scales of a fragment's four steps are one word, a byte a step.
+#define M4_K 256
+static __device__ __forceinline__ void mx_dma16(unsigned at, int off, lt_rsrc_t rs, int soff) {
+  // (assembly: told that a load writes LDS, the compiler would wait for all of them in front of every barrier and LDS read; the waits
+  // stand by hand)
+  __asm__ volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, %3 offen lds"
+                   :: "s"(at), "v"(off), "s"(rs), "s"(soff) : "memory", "m0");
+}
+static __device__ __forceinline__ void mx_dma4(unsigned at, int off, lt_rsrc_t rs, int soff) {
+  __asm__ volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dword %1, %2, %3 offen lds"
+                   :: "s"(at), "v"(off), "s"(rs), "s"(soff) : "memory", "m0");
+}
+typedef __attribute__((address_space(3))) const u32x4_t lds_u4;
+typedef __attribute__((address_space(3))) const u32 lds_u1;
+template <int S>
+static __device__ __forceinline__ f32x16_t mx_mfma32(u32x4_t a, u32x4_t b, f32x16_t c, u32 sa, u32 sb) {
+  const i32x8_t a8{(int)a[0], (int)a[1], (int)a[2], (int)a[3], 0, 0, 0, 0}, b8{(int)b[0], (int)b[1], (int)b[2], (int)b[3], 0, 0, 0, 0};
+  return __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(a8, b8, c, 4, 4, S, (int)sa, S, (int)sb);
+}
+// the bytes of a word of scales that stand for blocks in front of the last, `left` of them; what lies behind may be anything, NaN too
+static __device__ __forceinline__ u32 mx_mask(int left) { return left >= 4 ? ~0u : left <= 0 ? 0u : (1u << 8 * left) - 1u; }
+
+template <bool F16, bool GATED, int WM, int WN, int RING>
+__global__ __launch_bounds__(256, RING * (WM + WN) * 64 * 136 > 80 * 1024 ? 1 : 2) void k_mx4_tile(const MxArgs a) {
+  constexpr int BM = 64 * WM, BN = 64 * WN, NX = 2 * WM, NW = 2 * WN, NS = (WM + WN + 1) / 2, NG = WM * WN, NT = NX + NW + NS;
+  constexpr int CODES = (BM + BN) * 128, SLAB = CODES + NS * 1024, NC = GATED ? BN / 2 : BN;
+  __shared__ __align__(1024) unsigned char s_ring[RING * SLAB];
+  const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6), wm = w & 1, wn = w >> 1;
+  const int fr = lane & 31, q = lane >> 5;
+  MxTile t;
+  if (!mx_tile_of<BM, NC>(a, mx_run_of(), t)) return;
+  const unsigned lds = (unsigned)(uintptr_t)(__attribute__((address_space(3))) unsigned char *)s_ring;
+  const uint8_t *w0 = a.w[0] + t.e * a.ew + t.n0 * a.ldw, *w1 = a.w[GATED ? 1 : 0] + t.e * a.ew + t.n0 * a.ldw;
+  const uint8_t *ws0 = a.ws[0] + t.e * a.ews + t.n0 * a.ldws, *ws1 = a.ws[GATED ? 1 : 0] + t.e * a.ews + t.n0 * a.ldws;
+  const long long xbase = a.tok ? 0 : t.m0;
+  const lt_rsrc_t rx = lt_rsrc((const uint8_t *)a.x + xbase * a.ldx), rxs = lt_rsrc(a.xs + xbase * a.ldxs);
+  const lt_rsrc_t rw0 = lt_rsrc(w0), rw1 = lt_rsrc(w1), rs0 = lt_rsrc(ws0), rs1 = lt_rsrc(ws1);
+  auto xrow = [&](int i) {  // row i of the tile in x, from xbase on
+    const int m = min(t.m0 + i, t.m_end - 1);
+    return a.tok ? a.tok[m] : m - t.m0;
+  };
+  auto wrow = [&](int i) { return min(t.n0 + i, a.N - 1) - t.n0; };
+  // transfer i of wave w: rows 32 i + 8 w .. + 7, eight lanes a row; the lanes choose the chunk that belongs in their slot (chunk c of row
+  // r in slot c ^ ((r >> 1) & 7)).  Scales: 32 rows a transfer, a word for each half of the wave, transfer 4 i + w of x's blocks and then W's.
+  const int tr = 8 * w + (lane >> 3), chunk = (lane & 7) ^ ((tr >> 1) & 7);
+  int vx[NX], vw[NW], vs[NS];
+#pragma unroll
+  for (int i = 0; i < NX; ++i) vx[i] = xrow(32 * i + tr) * (int)a.ldx + 16 * chunk;
+#pragma unroll
+  for (int i = 0; i < NW; ++i) vw[i] = wrow(32 * (GATED ? i >> 1 : i) + tr) * (int)a.ldw + 16 * chunk;
+  lt_rsrc_t rsc[NS];
+#pragma unroll
+  for (int i = 0; i < NS; ++i) {
+    const int b = 4 * i + w, bw = b - NX;
+    if (b < NX) { vs[i] = xrow(32 * b + (lane >> 1)) * (int)a.ldxs + 4 * (lane & 1); rsc[i] = rxs; }
+    else {
+      vs[i] = b < NX + NW ? wrow(32 * (GATED ? bw >> 1 : bw) + (lane >> 1)) * (int)a.ldws + 4 * (lane & 1) : LT_OUT;
+      rsc[i] = GATED && (bw & 1) ? rs1 : rs0;
+    }
+  }
+  const int kt0 = t.split * a.slabs + min(t.split, a.extra), nk = kt0 + a.slabs + (t.split < a.extra);
+  const int blocks = min(a.K >> 5, nk * (M4_K / 32));        // (past the last block: zeros)
+  auto dma = [&](int i, int kt, int place) {
+    if (i < NX + NW) {
+      const bool in = kt * 8 + chunk < blocks;
+      mx_dma16(lds + (unsigned)(place + (i * 32 + 8 * w) * 128), in ? (i < NX ? vx[i < NX ? i : 0] : vw[i < NX ? 0 : i - NX]) : LT_OUT,
+               i < NX ? rx : (GATED && ((i - NX) & 1)) ? rw1 : rw0, kt * (M4_K / 2));
+    } else {
+      const int s = i - NX - NW;
+      const bool in = kt * 8 + 4 * (lane & 1) < blocks;
+      mx_dma4(lds + (unsigned)(place + CODES + (4 * s + w) * 256), in ? vs[s] : LT_OUT, rsc[s], kt * 8);
+    }
+  };
+  unsigned ax[4], aw[4];  // LDS address of the lane's fragment of step j in block 0, of rows that begin where the ring does
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    const unsigned c = (unsigned)(((4 * q + j) ^ ((fr >> 1) & 7)) * 16);
+    ax[j] = lds + (unsigned)((wm * WM * 32 + fr) * 128) + c;
+    aw[j] = lds + (unsigned)((BM + wn * WN * 32 + fr) * 128) + c;
+  }
+  const unsigned asx = lds + CODES + (unsigned)((wm * WM * 32 + fr) * 8 + 4 * q), asw = lds + CODES + (unsigned)((BM + wn * WN * 32 + fr) * 8 + 4 * q);
+  f32x16_t acc[WM][WN];
+#pragma unroll
+  for (int i = 0; i < WM; ++i)
+#pragma unroll
+    for (int b = 0; b < WN; ++b)
+#pragma unroll
+      for (int e = 0; e < 16; ++e) acc[i][b][e] = 0.f;
+  // A slab's products are short, a step of them shorter than an LDS read: the fragments of the whole next slab are read between this
+  // one's.  At the barrier everybody has this slab's fragments, so its slot is free, and the next has landed.
+#pragma unroll
+  for (int i = 0; i < RING; ++i)
+#pragma unroll
+    for (int d = 0; d < NT; ++d) dma(d, kt0 + i, i * SLAB);
+  LT_VM((RING - 1) * NT);
+  __builtin_amdgcn_s_barrier();
+  u32x4_t fx[2][4][WM], fw[2][4][WN];
+  u32 sx[2][WM], sw[2][WN];
+  auto read = [&](int p, int r, unsigned place) {  // fragment r of a slab: scales, then step by step
+    if (r < WM) sx[p][r] = *(lds_u1 *)(uintptr_t)(asx + place + (unsigned)(r * 256));
+    else if (r < WM + WN) sw[p][r - WM] = *(lds_u1 *)(uintptr_t)(asw + place + (unsigned)((r - WM) * 256));
+    else {
+      const int s = r - WM - WN, j = s / (WM + WN), i = s % (WM + WN);
+      if (i < WM) fx[p][j][i] = *(lds_u4 *)(uintptr_t)(ax[j] + place + (unsigned)(i * 32 * 128));
+      else fw[p][j][i - WM] = *(lds_u4 *)(uintptr_t)(aw[j] + place + (unsigned)((i - WM) * 32 * 128));
+    }
+  };
+  constexpr int NR = 5 * (WM + WN), NP = 4 * NG;
+#pragma unroll
+  for (int r = 0; r < NR; ++r) read(0, r, 0);
+  int slot = 0;
+  auto step = [&](auto p_, int kt) {
+    constexpr int p = decltype(p_)::value;
+    const int next = slot + 1 < RING ? slot + 1 : 0;
+    LT_LGKM0();
+    LT_VM((RING - 2) * NT);
+    __builtin_amdgcn_s_barrier();
+    const u32 mask = mx_mask(blocks - kt * 8 - 4 * q);
+#pragma unroll
+    for (int i = 0; i < WM; ++i) sx[p][i] &= mask;
+#pragma unroll
+    for (int i = 0; i < WN; ++i) sw[p][i] &= mask;
+    __builtin_amdgcn_sched_barrier(0);
+    lt_each<NP>([&](auto g_) {
+      constexpr int g = decltype(g_)::value, j = g / NG, i = g % NG / WN, b = g % WN;
+#pragma unroll
+      for (int r = 0; r < NR; ++r)
+        if (r * NP / NR == g) read(p ^ 1, r, (unsigned)(next * SLAB));
+#pragma unroll
+      for (int d = 0; d < NT; ++d)
+        if (d * NP / NT == g) dma(d, kt + RING, slot * SLAB);
+      __builtin_amdgcn_sched_barrier(0);
+      acc[i][b] = mx_mfma32<j>(fw[p][j][b], fx[p][j][i], acc[i][b], sw[p][b], sx[p][i]);
+      __builtin_amdgcn_sched_barrier(0);
+    });
+    slot = next;
+  };
+  // (always a pair of slabs: one past the end is zeros)
+  for (int kt = kt0; kt < nk; kt += 2) {
+    step(std::integral_constant<int, 0>(), kt);
+    step(std::integral_constant<int, 1>(), kt + 1);
+  }
+  static_assert(4 * 32 * (32 * WN + 4) * 4 <= RING * SLAB, "the sums of four waves fit the ring");
+  mx_tile_out<F16, GATED, WM, WN>(mx_out(a, t), acc, s_ring, t.m0, t.n0, t.split);
+}
+
 // ---- entry points -------------------------------------------------------------------------------------------------------------
 static bool mx_aligned(const void *codes, int64_t ldc, const void *scales, int64_t lds) {
   return !(((uintptr_t)codes | (uintptr_t)ldc) & 15) && !(((uintptr_t)scales | (uintptr_t)lds) & 3);
@@ -386,11 +677,42 @@ static int mx_check(const char *who, const MxArgs &a, int xkind, int64_t xrows, 
   }
   return MOE_OK;
 }
+struct MxPlan { int wm, wn, ring, splits; };    // wm 0: few rows
+static MxPlan mx_plan(int xkind, long long rows, int tiles_of, int N, int K, bool gated) {
+  const long long each = rows / tiles_of;
+  if (xkind != X_MX4 || each <= 16) return MxPlan{0, 0, 0, 1};
+  if (each <= 64) return MxPlan{1, 2, 4, 1};
+  return MxPlan{2, 2, 4, 1};
+}
 template <int X, bool F16, bool GATED>
 static int mx_launch(const MxArgs &a, int units, hipStream_t s) {
-  const dim3 grid((a.N + 15) / 16, units);
-  hipLaunchKernelGGL(HIP_KERNEL_NAME(k_mx4_rows<X, F16, GATED, 1>), grid, dim3(64 * MR_WAVES), 0, s, a);
-  return moe_check_launch("k_mx4_rows");
+  const MxPlan pl = mx_plan(X, a.M, a.units ? units : 1, a.N, a.K, GATED);
+  if (pl.wm == 0) {
+    const dim3 grid((a.N + 15) / 16, units);
+    hipLaunchKernelGGL(HIP_KERNEL_NAME(k_mx4_rows<X, F16, GATED, 1>), grid, dim3(64 * MR_WAVES), 0, s, a);
+    return moe_check_launch("k_mx4_rows");
+  }
+  if constexpr (X == X_MX4) {
+    MxArgs t = a;
+    const int bm = 64 * pl.wm, nc = 64 * pl.wn / (GATED ? 2 : 1);
+    t.nm = a.units ? 0 : (a.M + bm - 1) / bm;
+    t.nn = (a.N + nc - 1) / nc;
+    // (by expert: whole tiles, and one that is not for each expert at most)
+    const long long tiles = (a.units ? a.M / bm + units : t.nm) * (long long)t.nn * pl.splits;
+    if (tiles >= 1 << 24) {
+      moe_set_error("moe_mx4: %d x %d results are too many for one launch", a.M, a.N);
+      return MOE_EINVAL;
+    }
+    t.splits = pl.splits;
+    const int slabs = (a.K + M4_K - 1) / M4_K;
+    t.slabs = slabs / pl.splits;
+    t.extra = slabs % pl.splits;
+    const dim3 grid((unsigned)((tiles + 7) / 8 * 8));
+    if (pl.wm == 1) hipLaunchKernelGGL(HIP_KERNEL_NAME(k_mx4_tile<F16, GATED, 1, 2, 4>), grid, dim3(256), 0, s, t);
+    else hipLaunchKernelGGL(HIP_KERNEL_NAME(k_mx4_tile<F16, GATED, 2, 2, 4>), grid, dim3(256), 0, s, t);
+    return moe_check_launch("k_mx4_tile");
+  }
+  return MOE_EINVAL;
 }
 static int mx_run(const MxArgs &a, int xkind, int dtype, bool gated, int units, hipStream_t s) {
   const bool f16 = dtype == MOE_DT_FP16;
@@ -447,7 +769,7 @@ extern "C" int moe_mx4_experts(const void *x, int64_t ldx, const moe_mx4 *xq, co
   MxArgs a = mx_args(x, ldx, xq, w, w_up, bias, bias_up, nullptr, 0, y, ldy, P, N, K, act, y_fp32);
   a.counts = counts; a.offsets = offsets; a.units = units; a.tok = sorted_tok; a.E = E;
   const int xkind = xq ? X_MX4 : dtype == MOE_DT_FP16 ? X_FP16 : X_BF16;
-  if (E < 1 || E > 1024 || max_units < 0 || x_rows < 0 || (!sorted_tok && x_rows < P) || (P && N && (!counts || !offsets || !units))) {
+  if (E < 1 || E > 1024 || max_units < (E < P ? E : P) || x_rows < 0 || (!sorted_tok && x_rows < P) || (P && N && (!counts || !offsets || !units))) {
     moe_set_error("moe_mx4_experts: bad argument (E=%d P=%d max_units=%d rows of x %d)", E, P, max_units, x_rows);
     return MOE_EINVAL;
   }
@@ -456,6 +778,6 @@ extern "C" int moe_mx4_experts(const void *x, int64_t ldx, const moe_mx4 *xq, co
     moe_set_error("moe_mx4_experts: %d rows of tokens %lld bytes apart (less than 2 GiB are needed)", x_rows, a.ldx);
     return MOE_EINVAL;
   }
-  if (!P || !N || !max_units) return MOE_OK;
-  return mx_run(a, xkind, dtype, w_up != nullptr, max_units, (hipStream_t)stream);
+  if (!P || !N) return MOE_OK;
+  return mx_run(a, xkind, dtype, w_up != nullptr, E < P ? E : P, (hipStream_t)stream);
 }

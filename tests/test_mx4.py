@@ -37,7 +37,7 @@ def test_linear_refuses(kw):
     assert linear(up=desc(3 << 20, 3 << 21), **kw) == L.MOE_EINVAL
 
 
-@pytest.mark.parametrize("kw", BAD + [dict(P=-1), dict(E=0), dict(E=1025), dict(x_rows=3), dict(x_rows=-1), dict(max_units=-1), dict(counts=None),
+@pytest.mark.parametrize("kw", BAD + [dict(P=-1), dict(E=0), dict(E=1025), dict(x_rows=3), dict(x_rows=-1), dict(max_units=2), dict(counts=None),
                                       dict(offsets=None), dict(units=None)], ids=str)
 def test_experts_refuse(kw):
     from promoe_amd import _lib as L
@@ -64,7 +64,7 @@ def test_products_refuse_more():
     assert experts(x=1 << 50, x_rows=1 << 24, ldx=1 << 20, tok=64) == L.MOE_EINVAL and b"2 GiB" in L.lib.moe_last_error()
     for M, N in ((0, 8), (4, 0)):                                     # nothing to do
         assert linear(M=M, N=N, x=None, y=None, w=desc(None, None)) == 0
-    assert experts(P=0, x_rows=0, x=None, y=None) == 0 and experts(max_units=0) == 0
+    assert experts(P=0, x_rows=0, x=None, y=None) == 0 and experts(N=0, ldy=0) == 0
 
 
 def test_a_result_over_an_operand_is_refused():
