@@ -568,6 +568,154 @@ __global__ __launch_bounds__(256, RING * (WM + WN) * 64 * 136 > 80 * 1024 ? 1 : 
   mx_tile_out<F16, GATED, WM, WN>(mx_out(a, t), acc, s_ring, t.m0, t.n0, t.split);
 }
 
+static __device__ __forceinline__ f32x16_t mx_mfma32_bf16(u32x4_t a, u32x4_t b, f32x16_t c) {
+  return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8_t, a), __builtin_bit_cast(bf16x8_t, b), c, 0, 0, 0);
+}
+// x in 16 bits: the same tile, K 128 at a time (256 bytes of a row of x, 64 of codes, one word of scales).  Half q of the wave takes the
+// columns 64 q .. 64 q + 63 of a slab, eight a step: blocks 2 q and 2 q + 1 of W, which become bf16 in front of their products.
+// Chunk c (16 bytes) of row r of x stands in slot c ^ (r & 15), of W in slot c ^ ((r >> 2) & 3).
+#define M16_K 128
+template <int X, bool GATED, int WM, int WN, int RING>
+__global__ __launch_bounds__(256, RING * (WM * 64 * 256 + WN * 64 * 64 + 1024) > 80 * 1024 ? 1 : 2) void k_mx4_tile16(const MxArgs a) {
+  constexpr bool F16 = X == X_FP16;
+  constexpr int BM = 64 * WM, BN = 64 * WN, NX = 4 * WM, NW = WN, NG = WM * WN, NT = NX + NW + 1;
+  constexpr int XS = BM * 256, CODES = XS + BN * 64, SLAB = CODES + 1024, NC = GATED ? BN / 2 : BN;
+  __shared__ __align__(1024) unsigned char s_ring[RING * SLAB];
+  const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6), wm = w & 1, wn = w >> 1;
+  const int fr = lane & 31, q = lane >> 5;
+  MxTile t;
+  if (!mx_tile_of<BM, NC>(a, mx_run_of(), t)) return;
+  const unsigned lds = (unsigned)(uintptr_t)(__attribute__((address_space(3))) unsigned char *)s_ring;
+  const long long xbase = a.tok ? 0 : t.m0;
+  const lt_rsrc_t rx = lt_rsrc((const uint8_t *)a.x + xbase * a.ldx);
+  const lt_rsrc_t rw0 = lt_rsrc(a.w[0] + t.e * a.ew + t.n0 * a.ldw), rw1 = lt_rsrc(a.w[GATED ? 1 : 0] + t.e * a.ew + t.n0 * a.ldw);
+  const lt_rsrc_t rs0 = lt_rsrc(a.ws[0] + t.e * a.ews + t.n0 * a.ldws), rs1 = lt_rsrc(a.ws[GATED ? 1 : 0] + t.e * a.ews + t.n0 * a.ldws);
+  // transfer i of wave w: four rows of x from 16 i + 4 w on, sixteen lanes a row; sixteen rows of W from 64 i + 16 w on, four lanes a row.
+  // Scales: wave w (w < WN) 64 rows of W.
+  const int xr = 4 * w + (lane >> 4), xc = (lane & 15) ^ xr, wr = 16 * w + (lane >> 2), wc = (lane & 3) ^ ((wr >> 2) & 3);
+  auto wrow = [&](int i) {  // row i of the tile in its matrix, from n0 on
+    const int n = GATED ? 32 * (i >> 6) + (i & 31) : i;
+    return min(t.n0 + n, a.N - 1) - t.n0;
+  };
+  int vx[NX], vw[NW];
+#pragma unroll
+  for (int i = 0; i < NX; ++i) {
+    const int m = min(t.m0 + 16 * i + xr, t.m_end - 1);
+    vx[i] = (a.tok ? a.tok[m] : m - t.m0) * (int)a.ldx + 16 * xc;
+  }
+#pragma unroll
+  for (int i = 0; i < NW; ++i) vw[i] = wrow(64 * i + wr) * (int)a.ldw + 16 * wc;
+  // a gated pair's matrices change every 32 rows of the tile, so with the wave; its scales stand one matrix behind the other, 64 rows a wave
+  const lt_rsrc_t rw = GATED && (w & 2) ? rw1 : rw0, rs = GATED && w >= WN / 2 ? rs1 : rs0;
+  const int vs = w < WN ? (min(t.n0 + 64 * (GATED ? w % ((WN + 1) / 2) : w) + lane, a.N - 1) - t.n0) * (int)a.ldws : LT_OUT;
+  const int kt0 = t.split * a.slabs + min(t.split, a.extra), nk = kt0 + a.slabs + (t.split < a.extra);
+  const int blocks = min(a.K >> 5, nk * (M16_K / 32));  // (past the last block: zeros)
+  auto dma = [&](int i, int kt, int place) {
+    if (i < NX) {
+      const bool in = kt * 4 + (xc >> 2) < blocks;
+      mx_dma16(lds + (unsigned)(place + (i * 16 + 4 * w) * 256), in ? vx[i < NX ? i : 0] : LT_OUT, rx, kt * (M16_K * 2));
+    } else if (i < NX + NW) {
+      const bool in = kt * 4 + wc < blocks;
+      mx_dma16(lds + (unsigned)(place + XS + ((i - NX) * 64 + 16 * w) * 64), in ? vw[i < NX || i >= NX + NW ? 0 : i - NX] : LT_OUT, rw, kt * (M16_K / 2));
+    } else {
+      mx_dma4(lds + (unsigned)(place + CODES + w * 256), kt * 4 < blocks ? vs : LT_OUT, rs, kt * 4);
+    }
+  };
+  unsigned ax[8], aw[2], as[WN];  // LDS address of the lane's fragments in block 0 (scales: every block), of rows that begin where the ring does
+#pragma unroll
+  for (int j = 0; j < 8; ++j) ax[j] = lds + (unsigned)((wm * WM * 32 + fr) * 256 + ((8 * q + j) ^ (fr & 15)) * 16);
+#pragma unroll
+  for (int h = 0; h < 2; ++h) aw[h] = lds + (unsigned)(XS + (wn * WN * 32 + fr) * 64 + ((2 * q + h) ^ ((fr >> 2) & 3)) * 16);
+#pragma unroll
+  for (int b = 0; b < WN; ++b) {
+    const int block = wn * WN + b;
+    as[b] = lds + (unsigned)(CODES + (GATED ? (block & 1) * NC + 32 * (block >> 1) + fr : 32 * block + fr) * 4);
+  }
+  f32x16_t acc[WM][WN];
+#pragma unroll
+  for (int i = 0; i < WM; ++i)
+#pragma unroll
+    for (int b = 0; b < WN; ++b)
+#pragma unroll
+      for (int e = 0; e < 16; ++e) acc[i][b][e] = 0.f;
+#pragma unroll
+  for (int i = 0; i < RING; ++i)
+#pragma unroll
+    for (int d = 0; d < NT; ++d) dma(d, kt0 + i, i * SLAB);
+  LT_VM((RING - 1) * NT);
+  __builtin_amdgcn_s_barrier();
+  u32x4_t fx[2][8][WM], fw[2][2][WN];
+  u32 fs[2][WN];
+  auto read = [&](int p, int r, unsigned place) {  // fragment r of a slab: scales and W, then x step by step
+    if (r < WN) fs[p][r] = *(lds_u1 *)(uintptr_t)(as[r < WN ? r : 0] + place);
+    else if (r < 3 * WN) {
+      const int h = (r - WN) / WN, b = (r - WN) % WN;
+      fw[p][h & 1][b] = *(lds_u4 *)(uintptr_t)(aw[h & 1] + place + (unsigned)(b * 32 * 64));
+    } else {
+      const int j = (r - 3 * WN) / WM, i = (r - 3 * WN) % WM;
+      fx[p][j][i] = *(lds_u4 *)(uintptr_t)(ax[j] + place + (unsigned)(i * 32 * 256));
+    }
+  };
+  constexpr int NR = 3 * WN + 8 * WM, NP = 8 * NG;
+  // operands of a step, made during the step before
+  u32x4_t cw[2][WN], hi[2][WM], lo[2][WM];
+  float sv[WN][2];
+  constexpr int NC2 = WN + WM;
+  auto make = [&](int m, int j, int p, int kt) {
+    if (m < WN) {
+      const int b = m;
+      if (j == 0) {
+        const u32 two = (fs[p][b] & mx_mask(blocks - kt * 4)) >> (16 * q);
+        sv[b][0] = __uint_as_float((two & 255u) << 23);
+        sv[b][1] = __uint_as_float((two >> 8 & 255u) << 23);
+      }
+      cw[j & 1][b] = mx_bf16(fw[p][j >> 2][b][j & 3], sv[b][j >> 2]);
+    } else {
+      const int i = m - WN;
+      if constexpr (F16) mx_split(fx[p][j][i], hi[j & 1][i], lo[j & 1][i]);
+      else hi[j & 1][i] = fx[p][j][i];
+    }
+  };
+#pragma unroll
+  for (int r = 0; r < NR; ++r) read(0, r, 0);
+#pragma unroll
+  for (int m = 0; m < NC2; ++m) make(m, 0, 0, kt0);
+  int slot = 0;
+  auto step = [&](auto p_, int kt) {
+    constexpr int p = decltype(p_)::value;
+    const int next = slot + 1 < RING ? slot + 1 : 0;
+    LT_LGKM0();
+    LT_VM((RING - 2) * NT);
+    __builtin_amdgcn_s_barrier();
+    __builtin_amdgcn_sched_barrier(0);
+    lt_each<NP>([&](auto g_) {
+      constexpr int g = decltype(g_)::value, j = g / NG, i = g % NG / WN, b = g % WN, in = g % NG;
+      // (the next slab's fragments are all there in front of the last step, which makes the first operands of them)
+#pragma unroll
+      for (int r = 0; r < NR; ++r)
+        if (r * (NP - NG) / NR == g) read(p ^ 1, r, (unsigned)(next * SLAB));
+#pragma unroll
+      for (int d = 0; d < NT; ++d)
+        if (d * NP / NT == g) dma(d, kt + RING, slot * SLAB);
+#pragma unroll
+      for (int m = 0; m < NC2; ++m)
+        if (m * NG / NC2 == in) make(m, (j + 1) & 7, j == 7 ? p ^ 1 : p, j == 7 ? kt + 1 : kt);
+      __builtin_amdgcn_sched_barrier(0);
+      acc[i][b] = mx_mfma32_bf16(cw[j & 1][b], hi[j & 1][i], acc[i][b]);
+      if constexpr (F16) acc[i][b] = mx_mfma32_bf16(cw[j & 1][b], lo[j & 1][i], acc[i][b]);
+      __builtin_amdgcn_sched_barrier(0);
+    });
+    slot = next;
+  };
+  // (always a pair of slabs: one past the end is zeros)
+  for (int kt = kt0; kt < nk; kt += 2) {
+    step(std::integral_constant<int, 0>(), kt);
+    step(std::integral_constant<int, 1>(), kt + 1);
+  }
+  static_assert(4 * 32 * (32 * WN + 4) * 4 <= RING * SLAB, "the sums of four waves fit the ring");
+  mx_tile_out<F16, GATED, WM, WN>(mx_out(a, t), acc, s_ring, t.m0, t.n0, t.split);
+}
+
 // ---- entry points -------------------------------------------------------------------------------------------------------------
 static bool mx_aligned(const void *codes, int64_t ldc, const void *scales, int64_t lds) {
   return !(((uintptr_t)codes | (uintptr_t)ldc) & 15) && !(((uintptr_t)scales | (uintptr_t)lds) & 3);
@@ -680,9 +828,9 @@ static int mx_check(const char *who, const MxArgs &a, int xkind, int64_t xrows, 
 struct MxPlan { int wm, wn, ring, splits; };    // wm 0: few rows
 static MxPlan mx_plan(int xkind, long long rows, int tiles_of, int N, int K, bool gated) {
   const long long each = rows / tiles_of;
-  if (xkind != X_MX4 || each <= 16) return MxPlan{0, 0, 0, 1};
+  if (each <= 16) return MxPlan{0, 0, 0, 1};
   if (each <= 64) return MxPlan{1, 2, 4, 1};
-  return MxPlan{2, 2, 4, 1};
+  return xkind == X_MX4 ? MxPlan{2, 2, 4, 1} : MxPlan{2, 2, 3, 1};
 }
 template <int X, bool F16, bool GATED>
 static int mx_launch(const MxArgs &a, int units, hipStream_t s) {
@@ -692,27 +840,29 @@ static int mx_launch(const MxArgs &a, int units, hipStream_t s) {
     hipLaunchKernelGGL(HIP_KERNEL_NAME(k_mx4_rows<X, F16, GATED, 1>), grid, dim3(64 * MR_WAVES), 0, s, a);
     return moe_check_launch("k_mx4_rows");
   }
-  if constexpr (X == X_MX4) {
-    MxArgs t = a;
-    const int bm = 64 * pl.wm, nc = 64 * pl.wn / (GATED ? 2 : 1);
-    t.nm = a.units ? 0 : (a.M + bm - 1) / bm;
-    t.nn = (a.N + nc - 1) / nc;
-    // (by expert: whole tiles, and one that is not for each expert at most)
-    const long long tiles = (a.units ? a.M / bm + units : t.nm) * (long long)t.nn * pl.splits;
-    if (tiles >= 1 << 24) {
-      moe_set_error("moe_mx4: %d x %d results are too many for one launch", a.M, a.N);
-      return MOE_EINVAL;
-    }
-    t.splits = pl.splits;
-    const int slabs = (a.K + M4_K - 1) / M4_K;
-    t.slabs = slabs / pl.splits;
-    t.extra = slabs % pl.splits;
-    const dim3 grid((unsigned)((tiles + 7) / 8 * 8));
-    if (pl.wm == 1) hipLaunchKernelGGL(HIP_KERNEL_NAME(k_mx4_tile<F16, GATED, 1, 2, 4>), grid, dim3(256), 0, s, t);
-    else hipLaunchKernelGGL(HIP_KERNEL_NAME(k_mx4_tile<F16, GATED, 2, 2, 4>), grid, dim3(256), 0, s, t);
-    return moe_check_launch("k_mx4_tile");
+  MxArgs t = a;
+  const int bm = 64 * pl.wm, nc = 64 * pl.wn / (GATED ? 2 : 1);
+  t.nm = a.units ? 0 : (a.M + bm - 1) / bm;
+  t.nn = (a.N + nc - 1) / nc;
+  // (by expert: whole tiles, and one that is not for each expert at most)
+  const long long tiles = (a.units ? a.M / bm + units : t.nm) * (long long)t.nn * pl.splits;
+  if (tiles >= 1 << 24) {
+    moe_set_error("moe_mx4: %d x %d results are too many for one launch", a.M, a.N);
+    return MOE_EINVAL;
   }
-  return MOE_EINVAL;
+  t.splits = pl.splits;
+  constexpr int SLAB_K = X == X_MX4 ? M4_K : M16_K;
+  const int slabs = (a.K + SLAB_K - 1) / SLAB_K;
+  t.slabs = slabs / pl.splits;
+  t.extra = slabs % pl.splits;
+  const dim3 grid((unsigned)((tiles + 7) / 8 * 8));
+#define MT_LAUNCH(WM_, WN_, RING4, RING16)                                                                                      \
+  if constexpr (X == X_MX4) hipLaunchKernelGGL(HIP_KERNEL_NAME(k_mx4_tile<F16, GATED, WM_, WN_, RING4>), grid, dim3(256), 0, s, t); \
+  else hipLaunchKernelGGL(HIP_KERNEL_NAME(k_mx4_tile16<X, GATED, WM_, WN_, RING16>), grid, dim3(256), 0, s, t)
+  if (pl.wm == 1) { MT_LAUNCH(1, 2, 4, 5); }
+  else { MT_LAUNCH(2, 2, 4, 3); }
+#undef MT_LAUNCH
+  return moe_check_launch("k_mx4_tile");
 }
 static int mx_run(const MxArgs &a, int xkind, int dtype, bool gated, int units, hipStream_t s) {
   const bool f16 = dtype == MOE_DT_FP16;
