@@ -538,14 +538,14 @@ int moe_mx4_dequantize(const void *codes, int64_t ldc, const void *scales, int64
  * y_fp32) have the type dtype, and so has a 16-bit x.  K % 32 == 0; rows less than 4 MiB apart; sums in fp32, one rounding.  The other rules
  * as for moe_linear.
  * moe_mx4_experts: the same for every expert e of a dispatch: rows offsets[e] .. + counts[e] of y are the product of those rows of x, or,
- * with sorted_tok, of the rows sorted_tok[..] of x (x_rows of them), with matrix e; bias [E, N].  Rows behind the last pair are left as
+ * with sorted_tok, of the rows sorted_tok[..] of x (T of them, one for each token; else P), with matrix e; bias [E, N].  Rows behind the last pair are left as
  * they were.  E <= 1024, max_units >= min(E, P). */
 int moe_mx4_linear(const void *x, int64_t ldx, const moe_mx4 *xq_host, const moe_mx4 *w_host, const moe_mx4 *w_up_host, const void *bias,
                    const void *bias_up, const void *residual, int64_t ldr, void *y, int64_t ldy, int M, int N, int K, int dtype, int act,
                    int y_fp32, void *ws, int64_t ws_bytes, void *stream);
 int moe_mx4_experts(const void *x, int64_t ldx, const moe_mx4 *xq_host, const moe_mx4 *w_host, const moe_mx4 *w_up_host, const void *bias,
                     const void *bias_up, void *y, int64_t ldy, const int *counts, const int *offsets, const moe_unit *units, int max_units,
-                    const int *sorted_tok, int x_rows, int P, int E, int N, int K, int dtype, int act, int y_fp32, void *stream);
+                    const int *sorted_tok, int T, int P, int E, int N, int K, int dtype, int act, int y_fp32, void *stream);
 
 /* Per-kernel timing with HIP events recorded on the launch stream around every kernel
  * the launchers below start (no reference counterpart; used by the benchmark to report

@@ -171,14 +171,13 @@ static __device__ __forceinline__ void mx_split(u32x4_t x, u32x4_t &hi, u32x4_t 
 // in LDS.  A lane's load is one block, 32 columns of a row: with SH = 1 the 16 rows of the operand are 16 rows of W, with few rows of x
 // (at most 16 / SH) R rows of W by SH pieces of K: row s R + r and column s R + m hold piece s of both, and the products of unlike
 // pieces are left unread.  By expert the second dimension of the grid is a unit of the dispatch; more than 16 rows go in turn.
-#define MR_WAVES 8
-#define MR_U 2  // loads of a matrix in flight per wave, twice
-template <int X, bool F16, bool GATED, int SH>
-__global__ __launch_bounds__(64 * MR_WAVES) void k_mx4_rows(const MxArgs a) {
-  constexpr int NM = GATED ? 2 : 1, R = 16 / SH, STEP = 4 * SH * MR_U, SPAN = STEP * MR_WAVES, NX = X == X_MX4 ? 1 : 4;
-  __shared__ f32x4_t red[MR_WAVES][NM][64];
+// NB: sets of R rows a workgroup takes, all against the same operand of x; U: loads of a set in flight per wave, twice.
+template <int X, bool F16, bool GATED, int SH, int NB, int U, int WAVES>
+__global__ __launch_bounds__(64 * WAVES) void k_mx4_rows(const MxArgs a) {
+  constexpr int MATS = GATED ? 2 : 1, NM = MATS * NB, R = 16 / SH, STEP = 4 * SH * U, SPAN = STEP * WAVES, NX = X == X_MX4 ? 1 : 4;
+  __shared__ f32x4_t red[WAVES][NM][64];
   const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int r = (lane & 15) % R, s = (lane & 15) / R, n0 = blockIdx.x * R, blocks = a.K >> 5;
+  const int r = (lane & 15) % R, s = (lane & 15) / R, n0 = blockIdx.x * (R * NB), blocks = a.K >> 5;
   int e = 0, first = 0, rows = a.M;
   if (a.units) {
     const moe_unit u = a.units[blockIdx.y];
@@ -189,30 +188,36 @@ __global__ __launch_bounds__(64 * MR_WAVES) void k_mx4_rows(const MxArgs a) {
   if (o.bias[0]) o.bias[0] += (long long)e * a.N;
   if (GATED && o.bias[1]) o.bias[1] += (long long)e * a.N;
   const int k0 = (lane >> 4) * SH + s;                           // the lane's block among 4 SH
-  rsrc_t rw[NM], rs[NM];
+  rsrc_t rw[MATS], rs[MATS];
+  int vw[NB], vs[NB];
 #pragma unroll
-  for (int i = 0; i < NM; ++i) {
+  for (int i = 0; i < MATS; ++i) {
     rw[i] = make_rsrc(a.w[i] + e * a.ew + n0 * a.ldw, LT_OUT);
     rs[i] = make_rsrc(a.ws[i] + e * a.ews + n0 * a.ldws, LT_OUT);
   }
-  const int row = min(n0 + r, a.N - 1) - n0, vw = row * (int)a.ldw, vs = row * (int)a.ldws;
+#pragma unroll
+  for (int b = 0; b < NB; ++b) {
+    const int row = min(n0 + b * R + r, a.N - 1) - n0;
+    vw[b] = row * (int)a.ldw;
+    vs[b] = row * (int)a.ldws;
+  }
   for (int m0 = 0; m0 < rows; m0 += R) {
     const int m = first + m0 + min(r, rows - 1 - m0);
     const long long xrow = a.tok ? a.tok[m] : m, x0 = a.tok ? 0 : first + m0;  // (rows side by side from the block's first on)
     const rsrc_t rx = make_rsrc((const char *)a.x + x0 * a.ldx, LT_OUT), rxs = make_rsrc(X == X_MX4 ? a.xs + x0 * a.ldxs : (const uint8_t *)a.x, LT_OUT);
     const int vx = (int)((xrow - x0) * a.ldx), vxs = (int)((xrow - x0) * a.ldxs);
     f32x4_t acc[NM] = {};
-    uint4 fw[2][NM][MR_U], fx[2][MR_U][NX];
-    u32 sw[2][NM][MR_U], sx[2][MR_U];
+    uint4 fw[2][NM][U], fx[2][U][NX];
+    u32 sw[2][NM][U], sx[2][U];
     auto load = [&](int p, int base) {
 #pragma unroll
-      for (int u = 0; u < MR_U; ++u) {
+      for (int u = 0; u < U; ++u) {
         const int k = base + 4 * SH * u + k0;
         const bool in = k < blocks;                              // past the end: zeros on both sides
 #pragma unroll
         for (int i = 0; i < NM; ++i) {
-          fw[p][i][u] = bload16(rw[i], in ? vw + 16 * k : LT_OUT, 0);
-          sw[p][i][u] = bload1(rs[i], in ? vs + k : LT_OUT, 0);
+          fw[p][i][u] = bload16(rw[i % MATS], in ? vw[i / MATS] + 16 * k : LT_OUT, 0);
+          sw[p][i][u] = bload1(rs[i % MATS], in ? vs[i / MATS] + k : LT_OUT, 0);
         }
         if constexpr (X == X_MX4) {
           fx[p][u][0] = bload16(rx, in ? vx + 16 * k : LT_OUT, 0);
@@ -225,7 +230,7 @@ __global__ __launch_bounds__(64 * MR_WAVES) void k_mx4_rows(const MxArgs a) {
     };
     auto use = [&](int p) {
 #pragma unroll
-      for (int u = 0; u < MR_U; ++u) {
+      for (int u = 0; u < U; ++u) {
         if constexpr (X == X_MX4) {
 #pragma unroll
           for (int i = 0; i < NM; ++i)
@@ -257,21 +262,21 @@ __global__ __launch_bounds__(64 * MR_WAVES) void k_mx4_rows(const MxArgs a) {
     __syncthreads();
     // result (m, n): element n' % 4 of lane 16 (n' / 4) + m', n' = s R + n and m' = s R + m, over the pieces and the waves in order
     const int cnt = min(R, rows - m0);
-    for (int t = tid; t < R * cnt; t += 64 * MR_WAVES) {
-      const int n = t % R, i_m = t / R;
-      if (n0 + n >= a.N) continue;
-      float sum[NM];
+    for (int t = tid; t < R * NB * cnt; t += 64 * WAVES) {
+      const int n = t % R, b = t / R % NB, i_m = t / (R * NB);
+      if (n0 + b * R + n >= a.N) continue;
+      float sum[MATS];
 #pragma unroll
-      for (int i = 0; i < NM; ++i) {
+      for (int i = 0; i < MATS; ++i) {
         sum[i] = 0.f;
 #pragma unroll
         for (int p = 0; p < SH; ++p) {
           const int at = p * R + n;
 #pragma unroll
-          for (int v = 0; v < MR_WAVES; ++v) sum[i] += ((const float *)&red[v][i][16 * (at >> 2) + p * R + i_m])[at & 3];
+          for (int v = 0; v < WAVES; ++v) sum[i] += ((const float *)&red[v][b * MATS + i][16 * (at >> 2) + p * R + i_m])[at & 3];
         }
       }
-      lin_store<F16, GATED>(o, first + m0 + i_m, n0 + n, sum[0], sum[NM - 1]);
+      lin_store<F16, GATED>(o, first + m0 + i_m, n0 + b * R + n, sum[0], sum[MATS - 1]);
     }
     __syncthreads();
   }
@@ -833,11 +838,21 @@ static MxPlan mx_plan(int xkind, long long rows, int tiles_of, int N, int K, boo
   return xkind == X_MX4 ? MxPlan{2, 2, 4, 1} : MxPlan{2, 2, 3, 1};
 }
 template <int X, bool F16, bool GATED>
-static int mx_launch(const MxArgs &a, int units, hipStream_t s) {
+static int mx_launch(const MxArgs &a, int units, int most, hipStream_t s) {  // most: rows that one expert (or the product) can have
   const MxPlan pl = mx_plan(X, a.M, a.units ? units : 1, a.N, a.K, GATED);
   if (pl.wm == 0) {
-    const dim3 grid((a.N + 15) / 16, units);
-    hipLaunchKernelGGL(HIP_KERNEL_NAME(k_mx4_rows<X, F16, GATED, 1>), grid, dim3(64 * MR_WAVES), 0, s, a);
+#define MR_LAUNCH(SH_, NB_, W_)                                                                                                      \
+  hipLaunchKernelGGL(HIP_KERNEL_NAME(k_mx4_rows<X, F16, GATED, SH_, NB_, 1, W_>), dim3((a.N + 16 / SH_ * NB_ - 1) / (16 / SH_ * NB_), units), \
+                     dim3(64 * W_), 0, s, a)
+    const long long sets = (a.N + 15) / 16 * (long long)units;  // of 16 rows of W
+    if (most <= 8) {
+      if (sets >= 256) MR_LAUNCH(2, 2, 4);
+      else MR_LAUNCH(2, 1, 8);
+    } else {
+      if (sets >= 512) MR_LAUNCH(1, 2, 4);
+      else MR_LAUNCH(1, 1, 4);
+    }
+#undef MR_LAUNCH
     return moe_check_launch("k_mx4_rows");
   }
   MxArgs t = a;
@@ -864,17 +879,17 @@ static int mx_launch(const MxArgs &a, int units, hipStream_t s) {
 #undef MT_LAUNCH
   return moe_check_launch("k_mx4_tile");
 }
-static int mx_run(const MxArgs &a, int xkind, int dtype, bool gated, int units, hipStream_t s) {
+static int mx_run(const MxArgs &a, int xkind, int dtype, bool gated, int units, int most, hipStream_t s) {
   const bool f16 = dtype == MOE_DT_FP16;
   switch ((xkind == X_MX4 ? 0 : 4) + (f16 ? 2 : 0) + (gated ? 1 : 0)) {
-    case 0: return mx_launch<X_MX4, false, false>(a, units, s);
-    case 1: return mx_launch<X_MX4, false, true>(a, units, s);
-    case 2: return mx_launch<X_MX4, true, false>(a, units, s);
-    case 3: return mx_launch<X_MX4, true, true>(a, units, s);
-    case 4: return mx_launch<X_BF16, false, false>(a, units, s);
-    case 5: return mx_launch<X_BF16, false, true>(a, units, s);
-    case 6: return mx_launch<X_FP16, true, false>(a, units, s);
-    default: return mx_launch<X_FP16, true, true>(a, units, s);
+    case 0: return mx_launch<X_MX4, false, false>(a, units, most, s);
+    case 1: return mx_launch<X_MX4, false, true>(a, units, most, s);
+    case 2: return mx_launch<X_MX4, true, false>(a, units, most, s);
+    case 3: return mx_launch<X_MX4, true, true>(a, units, most, s);
+    case 4: return mx_launch<X_BF16, false, false>(a, units, most, s);
+    case 5: return mx_launch<X_BF16, false, true>(a, units, most, s);
+    case 6: return mx_launch<X_FP16, true, false>(a, units, most, s);
+    default: return mx_launch<X_FP16, true, true>(a, units, most, s);
   }
 }
 static MxArgs mx_args(const void *x, int64_t ldx, const moe_mx4 *xq, const moe_mx4 *w, const moe_mx4 *w_up, const void *bias,
@@ -908,26 +923,26 @@ extern "C" int moe_mx4_linear(const void *x, int64_t ldx, const moe_mx4 *xq, con
   const int xkind = xq ? X_MX4 : dtype == MOE_DT_FP16 ? X_FP16 : X_BF16;
   if (int rc = mx_check("moe_mx4_linear", a, xkind, M, 1, dtype, w_up != nullptr)) return rc;
   if (!M || !N) return MOE_OK;
-  return mx_run(a, xkind, dtype, w_up != nullptr, 1, (hipStream_t)stream);
+  return mx_run(a, xkind, dtype, w_up != nullptr, 1, M, (hipStream_t)stream);
 }
 
 extern "C" int moe_mx4_experts(const void *x, int64_t ldx, const moe_mx4 *xq, const moe_mx4 *w, const moe_mx4 *w_up, const void *bias,
                                const void *bias_up, void *y, int64_t ldy, const int *counts, const int *offsets, const moe_unit *units,
-                               int max_units, const int *sorted_tok, int x_rows, int P, int E, int N, int K, int dtype, int act, int y_fp32,
+                               int max_units, const int *sorted_tok, int T, int P, int E, int N, int K, int dtype, int act, int y_fp32,
                                void *stream) {
   if (int rc = mx_described("moe_mx4_experts", x, xq, w, w_up)) return rc;
   MxArgs a = mx_args(x, ldx, xq, w, w_up, bias, bias_up, nullptr, 0, y, ldy, P, N, K, act, y_fp32);
   a.counts = counts; a.offsets = offsets; a.units = units; a.tok = sorted_tok; a.E = E;
   const int xkind = xq ? X_MX4 : dtype == MOE_DT_FP16 ? X_FP16 : X_BF16;
-  if (E < 1 || E > 1024 || max_units < (E < P ? E : P) || x_rows < 0 || (!sorted_tok && x_rows < P) || (P && N && (!counts || !offsets || !units))) {
-    moe_set_error("moe_mx4_experts: bad argument (E=%d P=%d max_units=%d rows of x %d)", E, P, max_units, x_rows);
+  if (E < 1 || E > 1024 || max_units < (E < P ? E : P) || T < 0 || (P && !T) || (P && N && (!counts || !offsets || !units))) {
+    moe_set_error("moe_mx4_experts: bad argument (E=%d T=%d P=%d max_units=%d)", E, T, P, max_units);
     return MOE_EINVAL;
   }
-  if (int rc = mx_check("moe_mx4_experts", a, xkind, x_rows, E, dtype, w_up != nullptr)) return rc;
-  if (sorted_tok && x_rows * a.ldx >= 1ll << 31) {
-    moe_set_error("moe_mx4_experts: %d rows of tokens %lld bytes apart (less than 2 GiB are needed)", x_rows, a.ldx);
+  if (int rc = mx_check("moe_mx4_experts", a, xkind, sorted_tok ? T : P, E, dtype, w_up != nullptr)) return rc;
+  if (sorted_tok && T * a.ldx >= 1ll << 31) {
+    moe_set_error("moe_mx4_experts: %d rows of tokens %lld bytes apart (less than 2 GiB are needed)", T, a.ldx);
     return MOE_EINVAL;
   }
   if (!P || !N) return MOE_OK;
-  return mx_run(a, xkind, dtype, w_up != nullptr, E < P ? E : P, (hipStream_t)stream);
+  return mx_run(a, xkind, dtype, w_up != nullptr, E < P ? E : P, T, (hipStream_t)stream);
 }

@@ -744,7 +744,7 @@ def _product_mx4(what, x, mats, biases, act, residual, out, out_dtype, d=None, o
                                 L.ACTS[act], y32, 0, 0, _raw_stream(index))
     else:
         rc = lib.moe_mx4_experts(xp, ldx, xq, byref(wd), up, ptr(biases[0]), b_up, out.data_ptr(), ldy, d.counts.data_ptr(),
-                                 d.offsets.data_ptr(), d.units.data_ptr(), d.max_units, d.sorted_tok.data_ptr() if of_tokens else 0, rows,
+                                 d.offsets.data_ptr(), d.units.data_ptr(), d.max_units, d.sorted_tok.data_ptr() if of_tokens else 0, d.T,
                                  M, d.E, N, K, code, L.ACTS[act], y32, _raw_stream(index))
     if rc:
         check(rc, what)

@@ -17,12 +17,12 @@ def linear(M=4, N=8, K=64, x=1 << 16, ldx=64, xq=None, w=None, up=None, bias=Non
                                 ldy, M, N, K, dtype, act, y32, None, 0, None)
 
 
-def experts(P=4, x_rows=4, E=3, N=8, K=64, x=1 << 16, ldx=64, xq=None, w=None, up=None, y=1 << 22, ldy=8, counts=64, offsets=64, units=64,
+def experts(P=4, T=4, E=3, N=8, K=64, x=1 << 16, ldx=64, xq=None, w=None, up=None, y=1 << 22, ldy=8, counts=64, offsets=64, units=64,
             max_units=3, tok=None):
     from promoe_amd import _lib as L
     w = desc(next_c=256, next_s=32) if w is None else w
     return L.lib.moe_mx4_experts(x, ldx, None if xq is None else byref(xq), byref(w), None if up is None else byref(up), None, None, y, ldy,
-                                 counts, offsets, units, max_units, tok, x_rows, P, E, N, K, 0, 0, 0, None)
+                                 counts, offsets, units, max_units, tok, T, P, E, N, K, 0, 0, 0, None)
 
 
 BAD = [dict(N=-1), dict(K=0), dict(K=48), dict(K=-32), dict(ldx=56), dict(ldx=68), dict(ldx=1 << 21), dict(ldy=7), dict(x=None), dict(x=(1 << 16) + 8),
@@ -37,7 +37,7 @@ def test_linear_refuses(kw):
     assert linear(up=desc(3 << 20, 3 << 21), **kw) == L.MOE_EINVAL
 
 
-@pytest.mark.parametrize("kw", BAD + [dict(P=-1), dict(E=0), dict(E=1025), dict(x_rows=3), dict(x_rows=-1), dict(max_units=2), dict(counts=None),
+@pytest.mark.parametrize("kw", BAD + [dict(P=-1), dict(E=0), dict(E=1025), dict(T=0), dict(T=-1), dict(max_units=2), dict(counts=None),
                                       dict(offsets=None), dict(units=None)], ids=str)
 def test_experts_refuse(kw):
     from promoe_amd import _lib as L
@@ -61,10 +61,10 @@ def test_products_refuse_more():
     from promoe_amd import _lib as L
     assert linear(xq=desc(3 << 20, 3 << 21)) == L.MOE_EINVAL          # two x
     assert L.lib.moe_mx4_linear(1 << 16, 64, None, None, None, None, None, None, 0, 1 << 22, 8, 4, 8, 64, 0, 0, 0, None, 0, None) == L.MOE_EINVAL
-    assert experts(x=1 << 50, x_rows=1 << 24, ldx=1 << 20, tok=64) == L.MOE_EINVAL and b"2 GiB" in L.lib.moe_last_error()
+    assert experts(x=1 << 50, T=1 << 24, ldx=1 << 20, tok=64) == L.MOE_EINVAL and b"2 GiB" in L.lib.moe_last_error()
     for M, N in ((0, 8), (4, 0)):                                     # nothing to do
         assert linear(M=M, N=N, x=None, y=None, w=desc(None, None)) == 0
-    assert experts(P=0, x_rows=0, x=None, y=None) == 0 and experts(N=0, ldy=0) == 0
+    assert experts(P=0, T=0, x=None, y=None) == 0 and experts(N=0, ldy=0) == 0
 
 
 def test_a_result_over_an_operand_is_refused():
