@@ -518,21 +518,20 @@ int moe_unsort_rows_grad(const void *dy, int64_t lddy, const void *x, int64_t ld
 
 /* Matrices in microscaled 4-bit floating point: a code per value (two to a byte, the even column in the low half: sign, two bits of
  * exponent, one of mantissa, i.e. 0, 0.5, 1, 1.5, 2, 3, 4, 6) and a byte per 32 columns, value = code * 2^(byte - 127); byte 255: NaN.
- * Rows of K/2 bytes of codes ldc apart (16-byte boundaries) and of K/32 bytes of scales lds apart (4-byte boundaries; the bytes up to the
- * next such boundary behind a row's scales are read and not used).  next_c, next_s: bytes between the matrices of consecutive
- * experts. */
+ * Rows of K/2 bytes of codes ldc apart (16-byte boundaries).  Scales lie in blocks of 32 rows by 8 bytes (256 columns): byte kb of row r at
+ * ((r/32) * ceil(K/256) + kb/8) * 256 + (r%32) * 8 + kb%8 (4-byte boundaries), moe_mx4_scale_bytes(rows, K) in all; what belongs to no
+ * row or column may be anything.  next_c, next_s: bytes between the matrices of consecutive experts. */
 typedef struct moe_mx4 {
-  const void *codes, *scales;
-  int64_t ldc, lds, next_c, next_s;
+  void *codes, *scales;
+  int64_t ldc, next_c, next_s;
 } moe_mx4;
-/* M rows of K values (K % 32 == 0, rows ld elements apart on 16-byte boundaries, dtype any of three) to codes and scales and back.  The
- * scale of a block is 2^(floor(log2 of its largest magnitude) - 2), at least 2^-127; codes are rounded to the nearest, ties to the even
- * code, 6 beyond 6.  A block with a NaN or an infinity becomes NaN.  Back: rounded to dtype, which fp32 and bf16 do not need (beyond
- * their range codes become infinite). */
-int moe_mx4_quantize(const void *x, int64_t ldx, int dtype, int64_t M, int K, void *codes, int64_t ldc, void *scales, int64_t lds,
-                     void *stream);
-int moe_mx4_dequantize(const void *codes, int64_t ldc, const void *scales, int64_t lds, int64_t M, int K, void *y, int64_t ldy, int dtype,
-                       void *stream);
+int64_t moe_mx4_scale_bytes(int64_t rows, int K);
+/* E matrices of M rows of K values (K % 32 == 0, rows ld and matrices next elements apart, on 16-byte boundaries, dtype any of three) to
+ * codes and scales and back.  The scale of a block is 2^(floor(log2 of its largest magnitude) - 2), at least 2^-127; codes are rounded to
+ * the nearest, ties to the even code, 6 beyond 6.  A block with a NaN or an infinity becomes NaN.  Back: rounded to dtype, which fp32 and
+ * bf16 do not need (beyond their range codes become infinite).  M*K below 2^34, E below 2^16. */
+int moe_mx4_quantize(const void *x, int64_t ldx, int64_t next_x, int dtype, int E, int M, int K, const moe_mx4 *q_host, void *stream);
+int moe_mx4_dequantize(const moe_mx4 *q_host, int E, int M, int K, void *y, int64_t ldy, int64_t next_y, int dtype, void *stream);
 /* moe_linear and moe_linear_gated (w_up not NULL) with matrices in that form (descriptions on the host); x either 16-bit rows (ldx
  * elements apart; the products are those of the values as they are) or rows in the same form (xq, x NULL).  bias, residual and y (unless
  * y_fp32) have the type dtype, and so has a 16-bit x.  K % 32 == 0; rows less than 4 MiB apart; sums in fp32, one rounding.  The other rules

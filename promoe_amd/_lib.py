@@ -43,7 +43,7 @@ class RouteRule(C.Structure):
 
 
 class Mx4Desc(C.Structure):
-    _fields_ = [("codes", vp), ("scales", vp), ("ldc", i64), ("lds", i64), ("next_c", i64), ("next_s", i64)]
+    _fields_ = [("codes", vp), ("scales", vp), ("ldc", i64), ("next_c", i64), ("next_s", i64)]
 
 
 class MoeError(RuntimeError):
@@ -65,8 +65,9 @@ _sig("moe_linear_gated", [vp, i64, vp, vp, i64, vp, vp, vp, i64, i32, i32, i32, 
 _sig("moe_sort_rows", [vp, i64, vp, i64, vp, vp, i32, i32, i32, i32, vp])
 _sig("moe_unsort_rows", [vp, i64, vp, i64, vp, vp, i32, i32, i32, i32, vp])
 _sig("moe_unsort_rows_grad", [vp, i64, vp, i64, vp, vp, vp, vp, i64, vp, i32, i32, i32, i32, vp])
-_sig("moe_mx4_quantize", [vp, i64, i32, i64, i32, vp, i64, vp, i64, vp])
-_sig("moe_mx4_dequantize", [vp, i64, vp, i64, i64, i32, vp, i64, i32, vp])
+_sig("moe_mx4_scale_bytes", [i64, i32], i64)
+_sig("moe_mx4_quantize", [vp, i64, i64, i32, i32, i32, i32, vp, vp])
+_sig("moe_mx4_dequantize", [vp, i32, i32, i32, vp, i64, i64, i32, vp])
 _sig("moe_mx4_linear", [vp, i64, vp, vp, vp, vp, vp, vp, i64, vp, i64, i32, i32, i32, i32, i32, i32, vp, i64, vp])
 _sig("moe_mx4_experts", [vp, i64, vp, vp, vp, vp, vp, vp, i64, vp, vp, vp, i32, vp, i32, i32, i32, i32, i32, i32, i32, i32, vp])
 _sig("moe_group_topk", [vp, i32, i32, i32, i32, vp, vp, vp, vp, vp])

@@ -18,20 +18,26 @@ typedef float f32x2_t __attribute__((ext_vector_type(2)));
 typedef _Float16 f16x2_t __attribute__((ext_vector_type(2)));
 
 // ---- rows into codes and back ---------------------------------------------------------------------------------------------------
+// Scales lie in blocks of 32 rows by 8 bytes (256 columns, a slab of the products below), so that what 32 rows need of a slab is 256 bytes
+// in one piece: byte kb of row r at ((r / 32) slabs + kb / 8) 256 + (r % 32) 8 + kb % 8.  Row by row, as they are exchanged, every row would
+// cost the products a cache line for 8 bytes (4096 x 4096 x 14336 in 4 bits: 216 us, with blocks 167).
+static __host__ __device__ __forceinline__ int mx_slabs(int K) { return (K + 255) >> 8; }
+static __device__ __forceinline__ long long mx_scale_row(long long r, int slabs) { return (r >> 5) * (slabs * 256ll) + (r & 31) * 8; }
 struct QuantArgs {
-  const void *x;              // the rows that are read: values, or codes
-  void *y;                    // the rows that are written: codes, or values
+  const char *x;              // the rows that are read: values, or codes
+  char *y;                    // the rows that are written: codes, or values
   uint8_t *scales;
-  long long ldx, ldc, lds;    // elements between rows of values, bytes between rows of codes and of scales
-  long long n;                // pieces of 8 values
+  long long ldx, ldc;         // elements between rows of values, bytes between rows of codes
+  long long next_x, next_c, next_s;  // between matrices: elements, bytes, bytes
+  u32 n;                      // pieces of 8 values of a matrix
   u32 per, magic, shift;      // pieces of a row; i / per = (mulhi(i, magic) + i) >> shift for i < 2^31
+  int slabs;
 };
 struct Place { long long x, c, s; };
-template <bool FLAT>  // FLAT: the rows lie end to end
-static __device__ __forceinline__ Place place_of(const QuantArgs &a, long long i) {
-  if constexpr (FLAT) return Place{8 * i, 4 * i, i >> 2};
-  const u32 row = (__umulhi((u32)i, a.magic) + (u32)i) >> a.shift, col = (u32)i - row * a.per;
-  return Place{row * a.ldx + 8 * (long long)col, row * a.ldc + 4 * (long long)col, row * a.lds + (col >> 2)};
+static __device__ __forceinline__ Place place_of(const QuantArgs &a, u32 i) {
+  const u32 row = (__umulhi(i, a.magic) + i) >> a.shift, col = i - row * a.per;
+  return Place{blockIdx.y * a.next_x + row * a.ldx + 8ll * col, blockIdx.y * a.next_c + row * a.ldc + 4ll * col,
+               blockIdx.y * a.next_s + mx_scale_row(row, a.slabs) + (col >> 5) * 256 + (col >> 2 & 7)};
 }
 // the largest of the four lanes of a block
 static __device__ __forceinline__ u32 quad_max(u32 v) {
@@ -47,20 +53,20 @@ static __device__ __forceinline__ u32 scale_byte(u32 top) {
 // Four lanes a block, eight values each: one 16-byte load (two of fp32) and four bytes of codes, side by side over the lanes.  The
 // hardware's conversion divides by the scale, rounds to the nearest (ties to the even code) and goes no further than 6.
 #define QT_U 4  // pieces of a lane, all of them on their way at once
-template <int DT, bool FLAT>
+template <int DT>
 __global__ __launch_bounds__(256) void k_mx4_quantize(const QuantArgs a) {
-  const long long first = (long long)blockIdx.x * (256 * QT_U) + threadIdx.x;
+  const u32 first = blockIdx.x * (256 * QT_U) + threadIdx.x;
   u32x4_t v[QT_U][DT == MOE_DT_FP32 ? 2 : 1];
 #pragma unroll
   for (int u = 0; u < QT_U; ++u) {
-    const long long i = min(first + 256 * u, a.n - 1);  // (no condition around a load)
-    const char *p = (const char *)a.x + place_of<FLAT>(a, i).x * (DT == MOE_DT_FP32 ? 4 : 2);
+    const u32 i = min(first + 256 * u, a.n - 1);  // (no condition around a load)
+    const char *p = a.x + place_of(a, i).x * (DT == MOE_DT_FP32 ? 4 : 2);
     v[u][0] = *(const u32x4_t *)p;
     if constexpr (DT == MOE_DT_FP32) v[u][1] = *(const u32x4_t *)(p + 16);
   }
 #pragma unroll
   for (int u = 0; u < QT_U; ++u) {
-    const long long i = first + 256 * u;
+    const u32 i = first + 256 * u;
     if (i >= a.n) break;
     u32 top = 0;
     if constexpr (DT == MOE_DT_FP32) {
@@ -89,27 +95,27 @@ __global__ __launch_bounds__(256) void k_mx4_quantize(const QuantArgs a) {
         else c = __builtin_amdgcn_cvt_scalef32_pk_fp4_f16(c, __builtin_bit_cast(f16x2_t, p), s, J);
       }
     });
-    const Place at = place_of<FLAT>(a, i);
-    *(u32 *)((char *)a.y + at.c) = c;
+    const Place at = place_of(a, i);
+    *(u32 *)(a.y + at.c) = c;
     if ((threadIdx.x & 3) == 0) a.scales[at.s] = (uint8_t)byte;
   }
 }
-template <int DT, bool FLAT>
+template <int DT>
 __global__ __launch_bounds__(256) void k_mx4_dequantize(const QuantArgs a) {
-  const long long first = (long long)blockIdx.x * (256 * QT_U) + threadIdx.x;
+  const u32 first = blockIdx.x * (256 * QT_U) + threadIdx.x;
   u32 c[QT_U], b[QT_U];
 #pragma unroll
   for (int u = 0; u < QT_U; ++u) {
-    const Place at = place_of<FLAT>(a, min(first + 256 * u, a.n - 1));
-    c[u] = *(const u32 *)((const char *)a.x + at.c);
+    const Place at = place_of(a, min(first + 256 * u, a.n - 1));
+    c[u] = *(const u32 *)(a.x + at.c);
     b[u] = a.scales[at.s];
   }
 #pragma unroll
   for (int u = 0; u < QT_U; ++u) {
-    const long long i = first + 256 * u;
+    const u32 i = first + 256 * u;
     if (i >= a.n) break;
     const float s = __uint_as_float(b[u] << 23);
-    char *p = (char *)a.y + place_of<FLAT>(a, i).x * (DT == MOE_DT_FP32 ? 4 : 2);
+    char *p = a.y + place_of(a, i).x * (DT == MOE_DT_FP32 ? 4 : 2);
     f32x2_t f[4];
     f[0] = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(c[u], s, 0);
     f[1] = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(c[u], s, 1);
@@ -132,7 +138,7 @@ struct MxArgs {
   const uint8_t *w[2], *ws[2];               // codes and scales of the matrices; [1]: the second one of a gated pair
   const uint16_t *bias[2], *res;
   void *y;
-  long long ldx, ldxs, ldw, ldws, ew, ews;   // bytes between rows; ew, ews: between the matrices of consecutive experts
+  long long ldx, ldw, ew, ews;               // bytes between rows; ew, ews: between the matrices (scales) of consecutive experts
   long long ldr, ldy;                        // elements
   int M, N, K, act, y32;                     // M: rows of y
   int nm, nn, splits, ldp, slabs, extra;     // as in the products of 16-bit matrices
@@ -177,7 +183,7 @@ __global__ __launch_bounds__(64 * WAVES) void k_mx4_rows(const MxArgs a) {
   constexpr int MATS = GATED ? 2 : 1, NM = MATS * NB, R = 16 / SH, STEP = 4 * SH * U, SPAN = STEP * WAVES, NX = X == X_MX4 ? 1 : 4;
   __shared__ f32x4_t red[WAVES][NM][64];
   const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int r = (lane & 15) % R, s = (lane & 15) / R, n0 = blockIdx.x * (R * NB), blocks = a.K >> 5;
+  const int r = (lane & 15) % R, s = (lane & 15) / R, n0 = blockIdx.x * (R * NB), blocks = a.K >> 5, slabs = mx_slabs(a.K);
   int e = 0, first = 0, rows = a.M;
   if (a.units) {
     const moe_unit u = a.units[blockIdx.y];
@@ -193,19 +199,19 @@ __global__ __launch_bounds__(64 * WAVES) void k_mx4_rows(const MxArgs a) {
 #pragma unroll
   for (int i = 0; i < MATS; ++i) {
     rw[i] = make_rsrc(a.w[i] + e * a.ew + n0 * a.ldw, LT_OUT);
-    rs[i] = make_rsrc(a.ws[i] + e * a.ews + n0 * a.ldws, LT_OUT);
+    rs[i] = make_rsrc(a.ws[i] + e * a.ews + mx_scale_row(n0 & ~31, slabs), LT_OUT);
   }
 #pragma unroll
   for (int b = 0; b < NB; ++b) {
     const int row = min(n0 + b * R + r, a.N - 1) - n0;
     vw[b] = row * (int)a.ldw;
-    vs[b] = row * (int)a.ldws;
+    vs[b] = (int)mx_scale_row(row + (n0 & 31), slabs);
   }
   for (int m0 = 0; m0 < rows; m0 += R) {
     const int m = first + m0 + min(r, rows - 1 - m0);
     const long long xrow = a.tok ? a.tok[m] : m, x0 = a.tok ? 0 : first + m0;  // (rows side by side from the block's first on)
-    const rsrc_t rx = make_rsrc((const char *)a.x + x0 * a.ldx, LT_OUT), rxs = make_rsrc(X == X_MX4 ? a.xs + x0 * a.ldxs : (const uint8_t *)a.x, LT_OUT);
-    const int vx = (int)((xrow - x0) * a.ldx), vxs = (int)((xrow - x0) * a.ldxs);
+    const rsrc_t rx = make_rsrc((const char *)a.x + x0 * a.ldx, LT_OUT), rxs = make_rsrc(X == X_MX4 ? a.xs + mx_scale_row(x0 & ~31, slabs) : (const uint8_t *)a.x, LT_OUT);
+    const int vx = (int)((xrow - x0) * a.ldx), vxs = (int)mx_scale_row(xrow - (x0 & ~31), slabs);
     f32x4_t acc[NM] = {};
     uint4 fw[2][NM][U], fx[2][U][NX];
     u32 sw[2][NM][U], sx[2][U];
@@ -214,14 +220,15 @@ __global__ __launch_bounds__(64 * WAVES) void k_mx4_rows(const MxArgs a) {
       for (int u = 0; u < U; ++u) {
         const int k = base + 4 * SH * u + k0;
         const bool in = k < blocks;                              // past the end: zeros on both sides
+        const int ks = (k >> 3) * 256 + (k & 7);
 #pragma unroll
         for (int i = 0; i < NM; ++i) {
           fw[p][i][u] = bload16(rw[i % MATS], in ? vw[i / MATS] + 16 * k : LT_OUT, 0);
-          sw[p][i][u] = bload1(rs[i % MATS], in ? vs[i / MATS] + k : LT_OUT, 0);
+          sw[p][i][u] = bload1(rs[i % MATS], in ? vs[i / MATS] + ks : LT_OUT, 0);
         }
         if constexpr (X == X_MX4) {
           fx[p][u][0] = bload16(rx, in ? vx + 16 * k : LT_OUT, 0);
-          sx[p][u] = bload1(rxs, in ? vxs + k : LT_OUT, 0);
+          sx[p][u] = bload1(rxs, in ? vxs + ks : LT_OUT, 0);
         } else {
 #pragma unroll
           for (int j = 0; j < 4; ++j) fx[p][u][j] = bload16(rx, in ? vx + 64 * k + 16 * j : LT_OUT, 0);
@@ -460,9 +467,10 @@ __global__ __launch_bounds__(256, RING * (WM + WN) * 64 * 136 > 80 * 1024 ? 1 : 
   if (!mx_tile_of<BM, NC>(a, mx_run_of(), t)) return;
   const unsigned lds = (unsigned)(uintptr_t)(__attribute__((address_space(3))) unsigned char *)s_ring;
   const uint8_t *w0 = a.w[0] + t.e * a.ew + t.n0 * a.ldw, *w1 = a.w[GATED ? 1 : 0] + t.e * a.ew + t.n0 * a.ldw;
-  const uint8_t *ws0 = a.ws[0] + t.e * a.ews + t.n0 * a.ldws, *ws1 = a.ws[GATED ? 1 : 0] + t.e * a.ews + t.n0 * a.ldws;
+  const int slabs = mx_slabs(a.K);
+  const uint8_t *ws0 = a.ws[0] + t.e * a.ews + mx_scale_row(t.n0, slabs), *ws1 = a.ws[GATED ? 1 : 0] + t.e * a.ews + mx_scale_row(t.n0, slabs);
   const long long xbase = a.tok ? 0 : t.m0;
-  const lt_rsrc_t rx = lt_rsrc((const uint8_t *)a.x + xbase * a.ldx), rxs = lt_rsrc(a.xs + xbase * a.ldxs);
+  const lt_rsrc_t rx = lt_rsrc((const uint8_t *)a.x + xbase * a.ldx), rxs = lt_rsrc(a.xs + mx_scale_row(xbase & ~31ll, slabs));
   const lt_rsrc_t rw0 = lt_rsrc(w0), rw1 = lt_rsrc(w1), rs0 = lt_rsrc(ws0), rs1 = lt_rsrc(ws1);
   auto xrow = [&](int i) {  // row i of the tile in x, from xbase on
     const int m = min(t.m0 + i, t.m_end - 1);
@@ -481,9 +489,9 @@ __global__ __launch_bounds__(256, RING * (WM + WN) * 64 * 136 > 80 * 1024 ? 1 : 
 #pragma unroll
   for (int i = 0; i < NS; ++i) {
     const int b = 4 * i + w, bw = b - NX;
-    if (b < NX) { vs[i] = xrow(32 * b + (lane >> 1)) * (int)a.ldxs + 4 * (lane & 1); rsc[i] = rxs; }
+    if (b < NX) { vs[i] = (int)mx_scale_row(xrow(32 * b + (lane >> 1)) + (xbase & 31), slabs) + 4 * (lane & 1); rsc[i] = rxs; }
     else {
-      vs[i] = b < NX + NW ? wrow(32 * (GATED ? bw >> 1 : bw) + (lane >> 1)) * (int)a.ldws + 4 * (lane & 1) : LT_OUT;
+      vs[i] = b < NX + NW ? (int)mx_scale_row(wrow(32 * (GATED ? bw >> 1 : bw) + (lane >> 1)), slabs) + 4 * (lane & 1) : LT_OUT;
       rsc[i] = GATED && (bw & 1) ? rs1 : rs0;
     }
   }
@@ -497,7 +505,7 @@ __global__ __launch_bounds__(256, RING * (WM + WN) * 64 * 136 > 80 * 1024 ? 1 : 
     } else {
       const int s = i - NX - NW;
       const bool in = kt * 8 + 4 * (lane & 1) < blocks;
-      mx_dma4(lds + (unsigned)(place + CODES + (4 * s + w) * 256), in ? vs[s] : LT_OUT, rsc[s], kt * 8);
+      mx_dma4(lds + (unsigned)(place + CODES + (4 * s + w) * 256), in ? vs[s] : LT_OUT, rsc[s], kt * 256);
     }
   };
   unsigned ax[4], aw[4];  // LDS address of the lane's fragment of step j in block 0, of rows that begin where the ring does
@@ -594,7 +602,8 @@ __global__ __launch_bounds__(256, RING * (WM * 64 * 256 + WN * 64 * 64 + 1024) >
   const long long xbase = a.tok ? 0 : t.m0;
   const lt_rsrc_t rx = lt_rsrc((const uint8_t *)a.x + xbase * a.ldx);
   const lt_rsrc_t rw0 = lt_rsrc(a.w[0] + t.e * a.ew + t.n0 * a.ldw), rw1 = lt_rsrc(a.w[GATED ? 1 : 0] + t.e * a.ew + t.n0 * a.ldw);
-  const lt_rsrc_t rs0 = lt_rsrc(a.ws[0] + t.e * a.ews + t.n0 * a.ldws), rs1 = lt_rsrc(a.ws[GATED ? 1 : 0] + t.e * a.ews + t.n0 * a.ldws);
+  const int slabs = mx_slabs(a.K);
+  const lt_rsrc_t rs0 = lt_rsrc(a.ws[0] + t.e * a.ews + mx_scale_row(t.n0, slabs)), rs1 = lt_rsrc(a.ws[GATED ? 1 : 0] + t.e * a.ews + mx_scale_row(t.n0, slabs));
   // transfer i of wave w: four rows of x from 16 i + 4 w on, sixteen lanes a row; sixteen rows of W from 64 i + 16 w on, four lanes a row.
   // Scales: wave w (w < WN) 64 rows of W.
   const int xr = 4 * w + (lane >> 4), xc = (lane & 15) ^ xr, wr = 16 * w + (lane >> 2), wc = (lane & 3) ^ ((wr >> 2) & 3);
@@ -612,7 +621,7 @@ __global__ __launch_bounds__(256, RING * (WM * 64 * 256 + WN * 64 * 64 + 1024) >
   for (int i = 0; i < NW; ++i) vw[i] = wrow(64 * i + wr) * (int)a.ldw + 16 * wc;
   // a gated pair's matrices change every 32 rows of the tile, so with the wave; its scales stand one matrix behind the other, 64 rows a wave
   const lt_rsrc_t rw = GATED && (w & 2) ? rw1 : rw0, rs = GATED && w >= WN / 2 ? rs1 : rs0;
-  const int vs = w < WN ? (min(t.n0 + 64 * (GATED ? w % ((WN + 1) / 2) : w) + lane, a.N - 1) - t.n0) * (int)a.ldws : LT_OUT;
+  const int vs = w < WN ? (int)mx_scale_row(min(t.n0 + 64 * (GATED ? w % ((WN + 1) / 2) : w) + lane, a.N - 1) - t.n0, slabs) : LT_OUT;
   const int kt0 = t.split * a.slabs + min(t.split, a.extra), nk = kt0 + a.slabs + (t.split < a.extra);
   const int blocks = min(a.K >> 5, nk * (M16_K / 32));  // (past the last block: zeros)
   auto dma = [&](int i, int kt, int place) {
@@ -623,7 +632,7 @@ __global__ __launch_bounds__(256, RING * (WM * 64 * 256 + WN * 64 * 64 + 1024) >
       const bool in = kt * 4 + wc < blocks;
       mx_dma16(lds + (unsigned)(place + XS + ((i - NX) * 64 + 16 * w) * 64), in ? vw[i < NX || i >= NX + NW ? 0 : i - NX] : LT_OUT, rw, kt * (M16_K / 2));
     } else {
-      mx_dma4(lds + (unsigned)(place + CODES + w * 256), kt * 4 < blocks ? vs : LT_OUT, rs, kt * 4);
+      mx_dma4(lds + (unsigned)(place + CODES + w * 256), kt * 4 < blocks ? vs : LT_OUT, rs, (kt >> 1) * 256 + (kt & 1) * 4);
     }
   };
   unsigned ax[8], aw[2], as[WN];  // LDS address of the lane's fragments in block 0 (scales: every block), of rows that begin where the ring does
@@ -722,86 +731,73 @@ __global__ __launch_bounds__(256, RING * (WM * 64 * 256 + WN * 64 * 64 + 1024) >
 }
 
 // ---- entry points -------------------------------------------------------------------------------------------------------------
-static bool mx_aligned(const void *codes, int64_t ldc, const void *scales, int64_t lds) {
-  return !(((uintptr_t)codes | (uintptr_t)ldc) & 15) && !(((uintptr_t)scales | (uintptr_t)lds) & 3);
-}
 static bool mx_meet(const void *a, int64_t na, int64_t la, int64_t len_a, const void *b, int64_t nb, int64_t lb, int64_t len_b) {
   const char *p = (const char *)a, *q = (const char *)b;
   return p && q && na > 0 && nb > 0 && len_a > 0 && len_b > 0 && p < q + (nb - 1) * lb + len_b && q < p + (na - 1) * la + len_a;
 }
-static int quant_check(const char *who, const void *v, int64_t ldv, int dtype, int64_t M, int K, const void *codes, int64_t ldc,
-                       const void *scales, int64_t lds) {
-  if (M < 0 || K < 0 || K % 32 || dtype < MOE_DT_BF16 || dtype > MOE_DT_FP32 || ldv < K || ldc < K / 2 || lds < K / 32 || M >= 1ll << 40 ||
-      ldv >= 1ll << 40 || ldc >= 1ll << 40 || lds >= 1ll << 40) {
-    moe_set_error("%s: bad shape (M=%lld K=%d dtype=%d, rows %lld, %lld and %lld apart)", who, (long long)M, K, dtype, (long long)ldv,
-                  (long long)ldc, (long long)lds);
-    return MOE_EINVAL;
-  }
-  if (!M || !K) return MOE_OK;
+extern "C" int64_t moe_mx4_scale_bytes(int64_t rows, int K) {
+  return rows <= 0 || K <= 0 ? 0 : (rows + 31) / 32 * mx_slabs(K) * 256;
+}
+static int quant_run(const char *who, const void *v, int64_t ldv, int64_t next_v, int dtype, int E, int M, int K, const moe_mx4 *q, bool back,
+                     hipStream_t s) {
   const int size = dtype == MOE_DT_FP32 ? 4 : 2;
-  if (!v || !codes || !scales || ((uintptr_t)v & 15) || ldv * size % 16 || !mx_aligned(codes, ldc, scales, 0)) {
-    moe_set_error("%s: rows of values and of codes must be present and on 16-byte boundaries, scales on 4-byte ones", who);
+  const bool one = E <= 1;
+  if (!q || E < 0 || M < 0 || K < 0 || K % 32 || dtype < MOE_DT_BF16 || dtype > MOE_DT_FP32 || E > 65535 || ldv < K || ldv >= 1ll << 40 ||
+      q->ldc < K / 2 || q->ldc % 16 || q->ldc >= 1ll << 40 || ldv * size % 16 ||
+      (!one && (next_v < 0 || next_v * size % 16 || q->next_c < 0 || q->next_c % 16 || q->next_s < 0))) {
+    moe_set_error("%s: bad shape (E=%d M=%d K=%d dtype=%d, rows %lld and %lld apart)", who, E, M, K, dtype, (long long)ldv,
+                  q ? (long long)q->ldc : 0);
     return MOE_EINVAL;
   }
-  const int64_t n = M * (K / 8);
-  if (n / 1024 >= 1 << 24 || (n >= 1ll << 31 && !(ldv == K && ldc == K / 2 && lds == K / 32))) {
-    moe_set_error("%s: %lld x %d values are too many for one launch", who, (long long)M, K);
+  if (!E || !M || !K) return MOE_OK;
+  if (!v || !q->codes || !q->scales || (((uintptr_t)v | (uintptr_t)q->codes) & 15)) {
+    moe_set_error("%s: rows of values and of codes must be present and on 16-byte boundaries", who);
     return MOE_EINVAL;
   }
-  if (mx_meet(v, M, ldv * size, (int64_t)K * size, codes, M, ldc, K / 2) || mx_meet(v, M, ldv * size, (int64_t)K * size, scales, M, lds, K / 32) ||
-      mx_meet(codes, M, ldc, K / 2, scales, M, lds, K / 32)) {
+  const int64_t n = (int64_t)M * (K / 8);
+  if (n >= 1ll << 31) {
+    moe_set_error("%s: %d x %d values are too many for one matrix", who, M, K);
+    return MOE_EINVAL;
+  }
+  const int64_t nv = one ? 0 : next_v * size, nc = one ? 0 : q->next_c, ns = one ? 0 : q->next_s;
+  const int64_t all_v = (E - 1) * nv + (M - 1) * ldv * size + (int64_t)K * size, all_c = (E - 1) * nc + (M - 1) * q->ldc + K / 2;
+  const int64_t all_s = (E - 1) * ns + moe_mx4_scale_bytes(M, K);
+  if (mx_meet(v, 1, 0, all_v, q->codes, 1, 0, all_c) || mx_meet(v, 1, 0, all_v, q->scales, 1, 0, all_s) ||
+      mx_meet(q->codes, 1, 0, all_c, q->scales, 1, 0, all_s)) {
     moe_set_error("%s: values, codes and scales overlap", who);
     return MOE_EINVAL;
   }
-  return MOE_OK;
-}
-static QuantArgs quant_args(const void *x, void *y, void *scales, int64_t ldv, int64_t ldc, int64_t lds, int64_t M, int K, bool *flat) {
-  QuantArgs a{x, y, (uint8_t *)scales, ldv, ldc, lds, M * (K / 8), (u32)K / 8, 0, 0};
-  *flat = M == 1 || (ldv == K && ldc == K / 2 && lds == K / 32);
+  QuantArgs a{(const char *)(back ? q->codes : v), (char *)(back ? v : q->codes), (uint8_t *)q->scales, ldv, q->ldc, one ? 0 : next_v, nc, ns,
+              (u32)n, (u32)K / 8, 0, 0, mx_slabs(K)};
   while ((1ull << a.shift) < a.per) ++a.shift;
   a.magic = (u32)((((1ull << a.shift) - a.per) << 32) / a.per + 1);
-  return a;
-}
-#define QUANT_LAUNCH(KERNEL)                                                                                                     \
-  const dim3 grid((unsigned)((a.n + 256 * QT_U - 1) / (256 * QT_U)));                                                            \
-  hipStream_t s = (hipStream_t)stream;                                                                                           \
-  switch (dtype * 2 + (flat ? 1 : 0)) {                                                                                          \
-    case 0: hipLaunchKernelGGL(HIP_KERNEL_NAME(KERNEL<MOE_DT_BF16, false>), grid, dim3(256), 0, s, a); break;                    \
-    case 1: hipLaunchKernelGGL(HIP_KERNEL_NAME(KERNEL<MOE_DT_BF16, true>), grid, dim3(256), 0, s, a); break;                     \
-    case 2: hipLaunchKernelGGL(HIP_KERNEL_NAME(KERNEL<MOE_DT_FP16, false>), grid, dim3(256), 0, s, a); break;                    \
-    case 3: hipLaunchKernelGGL(HIP_KERNEL_NAME(KERNEL<MOE_DT_FP16, true>), grid, dim3(256), 0, s, a); break;                     \
-    case 4: hipLaunchKernelGGL(HIP_KERNEL_NAME(KERNEL<MOE_DT_FP32, false>), grid, dim3(256), 0, s, a); break;                    \
-    default: hipLaunchKernelGGL(HIP_KERNEL_NAME(KERNEL<MOE_DT_FP32, true>), grid, dim3(256), 0, s, a); break;                    \
+  const dim3 grid((unsigned)((n + 256 * QT_U - 1) / (256 * QT_U)), E);
+  switch (dtype * 2 + (back ? 1 : 0)) {
+    case 0: hipLaunchKernelGGL(k_mx4_quantize<MOE_DT_BF16>, grid, dim3(256), 0, s, a); break;
+    case 1: hipLaunchKernelGGL(k_mx4_dequantize<MOE_DT_BF16>, grid, dim3(256), 0, s, a); break;
+    case 2: hipLaunchKernelGGL(k_mx4_quantize<MOE_DT_FP16>, grid, dim3(256), 0, s, a); break;
+    case 3: hipLaunchKernelGGL(k_mx4_dequantize<MOE_DT_FP16>, grid, dim3(256), 0, s, a); break;
+    case 4: hipLaunchKernelGGL(k_mx4_quantize<MOE_DT_FP32>, grid, dim3(256), 0, s, a); break;
+    default: hipLaunchKernelGGL(k_mx4_dequantize<MOE_DT_FP32>, grid, dim3(256), 0, s, a); break;
   }
-extern "C" int moe_mx4_quantize(const void *x, int64_t ldx, int dtype, int64_t M, int K, void *codes, int64_t ldc, void *scales,
-                                int64_t lds, void *stream) {
-  if (int rc = quant_check("moe_mx4_quantize", x, ldx, dtype, M, K, codes, ldc, scales, lds)) return rc;
-  if (!M || !K) return MOE_OK;
-  bool flat;
-  const QuantArgs a = quant_args(x, codes, scales, ldx, ldc, lds, M, K, &flat);
-  QUANT_LAUNCH(k_mx4_quantize)
-  return moe_check_launch("k_mx4_quantize");
+  return moe_check_launch(back ? "k_mx4_dequantize" : "k_mx4_quantize");
 }
-extern "C" int moe_mx4_dequantize(const void *codes, int64_t ldc, const void *scales, int64_t lds, int64_t M, int K, void *y, int64_t ldy,
-                                  int dtype, void *stream) {
-  if (int rc = quant_check("moe_mx4_dequantize", y, ldy, dtype, M, K, codes, ldc, scales, lds)) return rc;
-  if (!M || !K) return MOE_OK;
-  bool flat;
-  const QuantArgs a = quant_args(codes, y, (void *)scales, ldy, ldc, lds, M, K, &flat);
-  QUANT_LAUNCH(k_mx4_dequantize)
-  return moe_check_launch("k_mx4_dequantize");
+extern "C" int moe_mx4_quantize(const void *x, int64_t ldx, int64_t next_x, int dtype, int E, int M, int K, const moe_mx4 *q, void *stream) {
+  return quant_run("moe_mx4_quantize", x, ldx, next_x, dtype, E, M, K, q, false, (hipStream_t)stream);
+}
+extern "C" int moe_mx4_dequantize(const moe_mx4 *q, int E, int M, int K, void *y, int64_t ldy, int64_t next_y, int dtype, void *stream) {
+  return quant_run("moe_mx4_dequantize", y, ldy, next_y, dtype, E, M, K, q, true, (hipStream_t)stream);
 }
 
 // What the products of both kinds check; xrows: rows of x, experts: matrices
 static int mx_check(const char *who, const MxArgs &a, int xkind, int64_t xrows, int experts, int dtype, bool gated) {
-  const int64_t xlen = xkind == X_MX4 ? a.K / 2 : a.K * 2ll, wlen = a.K / 2, slen = a.K / 32;
+  const int64_t xlen = xkind == X_MX4 ? a.K / 2 : a.K * 2ll, wlen = a.K / 2;
   const bool empty = a.M == 0 || a.N == 0;
   if (a.M < 0 || a.N < 0 || a.K <= 0 || a.K % 32 || (dtype != MOE_DT_BF16 && dtype != MOE_DT_FP16) || a.act < MOE_ACT_NONE ||
       a.act > MOE_ACT_RELU2 || a.ldx < xlen || a.ldx % 16 || a.ldx >= 1 << 22 || a.ldw < wlen || a.ldw % 16 || a.ldw >= 1 << 22 ||
-      (xkind == X_MX4 && (a.ldxs < slen || a.ldxs % 4 || a.ldxs >= 1 << 22)) || a.ldws < slen || a.ldws % 4 || a.ldws >= 1 << 22 ||
       a.ew < 0 || a.ews < 0 || a.ew % 16 || a.ews % 4 || a.ldy < a.N || (a.res && a.ldr < a.N) || a.M > 1 << 26 || a.N > 1 << 26) {
-    moe_set_error("%s: bad shape (M=%d N=%d K=%d dtype=%d act=%d, rows %lld %lld %lld %lld %lld %lld apart)", who, a.M, a.N, a.K, dtype,
-                  a.act, a.ldx, a.ldxs, a.ldw, a.ldws, a.res ? a.ldr : 0, a.ldy);
+    moe_set_error("%s: bad shape (M=%d N=%d K=%d dtype=%d act=%d, rows %lld %lld %lld %lld apart)", who, a.M, a.N, a.K, dtype,
+                  a.act, a.ldx, a.ldw, a.res ? a.ldr : 0, a.ldy);
     return MOE_EINVAL;
   }
   if (empty) return MOE_OK;
@@ -818,10 +814,10 @@ static int mx_check(const char *who, const MxArgs &a, int xkind, int64_t xrows, 
   }
   const int64_t e = a.y32 ? 4 : 2, ylen = a.N * e, yld = a.ldy * e;
   auto meets = [&](const void *p, int64_t rows, int64_t ld, int64_t len) { return mx_meet(a.y, a.M, yld, ylen, p, rows, ld, len); };
-  bool shares = meets(a.x, xrows, a.ldx, xlen) || (xkind == X_MX4 && meets(a.xs, xrows, a.ldxs, slen));
+  bool shares = meets(a.x, xrows, a.ldx, xlen) || (xkind == X_MX4 && meets(a.xs, 1, 0, moe_mx4_scale_bytes(xrows, a.K)));
   for (int i = 0; i < (gated ? 2 : 1); ++i) {
     shares = shares || meets(a.w[i], 1, 0, (experts - 1) * a.ew + (a.N - 1) * a.ldw + wlen) ||
-             meets(a.ws[i], 1, 0, (experts - 1) * a.ews + (a.N - 1) * a.ldws + slen) || meets(a.bias[i], 1, 0, 2ll * experts * a.N);
+             meets(a.ws[i], 1, 0, (experts - 1) * a.ews + moe_mx4_scale_bytes(a.N, a.K)) || meets(a.bias[i], 1, 0, 2ll * experts * a.N);
   }
   const bool in_place = a.res == a.y && !a.y32 && (a.ldr == a.ldy || a.M == 1);
   if (shares || (!in_place && meets(a.res, a.M, a.ldr * 2, a.N * 2ll))) {
@@ -835,6 +831,7 @@ static MxPlan mx_plan(int xkind, long long rows, int tiles_of, int N, int K, boo
   const long long each = rows / tiles_of;
   if (each <= 16) return MxPlan{0, 0, 0, 1};
   if (each <= 64) return MxPlan{1, 2, 4, 1};
+  if (rows >= 4096 && each >= 256) return MxPlan{2, 4, 3, 1};
   return xkind == X_MX4 ? MxPlan{2, 2, 4, 1} : MxPlan{2, 2, 3, 1};
 }
 template <int X, bool F16, bool GATED>
@@ -875,7 +872,8 @@ static int mx_launch(const MxArgs &a, int units, int most, hipStream_t s) {  // 
   if constexpr (X == X_MX4) hipLaunchKernelGGL(HIP_KERNEL_NAME(k_mx4_tile<F16, GATED, WM_, WN_, RING4>), grid, dim3(256), 0, s, t); \
   else hipLaunchKernelGGL(HIP_KERNEL_NAME(k_mx4_tile16<X, GATED, WM_, WN_, RING16>), grid, dim3(256), 0, s, t)
   if (pl.wm == 1) { MT_LAUNCH(1, 2, 4, 5); }
-  else { MT_LAUNCH(2, 2, 4, 3); }
+  else if (pl.wn == 2) { MT_LAUNCH(2, 2, 4, 3); }
+  else { MT_LAUNCH(2, 4, 3, 3); }
 #undef MT_LAUNCH
   return moe_check_launch("k_mx4_tile");
 }
@@ -898,17 +896,16 @@ static MxArgs mx_args(const void *x, int64_t ldx, const moe_mx4 *xq, const moe_m
   a.x = xq ? xq->codes : x;
   a.xs = xq ? (const uint8_t *)xq->scales : nullptr;
   a.ldx = xq ? xq->ldc : ldx < 1ll << 40 ? ldx * 2 : ldx;
-  a.ldxs = xq ? xq->lds : 0;
   a.w[0] = (const uint8_t *)w->codes; a.ws[0] = (const uint8_t *)w->scales;
   if (w_up) { a.w[1] = (const uint8_t *)w_up->codes; a.ws[1] = (const uint8_t *)w_up->scales; }
-  a.ldw = w->ldc; a.ldws = w->lds; a.ew = w->next_c; a.ews = w->next_s;
+  a.ldw = w->ldc; a.ew = w->next_c; a.ews = w->next_s;
   a.bias[0] = (const uint16_t *)bias; a.bias[1] = (const uint16_t *)bias_up; a.res = (const uint16_t *)residual;
   a.y = y; a.ldr = ldr; a.ldy = ldy; a.M = M; a.N = N; a.K = K; a.act = act; a.y32 = y_fp32 != 0;
   return a;
 }
 // the descriptions themselves
 static int mx_described(const char *who, const void *x, const moe_mx4 *xq, const moe_mx4 *w, const moe_mx4 *w_up) {
-  if (!w || (x && xq) || (w_up && (w_up->ldc != w->ldc || w_up->lds != w->lds || w_up->next_c != w->next_c || w_up->next_s != w->next_s))) {
+  if (!w || (x && xq) || (w_up && (w_up->ldc != w->ldc || w_up->next_c != w->next_c || w_up->next_s != w->next_s))) {
     moe_set_error("%s: one x, a matrix, and for a pair a second one laid out like the first", who);
     return MOE_EINVAL;
   }

@@ -582,14 +582,19 @@ def linear_gated(x: torch.Tensor, w_gate: torch.Tensor, w_up: torch.Tensor, b_ga
     return _product("linear_gated", x, (w_gate, w_up), (b_gate, b_up), act, None, out, out_dtype)
 
 
+def _scale_shape(lead, N, K):
+    """Blocks of 32 rows by 8 scales: [..., ceil(N / 32), ceil(K / 256), 32, 8]"""
+    return (*lead, (N + 31) // 32, (K + 255) // 256, 32, 8)
+
+
 class Mx4:
     """Rows [..., K] of values in microscaled 4-bit floating point: codes uint8 [..., K / 2], two to a byte with the even column in the
     low half (sign, two bits of exponent, one of mantissa: 0, 0.5, 1, 1.5, 2, 3, 4, 6), and scales uint8 [..., K / 32], a byte e per 32
     columns that stands for 2^(e - 127); 255 makes the block NaN.  One matrix [N, K] or one per expert [E, N, K], K a multiple of 32.
-    The tensors are kept as they are where the kernels can read them so: rows of codes on 16-byte and of scales on 4-byte boundaries, with
-    the bytes up to the next one in the same storage.  Others are copied here, once (new tensors of quantize_mx4 never are)."""
+    Codes are kept as they are if their rows are on 16-byte boundaries and copied otherwise; scales are laid out anew, in the blocks that
+    the kernels read, and `scales` is a new tensor at every access."""
 
-    __slots__ = ("codes", "scales", "shape", "desc")
+    __slots__ = ("shape", "desc", "_codes", "_blocks", "_buffer")
 
     def __init__(self, codes: torch.Tensor, scales: torch.Tensor):
         if codes.dtype != torch.uint8 or scales.dtype != torch.uint8 or codes.dim() not in (2, 3) or codes.dim() != scales.dim():
@@ -599,63 +604,88 @@ class Mx4:
             raise L.MoeError("Mx4: codes %s and scales %s (K a multiple of 32, a scale per 32 columns, one device)"
                              % (tuple(codes.shape), tuple(scales.shape)))
         if codes.numel():
-            apart = [(n, st) for n, st in zip(codes.shape[:-1], codes.stride()) if n > 1]
-            if codes.stride(-1) != 1 or codes.data_ptr() % 16 or any(st % 16 for _, st in apart) or \
+            apart = [st for n, st in zip(codes.shape[:-1], codes.stride()) if n > 1]
+            if codes.stride(-1) != 1 or codes.data_ptr() % 16 or any(st % 16 for st in apart) or \
                     (codes.shape[-2] > 1 and codes.stride(-2) < K // 2):
                 codes = codes.clone(memory_format=torch.contiguous_format)
-            blocks, tail = K // 32, (K // 32 + 3) // 4 * 4
-            apart = [(n, st) for n, st in zip(scales.shape[:-1], scales.stride()) if n > 1]
-            last = scales.storage_offset() + sum((n - 1) * st for n, st in apart) + tail
-            if (scales.stride(-1) != 1 and blocks > 1) or scales.data_ptr() % 4 or any(st % 4 for _, st in apart) or \
-                    (scales.shape[-2] > 1 and scales.stride(-2) < blocks) or last > scales.untyped_storage().nbytes():
-                wide = torch.zeros(*scales.shape[:-1], tail, dtype=torch.uint8, device=scales.device)
-                wide[..., :blocks] = scales
-                scales = wide[..., :blocks]
-        self._set(codes, scales)
-
-    def _set(self, codes, scales):
+        *lead, N = codes.shape[:-1]
+        shape = _scale_shape(lead, N, K)
+        rows = torch.nn.functional.pad(scales, (0, shape[-3] * 8 - K // 32, 0, shape[-4] * 32 - N))
+        blocks = rows.unflatten(-1, (-1, 8)).unflatten(-3, (-1, 32)).transpose(-3, -2).contiguous() if N else rows.new_empty(shape)
+        self._codes, self._blocks, self._buffer, self.shape = codes, blocks, None, (*lead, N, K)
         # (of one row the distance to the next is whatever the tensor says: the kernels get one that holds the row)
-        K2, blocks = codes.shape[-1], scales.shape[-1]
-        n = codes.shape[-2]
-        ldc, lds = (codes.stride(-2), scales.stride(-2)) if n > 1 else (K2, (blocks + 3) // 4 * 4)
-        next_c, next_s = (codes.stride(0), scales.stride(0)) if codes.dim() == 3 and codes.shape[0] > 1 else (0, 0)
-        self.codes, self.scales, self.shape = codes, scales, (*codes.shape[:-1], 2 * K2)
-        self.desc = L.Mx4Desc(codes.data_ptr(), scales.data_ptr(), ldc, lds, next_c, next_s)
-        return self
+        self.desc = L.Mx4Desc(codes.data_ptr(), blocks.data_ptr(), codes.stride(-2) if N > 1 else K // 2,
+                              codes.stride(0) if lead and lead[0] > 1 else 0, blocks.stride(0) if lead and lead[0] > 1 else 0)
+
+    @classmethod
+    def _empty(cls, shape, device):
+        """Codes and scales in one new allocation, looked at as tensors only when somebody does."""
+        q = cls.__new__(cls)
+        *lead, N, K = shape
+        E = lead[0] if lead else 1
+        n_c, n_s = N * K // 2, (N + 31) // 32 * ((K + 255) // 256) * 256
+        q._buffer = torch.empty(E * (n_c + n_s), dtype=torch.uint8, device=device)
+        at = q._buffer.data_ptr()
+        q._codes = q._blocks = None
+        q.shape = (*shape,)
+        q.desc = L.Mx4Desc(at, at + E * n_c, K // 2, *((n_c, n_s) if E > 1 else (0, 0)))
+        return q
+
+    @property
+    def codes(self) -> torch.Tensor:
+        if self._codes is None:
+            *lead, N, K = self.shape
+            n = (lead[0] if lead else 1) * N * K // 2
+            self._codes = self._buffer[:n].view(*lead, N, K // 2)
+        return self._codes
+
+    @property
+    def blocks(self) -> torch.Tensor:
+        """The scales as the kernels read them: [..., ceil(N / 32), ceil(K / 256), 32, 8]"""
+        if self._blocks is None:
+            *lead, N, K = self.shape
+            n = (lead[0] if lead else 1) * N * K // 2
+            self._blocks = self._buffer[n:].view(_scale_shape(lead, N, K))
+        return self._blocks
+
+    @property
+    def scales(self) -> torch.Tensor:
+        N, K = self.shape[-2:]
+        return self.blocks.transpose(-3, -2).flatten(-2).flatten(-3, -2)[..., :N, : K // 32].contiguous()
+
+    @property
+    def _tensor(self) -> torch.Tensor:
+        return self._codes if self._buffer is None else self._buffer
+
+    @property
+    def device(self) -> torch.device:
+        return self._tensor.device
 
     def __repr__(self):
-        return "Mx4(%s, %s)" % (list(self.shape), self.codes.device)
+        return "Mx4(%s, %s)" % (list(self.shape), self.device)
 
 
 def quantize_mx4(x: torch.Tensor) -> Mx4:
     """Rows [..., K] of bf16, fp16 or fp32 to microscaled 4-bit floating point (moe_mx4_quantize): the scale of 32 columns is
     2^(floor(log2 of their largest magnitude) - 2), at least 2^-127, codes go to the nearest (ties to the even code, 6 beyond 6); a block
-    with a NaN or an infinity becomes NaN.  K is a multiple of 32; x [N, K] may have its rows further apart (16-byte boundaries), x [E, N, K]
-    is contiguous."""
+    with a NaN or an infinity becomes NaN.  K is a multiple of 32; rows may be further apart (16-byte boundaries)."""
     code = L.ROW_DTYPES.get(x.dtype)
-    if code is None or x.dim() not in (2, 3) or x.shape[-1] == 0 or x.shape[-1] % 32:
+    shape = x.shape
+    if code is None or len(shape) not in (2, 3) or shape[-1] == 0 or shape[-1] % 32:
         raise L.MoeError("quantize_mx4: bf16, fp16 or fp32 [N, K] or [E, N, K] with K a multiple of 32 are needed, not %s %s"
-                         % (x.dtype, tuple(x.shape)))
+                         % (x.dtype, tuple(shape)))
     index = _operands("quantize_mx4", x)
     if index != torch.cuda.current_device():
         with torch.cuda.device(index):
             return quantize_mx4(x)
-    K = x.shape[-1]
-    M = x.numel() // K
-    if x.dim() == 2:
-        ldx = _rows("quantize_mx4", x, M, K)
-    elif x.is_contiguous():
-        ldx = K
-    else:
-        raise L.MoeError("quantize_mx4: [E, N, K] must be contiguous")
-    blocks = K // 32
-    lds = (blocks + 3) // 4 * 4
-    codes = torch.empty((*x.shape[:-1], K // 2), dtype=torch.uint8, device=x.device)
-    scales = torch.empty((*x.shape[:-1], lds), dtype=torch.uint8, device=x.device)
-    rc = lib.moe_mx4_quantize(x.data_ptr(), ldx, code, M, K, codes.data_ptr(), K // 2, scales.data_ptr(), lds, _raw_stream(index))
+    E = shape[0] if len(shape) == 3 else 1
+    M, K = shape[-2:]
+    ldx = _rows("quantize_mx4", x if len(shape) == 2 or not E else x[0], M, K)
+    q = Mx4._empty(shape, x.device)
+    rc = lib.moe_mx4_quantize(x.data_ptr(), ldx, x.stride(0) if E > 1 else 0, code, E, M, K, byref(q.desc), _raw_stream(index))
     if rc:
         check(rc, "quantize_mx4")
-    return Mx4.__new__(Mx4)._set(codes, scales if lds == blocks else scales[..., :blocks])
+    return q
 
 
 def dequantize_mx4(q: Mx4, dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
@@ -664,19 +694,16 @@ def dequantize_mx4(q: Mx4, dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
     code = L.ROW_DTYPES.get(dtype)
     if code is None or not isinstance(q, Mx4):
         raise L.MoeError("dequantize_mx4: an Mx4 into bf16, fp16 or fp32")
-    index = _operands("dequantize_mx4", q.codes, q.scales)
+    index = _operands("dequantize_mx4", q._tensor)
     if index != torch.cuda.current_device():
         with torch.cuda.device(index):
             return dequantize_mx4(q, dtype)
-    N, K = q.shape[-2:]
-    y = torch.empty(q.shape, dtype=dtype, device=q.codes.device)
-    d, size = q.desc, y.element_size()
-    parts = [(0, y.numel() // K)]
-    if len(q.shape) == 3 and q.shape[0] > 1 and N and not (d.next_c == N * d.ldc and d.next_s == N * d.lds):
-        parts = [(e, N) for e in range(q.shape[0])]       # (matrices that are not end to end go one by one)
-    for e, rows in parts:
-        check(lib.moe_mx4_dequantize((d.codes or 0) + e * d.next_c, d.ldc, (d.scales or 0) + e * d.next_s, d.lds, rows, K,
-                                     y.data_ptr() + e * N * K * size, K, code, _raw_stream(index)), "dequantize_mx4")
+    shape = q.shape
+    N, K = shape[-2:]
+    y = torch.empty(shape, dtype=dtype, device=q._tensor.device)
+    rc = lib.moe_mx4_dequantize(byref(q.desc), shape[0] if len(shape) == 3 else 1, N, K, y.data_ptr(), K, N * K, code, _raw_stream(index))
+    if rc:
+        check(rc, "dequantize_mx4")
     return y
 
 
@@ -694,9 +721,8 @@ def _product_mx4(what, x, mats, biases, act, residual, out, out_dtype, d=None, o
     code = L.DTYPES.get(dtype)
     if code is None or act not in L.ACTS:
         raise L.MoeError("%s: an x of bf16, fp16 or Mx4 and one of the activations %s" % (what, sorted(L.ACTS)))
-    parts = [t for m in mats for t in (m.codes, m.scales)]
-    first = x.codes if quantised else x
-    index = _operands(what, first, *parts, *((x.scales,) if quantised else ()), *biases, residual, out,
+    first = x._tensor if quantised else x
+    index = _operands(what, first, *[m._tensor for m in mats], *biases, residual, out,
                       *((d.counts, d.offsets, d.units, d.sorted_tok) if d is not None else ()))
     if index != torch.cuda.current_device():
         with torch.cuda.device(index):
@@ -717,7 +743,7 @@ def _product_mx4(what, x, mats, biases, act, residual, out, out_dtype, d=None, o
     wd = w.desc
     for m in mats[1:]:
         md = m.desc
-        if (md.ldc, md.lds, md.next_c, md.next_s) != (wd.ldc, wd.lds, wd.next_c, wd.next_s):
+        if (md.ldc, md.next_c, md.next_s) != (wd.ldc, wd.next_c, wd.next_s):
             raise L.MoeError("%s: both matrices of a pair must have the same strides" % what)
     for b in biases:
         if b is not None and (b.dtype != dtype or b.shape != w.shape[:-1] or not b.is_contiguous()):

@@ -96,7 +96,7 @@ def test_quantize_infinities_nan_and_three_dimensions(cuda):
 
 
 def test_quantize_many_rows_past_32_bits_of_offsets(cuda):
-    """2.2e9 values in one call: offsets of values pass 2^32 bytes, their number 2^31."""
+    """2.2e9 values in one call: offsets of values pass 2^32 bytes, their number 2^31.  Rows of zeros have zeros for codes."""
     from promoe_amd import ops
     print("case quantize_large", flush=True)
     M, K = 1 << 20, 2112
@@ -123,16 +123,17 @@ def matrix(shape, gen, dev, spread=3):
 
 
 def spaced(q, gap, dev):
-    """The same values with the rows further apart, NaN scales and other codes between them and behind the last."""
+    """The same values with rows of codes further apart, other codes between them and NaN wherever a block of scales belongs to no row or
+    column."""
     from promoe_amd import ops
     *lead, N, K = q.shape
-    codes = torch.full((*lead, N + 1, K // 2 + 16 * gap), 0x77, dtype=torch.uint8, device=dev)
-    scales = torch.full((*lead, N + 1, (K // 32 + 3) // 4 * 4 + 4 * gap), 255, dtype=torch.uint8, device=dev)
-    codes, scales = codes[..., :N, : K // 2], scales[..., :N, : K // 32]
+    codes = torch.full((*lead, N + 1, K // 2 + 16 * gap), 0x77, dtype=torch.uint8, device=dev)[..., :N, : K // 2]
     codes.copy_(q.codes)
-    scales.copy_(q.scales)
-    s = ops.Mx4(codes, scales)
-    assert s.codes.data_ptr() == codes.data_ptr() and s.scales.data_ptr() == scales.data_ptr()
+    s = ops.Mx4(codes, q.scales)
+    assert s.codes.data_ptr() == codes.data_ptr()
+    rows = torch.nn.functional.pad(q.scales, (0, -(K // 32) % 8, 0, -N % 32), value=255)
+    s.blocks.copy_(rows.unflatten(-1, (-1, 8)).unflatten(-3, (-1, 32)).transpose(-3, -2))
+    assert torch.equal(s.scales, q.scales)
     return s
 
 
@@ -229,8 +230,10 @@ def test_nan_and_infinities_stay_in_their_rows_and_columns(cuda, M):
     gen = torch.Generator(device=cuda).manual_seed(M)
     x = rows((M, K), 1.0, torch.float16, gen, cuda)
     w = matrix((N, K), gen, cuda)
-    w.scales[17, 5] = 255
-    w.scales[N - 1, K // 32 - 1] = 255
+    scales = w.scales
+    scales[17, 5] = 255
+    scales[N - 1, K // 32 - 1] = 255
+    w = ops.Mx4(w.codes, scales)
     if M > 1:
         x[M - 1, K - 1] = float("nan")
         x[0, 0] = float("inf")
@@ -479,25 +482,39 @@ def test_two_streams_at_once(cuda):
         assert all(torch.equal(g, want[i]) for g in got[i])
 
 
-def test_matrices_that_have_to_be_copied(cuda):
-    """Scales of 3 bytes a row, codes off 16-byte boundaries, a last row without the bytes behind it."""
+def test_matrices_as_they_come(cuda):
+    """Scales in any order, codes off 16-byte boundaries (copied) or far apart (kept), parts of stacked matrices, matrices from quantize_mx4."""
     from promoe_amd import ops
-    print("case mx4_copied", flush=True)
+    print("case mx4_layouts", flush=True)
     gen = torch.Generator(device=cuda).manual_seed(6)
     N, K = 37, 96
     q = matrix((N, K), gen, cuda)
     v = values(q.codes, q.scales)
-    tight = torch.empty(N * 3 + 1, dtype=torch.uint8, device=cuda)[1:].view(N, 3)
-    tight.copy_(q.scales)
     off = torch.empty(N * 48 + 8, dtype=torch.uint8, device=cuda)[8:].view(N, 48)
     off.copy_(q.codes)
     x = torch.randn(50, K, device=cuda, generator=gen).to(torch.bfloat16)
     y, e = expect(x.double(), [v], [None], "none")
-    for codes, scales in ((q.codes, tight), (off, q.scales), (off, tight), (off.t().contiguous().t(), tight.t().contiguous().t())):
+    for codes, scales in ((off, q.scales), (off.t().contiguous().t(), q.scales.t().contiguous().t())):
         m = ops.Mx4(codes, scales)
         assert torch.equal(m.codes, q.codes) and torch.equal(m.scales, q.scales)
         check(ops.linear_mx4(x, m), y, e)
         assert torch.equal(ops.dequantize_mx4(m, torch.float32).double(), v)
     three = matrix((3, N, K), gen, cuda)
     part = ops.Mx4(three.codes[:, 5:30], three.scales[:, 5:30])
+    assert part.codes.data_ptr() == three.codes[:, 5:30].data_ptr()
     assert torch.equal(ops.dequantize_mx4(part, torch.float32).double(), values(three.codes[:, 5:30], three.scales[:, 5:30]))
+    # a pair, one quantised here and one given as codes and scales
+    w = ops.quantize_mx4(torch.randn(N, K, device=cuda, generator=gen))
+    y, e = expect(x.double(), [values(w.codes, w.scales), v], [None, None], "silu")
+    check(ops.linear_gated_mx4(x, w, q), y, e)
+    # matrices of experts quantised from rows that lie apart
+    src = torch.randn(4, N + 3, 2 * K, device=cuda, generator=gen)[:, :N, :K]
+    w = ops.quantize_mx4(src)
+    same(w, src)
+    idx, d = routed(50, 4, 2, gen, cuda)
+    got = ops.experts_linear_mx4(x, w, d, of_tokens=True, out_dtype=torch.float32)
+    order = torch.sort(idx.reshape(-1), stable=True).indices
+    for e_ in range(4):
+        at = torch.nonzero(idx.reshape(-1)[order] == e_)[:, 0]
+        y, e = expect(x.double()[order[at] // 2], [values(w.codes[e_], w.scales[e_])], [None], "none")
+        check(got[at], y, e)
