@@ -581,6 +581,130 @@ __global__ __launch_bounds__(256, RING * (WM + WN) * 64 * 136 > 80 * 1024 ? 1 : 
   mx_tile_out<F16, GATED, WM, WN>(mx_out(a, t), acc, s_ring, t.m0, t.n0, t.split);
 }
 
+// ---- wide tiles, x in 4 bits: 256 x 256 -------------------------------------------------------------------------------------------
+// The same four waves, each on 4 x 4 blocks of 32 x 32: a step (a quarter of a slab) is 16 products, which last many times an LDS read, so that
+// fragments are read step by step.  Two slabs in LDS.  The fragments of a whole slab fit the registers (four steps of eight), and they are
+// read as early as the slab is there: in the middle of its step 1 everybody has all of it, so its place takes the slab after next from
+// then on, more than a slab's time in front of the first read of that.
+template <bool F16, bool GATED>
+__global__ __launch_bounds__(256, 1) void k_mx4_wide(const MxArgs a) {
+  constexpr int B = 256, NB = 4, NX = 8, NW = 8, NS = 4, NT = NX + NW + NS;
+  constexpr int CODES = 2 * B * 128, SLAB = CODES + NS * 1024, NC = GATED ? B / 2 : B;
+  constexpr int FREE = 28, SENT = 60;  // product (of 64) in front of which a slab's place is free; the last that a transfer goes with
+  __shared__ __align__(1024) unsigned char s_ring[2 * SLAB];
+  const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6), wm = w & 1, wn = w >> 1;
+  const int fr = lane & 31, q = lane >> 5;
+  MxTile t;
+  if (!mx_tile_of<B, NC>(a, mx_run_of(), t)) return;
+  const unsigned lds = (unsigned)(uintptr_t)(__attribute__((address_space(3))) unsigned char *)s_ring;
+  const int slabs = mx_slabs(a.K), blocks_k = a.K >> 5;
+  const long long xbase = a.tok ? 0 : t.m0;
+  const lt_rsrc_t rx = lt_rsrc((const uint8_t *)a.x + xbase * a.ldx), rxs = lt_rsrc(a.xs + mx_scale_row(xbase & ~31ll, slabs));
+  const lt_rsrc_t rw0 = lt_rsrc(a.w[0] + t.e * a.ew + t.n0 * a.ldw), rw1 = lt_rsrc(a.w[GATED ? 1 : 0] + t.e * a.ew + t.n0 * a.ldw);
+  const lt_rsrc_t rs0 = lt_rsrc(a.ws[0] + t.e * a.ews + mx_scale_row(t.n0, slabs)), rs1 = lt_rsrc(a.ws[GATED ? 1 : 0] + t.e * a.ews + mx_scale_row(t.n0, slabs));
+  auto xrow = [&](int i) {
+    const int m = min(t.m0 + i, t.m_end - 1);
+    return a.tok ? a.tok[m] : m - t.m0;
+  };
+  auto wrow = [&](int i) { return min(t.n0 + i, a.N - 1) - t.n0; };
+  // transfers as in k_mx4_tile; scales: transfers 0 and 1 x's blocks w and 4 + w, 2 and 3 W's
+  const int tr = 8 * w + (lane >> 3), chunk = (lane & 7) ^ ((tr >> 1) & 7);
+  int vx[NX], vw[NW], vs[NS];
+#pragma unroll
+  for (int i = 0; i < NX; ++i) vx[i] = xrow(32 * i + tr) * (int)a.ldx + 16 * chunk;
+#pragma unroll
+  for (int i = 0; i < NW; ++i) vw[i] = wrow(32 * (GATED ? i >> 1 : i) + tr) * (int)a.ldw + 16 * chunk;
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    const int b = 4 * i + w;
+    vs[i] = (int)mx_scale_row(xrow(32 * b + (lane >> 1)) + (xbase & 31), slabs) + 4 * (lane & 1);
+    vs[2 + i] = (int)mx_scale_row(wrow(32 * (GATED ? b >> 1 : b) + (lane >> 1)), slabs) + 4 * (lane & 1);
+  }
+  const lt_rsrc_t rsw = GATED && (w & 1) ? rs1 : rs0;
+  const int kt0 = t.split * a.slabs + min(t.split, a.extra), nk = kt0 + a.slabs + (t.split < a.extra);
+  const int blocks = min(blocks_k, nk * (M4_K / 32));
+  auto dma = [&](int i, int kt, int place) {
+    if (i < NX + NW) {
+      const bool in = kt * 8 + chunk < blocks;
+      mx_dma16(lds + (unsigned)(place + (i * 32 + 8 * w) * 128), in ? (i < NX ? vx[i < NX ? i : 0] : vw[i < NX || i >= NX + NW ? 0 : i - NX]) : LT_OUT,
+               i < NX ? rx : (GATED && (i & 1)) ? rw1 : rw0, kt * (M4_K / 2));
+    } else {
+      const int s = i - NX - NW;
+      const bool in = kt * 8 + 4 * (lane & 1) < blocks;
+      mx_dma4(lds + (unsigned)(place + CODES + (4 * s + w) * 256), in ? vs[s] : LT_OUT, s < 2 ? rxs : rsw, kt * 256);
+    }
+  };
+  unsigned ax[4], aw[4];
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    const unsigned c = (unsigned)(((4 * q + j) ^ ((fr >> 1) & 7)) * 16);
+    ax[j] = lds + (unsigned)((wm * 128 + fr) * 128) + c;
+    aw[j] = lds + (unsigned)((B + wn * 128 + fr) * 128) + c;
+  }
+  const unsigned asx = lds + CODES + (unsigned)((wm * 128 + fr) * 8 + 4 * q), asw = lds + CODES + (unsigned)((B + wn * 128 + fr) * 8 + 4 * q);
+  f32x16_t acc[NB][NB];
+#pragma unroll
+  for (int i = 0; i < NB; ++i)
+#pragma unroll
+    for (int b = 0; b < NB; ++b)
+#pragma unroll
+      for (int e = 0; e < 16; ++e) acc[i][b][e] = 0.f;
+  u32x4_t fx[4][NB], fw[4][NB];
+  u32 sx[2][NB], sw[2][NB];
+  auto read = [&](int j, int r, unsigned place) {  // fragment r of step j in the order of need: W's first, then x's
+    if (r < NB) fw[j][r & 3] = *(lds_u4 *)(uintptr_t)(aw[j] + place + (unsigned)((r & 3) * 32 * 128));
+    else fx[j][r & 3] = *(lds_u4 *)(uintptr_t)(ax[j] + place + (unsigned)((r & 3) * 32 * 128));
+  };
+  auto read_s = [&](int p, int r, unsigned place) {
+    if (r < NB) sw[p][r & 3] = *(lds_u1 *)(uintptr_t)(asw + place + (unsigned)((r & 3) * 256));
+    else sx[p][r & 3] = *(lds_u1 *)(uintptr_t)(asx + place + (unsigned)((r & 3) * 256));
+  };
+#pragma unroll
+  for (int i = 0; i < 2; ++i)
+#pragma unroll
+    for (int d = 0; d < NT; ++d) dma(d, kt0 + i, i * SLAB);
+  LT_VM(NT);
+  __builtin_amdgcn_s_barrier();
+#pragma unroll
+  for (int r = 0; r < 2 * NB; ++r) { read_s(0, r, 0); read(0, r, 0); }
+  // slab kt in place p; transfers that are sent in front of product g of the slab's 64: those of slab kt + 2, from FREE on
+  auto sent = [](int g) { return g < FREE ? 0 : g >= SENT ? NT : (g - FREE) * NT / (SENT - FREE); };
+  auto slab = [&](auto p_, int kt) {
+    constexpr int p = decltype(p_)::value;
+    constexpr int PLACE = p * SLAB, NEXT = (p ^ 1) * SLAB;
+    const u32 mask = mx_mask(blocks - kt * 8 - 4 * q);
+    LT_LGKM0();
+#pragma unroll
+    for (int i = 0; i < NB; ++i) { sx[p][i] &= mask; sw[p][i] &= mask; }
+    __builtin_amdgcn_sched_barrier(0);
+    lt_each<64>([&](auto g_) {
+      constexpr int g = decltype(g_)::value, j = g / 16, i = g % 16 / NB, b = g % NB;
+      if constexpr (g < 24) read(1 + g / 8, g % 8, PLACE);                     // (as fast as LDS gives them to four waves)
+      if constexpr (g == FREE) {
+        LT_LGKM0();
+        __builtin_amdgcn_s_barrier();
+      }
+      if constexpr (g == 48) {                                                 // the next slab has landed
+        LT_VM(sent(48));
+        __builtin_amdgcn_s_barrier();
+      }
+      if constexpr (g >= 48 && g < 56) { read_s(p ^ 1, g - 48, NEXT); read(0, g - 48, NEXT); }
+#pragma unroll
+      for (int d = 0; d < NT; ++d)
+        if (d >= sent(g) && d < sent(g + 1)) dma(d, kt + 2, PLACE);
+      __builtin_amdgcn_sched_barrier(0);
+      acc[i][b] = mx_mfma32<j>(fw[j][b], fx[j][i], acc[i][b], sw[p][b], sx[p][i]);
+      __builtin_amdgcn_sched_barrier(0);
+    });
+  };
+  for (int kt = kt0; kt < nk; kt += 2) {  // (always a pair of slabs: one past the end is zeros)
+    slab(std::integral_constant<int, 0>(), kt);
+    slab(std::integral_constant<int, 1>(), kt + 1);
+  }
+  static_assert(4 * 32 * (32 * NB + 4) * 4 <= 2 * SLAB, "the sums of four waves fit the ring");
+  mx_tile_out<F16, GATED, NB, NB>(mx_out(a, t), acc, s_ring, t.m0, t.n0, t.split);
+}
+
 static __device__ __forceinline__ f32x16_t mx_mfma32_bf16(u32x4_t a, u32x4_t b, f32x16_t c) {
   return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8_t, a), __builtin_bit_cast(bf16x8_t, b), c, 0, 0, 0);
 }
@@ -831,7 +955,7 @@ static MxPlan mx_plan(int xkind, long long rows, int tiles_of, int N, int K, boo
   const long long each = rows / tiles_of;
   if (each <= 16) return MxPlan{0, 0, 0, 1};
   if (each <= 64) return MxPlan{1, 2, 4, 1};
-  if (rows >= 4096 && each >= 256) return MxPlan{2, 4, 3, 1};
+  if (rows >= 4096 && each >= 256) return xkind == X_MX4 ? MxPlan{4, 4, 2, 1} : MxPlan{2, 4, 3, 1};
   return xkind == X_MX4 ? MxPlan{2, 2, 4, 1} : MxPlan{2, 2, 3, 1};
 }
 template <int X, bool F16, bool GATED>
@@ -873,7 +997,8 @@ static int mx_launch(const MxArgs &a, int units, int most, hipStream_t s) {  // 
   else hipLaunchKernelGGL(HIP_KERNEL_NAME(k_mx4_tile16<X, GATED, WM_, WN_, RING16>), grid, dim3(256), 0, s, t)
   if (pl.wm == 1) { MT_LAUNCH(1, 2, 4, 5); }
   else if (pl.wn == 2) { MT_LAUNCH(2, 2, 4, 3); }
-  else { MT_LAUNCH(2, 4, 3, 3); }
+  else if (pl.wm == 2) { MT_LAUNCH(2, 4, 3, 3); }
+  else if constexpr (X == X_MX4) hipLaunchKernelGGL(HIP_KERNEL_NAME(k_mx4_wide<F16, GATED>), grid, dim3(256), 0, s, t);
 #undef MT_LAUNCH
   return moe_check_launch("k_mx4_tile");
 }
