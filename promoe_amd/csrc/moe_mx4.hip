@@ -376,9 +376,37 @@ static __device__ __forceinline__ void mx_tile_out(const MxArgs &a, const f32x16
   const int col = 8 * (lane % LPR), n = n0 + wn * (NC / 2) + col;
   const int at = GATED ? (col >> 5) * 64 + (col & 31) : col;
   const LinColumns<F16, GATED> c(a, n);
+  const bool inside = !a.y32 && !a.part && n0 + NC <= a.N;
+  constexpr int NP = 32 / RPP;
+  // eight columns of row r of the block: gated the second eight of the second matrix
+  auto fetch = [&](int r, float (&s0)[8], float (&s1)[8]) {
+#pragma unroll
+    for (int k = 0; k < (GATED ? 4 : 2); ++k) {
+      const f32x4_t f = *(const f32x4_t *)(buf + r * LDE + at + (k & 1) * 4 + (k >> 1) * 32);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) (k >> 1 ? s1 : s0)[4 * (k & 1) + e] = f[e];
+    }
+  };
+  // whole columns in 16 bits: every load of a residual in front of the sums' way through LDS, the activation chosen once
+  auto plain = [&](int first, const u32x4_t (&res)[NP], auto act_) {
+#pragma unroll
+    for (int p = 0; p < NP; ++p) {
+      float s0[8], s1[8];
+      fetch(lane / LPR + p * RPP, s0, s1);
+      c.template finish<decltype(act_)::value>(s0, s1);
+      if (!GATED && a.res) lin_add<F16>(s0, res[p]);
+      const int m = first + p * RPP;
+      if (m < a.M) *(u32x4_any *)((uint16_t *)a.y + m * a.ldy + n) = lin_pack<F16>(s0);
+    }
+  };
   // (one copy of the loop for all blocks: code that runs once a tile waits for its instructions, line by line)
 #pragma clang loop unroll(disable)
   for (int i = 0; i < WM; ++i) {
+    const int first = m0 + 32 * (wm * WM + i) + lane / LPR;
+    u32x4_t res[NP];
+    if (!GATED && inside && a.res)
+#pragma unroll
+      for (int p = 0; p < NP; ++p) res[p] = *(const u32x4_any *)(a.res + (long long)min(first + p * RPP, a.M - 1) * a.ldr + n);
     lt_each<WM>([&](auto i_) {
       if (i == decltype(i_)::value) {
 #pragma unroll
@@ -392,17 +420,28 @@ static __device__ __forceinline__ void mx_tile_out(const MxArgs &a, const f32x16
       }
     });
     __builtin_amdgcn_wave_barrier();
-    const int first = m0 + 32 * (wm * WM + i) + lane / LPR;
-    u32x4_t res = c.residual(a, first);
+    switch (inside ? a.act : -1) {
+      case MOE_ACT_NONE: plain(first, res, std::integral_constant<int, MOE_ACT_NONE>()); break;
+      case MOE_ACT_SILU: plain(first, res, std::integral_constant<int, MOE_ACT_SILU>()); break;
+      case MOE_ACT_GELU: plain(first, res, std::integral_constant<int, MOE_ACT_GELU>()); break;
+      case MOE_ACT_GELU_TANH: plain(first, res, std::integral_constant<int, MOE_ACT_GELU_TANH>()); break;
+      case MOE_ACT_RELU: plain(first, res, std::integral_constant<int, MOE_ACT_RELU>()); break;
+      case MOE_ACT_RELU2: plain(first, res, std::integral_constant<int, MOE_ACT_RELU2>()); break;
+      default: {
+        u32x4_t r0 = c.residual(a, first);
 #pragma clang loop unroll(disable)
-    for (int r = lane / LPR; r < 32; r += RPP) {
-      const int m = first - lane / LPR + r;
-      const u32x4_t ahead = c.residual(a, r + RPP < 32 ? m + RPP : a.M);
-      if (m < a.M) {
-        if (a.part) c.partial(a, split, m, buf + r * LDE + at, buf + r * LDE + at + 32);
-        else c.store(a, m, buf + r * LDE + at, buf + r * LDE + at + 32, res);
+        for (int p = 0; p < NP; ++p) {
+          const int m = first + p * RPP;
+          const u32x4_t ahead = c.residual(a, p + 1 < NP ? m + RPP : a.M);
+          float s0[8], s1[8];
+          fetch(lane / LPR + p * RPP, s0, s1);
+          if (m < a.M) {
+            if (a.part) c.partial(a, split, m, s0, s1);
+            else c.store(a, m, s0, s1, r0);
+          }
+          r0 = ahead;
+        }
       }
-      res = ahead;
     }
     __builtin_amdgcn_wave_barrier();
   }
