@@ -402,7 +402,8 @@ static __device__ __forceinline__ void mx_tile_out(const MxArgs &a, const f32x16
   // (one copy of the loop for all blocks: code that runs once a tile waits for its instructions, line by line)
 #pragma clang loop unroll(disable)
   for (int i = 0; i < WM; ++i) {
-    const int first = m0 + 32 * (wm * WM + i) + lane / LPR;
+    if (m0 + 32 * (2 * i + wm) >= a.M) break;
+    const int first = m0 + 32 * (2 * i + wm) + lane / LPR;
     u32x4_t res[NP];
     if (!GATED && inside && a.res)
 #pragma unroll
@@ -469,7 +470,8 @@ __global__ __launch_bounds__(256) void k_mx4_join(const MxArgs a) {
   c.store(a, m, s[0], s[1], c.residual(a, m));
 }
 
-// x in 4 bits.  Four waves (2 x 2), wave (wm, wn) on WM x WN blocks of 32 x 32: a tile of 64 WM rows of x by 64 WN rows of W.  A gated
+// x in 4 bits.  Four waves (2 x 2), wave (wm, wn) on WM x WN blocks of 32 x 32: a tile of 64 WM rows of x (block i of wave wm: rows 32 (2 i +
+// wm) ..) by 64 WN rows of W.  A gated
 // pair's W blocks alternate between the two matrices (block b: matrix b & 1, its columns 32 (b >> 1) ..), so that a lane holds both sums
 // of a column.  K advances 256 at a time (a slab: 128 bytes of codes and 8 of scales a row); slabs go global -> LDS directly, RING of them
 // in LDS.  A lane's operand of a product is one block of 32 columns: half q of the wave takes the blocks 4 q .. 4 q + 3 of a slab, so that
@@ -551,10 +553,10 @@ __global__ __launch_bounds__(256, RING * (WM + WN) * 64 * 136 > 80 * 1024 ? 1 : 
 #pragma unroll
   for (int j = 0; j < 4; ++j) {
     const unsigned c = (unsigned)(((4 * q + j) ^ ((fr >> 1) & 7)) * 16);
-    ax[j] = lds + (unsigned)((wm * WM * 32 + fr) * 128) + c;
+    ax[j] = lds + (unsigned)((wm * 32 + fr) * 128) + c;
     aw[j] = lds + (unsigned)((BM + wn * WN * 32 + fr) * 128) + c;
   }
-  const unsigned asx = lds + CODES + (unsigned)((wm * WM * 32 + fr) * 8 + 4 * q), asw = lds + CODES + (unsigned)((BM + wn * WN * 32 + fr) * 8 + 4 * q);
+  const unsigned asx = lds + CODES + (unsigned)((wm * 32 + fr) * 8 + 4 * q), asw = lds + CODES + (unsigned)((BM + wn * WN * 32 + fr) * 8 + 4 * q);
   f32x16_t acc[WM][WN];
 #pragma unroll
   for (int i = 0; i < WM; ++i)
@@ -573,11 +575,11 @@ __global__ __launch_bounds__(256, RING * (WM + WN) * 64 * 136 > 80 * 1024 ? 1 : 
   u32x4_t fx[2][4][WM], fw[2][4][WN];
   u32 sx[2][WM], sw[2][WN];
   auto read = [&](int p, int r, unsigned place) {  // fragment r of a slab: scales, then step by step
-    if (r < WM) sx[p][r] = *(lds_u1 *)(uintptr_t)(asx + place + (unsigned)(r * 256));
+    if (r < WM) sx[p][r] = *(lds_u1 *)(uintptr_t)(asx + place + (unsigned)(r * 512));
     else if (r < WM + WN) sw[p][r - WM] = *(lds_u1 *)(uintptr_t)(asw + place + (unsigned)((r - WM) * 256));
     else {
       const int s = r - WM - WN, j = s / (WM + WN), i = s % (WM + WN);
-      if (i < WM) fx[p][j][i] = *(lds_u4 *)(uintptr_t)(ax[j] + place + (unsigned)(i * 32 * 128));
+      if (i < WM) fx[p][j][i] = *(lds_u4 *)(uintptr_t)(ax[j] + place + (unsigned)(i * 64 * 128));
       else fw[p][j][i - WM] = *(lds_u4 *)(uintptr_t)(aw[j] + place + (unsigned)((i - WM) * 32 * 128));
     }
   };
@@ -650,7 +652,7 @@ __global__ __launch_bounds__(256, 1) void k_mx4_wide(const MxArgs a) {
   const int tr = 8 * w + (lane >> 3), chunk = (lane & 7) ^ ((tr >> 1) & 7);
   int vx[NX], vw[NW], vs[NS];
 #pragma unroll
-  for (int i = 0; i < NX; ++i) vx[i] = xrow(32 * i + tr) * (int)a.ldx + 16 * chunk;
+  for (int i = 0; i < NX; ++i) vx[i] = t.m0 + 32 * i < t.m_end ? xrow(32 * i + tr) * (int)a.ldx + 16 * chunk : LT_OUT;  // (blocks without a row: zeros)
 #pragma unroll
   for (int i = 0; i < NW; ++i) vw[i] = wrow(32 * (GATED ? i >> 1 : i) + tr) * (int)a.ldw + 16 * chunk;
 #pragma unroll
@@ -677,10 +679,10 @@ __global__ __launch_bounds__(256, 1) void k_mx4_wide(const MxArgs a) {
 #pragma unroll
   for (int j = 0; j < 4; ++j) {
     const unsigned c = (unsigned)(((4 * q + j) ^ ((fr >> 1) & 7)) * 16);
-    ax[j] = lds + (unsigned)((wm * 128 + fr) * 128) + c;
+    ax[j] = lds + (unsigned)((wm * 32 + fr) * 128) + c;
     aw[j] = lds + (unsigned)((B + wn * 128 + fr) * 128) + c;
   }
-  const unsigned asx = lds + CODES + (unsigned)((wm * 128 + fr) * 8 + 4 * q), asw = lds + CODES + (unsigned)((B + wn * 128 + fr) * 8 + 4 * q);
+  const unsigned asx = lds + CODES + (unsigned)((wm * 32 + fr) * 8 + 4 * q), asw = lds + CODES + (unsigned)((B + wn * 128 + fr) * 8 + 4 * q);
   f32x16_t acc[NB][NB];
 #pragma unroll
   for (int i = 0; i < NB; ++i)
@@ -692,11 +694,11 @@ __global__ __launch_bounds__(256, 1) void k_mx4_wide(const MxArgs a) {
   u32 sx[2][NB], sw[2][NB];
   auto read = [&](int j, int r, unsigned place) {  // fragment r of step j in the order of need: W's first, then x's
     if (r < NB) fw[j][r & 3] = *(lds_u4 *)(uintptr_t)(aw[j] + place + (unsigned)((r & 3) * 32 * 128));
-    else fx[j][r & 3] = *(lds_u4 *)(uintptr_t)(ax[j] + place + (unsigned)((r & 3) * 32 * 128));
+    else fx[j][r & 3] = *(lds_u4 *)(uintptr_t)(ax[j] + place + (unsigned)((r & 3) * 64 * 128));
   };
   auto read_s = [&](int p, int r, unsigned place) {
     if (r < NB) sw[p][r & 3] = *(lds_u1 *)(uintptr_t)(asw + place + (unsigned)((r & 3) * 256));
-    else sx[p][r & 3] = *(lds_u1 *)(uintptr_t)(asx + place + (unsigned)((r & 3) * 256));
+    else sx[p][r & 3] = *(lds_u1 *)(uintptr_t)(asx + place + (unsigned)((r & 3) * 512));
   };
 #pragma unroll
   for (int i = 0; i < 2; ++i)
@@ -708,8 +710,8 @@ __global__ __launch_bounds__(256, 1) void k_mx4_wide(const MxArgs a) {
   for (int r = 0; r < 2 * NB; ++r) { read_s(0, r, 0); read(0, r, 0); }
   // slab kt in place p; transfers that are sent in front of product g of the slab's 64: those of slab kt + 2, from FREE on
   auto sent = [](int g) { return g < FREE ? 0 : g >= SENT ? NT : (g - FREE) * NT / (SENT - FREE); };
-  auto slab = [&](auto p_, int kt) {
-    constexpr int p = decltype(p_)::value;
+  auto slab = [&](auto p_, auto ni_, int kt) {
+    constexpr int p = decltype(p_)::value, NI = decltype(ni_)::value;
     constexpr int PLACE = p * SLAB, NEXT = (p ^ 1) * SLAB;
     const u32 mask = mx_mask(blocks - kt * 8 - 4 * q);
     LT_LGKM0();
@@ -718,7 +720,7 @@ __global__ __launch_bounds__(256, 1) void k_mx4_wide(const MxArgs a) {
     __builtin_amdgcn_sched_barrier(0);
     lt_each<64>([&](auto g_) {
       constexpr int g = decltype(g_)::value, j = g / 16, i = g % 16 / NB, b = g % NB;
-      if constexpr (g < 24) read(1 + g / 8, g % 8, PLACE);                     // (as fast as LDS gives them to four waves)
+      if constexpr (g < 24 && g % 8 < NB + NI) read(1 + g / 8, g % 8, PLACE);                     // (as fast as LDS gives them to four waves)
       if constexpr (g == FREE) {
         LT_LGKM0();
         __builtin_amdgcn_s_barrier();
@@ -727,18 +729,28 @@ __global__ __launch_bounds__(256, 1) void k_mx4_wide(const MxArgs a) {
         LT_VM(sent(48));
         __builtin_amdgcn_s_barrier();
       }
-      if constexpr (g >= 48 && g < 56) { read_s(p ^ 1, g - 48, NEXT); read(0, g - 48, NEXT); }
+      if constexpr (g >= 48 && g < 52 + NI) { read_s(p ^ 1, g - 48, NEXT); read(0, g - 48, NEXT); }
 #pragma unroll
       for (int d = 0; d < NT; ++d)
         if (d >= sent(g) && d < sent(g + 1)) dma(d, kt + 2, PLACE);
       __builtin_amdgcn_sched_barrier(0);
-      acc[i][b] = mx_mfma32<j>(fw[j][b], fx[j][i], acc[i][b], sw[p][b], sx[p][i]);
+      if constexpr (i < NI) acc[i][b] = mx_mfma32<j>(fw[j][b], fx[j][i], acc[i][b], sw[p][b], sx[p][i]);
       __builtin_amdgcn_sched_barrier(0);
     });
   };
-  for (int kt = kt0; kt < nk; kt += 2) {  // (always a pair of slabs: one past the end is zeros)
-    slab(std::integral_constant<int, 0>(), kt);
-    slab(std::integral_constant<int, 1>(), kt + 1);
+  auto run = [&](auto ni) {
+    for (int kt = kt0; kt < nk; kt += 2) {  // (always a pair of slabs: one past the end is zeros)
+      slab(std::integral_constant<int, 0>(), ni, kt);
+      slab(std::integral_constant<int, 1>(), ni, kt + 1);
+    }
+  };
+  // an expert's last rows: a wave leaves out the products of blocks that have none (the waits and barriers are the same for all)
+  switch (min(NB, ((t.m_end - t.m0 + 31) / 32 - wm + 1) / 2)) {
+    case 4: run(std::integral_constant<int, 4>()); break;
+    case 3: run(std::integral_constant<int, 3>()); break;
+    case 2: run(std::integral_constant<int, 2>()); break;
+    case 1: run(std::integral_constant<int, 1>()); break;
+    default: run(std::integral_constant<int, 0>()); break;
   }
   static_assert(4 * 32 * (32 * NB + 4) * 4 <= 2 * SLAB, "the sums of four waves fit the ring");
   mx_tile_out<F16, GATED, NB, NB>(mx_out(a, t), acc, s_ring, t.m0, t.n0, t.split);
@@ -800,7 +812,7 @@ __global__ __launch_bounds__(256, RING * (WM * 64 * 256 + WN * 64 * 64 + 1024) >
   };
   unsigned ax[8], aw[2], as[WN];  // LDS address of the lane's fragments in block 0 (scales: every block), of rows that begin where the ring does
 #pragma unroll
-  for (int j = 0; j < 8; ++j) ax[j] = lds + (unsigned)((wm * WM * 32 + fr) * 256 + ((8 * q + j) ^ (fr & 15)) * 16);
+  for (int j = 0; j < 8; ++j) ax[j] = lds + (unsigned)((wm * 32 + fr) * 256 + ((8 * q + j) ^ (fr & 15)) * 16);
 #pragma unroll
   for (int h = 0; h < 2; ++h) aw[h] = lds + (unsigned)(XS + (wn * WN * 32 + fr) * 64 + ((2 * q + h) ^ ((fr >> 2) & 3)) * 16);
 #pragma unroll
@@ -830,7 +842,7 @@ __global__ __launch_bounds__(256, RING * (WM * 64 * 256 + WN * 64 * 64 + 1024) >
       fw[p][h & 1][b] = *(lds_u4 *)(uintptr_t)(aw[h & 1] + place + (unsigned)(b * 32 * 64));
     } else {
       const int j = (r - 3 * WN) / WM, i = (r - 3 * WN) % WM;
-      fx[p][j][i] = *(lds_u4 *)(uintptr_t)(ax[j] + place + (unsigned)(i * 32 * 256));
+      fx[p][j][i] = *(lds_u4 *)(uintptr_t)(ax[j] + place + (unsigned)(i * 64 * 256));
     }
   };
   constexpr int NR = 3 * WN + 8 * WM, NP = 8 * NG;
