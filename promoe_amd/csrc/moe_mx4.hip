@@ -351,6 +351,19 @@ static __device__ __forceinline__ int mx_run_of() {
   const int per = (int)gridDim.x >> 3;
   return ((int)blockIdx.x & 7) * per + ((int)blockIdx.x >> 3);
 }
+// Rows of x that a lane's transfers read, behind xbase: all lookups of a gathered x on their way at once
+template <int N, class F>
+static __device__ __forceinline__ void mx_rows_of_x(const MxArgs &a, const MxTile &t, int (&row)[N], const F &of) {
+#pragma unroll
+  for (int i = 0; i < N; ++i) row[i] = min(t.m0 + of(i), t.m_end - 1);
+  if (a.tok) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) row[i] = a.tok[row[i]];
+  } else {
+#pragma unroll
+    for (int i = 0; i < N; ++i) row[i] -= t.m0;
+  }
+}
 // what the epilogue of a tile goes by
 static __device__ __forceinline__ MxArgs mx_out(const MxArgs &a, const MxTile &t) {
   MxArgs o = a;
@@ -513,24 +526,21 @@ __global__ __launch_bounds__(256, RING * (WM + WN) * 64 * 136 > 80 * 1024 ? 1 : 
   const long long xbase = a.tok ? 0 : t.m0;
   const lt_rsrc_t rx = lt_rsrc((const uint8_t *)a.x + xbase * a.ldx), rxs = lt_rsrc(a.xs + mx_scale_row(xbase & ~31ll, slabs));
   const lt_rsrc_t rw0 = lt_rsrc(w0), rw1 = lt_rsrc(w1), rs0 = lt_rsrc(ws0), rs1 = lt_rsrc(ws1);
-  auto xrow = [&](int i) {  // row i of the tile in x, from xbase on
-    const int m = min(t.m0 + i, t.m_end - 1);
-    return a.tok ? a.tok[m] : m - t.m0;
-  };
   auto wrow = [&](int i) { return min(t.n0 + i, a.N - 1) - t.n0; };
   // transfer i of wave w: rows 32 i + 8 w .. + 7, eight lanes a row; the lanes choose the chunk that belongs in their slot (chunk c of row
   // r in slot c ^ ((r >> 1) & 7)).  Scales: 32 rows a transfer, a word for each half of the wave, transfer 4 i + w of x's blocks and then W's.
   const int tr = 8 * w + (lane >> 3), chunk = (lane & 7) ^ ((tr >> 1) & 7);
-  int vx[NX], vw[NW], vs[NS];
+  int vx[NX], vw[NW], vs[NS], row[NX + NS];
+  mx_rows_of_x(a, t, row, [&](int i) { return i < NX ? 32 * i + tr : 32 * min(4 * (i - NX) + w, NX - 1) + (lane >> 1); });
 #pragma unroll
-  for (int i = 0; i < NX; ++i) vx[i] = xrow(32 * i + tr) * (int)a.ldx + 16 * chunk;
+  for (int i = 0; i < NX; ++i) vx[i] = row[i] * (int)a.ldx + 16 * chunk;
 #pragma unroll
   for (int i = 0; i < NW; ++i) vw[i] = wrow(32 * (GATED ? i >> 1 : i) + tr) * (int)a.ldw + 16 * chunk;
   lt_rsrc_t rsc[NS];
 #pragma unroll
   for (int i = 0; i < NS; ++i) {
     const int b = 4 * i + w, bw = b - NX;
-    if (b < NX) { vs[i] = (int)mx_scale_row(xrow(32 * b + (lane >> 1)) + (xbase & 31), slabs) + 4 * (lane & 1); rsc[i] = rxs; }
+    if (b < NX) { vs[i] = (int)mx_scale_row(row[NX + i] + (xbase & 31), slabs) + 4 * (lane & 1); rsc[i] = rxs; }
     else {
       vs[i] = b < NX + NW ? (int)mx_scale_row(wrow(32 * (GATED ? bw >> 1 : bw) + (lane >> 1)), slabs) + 4 * (lane & 1) : LT_OUT;
       rsc[i] = GATED && (bw & 1) ? rs1 : rs0;
@@ -643,22 +653,19 @@ __global__ __launch_bounds__(256, 1) void k_mx4_wide(const MxArgs a) {
   const lt_rsrc_t rx = lt_rsrc((const uint8_t *)a.x + xbase * a.ldx), rxs = lt_rsrc(a.xs + mx_scale_row(xbase & ~31ll, slabs));
   const lt_rsrc_t rw0 = lt_rsrc(a.w[0] + t.e * a.ew + t.n0 * a.ldw), rw1 = lt_rsrc(a.w[GATED ? 1 : 0] + t.e * a.ew + t.n0 * a.ldw);
   const lt_rsrc_t rs0 = lt_rsrc(a.ws[0] + t.e * a.ews + mx_scale_row(t.n0, slabs)), rs1 = lt_rsrc(a.ws[GATED ? 1 : 0] + t.e * a.ews + mx_scale_row(t.n0, slabs));
-  auto xrow = [&](int i) {
-    const int m = min(t.m0 + i, t.m_end - 1);
-    return a.tok ? a.tok[m] : m - t.m0;
-  };
   auto wrow = [&](int i) { return min(t.n0 + i, a.N - 1) - t.n0; };
   // transfers as in k_mx4_tile; scales: transfers 0 and 1 x's blocks w and 4 + w, 2 and 3 W's
   const int tr = 8 * w + (lane >> 3), chunk = (lane & 7) ^ ((tr >> 1) & 7);
-  int vx[NX], vw[NW], vs[NS];
+  int vx[NX], vw[NW], vs[NS], row[NX + 2];
+  mx_rows_of_x(a, t, row, [&](int i) { return i < NX ? 32 * i + tr : 32 * (4 * (i - NX) + w) + (lane >> 1); });
 #pragma unroll
-  for (int i = 0; i < NX; ++i) vx[i] = t.m0 + 32 * i < t.m_end ? xrow(32 * i + tr) * (int)a.ldx + 16 * chunk : LT_OUT;  // (blocks without a row: zeros)
+  for (int i = 0; i < NX; ++i) vx[i] = t.m0 + 32 * i < t.m_end ? row[i] * (int)a.ldx + 16 * chunk : LT_OUT;  // (blocks without a row: zeros)
 #pragma unroll
   for (int i = 0; i < NW; ++i) vw[i] = wrow(32 * (GATED ? i >> 1 : i) + tr) * (int)a.ldw + 16 * chunk;
 #pragma unroll
   for (int i = 0; i < 2; ++i) {
     const int b = 4 * i + w;
-    vs[i] = (int)mx_scale_row(xrow(32 * b + (lane >> 1)) + (xbase & 31), slabs) + 4 * (lane & 1);
+    vs[i] = (int)mx_scale_row(row[NX + i] + (xbase & 31), slabs) + 4 * (lane & 1);
     vs[2 + i] = (int)mx_scale_row(wrow(32 * (GATED ? b >> 1 : b) + (lane >> 1)), slabs) + 4 * (lane & 1);
   }
   const lt_rsrc_t rsw = GATED && (w & 1) ? rs1 : rs0;
@@ -787,11 +794,9 @@ __global__ __launch_bounds__(256, RING * (WM * 64 * 256 + WN * 64 * 64 + 1024) >
     return min(t.n0 + n, a.N - 1) - t.n0;
   };
   int vx[NX], vw[NW];
+  mx_rows_of_x(a, t, vx, [&](int i) { return 16 * i + xr; });
 #pragma unroll
-  for (int i = 0; i < NX; ++i) {
-    const int m = min(t.m0 + 16 * i + xr, t.m_end - 1);
-    vx[i] = (a.tok ? a.tok[m] : m - t.m0) * (int)a.ldx + 16 * xc;
-  }
+  for (int i = 0; i < NX; ++i) vx[i] = vx[i] * (int)a.ldx + 16 * xc;
 #pragma unroll
   for (int i = 0; i < NW; ++i) vw[i] = wrow(64 * i + wr) * (int)a.ldw + 16 * wc;
   // a gated pair's matrices change every 32 rows of the tile, so with the wave; its scales stand one matrix behind the other, 64 rows a wave
