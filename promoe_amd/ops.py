@@ -808,104 +808,106 @@ def experts_gated_mx4(x, w_gate: Mx4, w_up: Mx4, d: Dispatch, b_gate: torch.Tens
     return _product_mx4("experts_gated_mx4", x, (w_gate, w_up), (b_gate, b_up), act, None, out, out_dtype, d, of_tokens)
 
 
-def _sort(x, d, out=None):
+def _sort(x, d, ldx):
     T, k, H = d.T, d.k, x.shape[1]
-    ldx = _rows("sort_tokens", x, T, H)
-    y = torch.empty(T * k, H, dtype=x.dtype, device=x.device) if out is None else out
-    index = x.get_device()
-    rc = lib.moe_sort_rows(x.data_ptr(), ldx, y.data_ptr(), _rows("sort_tokens", y, T * k, H), d.pos_of_pair.data_ptr(),
-                           d.offsets.data_ptr() + 4 * d.E, T, k, H, L.ROW_DTYPES[x.dtype], _raw_stream(index))
+    y = torch.empty((T * k, H), dtype=x.dtype, device=x.device)
+    rc = lib.moe_sort_rows(x.data_ptr(), ldx, y.data_ptr(), H, d.pos_of_pair.data_ptr(), d.offsets.data_ptr() + 4 * d.E, T, k, H,
+                           L.ROW_DTYPES[x.dtype], _raw_stream(x.get_device()))
     if rc:
         check(rc, "sort_tokens")
     return y
 
 
-def _unsort(x, d, w, out=None):
+def _unsort(x, d, w, ldx):
     T, k, H = d.T, d.k, x.shape[1]
-    ldx = _rows("unsort_tokens", x, T * k, H)
-    y = torch.empty(T, H, dtype=x.dtype, device=x.device) if out is None else out
-    rc = lib.moe_unsort_rows(x.data_ptr(), ldx, y.data_ptr(), _rows("unsort_tokens", y, T, H), d.pos_of_pair.data_ptr(), ptr(w), T, k, H,
-                             L.ROW_DTYPES[x.dtype], _raw_stream(x.get_device()))
+    y = torch.empty((T, H), dtype=x.dtype, device=x.device)
+    rc = lib.moe_unsort_rows(x.data_ptr(), ldx, y.data_ptr(), H, d.pos_of_pair.data_ptr(), ptr(w), T, k, H, L.ROW_DTYPES[x.dtype],
+                             _raw_stream(x.get_device()))
     if rc:
         check(rc, "unsort_tokens")
     return y
 
 
-def _whole_rows(t):
-    """A gradient as autograd hands it over (an expanded one, say) with rows that the kernels can read."""
-    return t if t.dim() == 2 and (t.stride(1) == 1 or t.shape[1] <= 1) and t.stride(0) >= t.shape[1] else t.contiguous()
+def _gradient_rows(what, t):
+    """A gradient as autograd hands it over (an expanded one, say) with rows that the kernels can read, and their distance."""
+    if torch.is_grad_enabled():
+        raise L.MoeError("%s has no second gradient" % what)
+    if not (t.stride(1) == 1 or t.shape[1] <= 1) or t.stride(0) < t.shape[1]:
+        t = t.contiguous()
+    return t, _rows(what, t, *t.shape)
 
 
 class _SortTokens(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, x, d):
+    def forward(ctx, x, d, ldx):
         ctx.d = d
-        return _sort(x, d)
+        return _sort(x, d, ldx)
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
     def backward(ctx, dy):
-        with torch.cuda.device(dy.device):
-            return _unsort(_whole_rows(dy), ctx.d, None), None
+        dy, ld = _gradient_rows("sort_tokens", dy)
+        return _unsort(dy, ctx.d, None, ld), None, None
 
 
 class _UnsortTokens(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, x, w, d):
-        ctx.d = d
-        ctx.save_for_backward(x, w)
-        return _unsort(x, d, w)
+    def forward(ctx, x, w, d, ldx):
+        ctx.d, ctx.ldx = d, ldx
+        if w is not None:
+            ctx.save_for_backward(x, w)
+        return _unsort(x, d, w, ldx)
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
     def backward(ctx, dy):
-        d, (x, w), dy = ctx.d, ctx.saved_tensors, _whole_rows(dy)
-        need_x, need_w = ctx.needs_input_grad[0], w is not None and ctx.needs_input_grad[1]
-        with torch.cuda.device(dy.device):
-            if w is None:
-                return _sort(dy, d), None, None
-            T, k, H = d.T, d.k, x.shape[1]
-            dx = torch.empty(x.shape, dtype=x.dtype, device=x.device) if need_x else None
-            dw = torch.empty(T, k, dtype=torch.float32, device=x.device) if need_w else None
-            check(lib.moe_unsort_rows_grad(dy.data_ptr(), _rows("unsort_tokens", dy, T, H), x.data_ptr(), _rows("unsort_tokens", x, T * k, H),
-                                           d.pos_of_pair.data_ptr(), w.data_ptr(), d.offsets.data_ptr() + 4 * d.E, ptr(dx), H, ptr(dw),
-                                           T, k, H, L.ROW_DTYPES[x.dtype], _raw_stream(x.get_device())), "unsort_tokens")
-        return dx, dw, None
+        d = ctx.d
+        dy, ld = _gradient_rows("unsort_tokens", dy)
+        if not ctx.saved_tensors:
+            return _sort(dy, d, ld), None, None, None
+        x, w = ctx.saved_tensors
+        need_x, need_w = ctx.needs_input_grad[:2]
+        T, k, H = d.T, d.k, x.shape[1]
+        dx = torch.empty((T * k, H), dtype=x.dtype, device=x.device) if need_x else None
+        dw = torch.empty((T, k), dtype=torch.float32, device=x.device) if need_w else None
+        check(lib.moe_unsort_rows_grad(dy.data_ptr(), ld, x.data_ptr(), ctx.ldx, d.pos_of_pair.data_ptr(), w.data_ptr(),
+                                       d.offsets.data_ptr() + 4 * d.E, ptr(dx), H, ptr(dw), T, k, H, L.ROW_DTYPES[x.dtype],
+                                       _raw_stream(x.get_device())), "unsort_tokens")
+        return dx, dw, None, None
 
 
 def _move_args(what, x, d, rows, w):
+    """(GPU, elements between the rows of x)"""
     if x.dim() != 2 or x.dtype not in L.ROW_DTYPES or x.shape[0] != rows:
         raise L.MoeError("%s: bf16, fp16 or fp32 [%d, H] is needed, not %s %s" % (what, rows, x.dtype, tuple(x.shape)))
     if w is not None and (w.dtype != torch.float32 or w.shape != (d.T, d.k) or not w.is_contiguous()):
         raise L.MoeError("%s: weights must be fp32 [%d, %d], contiguous" % (what, d.T, d.k))
     index = x.get_device()
-    if index < 0 or any(t is not None and t.get_device() != index for t in (w, d.pos_of_pair, d.offsets)):
+    if index < 0 or (w is not None and w.get_device() != index) or d.pos_of_pair.get_device() != index or d.offsets.get_device() != index:
         raise L.MoeError("%s: x, weights and dispatch must be on one GPU" % what)
-    _rows(what, x, rows, x.shape[1])
-    return index
+    return index, _rows(what, x, rows, x.shape[1])
 
 
 def sort_tokens(x: torch.Tensor, d: Dispatch) -> torch.Tensor:
     """The tokens' rows x [T, H] in the order of their experts: [T*k, H], a token's row once for each of its choices (moe_sort_rows).
     Choices of no expert (idx outside 0 .. E - 1) have no row; the rows behind the last one are zero.  Any alignment and row stride, bf16,
-    fp16 or fp32.  With a gradient (each token the sum of its rows', in fp32): d has to keep its contents until the backward pass."""
-    index = _move_args("sort_tokens", x, d, d.T, None)
+    fp16 or fp32.  With a gradient, not a second one (each token the sum of its rows', in fp32): d has to keep its contents until the
+    backward pass."""
+    index, ldx = _move_args("sort_tokens", x, d, d.T, None)
     if index != torch.cuda.current_device():
         with torch.cuda.device(index):
             return sort_tokens(x, d)
-    if torch.is_grad_enabled() and x.requires_grad:
-        return _SortTokens.apply(x, d)
-    return _sort(x, d)
+    if x.requires_grad and torch.is_grad_enabled():
+        return _SortTokens.apply(x, d, ldx)
+    return _sort(x, d, ldx)
 
 
 def unsort_tokens(x: torch.Tensor, d: Dispatch, w: torch.Tensor | None = None) -> torch.Tensor:
     """The experts' rows x [T*k, H] back to their tokens: y[t] = sum over the choices of w[t, j] x[row of (t, j)] (moe_unsort_rows; w fp32
     [T, k], or 1), in fp32 and in the order of the choices, rounded once to x's type.  Choices of no expert add nothing, whatever lies
-    behind the last row.  With gradients of x and w: d has to keep its contents until the backward pass."""
-    index = _move_args("unsort_tokens", x, d, d.T * d.k, w)
+    behind the last row.  With gradients of x and w, not second ones: d has to keep its contents until the backward pass."""
+    index, ldx = _move_args("unsort_tokens", x, d, d.T * d.k, w)
     if index != torch.cuda.current_device():
         with torch.cuda.device(index):
             return unsort_tokens(x, d, w)
-    if torch.is_grad_enabled() and (x.requires_grad or (w is not None and w.requires_grad)):
-        return _UnsortTokens.apply(x, w, d)
-    return _unsort(x, d, w)
+    if (x.requires_grad or (w is not None and w.requires_grad)) and torch.is_grad_enabled():
+        return _UnsortTokens.apply(x, w, d, ldx)
+    return _unsort(x, d, w, ldx)

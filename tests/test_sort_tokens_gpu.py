@@ -120,6 +120,11 @@ def test_a_strange_gradient_streams_graphs_and_refusals(cuda):
     a = torch.autograd.grad(ops.unsort_tokens(rl, d, wl), [rl, wl], turned)
     b = torch.autograd.grad(ops.unsort_tokens(rl, d, wl), [rl, wl], turned.contiguous())
     assert all(torch.equal(p, q) for p, q in zip(a, b))
+    # no second gradient
+    with pytest.raises(L.MoeError, match="second"):
+        torch.autograd.grad(ops.sort_tokens(xl, d), [xl], torch.ones_like(r), create_graph=True)
+    with pytest.raises(L.MoeError, match="second"):
+        torch.autograd.grad(ops.unsort_tokens(rl, d, wl), [rl], torch.ones_like(x), create_graph=True)
     # the same bits every time, on another stream and from a graph
     want = ops.unsort_tokens(ops.sort_tokens(x, d), d, w)
     st = torch.cuda.Stream()
