@@ -291,66 +291,75 @@ __global__ __launch_bounds__(64 * WAVES) void k_mx4_rows(const MxArgs a) {
 
 // ---- tiles ----------------------------------------------------------------------------------------------------------------------
 // Where a workgroup works.  Dense: tile (mt, nt) of rows and columns and a piece of K.  By expert: the tiles of an expert's rows by nt; the
-// counts of all experts are added up by every wave, the host does not know them.
-struct MxTile { int m0, m_end, n0, e, split; };  // rows m0 .. m_end - 1 of y at most
+// counts of all experts are added up by every wave, the host does not know them.  Workgroup i runs on XCD i % 8: each XCD takes a
+// contiguous run of tiles, four rows of tiles wide.
+struct MxTile { int m0, m_end, n0, e, split, kt0, nk; };  // rows m0 .. m_end - 1 of y at most; slabs kt0 .. nk - 1
 template <int BM, int NC>
-static __device__ __forceinline__ bool mx_tile_of(const MxArgs &a, int v, MxTile &t) {
-  const int lane = threadIdx.x & 63;
-  int nm = a.nm, r, first = 0, rows = a.M, e = 0;
-  if (!a.units) {
-    const int tiles = nm * a.nn;
-    if (v >= tiles * a.splits) return false;
-    t.split = v / tiles;
-    r = v - t.split * tiles;
-  } else {
-    // lane l has the experts per l .. per l + per - 1
-    const int per = (a.E + 63) >> 6;
-    int mine = 0;
-    for (int i = 0; i < per; ++i) {
-      const int x = per * lane + i;
-      mine += x < a.E ? (a.counts[x] + BM - 1) / BM : 0;
-    }
-    int upto = mine;
+struct MxTiles {
+  // by expert: lane l has experts per l .. per l + per - 1, their tiles, those up to them, the first row and how many there are
+  int total, per, mine, upto, first, have;
+  __device__ __forceinline__ MxTiles(const MxArgs &a) : per(0), mine(0), upto(0), first(0), have(0) {
+    total = a.nm * a.nn * a.splits;
+    if (a.units) {
+      const int lane = threadIdx.x & 63;
+      per = (a.E + 63) >> 6;
+      for (int i = 0; i < per; ++i) {
+        const int x = per * lane + i;
+        const int c = x < a.E ? a.counts[x] : 0;
+        mine += (c + BM - 1) / BM;
+        have += c;
+      }
+      first = a.offsets[min(per * lane, a.E)];
+      upto = mine;
 #pragma unroll
-    for (int d = 1; d < 64; d <<= 1) {
-      const int o = __shfl_up(upto, d, 64);
-      if (lane >= d) upto += o;
+      for (int d = 1; d < 64; d <<= 1) {
+        const int o = __shfl_up(upto, d, 64);
+        if (lane >= d) upto += o;
+      }
+      total = __builtin_amdgcn_readlane(upto, 63) * a.nn;
     }
-    const int mt_all = __builtin_amdgcn_readlane(upto, 63);
-    if (v >= mt_all * a.nn) return false;
-    // (tiles come expert by expert: v / nn is one of its tiles' rows, whichever)
-    const int at = v / a.nn;
-    const unsigned long long over = __ballot(upto > at);
-    const int l = (int)__builtin_ctzll(over);
-    int before = __builtin_amdgcn_readlane(upto - mine, l);
-    e = per * l;
-    int count = 0;
-    for (;; ++e) {
-      count = a.counts[e];
-      nm = (count + BM - 1) / BM;
-      if (before + nm > at || e == a.E - 1) break;
-      before += nm;
-    }
-    r = v - before * a.nn;
-    first = a.offsets[e];
-    rows = count;
-    t.split = 0;
   }
-  // four rows of tiles wide
-  const int group = r / (4 * a.nn), in = r - group * 4 * a.nn, wide = min(4, nm - 4 * group);
-  const int nt = in / wide, mt = 4 * group + in - nt * wide;
-  t.m0 = __builtin_amdgcn_readfirstlane(first + mt * BM);
-  t.m_end = __builtin_amdgcn_readfirstlane(first + rows);
-  t.n0 = __builtin_amdgcn_readfirstlane(nt * NC);
-  t.e = __builtin_amdgcn_readfirstlane(e);
-  t.split = __builtin_amdgcn_readfirstlane(t.split);
-  return true;
-}
-// workgroup i runs on XCD i % 8: each XCD takes a contiguous run of tiles
-static __device__ __forceinline__ int mx_run_of() {
-  const int per = (int)gridDim.x >> 3;
-  return ((int)blockIdx.x & 7) * per + ((int)blockIdx.x >> 3);
-}
+  // the run of this workgroup's XCD: its first tile, the end, and the workgroups that share it
+  __device__ __forceinline__ int begin() const { return ((int)blockIdx.x & 7) * ((total + 7) >> 3) + ((int)blockIdx.x >> 3); }
+  __device__ __forceinline__ int end() const { return min(total, (((int)blockIdx.x & 7) + 1) * ((total + 7) >> 3)); }
+  __device__ __forceinline__ MxTile at(const MxArgs &a, int v) const {
+    MxTile t{};
+    int nm = a.nm, r, e = 0, row0 = 0, rows = a.M;
+    if (!a.units) {
+      const int tiles = nm * a.nn;
+      t.split = v / tiles;
+      r = v - t.split * tiles;
+    } else {
+      const int row = v / a.nn;  // (tiles come expert by expert: one of its rows of tiles, whichever)
+      const int l = (int)__builtin_ctzll(__ballot(upto > row) | 1ull << 63);
+      int before = __builtin_amdgcn_readlane(upto - mine, l);
+      e = per * l;
+      row0 = __builtin_amdgcn_readlane(first, l);
+      rows = __builtin_amdgcn_readlane(have, l);
+      nm = (rows + BM - 1) / BM;
+      if (per > 1)                 // (a lane's experts one after the other)
+        for (;; ++e) {
+          rows = a.counts[e];
+          nm = (rows + BM - 1) / BM;
+          if (before + nm > row || e + 1 >= min(a.E, per * (l + 1))) break;
+          before += nm;
+          row0 += rows;
+        }
+      r = v - before * a.nn;
+    }
+    const int group = r / (4 * a.nn), in = r - group * 4 * a.nn, wide = min(4, nm - 4 * group);
+    const int nt = in / wide, mt = 4 * group + in - nt * wide;
+    // (scalars, whatever the divisions are made of)
+    t.m0 = __builtin_amdgcn_readfirstlane(row0 + mt * BM);
+    t.m_end = __builtin_amdgcn_readfirstlane(row0 + rows);
+    t.n0 = __builtin_amdgcn_readfirstlane(nt * NC);
+    t.e = __builtin_amdgcn_readfirstlane(e);
+    t.split = __builtin_amdgcn_readfirstlane(t.split);
+    t.kt0 = t.split * a.slabs + min(t.split, a.extra);
+    t.nk = t.kt0 + a.slabs + (t.split < a.extra);
+    return t;
+  }
+};
 // Rows of x that a lane's transfers read, behind xbase: all lookups of a gathered x on their way at once
 template <int N, class F>
 static __device__ __forceinline__ void mx_rows_of_x(const MxArgs &a, const MxTile &t, int (&row)[N], const F &of) {
@@ -517,8 +526,10 @@ __global__ __launch_bounds__(256, RING * (WM + WN) * 64 * 136 > 80 * 1024 ? 1 : 
   __shared__ __align__(1024) unsigned char s_ring[RING * SLAB];
   const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6), wm = w & 1, wn = w >> 1;
   const int fr = lane & 31, q = lane >> 5;
-  MxTile t;
-  if (!mx_tile_of<BM, NC>(a, mx_run_of(), t)) return;
+  const MxTiles<BM, NC> tiles(a);
+  const int v = tiles.begin();
+  if (v >= tiles.end()) return;
+  const MxTile t = tiles.at(a, v);
   const unsigned lds = (unsigned)(uintptr_t)(__attribute__((address_space(3))) unsigned char *)s_ring;
   const uint8_t *w0 = a.w[0] + t.e * a.ew + t.n0 * a.ldw, *w1 = a.w[GATED ? 1 : 0] + t.e * a.ew + t.n0 * a.ldw;
   const int slabs = mx_slabs(a.K);
@@ -546,8 +557,7 @@ __global__ __launch_bounds__(256, RING * (WM + WN) * 64 * 136 > 80 * 1024 ? 1 : 
       rsc[i] = GATED && (bw & 1) ? rs1 : rs0;
     }
   }
-  const int kt0 = t.split * a.slabs + min(t.split, a.extra), nk = kt0 + a.slabs + (t.split < a.extra);
-  const int blocks = min(a.K >> 5, nk * (M4_K / 32));        // (past the last block: zeros)
+  const int kt0 = t.kt0, nk = t.nk, blocks = min(a.K >> 5, nk * (M4_K / 32));  // (past the last block: zeros)
   auto dma = [&](int i, int kt, int place) {
     if (i < NX + NW) {
       const bool in = kt * 8 + chunk < blocks;
@@ -645,10 +655,12 @@ __global__ __launch_bounds__(256, 1) void k_mx4_wide(const MxArgs a) {
   __shared__ __align__(1024) unsigned char s_ring[2 * SLAB];
   const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6), wm = w & 1, wn = w >> 1;
   const int fr = lane & 31, q = lane >> 5;
-  MxTile t;
-  if (!mx_tile_of<B, NC>(a, mx_run_of(), t)) return;
+  const MxTiles<B, NC> tiles(a);
+  const int v = tiles.begin();
+  if (v >= tiles.end()) return;
+  const MxTile t = tiles.at(a, v);
   const unsigned lds = (unsigned)(uintptr_t)(__attribute__((address_space(3))) unsigned char *)s_ring;
-  const int slabs = mx_slabs(a.K), blocks_k = a.K >> 5;
+  const int slabs = mx_slabs(a.K);
   const long long xbase = a.tok ? 0 : t.m0;
   const lt_rsrc_t rx = lt_rsrc((const uint8_t *)a.x + xbase * a.ldx), rxs = lt_rsrc(a.xs + mx_scale_row(xbase & ~31ll, slabs));
   const lt_rsrc_t rw0 = lt_rsrc(a.w[0] + t.e * a.ew + t.n0 * a.ldw), rw1 = lt_rsrc(a.w[GATED ? 1 : 0] + t.e * a.ew + t.n0 * a.ldw);
@@ -669,8 +681,7 @@ __global__ __launch_bounds__(256, 1) void k_mx4_wide(const MxArgs a) {
     vs[2 + i] = (int)mx_scale_row(wrow(32 * (GATED ? b >> 1 : b) + (lane >> 1)), slabs) + 4 * (lane & 1);
   }
   const lt_rsrc_t rsw = GATED && (w & 1) ? rs1 : rs0;
-  const int kt0 = t.split * a.slabs + min(t.split, a.extra), nk = kt0 + a.slabs + (t.split < a.extra);
-  const int blocks = min(blocks_k, nk * (M4_K / 32));
+  const int kt0 = t.kt0, nk = t.nk, blocks = min(a.K >> 5, nk * (M4_K / 32));
   auto dma = [&](int i, int kt, int place) {
     if (i < NX + NW) {
       const bool in = kt * 8 + chunk < blocks;
@@ -778,8 +789,10 @@ __global__ __launch_bounds__(256, RING * (WM * 64 * 256 + WN * 64 * 64 + 1024) >
   __shared__ __align__(1024) unsigned char s_ring[RING * SLAB];
   const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6), wm = w & 1, wn = w >> 1;
   const int fr = lane & 31, q = lane >> 5;
-  MxTile t;
-  if (!mx_tile_of<BM, NC>(a, mx_run_of(), t)) return;
+  const MxTiles<BM, NC> tiles(a);
+  const int v = tiles.begin();
+  if (v >= tiles.end()) return;
+  const MxTile t = tiles.at(a, v);
   const unsigned lds = (unsigned)(uintptr_t)(__attribute__((address_space(3))) unsigned char *)s_ring;
   const long long xbase = a.tok ? 0 : t.m0;
   const lt_rsrc_t rx = lt_rsrc((const uint8_t *)a.x + xbase * a.ldx);
@@ -802,8 +815,7 @@ __global__ __launch_bounds__(256, RING * (WM * 64 * 256 + WN * 64 * 64 + 1024) >
   // a gated pair's matrices change every 32 rows of the tile, so with the wave; its scales stand one matrix behind the other, 64 rows a wave
   const lt_rsrc_t rw = GATED && (w & 2) ? rw1 : rw0, rs = GATED && w >= WN / 2 ? rs1 : rs0;
   const int vs = w < WN ? (int)mx_scale_row(min(t.n0 + 64 * (GATED ? w % ((WN + 1) / 2) : w) + lane, a.N - 1) - t.n0, slabs) : LT_OUT;
-  const int kt0 = t.split * a.slabs + min(t.split, a.extra), nk = kt0 + a.slabs + (t.split < a.extra);
-  const int blocks = min(a.K >> 5, nk * (M16_K / 32));  // (past the last block: zeros)
+  const int kt0 = t.kt0, nk = t.nk, blocks = min(a.K >> 5, nk * (M16_K / 32));  // (past the last block: zeros)
   auto dma = [&](int i, int kt, int place) {
     if (i < NX) {
       const bool in = kt * 4 + (xc >> 2) < blocks;
