@@ -535,10 +535,11 @@ int moe_mx4_dequantize(const moe_mx4 *q_host, int E, int M, int K, void *y, int6
 /* moe_linear and moe_linear_gated (w_up not NULL) with matrices in that form (descriptions on the host); x either 16-bit rows (ldx
  * elements apart; the products are those of the values as they are) or rows in the same form (xq, x NULL).  bias, residual and y (unless
  * y_fp32) have the type dtype, and so has a 16-bit x.  K % 32 == 0; rows less than 4 MiB apart; sums in fp32, one rounding.  The other rules
- * as for moe_linear.
+ * as for moe_linear; ws: moe_mx4_linear_workspace_bytes of device memory (x_mx4: whether xq is given).
  * moe_mx4_experts: the same for every expert e of a dispatch: rows offsets[e] .. + counts[e] of y are the product of those rows of x, or,
  * with sorted_tok, of the rows sorted_tok[..] of x (T of them, one for each token; else P), with matrix e; bias [E, N].  Rows behind the last pair are left as
  * they were.  E <= 1024, max_units >= min(E, P). */
+int64_t moe_mx4_linear_workspace_bytes(int M, int N, int K, int x_mx4, int gated);
 int moe_mx4_linear(const void *x, int64_t ldx, const moe_mx4 *xq_host, const moe_mx4 *w_host, const moe_mx4 *w_up_host, const void *bias,
                    const void *bias_up, const void *residual, int64_t ldr, void *y, int64_t ldy, int M, int N, int K, int dtype, int act,
                    int y_fp32, void *ws, int64_t ws_bytes, void *stream);

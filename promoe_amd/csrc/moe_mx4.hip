@@ -6,6 +6,7 @@
 // registers, exactly; an fp16 value is the sum of two bf16 (11 bits of mantissa), so that nothing of it is lost either.
 #include <hip/hip_runtime.h>
 #include <stdint.h>
+#include <algorithm>
 
 #include "moe_common.h"
 #include "moe_kernels.h"
@@ -398,36 +399,45 @@ static __device__ __forceinline__ void mx_tile_out(const MxArgs &a, const f32x16
   const int col = 8 * (lane % LPR), n = n0 + wn * (NC / 2) + col;
   const int at = GATED ? (col >> 5) * 64 + (col & 31) : col;
   const LinColumns<F16, GATED> c(a, n);
-  const bool inside = !a.y32 && !a.part && n0 + NC <= a.N;
   constexpr int NP = 32 / RPP;
-  // eight columns of row r of the block: gated the second eight of the second matrix
-  auto fetch = [&](int r, float (&s0)[8], float (&s1)[8]) {
+  // eight columns of row r of the block, from column k of the wave's sums on: gated the second eight of the second matrix
+  auto fetch = [&](int r, int k, float (&s0)[8], float (&s1)[8]) {
 #pragma unroll
-    for (int k = 0; k < (GATED ? 4 : 2); ++k) {
-      const f32x4_t f = *(const f32x4_t *)(buf + r * LDE + at + (k & 1) * 4 + (k >> 1) * 32);
+    for (int h = 0; h < (GATED ? 4 : 2); ++h) {
+      const f32x4_t f = *(const f32x4_t *)(buf + r * LDE + k + (h & 1) * 4 + (h >> 1) * 32);
 #pragma unroll
-      for (int e = 0; e < 4; ++e) (k >> 1 ? s1 : s0)[4 * (k & 1) + e] = f[e];
+      for (int e = 0; e < 4; ++e) (h >> 1 ? s1 : s0)[4 * (h & 1) + e] = f[e];
     }
   };
-  // whole columns in 16 bits: every load of a residual in front of the sums' way through LDS, the activation chosen once
+  // all rows of a block: every load of a residual in front of the sums' way through LDS, the activation chosen once
   auto plain = [&](int first, const u32x4_t (&res)[NP], auto act_) {
 #pragma unroll
     for (int p = 0; p < NP; ++p) {
       float s0[8], s1[8];
-      fetch(lane / LPR + p * RPP, s0, s1);
+      fetch(lane / LPR + p * RPP, at, s0, s1);
       c.template finish<decltype(act_)::value>(s0, s1);
       if (!GATED && a.res) lin_add<F16>(s0, res[p]);
       const int m = first + p * RPP;
-      if (m < a.M) *(u32x4_any *)((uint16_t *)a.y + m * a.ldy + n) = lin_pack<F16>(s0);
+      if (m < a.M && c.count == 8) {
+        if (a.y32) {
+          float *y = (float *)a.y + m * a.ldy + n;
+          *(f32x4_any *)y = f32x4_t{s0[0], s0[1], s0[2], s0[3]};
+          *(f32x4_any *)(y + 4) = f32x4_t{s0[4], s0[5], s0[6], s0[7]};
+        } else {
+          *(u32x4_any *)((uint16_t *)a.y + m * a.ldy + n) = lin_pack<F16>(s0);
+        }
+      }
     }
   };
+  // fewer than eight columns at the end of a row: a row a lane
+  const int tail = (a.N & 7) ? (a.N & ~7) - (n0 + wn * (NC / 2)) : -1;  // where they begin among the wave's
   // (one copy of the loop for all blocks: code that runs once a tile waits for its instructions, line by line)
 #pragma clang loop unroll(disable)
   for (int i = 0; i < WM; ++i) {
     if (m0 + 32 * (2 * i + wm) >= a.M) break;
     const int first = m0 + 32 * (2 * i + wm) + lane / LPR;
     u32x4_t res[NP];
-    if (!GATED && inside && a.res)
+    if (!GATED && a.res && !a.part && c.count == 8)
 #pragma unroll
       for (int p = 0; p < NP; ++p) res[p] = *(const u32x4_any *)(a.res + (long long)min(first + p * RPP, a.M - 1) * a.ldr + n);
     lt_each<WM>([&](auto i_) {
@@ -443,28 +453,26 @@ static __device__ __forceinline__ void mx_tile_out(const MxArgs &a, const f32x16
       }
     });
     __builtin_amdgcn_wave_barrier();
-    switch (inside ? a.act : -1) {
+    switch (a.part ? -1 : a.act) {
       case MOE_ACT_NONE: plain(first, res, std::integral_constant<int, MOE_ACT_NONE>()); break;
       case MOE_ACT_SILU: plain(first, res, std::integral_constant<int, MOE_ACT_SILU>()); break;
       case MOE_ACT_GELU: plain(first, res, std::integral_constant<int, MOE_ACT_GELU>()); break;
       case MOE_ACT_GELU_TANH: plain(first, res, std::integral_constant<int, MOE_ACT_GELU_TANH>()); break;
       case MOE_ACT_RELU: plain(first, res, std::integral_constant<int, MOE_ACT_RELU>()); break;
       case MOE_ACT_RELU2: plain(first, res, std::integral_constant<int, MOE_ACT_RELU2>()); break;
-      default: {
-        u32x4_t r0 = c.residual(a, first);
-#pragma clang loop unroll(disable)
+      default:
+#pragma unroll
         for (int p = 0; p < NP; ++p) {
-          const int m = first + p * RPP;
-          const u32x4_t ahead = c.residual(a, p + 1 < NP ? m + RPP : a.M);
           float s0[8], s1[8];
-          fetch(lane / LPR + p * RPP, s0, s1);
-          if (m < a.M) {
-            if (a.part) c.partial(a, split, m, s0, s1);
-            else c.store(a, m, s0, s1, r0);
-          }
-          r0 = ahead;
+          fetch(lane / LPR + p * RPP, at, s0, s1);
+          if (first + p * RPP < a.M) c.partial(a, split, first + p * RPP, s0, s1);
         }
-      }
+    }
+    if (!a.part && tail >= 0 && tail < NC / 2 && lane < 32) {
+      const int m = first - lane / LPR + lane;
+      float s0[8], s1[8];
+      fetch(lane, GATED ? (tail >> 5) * 64 + (tail & 31) : tail, s0, s1);
+      if (m < a.M) LinColumns<F16, GATED>(a, a.N & ~7).store(a, m, s0, s1, u32x4_t{0, 0, 0, 0});
     }
     __builtin_amdgcn_wave_barrier();
   }
@@ -1018,17 +1026,58 @@ static int mx_check(const char *who, const MxArgs &a, int xkind, int64_t xrows, 
   }
   return MOE_OK;
 }
-struct MxPlan { int wm, wn, ring, splits; };    // wm 0: few rows
-static MxPlan mx_plan(int xkind, long long rows, int tiles_of, int N, int K, bool gated) {
-  const long long each = rows / tiles_of;
-  if (each <= 16) return MxPlan{0, 0, 0, 1};
-  if (each <= 64) return MxPlan{1, 2, 4, 1};
-  if (rows >= 4096 && each >= 256) return xkind == X_MX4 ? MxPlan{4, 4, 2, 1} : MxPlan{2, 4, 3, 1};
-  return xkind == X_MX4 ? MxPlan{2, 2, 4, 1} : MxPlan{2, 2, 3, 1};
+// Which kernel a product takes: few rows (wm 0), or tiles of 64 wm x 64 wn with `ring` slabs in LDS (4 x 4: the wide kernel), dense ones
+// with K in `splits` pieces.  The plan of the least time after a model of one launch, us, fitted to 11000 measured times of 140 shapes (17 to 4096
+// rows; the chosen plan is 2 % slower than the best of all on average, 31 % at worst):
+//   start + rounds x (slabs x (c0 + c1 x share of the compute units in use) + f),  with pieces j0 + j1 a piece + j2 per MB of partial sums
+// c0, c1: a slab of a workgroup on an idle chip, and what the others' traffic adds; f: first slab and epilogue.
+struct MxPlan { int wm, wn, ring, splits; float us; };
+struct MxTileKind { int wm, wn, ring, per_cu; float c0, c1, f; };
+struct MxModel { MxTileKind tile[7]; int tiles; float start, j0, j1, j2; };
+static const MxModel MX_MODEL4 = {{{1, 1, 4, 2, .163f, .111f, 2.46f}, {1, 2, 2, 2, .484f, .114f, 1.94f}, {1, 2, 4, 1, .284f, .133f, 2.59f},
+                                   {2, 2, 2, 2, .534f, .307f, 2.32f}, {2, 2, 3, 1, .374f, .259f, 2.97f}, {2, 4, 3, 1, .680f, .397f, 3.98f},
+                                   {4, 4, 2, 1, 1.072f, .633f, 3.98f}}, 7, 3.43f, 3.50f, .161f, .166f};
+static const MxModel MX_MODEL16 = {{{1, 1, 3, 2, .264f, .118f, 2.32f}, {1, 2, 3, 2, .401f, .227f, 2.63f}, {1, 4, 2, 2, .742f, .386f, 2.49f},
+                                    {2, 2, 3, 1, .633f, .222f, 3.08f}, {2, 4, 3, 1, 1.146f, .333f, 4.13f}}, 5, 3.62f, 2.90f, .217f, .174f};
+// rows of all `units` products together; units 0: a dense one
+static MxPlan mx_plan(int xkind, long long rows, int units, int N, int K, bool gated) {
+  const long long each = units ? rows / units : rows;
+  if (each <= 16) return MxPlan{0, 0, 0, 1, 0.f};
+  static const int pieces[] = {1, 2, 3, 4, 6, 8, 12};
+  const MxModel &model = xkind == X_MX4 ? MX_MODEL4 : MX_MODEL16;
+  const int slab = xkind == X_MX4 ? M4_K : M16_K;
+  const long long slabs = (K + slab - 1) / slab;
+  MxPlan best{2, 2, 3, 1, 1e30f};
+  for (int i = 0; i < model.tiles; ++i) {
+    const MxTileKind &t = model.tile[i];
+    if (gated && t.wn == 1) continue;  // (a pair needs both matrices' blocks in a wave)
+    const int bm = 64 * t.wm, cols = 64 * t.wn / (gated ? 2 : 1);
+    // by expert the last tile of each is half full on average (the counts are not known here), and the wide kernel leaves its empty blocks out
+    const float full = (float)each / (float)bm;
+    const float down = !units ? (float)((rows + bm - 1) / bm) : (float)units * (full >= 1.f ? full + .5f : 1.f + std::max(0.f, full - .7f) * 1.67f);
+    const float fill = units && t.wm == 4 ? .3f + .7f * (float)rows / (down * (float)bm) : 1.f;
+    const long long n = (long long)(down * (float)((N + cols - 1) / cols));
+    for (int s : pieces) {
+      if (s > slabs || (s > 1 && (units || n * s > 640))) break;
+      const long long wgs = n * s, at_once = 256 * t.per_cu;
+      const float use = wgs > 256 ? (float)t.per_cu : (float)wgs / 256.f;
+      // (by expert rounds end at different times)
+      const float rounds = units && wgs > at_once ? (float)wgs / (float)at_once + .25f : (float)((wgs + at_once - 1) / at_once);
+      float us = model.start + rounds * ((float)((slabs + s - 1) / s) * (t.c0 + t.c1 * use) * fill + t.f);
+      if (s > 1) us += model.j0 + model.j1 * (float)s + model.j2 * 8e-6f * (float)s * (gated ? 2.f : 1.f) * (float)rows * (float)N;
+      if (us < best.us) best = MxPlan{t.wm, t.wn, t.ring, s, us};
+    }
+  }
+  return best;
+}
+extern "C" int64_t moe_mx4_linear_workspace_bytes(int M, int N, int K, int x_mx4, int gated) {
+  if (M <= 0 || N <= 0 || K <= 0) return 0;
+  const MxPlan p = mx_plan(x_mx4 ? X_MX4 : X_BF16, M, 0, N, K, gated != 0);
+  return p.splits > 1 ? (int64_t)p.splits * (gated ? 2 : 1) * M * ((N + 7) & ~7) * 4 : 0;
 }
 template <int X, bool F16, bool GATED>
-static int mx_launch(const MxArgs &a, int units, int most, hipStream_t s) {  // most: rows that one expert (or the product) can have
-  const MxPlan pl = mx_plan(X, a.M, a.units ? units : 1, a.N, a.K, GATED);
+static int mx_launch(const MxArgs &a, int units, int most, float *ws, hipStream_t s) {  // most: rows that one expert (or the product) can have
+  const MxPlan pl = mx_plan(X, a.M, a.units ? units : 0, a.N, a.K, GATED);
   if (pl.wm == 0) {
 #define MR_LAUNCH(SH_, NB_, W_)                                                                                                      \
   hipLaunchKernelGGL(HIP_KERNEL_NAME(k_mx4_rows<X, F16, GATED, SH_, NB_, 1, W_>), dim3((a.N + 16 / SH_ * NB_ - 1) / (16 / SH_ * NB_), units), \
@@ -1055,32 +1104,47 @@ static int mx_launch(const MxArgs &a, int units, int most, hipStream_t s) {  // 
     return MOE_EINVAL;
   }
   t.splits = pl.splits;
+  t.ldp = (a.N + 7) & ~7;
+  t.part = pl.splits > 1 ? ws : nullptr;
   constexpr int SLAB_K = X == X_MX4 ? M4_K : M16_K;
   const int slabs = (a.K + SLAB_K - 1) / SLAB_K;
   t.slabs = slabs / pl.splits;
   t.extra = slabs % pl.splits;
   const dim3 grid((unsigned)((tiles + 7) / 8 * 8));
-#define MT_LAUNCH(WM_, WN_, RING4, RING16)                                                                                      \
-  if constexpr (X == X_MX4) hipLaunchKernelGGL(HIP_KERNEL_NAME(k_mx4_tile<F16, GATED, WM_, WN_, RING4>), grid, dim3(256), 0, s, t); \
-  else hipLaunchKernelGGL(HIP_KERNEL_NAME(k_mx4_tile16<X, GATED, WM_, WN_, RING16>), grid, dim3(256), 0, s, t)
-  if (pl.wm == 1) { MT_LAUNCH(1, 2, 4, 5); }
-  else if (pl.wn == 2) { MT_LAUNCH(2, 2, 4, 3); }
-  else if (pl.wm == 2) { MT_LAUNCH(2, 4, 3, 3); }
-  else if constexpr (X == X_MX4) hipLaunchKernelGGL(HIP_KERNEL_NAME(k_mx4_wide<F16, GATED>), grid, dim3(256), 0, s, t);
+#define MT_LAUNCH(WM_, WN_, RING_)                                                                                                 \
+  if constexpr (X == X_MX4) hipLaunchKernelGGL(HIP_KERNEL_NAME(k_mx4_tile<F16, GATED, WM_, WN_, RING_>), grid, dim3(256), 0, s, t); \
+  else hipLaunchKernelGGL(HIP_KERNEL_NAME(k_mx4_tile16<X, GATED, WM_, WN_, RING_>), grid, dim3(256), 0, s, t)
+  switch (pl.wm * 100 + pl.wn * 10 + pl.ring) {
+    case 114: if constexpr (X == X_MX4 && !GATED) { MT_LAUNCH(1, 1, 4); } break;
+    case 113: if constexpr (X != X_MX4 && !GATED) { MT_LAUNCH(1, 1, 3); } break;
+    case 124: if constexpr (X == X_MX4) { MT_LAUNCH(1, 2, 4); } break;
+    case 123: if constexpr (X != X_MX4) { MT_LAUNCH(1, 2, 3); } break;
+    case 122: if constexpr (X == X_MX4) { MT_LAUNCH(1, 2, 2); } break;
+    case 142: if constexpr (X != X_MX4) { MT_LAUNCH(1, 4, 2); } break;
+    case 223: MT_LAUNCH(2, 2, 3); break;
+    case 222: if constexpr (X == X_MX4) { MT_LAUNCH(2, 2, 2); } break;
+    case 243: MT_LAUNCH(2, 4, 3); break;
+    case 442: if constexpr (X == X_MX4) hipLaunchKernelGGL(HIP_KERNEL_NAME(k_mx4_wide<F16, GATED>), grid, dim3(256), 0, s, t); break;
+    default: moe_set_error("moe_mx4: no tile %d x %d", pl.wm, pl.wn); return MOE_EINVAL;
+  }
 #undef MT_LAUNCH
-  return moe_check_launch("k_mx4_tile");
+  if (int rc = moe_check_launch("k_mx4_tile")) return rc;
+  if (!t.part) return MOE_OK;
+  const long long pieces = (long long)a.M * (t.ldp >> 3);
+  hipLaunchKernelGGL(HIP_KERNEL_NAME(k_mx4_join<F16, GATED>), dim3((unsigned)((pieces + 255) / 256)), dim3(256), 0, s, t);
+  return moe_check_launch("k_mx4_join");
 }
-static int mx_run(const MxArgs &a, int xkind, int dtype, bool gated, int units, int most, hipStream_t s) {
+static int mx_run(const MxArgs &a, int xkind, int dtype, bool gated, int units, int most, float *ws, hipStream_t s) {
   const bool f16 = dtype == MOE_DT_FP16;
   switch ((xkind == X_MX4 ? 0 : 4) + (f16 ? 2 : 0) + (gated ? 1 : 0)) {
-    case 0: return mx_launch<X_MX4, false, false>(a, units, most, s);
-    case 1: return mx_launch<X_MX4, false, true>(a, units, most, s);
-    case 2: return mx_launch<X_MX4, true, false>(a, units, most, s);
-    case 3: return mx_launch<X_MX4, true, true>(a, units, most, s);
-    case 4: return mx_launch<X_BF16, false, false>(a, units, most, s);
-    case 5: return mx_launch<X_BF16, false, true>(a, units, most, s);
-    case 6: return mx_launch<X_FP16, true, false>(a, units, most, s);
-    default: return mx_launch<X_FP16, true, true>(a, units, most, s);
+    case 0: return mx_launch<X_MX4, false, false>(a, units, most, ws, s);
+    case 1: return mx_launch<X_MX4, false, true>(a, units, most, ws, s);
+    case 2: return mx_launch<X_MX4, true, false>(a, units, most, ws, s);
+    case 3: return mx_launch<X_MX4, true, true>(a, units, most, ws, s);
+    case 4: return mx_launch<X_BF16, false, false>(a, units, most, ws, s);
+    case 5: return mx_launch<X_BF16, false, true>(a, units, most, ws, s);
+    case 6: return mx_launch<X_FP16, true, false>(a, units, most, ws, s);
+    default: return mx_launch<X_FP16, true, true>(a, units, most, ws, s);
   }
 }
 static MxArgs mx_args(const void *x, int64_t ldx, const moe_mx4 *xq, const moe_mx4 *w, const moe_mx4 *w_up, const void *bias,
@@ -1113,7 +1177,12 @@ extern "C" int moe_mx4_linear(const void *x, int64_t ldx, const moe_mx4 *xq, con
   const int xkind = xq ? X_MX4 : dtype == MOE_DT_FP16 ? X_FP16 : X_BF16;
   if (int rc = mx_check("moe_mx4_linear", a, xkind, M, 1, dtype, w_up != nullptr)) return rc;
   if (!M || !N) return MOE_OK;
-  return mx_run(a, xkind, dtype, w_up != nullptr, 1, M, (hipStream_t)stream);
+  const int64_t need = moe_mx4_linear_workspace_bytes(M, N, K, xq != nullptr, w_up != nullptr);
+  if (need && (!ws || ws_bytes < need || ((uintptr_t)ws & 15))) {
+    moe_set_error("moe_mx4_linear: a workspace of %lld bytes on a 16-byte boundary is needed", (long long)need);
+    return MOE_EINVAL;
+  }
+  return mx_run(a, xkind, dtype, w_up != nullptr, 1, M, (float *)ws, (hipStream_t)stream);
 }
 
 extern "C" int moe_mx4_experts(const void *x, int64_t ldx, const moe_mx4 *xq, const moe_mx4 *w, const moe_mx4 *w_up, const void *bias,
@@ -1134,5 +1203,5 @@ extern "C" int moe_mx4_experts(const void *x, int64_t ldx, const moe_mx4 *xq, co
     return MOE_EINVAL;
   }
   if (!P || !N) return MOE_OK;
-  return mx_run(a, xkind, dtype, w_up != nullptr, E < P ? E : P, T, (hipStream_t)stream);
+  return mx_run(a, xkind, dtype, w_up != nullptr, E < P ? E : P, T, nullptr, (hipStream_t)stream);
 }

@@ -766,8 +766,12 @@ def _product_mx4(what, x, mats, biases, act, residual, out, out_dtype, d=None, o
     xp, xq = (0, byref(x.desc)) if quantised else (x.data_ptr(), None)
     up, b_up = (byref(mats[1].desc), ptr(biases[1])) if len(mats) == 2 else (None, 0)
     if d is None:
+        ws_ptr, n_ws = 0, lib.moe_mx4_linear_workspace_bytes(M, N, K, quantised, len(mats) == 2)
+        if n_ws:
+            ws = torch.empty(n_ws, dtype=torch.uint8, device=first.device)
+            ws_ptr = ws.data_ptr()
         rc = lib.moe_mx4_linear(xp, ldx, xq, byref(wd), up, ptr(biases[0]), b_up, ptr(residual), ldr, out.data_ptr(), ldy, M, N, K, code,
-                                L.ACTS[act], y32, 0, 0, _raw_stream(index))
+                                L.ACTS[act], y32, ws_ptr, n_ws, _raw_stream(index))
     else:
         rc = lib.moe_mx4_experts(xp, ldx, xq, byref(wd), up, ptr(biases[0]), b_up, out.data_ptr(), ldy, d.counts.data_ptr(),
                                  d.offsets.data_ptr(), d.units.data_ptr(), d.max_units, d.sorted_tok.data_ptr() if of_tokens else 0, d.T,
