@@ -161,6 +161,14 @@ static __device__ __forceinline__ u32x4_t mx_bf16(u32 c, float s) {
                  __builtin_bit_cast(u32, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(c, s, 2)),
                  __builtin_bit_cast(u32, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(c, s, 3))};
 }
+// the same as fp16, exactly where the scale is between 2^-23 and 2^13 (mx_fits_f16)
+static __device__ __forceinline__ u32x4_t mx_f16(u32 c, float s) {
+  return u32x4_t{__builtin_bit_cast(u32, __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(c, s, 0)),
+                 __builtin_bit_cast(u32, __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(c, s, 1)),
+                 __builtin_bit_cast(u32, __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(c, s, 2)),
+                 __builtin_bit_cast(u32, __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(c, s, 3))};
+}
+static __device__ __forceinline__ bool mx_fits_f16(u32 byte) { return byte - 104u <= 36u; }
 // eight fp16 values as the sums of two bf16: the first to the nearest, the second what is left (at most 4 bits)
 static __device__ __forceinline__ void mx_split(u32x4_t x, u32x4_t &hi, u32x4_t &lo) {
 #pragma unroll
@@ -225,7 +233,8 @@ __global__ __launch_bounds__(64 * WAVES) void k_mx4_rows(const MxArgs a) {
 #pragma unroll
         for (int i = 0; i < NM; ++i) {
           fw[p][i][u] = bload16(rw[i % MATS], in ? vw[i / MATS] + 16 * k : LT_OUT, 0);
-          sw[p][i][u] = bload1(rs[i % MATS], in ? vs[i / MATS] + ks : LT_OUT, 0);
+          const u32 b = bload1(rs[i % MATS], in ? vs[i / MATS] + ks : LT_OUT, 0);
+          sw[p][i][u] = X == X_FP16 && !in ? 127u : b;           // (of zeros any scale will do)
         }
         if constexpr (X == X_MX4) {
           fx[p][u][0] = bload16(rx, in ? vx + 16 * k : LT_OUT, 0);
@@ -244,6 +253,20 @@ __global__ __launch_bounds__(64 * WAVES) void k_mx4_rows(const MxArgs a) {
           for (int i = 0; i < NM; ++i)
             acc[i] = mx_mfma16(__builtin_bit_cast(u32x4_t, fw[p][i][u]), __builtin_bit_cast(u32x4_t, fx[p][u][0]), acc[i], sw[p][i][u], sx[p][u]);
         } else {
+          if constexpr (X == X_FP16) {  // weights in fp16 where the whole wave's can be
+            bool fits = true;
+#pragma unroll
+            for (int i = 0; i < NM; ++i) fits = fits && mx_fits_f16(sw[p][i][u]);
+            if (__all(fits)) {
+#pragma unroll
+              for (int j = 0; j < 4; ++j)
+#pragma unroll
+                for (int i = 0; i < NM; ++i)
+                  acc[i] = lin_mfma16<true>(mx_f16(__builtin_bit_cast(u32x4_t, fw[p][i][u])[j], __uint_as_float(sw[p][i][u] << 23)),
+                                            __builtin_bit_cast(u32x4_t, fx[p][u][j]), acc[i]);
+              continue;
+            }
+          }
 #pragma unroll
           for (int j = 0; j < 4; ++j) {
             u32x4_t x = __builtin_bit_cast(u32x4_t, fx[p][u][j]), lo;
@@ -856,6 +879,28 @@ __global__ __launch_bounds__(256, RING * (WM * 64 * 256 + WN * 64 * 64 + 1024) >
   for (int i = 0; i < RING; ++i)
 #pragma unroll
     for (int d = 0; d < NT; ++d) dma(d, kt0 + i, i * SLAB);
+  // fp16: can all weights of this wave be fp16?  Decided by all of their scales (a sixteenth of the codes' bytes) while the ring fills
+  bool fits = false;
+  if constexpr (F16) {
+    u16x2_t least{127, 127}, most{127, 127};
+    for (int b = 0; b < WN; ++b) {
+      const int block = wn * WN + b, row0 = t.n0 + 32 * (GATED ? block >> 1 : block);
+      const uint8_t *base = a.ws[GATED ? block & 1 : 0] + t.e * a.ews + mx_scale_row(row0, slabs);
+      if (row0 < a.N)
+        for (int i = lane; i < slabs * 16; i += 64) {  // 16 bytes: two rows of a slab
+          const u32x4_t v = *(const u32x4_t *)(base + 16 * i);
+#pragma unroll
+          for (int d = 0; d < 4; ++d) {
+            const u32 mask = row0 + 2 * (i & 15) + (d >> 1) < a.N ? mx_mask((a.K >> 5) - 8 * (i >> 4) - 4 * (d & 1)) : 0u;
+            const u32 w4 = (v[d] & mask) | (0x7f7f7f7fu & ~mask);
+            const u16x2_t even = __builtin_bit_cast(u16x2_t, w4 & 0x00ff00ffu), odd = __builtin_bit_cast(u16x2_t, w4 >> 8 & 0x00ff00ffu);
+            least = __builtin_elementwise_min(least, __builtin_elementwise_min(even, odd));
+            most = __builtin_elementwise_max(most, __builtin_elementwise_max(even, odd));
+          }
+        }
+    }
+    fits = __all(mx_fits_f16(min(least[0], least[1])) && mx_fits_f16(max(most[0], most[1])));
+  }
   LT_VM((RING - 1) * NT);
   __builtin_amdgcn_s_barrier();
   u32x4_t fx[2][8][WM], fw[2][2][WN];
@@ -871,32 +916,30 @@ __global__ __launch_bounds__(256, RING * (WM * 64 * 256 + WN * 64 * 64 + 1024) >
     }
   };
   constexpr int NR = 3 * WN + 8 * WM, NP = 8 * NG;
-  // operands of a step, made during the step before
+  // operands of a step, made during the step before.  FAST (fp16): the weights become fp16 and x stays as it is; otherwise x is two
+  // bf16 and the products are twice as many.
   u32x4_t cw[2][WN], hi[2][WM], lo[2][WM];
   float sv[WN][2];
-  constexpr int NC2 = WN + WM;
-  auto make = [&](int m, int j, int p, int kt) {
+  constexpr int NC2 = WN + (F16 ? WM : 0);
+  auto make = [&](auto fast_, int m, int j, int p, int kt) {
+    constexpr bool FAST = decltype(fast_)::value;
     if (m < WN) {
-      const int b = m;
+      const int b = m < WN ? m : 0;
       if (j == 0) {
         const u32 two = (fs[p][b] & mx_mask(blocks - kt * 4)) >> (16 * q);
         sv[b][0] = __uint_as_float((two & 255u) << 23);
         sv[b][1] = __uint_as_float((two >> 8 & 255u) << 23);
       }
-      cw[j & 1][b] = mx_bf16(fw[p][j >> 2][b][j & 3], sv[b][j >> 2]);
-    } else {
-      const int i = m - WN;
-      if constexpr (F16) mx_split(fx[p][j][i], hi[j & 1][i], lo[j & 1][i]);
-      else hi[j & 1][i] = fx[p][j][i];
+      cw[j & 1][b] = FAST ? mx_f16(fw[p][j >> 2][b][j & 3], sv[b][j >> 2]) : mx_bf16(fw[p][j >> 2][b][j & 3], sv[b][j >> 2]);
+    } else if constexpr (F16 && !FAST) {
+      const int i = m < WN ? 0 : m - WN;
+      mx_split(fx[p][j][i], hi[j & 1][i], lo[j & 1][i]);
     }
   };
-#pragma unroll
-  for (int r = 0; r < NR; ++r) read(0, r, 0);
-#pragma unroll
-  for (int m = 0; m < NC2; ++m) make(m, 0, 0, kt0);
   int slot = 0;
-  auto step = [&](auto p_, int kt) {
+  auto step = [&](auto p_, auto fast_, int kt) __attribute__((always_inline)) {
     constexpr int p = decltype(p_)::value;
+    constexpr bool FAST = decltype(fast_)::value;
     const int next = slot + 1 < RING ? slot + 1 : 0;
     LT_LGKM0();
     LT_VM((RING - 2) * NT);
@@ -913,18 +956,33 @@ __global__ __launch_bounds__(256, RING * (WM * 64 * 256 + WN * 64 * 64 + 1024) >
         if (d * NP / NT == g) dma(d, kt + RING, slot * SLAB);
 #pragma unroll
       for (int m = 0; m < NC2; ++m)
-        if (m * NG / NC2 == in) make(m, (j + 1) & 7, j == 7 ? p ^ 1 : p, j == 7 ? kt + 1 : kt);
+        if (m * NG / NC2 == in) make(fast_, m, (j + 1) & 7, j == 7 ? p ^ 1 : p, j == 7 ? kt + 1 : kt);
       __builtin_amdgcn_sched_barrier(0);
-      acc[i][b] = mx_mfma32_bf16(cw[j & 1][b], hi[j & 1][i], acc[i][b]);
-      if constexpr (F16) acc[i][b] = mx_mfma32_bf16(cw[j & 1][b], lo[j & 1][i], acc[i][b]);
+      if constexpr (FAST) {
+        acc[i][b] = __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8_t, cw[j & 1][b]), __builtin_bit_cast(f16x8_t, fx[p][j][i]), acc[i][b], 0, 0, 0);
+      } else {
+        acc[i][b] = mx_mfma32_bf16(cw[j & 1][b], F16 ? hi[j & 1][i] : fx[p][j][i], acc[i][b]);
+        if constexpr (F16) acc[i][b] = mx_mfma32_bf16(cw[j & 1][b], lo[j & 1][i], acc[i][b]);
+      }
       __builtin_amdgcn_sched_barrier(0);
     });
     slot = next;
   };
-  // (always a pair of slabs: one past the end is zeros)
-  for (int kt = kt0; kt < nk; kt += 2) {
-    step(std::integral_constant<int, 0>(), kt);
-    step(std::integral_constant<int, 1>(), kt + 1);
+  auto run = [&](auto fast) __attribute__((always_inline)) {
+#pragma unroll
+    for (int r = 0; r < NR; ++r) read(0, r, 0);
+#pragma unroll
+    for (int m = 0; m < NC2; ++m) make(fast, m, 0, 0, kt0);
+    for (int kt = kt0; kt < nk; kt += 2) {  // (always a pair of slabs: one past the end is zeros)
+      step(std::integral_constant<int, 0>(), fast, kt);
+      step(std::integral_constant<int, 1>(), fast, kt + 1);
+    }
+  };
+  if constexpr (F16) {
+    if (fits) run(std::true_type());
+    else run(std::false_type());
+  } else {
+    run(std::false_type());
   }
   static_assert(4 * 32 * (32 * WN + 4) * 4 <= RING * SLAB, "the sums of four waves fit the ring");
   mx_tile_out<F16, GATED, WM, WN>(mx_out(a, t), acc, s_ring, t.m0, t.n0, t.split);

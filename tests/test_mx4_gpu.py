@@ -276,6 +276,25 @@ def test_scales_of_the_whole_range(cuda, M):
             check(ops.linear_mx4(xs, w, out_dtype=torch.float32), y, e)
 
 
+@pytest.mark.parametrize("M", [1, 12, 40, 300])
+def test_fp16_rows_at_the_ends_of_what_fp16_weights_can_be(cuda, M):
+    """Scales of 2^-23 and 2^13 (the last whose codes are all fp16), one step further, and rows of the smallest fp16 values."""
+    from promoe_amd import ops
+    print(f"case mx4_fp16 M={M}", flush=True)
+    N, K = 200, 1056
+    gen = torch.Generator(device=cuda).manual_seed(M)
+    codes = matrix((N, K), gen, cuda).codes
+    x = rows((M, K), 1.0, torch.float16, gen, cuda)
+    x[::2] *= 2.0 ** -22
+    for low, high in ((104, 105), (139, 140), (103, 105), (139, 141), (104, 140), (127, 128)):
+        s = torch.randint(low, high + 1, (N, K // 32), device=cuda, generator=gen, dtype=torch.uint8)
+        w = ops.Mx4(codes, s)
+        y, e = expect(x.double(), [values(codes, s)], [None], "none")
+        check(ops.linear_mx4(x, w, out_dtype=torch.float32), y, e)
+        y, e = expect(x.double(), [values(codes, s)] * 2, [None] * 2, "relu")
+        check(ops.linear_gated_mx4(x, w, w, act="relu", out_dtype=torch.float32), y, e)
+
+
 def routed(T, E, k, gen, dev, skew=0.0, left=0.0):
     from promoe_amd import ops
     s = torch.randn(T, E, device=dev, generator=gen) - skew * torch.log1p(torch.arange(E, device=dev))
