@@ -1100,7 +1100,7 @@ static const MxModel MX_MODEL16 = {{{1, 1, 3, 2, .264f, .118f, 2.32f}, {1, 2, 3,
 // rows of all `units` products together; units 0: a dense one
 static MxPlan mx_plan(int xkind, long long rows, int units, int N, int K, bool gated) {
   const long long each = units ? rows / units : rows;
-  if (each <= 16) return MxPlan{0, 0, 0, 1, 0.f};
+  if (each <= (xkind == X_MX4 ? 8 : 16)) return MxPlan{0, 0, 0, 1, 0.f};
   static const int pieces[] = {1, 2, 3, 4, 6, 8, 12};
   const MxModel &model = xkind == X_MX4 ? MX_MODEL4 : MX_MODEL16;
   const int slab = xkind == X_MX4 ? M4_K : M16_K;

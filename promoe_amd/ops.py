@@ -594,7 +594,7 @@ class Mx4:
     Codes are kept as they are if their rows are on 16-byte boundaries and copied otherwise; scales are laid out anew, in the blocks that
     the kernels read, and `scales` is a new tensor at every access."""
 
-    __slots__ = ("shape", "desc", "_codes", "_blocks", "_buffer")
+    __slots__ = ("shape", "desc", "index", "_codes", "_blocks", "_buffer")
 
     def __init__(self, codes: torch.Tensor, scales: torch.Tensor):
         if codes.dtype != torch.uint8 or scales.dtype != torch.uint8 or codes.dim() not in (2, 3) or codes.dim() != scales.dim():
@@ -612,7 +612,7 @@ class Mx4:
         shape = _scale_shape(lead, N, K)
         rows = torch.nn.functional.pad(scales, (0, shape[-3] * 8 - K // 32, 0, shape[-4] * 32 - N))
         blocks = rows.unflatten(-1, (-1, 8)).unflatten(-3, (-1, 32)).transpose(-3, -2).contiguous() if N else rows.new_empty(shape)
-        self._codes, self._blocks, self._buffer, self.shape = codes, blocks, None, (*lead, N, K)
+        self._codes, self._blocks, self._buffer, self.shape, self.index = codes, blocks, None, (*lead, N, K), codes.get_device()
         # (of one row the distance to the next is whatever the tensor says: the kernels get one that holds the row)
         self.desc = L.Mx4Desc(codes.data_ptr(), blocks.data_ptr(), codes.stride(-2) if N > 1 else K // 2,
                               codes.stride(0) if lead and lead[0] > 1 else 0, blocks.stride(0) if lead and lead[0] > 1 else 0)
@@ -626,6 +626,7 @@ class Mx4:
         n_c, n_s = N * K // 2, (N + 31) // 32 * ((K + 255) // 256) * 256
         q._buffer = torch.empty(E * (n_c + n_s), dtype=torch.uint8, device=device)
         at = q._buffer.data_ptr()
+        q.index = q._buffer.get_device()
         q._codes = q._blocks = None
         q.shape = (*shape,)
         q.desc = L.Mx4Desc(at, at + E * n_c, K // 2, *((n_c, n_s) if E > 1 else (0, 0)))
@@ -707,26 +708,34 @@ def dequantize_mx4(q: Mx4, dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
     return y
 
 
-def _product_mx4(what, x, mats, biases, act, residual, out, out_dtype, d=None, of_tokens=False):
-    w = mats[0]
-    quantised = isinstance(x, Mx4)
-    if not all(isinstance(m, Mx4) for m in mats) or len(w.shape) != (2 if d is None else 3) or any(m.shape != w.shape for m in mats):
+def _product_mx4(what, x, w, w_up, bias, b_up, act, residual, out, out_dtype, d=None, of_tokens=False):
+    quantised = type(x) is Mx4
+    if type(w) is not Mx4 or len(w.shape) != (2 if d is None else 3) or (w_up is not None and (type(w_up) is not Mx4 or w_up.shape != w.shape)):
         raise L.MoeError("%s: weights must be Mx4 %s, both of a pair of one shape" % (what, "[N, K]" if d is None else "[E, N, K]"))
     if quantised:
         dtype = next((t for t in (out_dtype, None if out is None else out.dtype) if t in L.DTYPES), None)
         if dtype is None:
-            dtype = next((t.dtype for t in (*biases, residual) if t is not None), torch.bfloat16)
+            dtype = next((t.dtype for t in (bias, b_up, residual) if t is not None), torch.bfloat16)
+        index = x.index
+        if index < 0:
+            raise L.MoeError("%s: tensors of a GPU are needed, not of %s" % (what, x.device))
     else:
         dtype = x.dtype
+        index = -1
     code = L.DTYPES.get(dtype)
     if code is None or act not in L.ACTS:
         raise L.MoeError("%s: an x of bf16, fp16 or Mx4 and one of the activations %s" % (what, sorted(L.ACTS)))
-    first = x._tensor if quantised else x
-    index = _operands(what, first, *[m._tensor for m in mats], *biases, residual, out,
-                      *((d.counts, d.offsets, d.units, d.sorted_tok) if d is not None else ()))
+    if not quantised:
+        index = _operands(what, x)
+    for t in (bias, b_up, residual, out):
+        if t is not None and (t.get_device() != index or (t.requires_grad and torch.is_grad_enabled())):
+            _operands(what, t)
+            raise L.MoeError("%s: tensors of GPU %d and of %s" % (what, index, t.device))
+    if w.index != index or (w_up is not None and w_up.index != index) or (d is not None and d.counts.get_device() != index):
+        raise L.MoeError("%s: x, weights and dispatch must be on one GPU" % what)
     if index != torch.cuda.current_device():
         with torch.cuda.device(index):
-            return _product_mx4(what, x, mats, biases, act, residual, out, out_dtype, d, of_tokens)
+            return _product_mx4(what, x, w, w_up, bias, b_up, act, residual, out, out_dtype, d, of_tokens)
     if len(x.shape) != 2:
         raise L.MoeError("%s: x must be [M, K]" % what)
     rows, K = x.shape
@@ -741,11 +750,13 @@ def _product_mx4(what, x, mats, biases, act, residual, out, out_dtype, d=None, o
                              % (what, rows, w.shape[0], d.T, d.k, d.E))
     ldx = 0 if quantised else _rows(what, x, rows, K)
     wd = w.desc
-    for m in mats[1:]:
-        md = m.desc
-        if (md.ldc, md.next_c, md.next_s) != (wd.ldc, wd.next_c, wd.next_s):
+    up = None
+    if w_up is not None:
+        up = w_up.desc
+        if up.ldc != wd.ldc or up.next_c != wd.next_c or up.next_s != wd.next_s:
             raise L.MoeError("%s: both matrices of a pair must have the same strides" % what)
-    for b in biases:
+        up = byref(up)
+    for b in (bias, b_up):
         if b is not None and (b.dtype != dtype or b.shape != w.shape[:-1] or not b.is_contiguous()):
             raise L.MoeError("%s: a bias must be %s %s, contiguous" % (what, dtype, list(w.shape[:-1])))
     ldr = 0
@@ -754,28 +765,29 @@ def _product_mx4(what, x, mats, biases, act, residual, out, out_dtype, d=None, o
             raise L.MoeError("%s: the residual must be %s" % (what, dtype))
         ldr = _rows(what, residual, M, N)
     if out is None:
-        out = torch.empty((M, N), dtype=out_dtype or dtype, device=first.device)
+        y_dtype = out_dtype or dtype
+        out = torch.empty((M, N), dtype=y_dtype, device=w.device if quantised else x.device)
         ldy = N
     else:
         ldy = _rows(what, out, M, N)
-        if out_dtype is not None and out.dtype != out_dtype:
-            raise L.MoeError("%s: out is %s, asked for was %s" % (what, out.dtype, out_dtype))
-    y32 = out.dtype == torch.float32
-    if not y32 and out.dtype != dtype:
+        y_dtype = out.dtype
+        if out_dtype is not None and y_dtype != out_dtype:
+            raise L.MoeError("%s: out is %s, asked for was %s" % (what, y_dtype, out_dtype))
+    y32 = y_dtype == torch.float32
+    if not y32 and y_dtype != dtype:
         raise L.MoeError("%s: results are %s or fp32" % (what, dtype))
     xp, xq = (0, byref(x.desc)) if quantised else (x.data_ptr(), None)
-    up, b_up = (byref(mats[1].desc), ptr(biases[1])) if len(mats) == 2 else (None, 0)
     if d is None:
-        ws_ptr, n_ws = 0, lib.moe_mx4_linear_workspace_bytes(M, N, K, quantised, len(mats) == 2)
+        ws_ptr, n_ws = 0, lib.moe_mx4_linear_workspace_bytes(M, N, K, quantised, up is not None) if M > 8 else 0
         if n_ws:
-            ws = torch.empty(n_ws, dtype=torch.uint8, device=first.device)
+            ws = torch.empty(n_ws, dtype=torch.uint8, device=w.device)
             ws_ptr = ws.data_ptr()
-        rc = lib.moe_mx4_linear(xp, ldx, xq, byref(wd), up, ptr(biases[0]), b_up, ptr(residual), ldr, out.data_ptr(), ldy, M, N, K, code,
+        rc = lib.moe_mx4_linear(xp, ldx, xq, byref(wd), up, ptr(bias), ptr(b_up), ptr(residual), ldr, out.data_ptr(), ldy, M, N, K, code,
                                 L.ACTS[act], y32, ws_ptr, n_ws, _raw_stream(index))
     else:
-        rc = lib.moe_mx4_experts(xp, ldx, xq, byref(wd), up, ptr(biases[0]), b_up, out.data_ptr(), ldy, d.counts.data_ptr(),
-                                 d.offsets.data_ptr(), d.units.data_ptr(), d.max_units, d.sorted_tok.data_ptr() if of_tokens else 0, d.T,
-                                 M, d.E, N, K, code, L.ACTS[act], y32, _raw_stream(index))
+        rc = lib.moe_mx4_experts(xp, ldx, xq, byref(wd), up, ptr(bias), ptr(b_up), out.data_ptr(), ldy, d.counts.data_ptr(),
+                                 d.offsets.data_ptr(), d.units.data_ptr(), d.max_units, d.sorted_tok.data_ptr() if of_tokens else 0, d.T, M,
+                                 d.E, N, K, code, L.ACTS[act], y32, _raw_stream(index))
     if rc:
         check(rc, what)
     return out
@@ -787,13 +799,19 @@ def linear_mx4(x, w: Mx4, bias: torch.Tensor | None = None, act: str = "none", r
     as they are, or an Mx4 (quantize_mx4), then both operands go to the matrix cores in 4 bits.  bias, residual and the result are of
     x's type, or for an Mx4 all bf16 or all fp16 (the result: out_dtype, else theirs, else bf16); out_dtype fp32 leaves the sums in 32
     bits.  Activations, strides and the rest as in linear, K a multiple of 32."""
-    return _product_mx4("linear_mx4", x, (w,), (bias,), act, residual, out, out_dtype)
+    return _product_mx4("linear_mx4", x, w, None, bias, None, act, residual, out, out_dtype)
+
+
+def _second(w_up):
+    if w_up is None:
+        raise L.MoeError("a gated product needs both matrices")
+    return w_up
 
 
 def linear_gated_mx4(x, w_gate: Mx4, w_up: Mx4, b_gate: torch.Tensor | None = None, b_up: torch.Tensor | None = None, act: str = "silu",
                      out: torch.Tensor | None = None, out_dtype: torch.dtype | None = None):
     """act(x w_gate^T + b_gate) * (x w_up^T + b_up) in one pass; types as in linear_mx4, both matrices with the same strides."""
-    return _product_mx4("linear_gated_mx4", x, (w_gate, w_up), (b_gate, b_up), act, None, out, out_dtype)
+    return _product_mx4("linear_gated_mx4", x, w_gate, _second(w_up), b_gate, b_up, act, None, out, out_dtype)
 
 
 def experts_linear_mx4(x, w: Mx4, d: Dispatch, bias: torch.Tensor | None = None, act: str = "none", of_tokens: bool = False,
@@ -802,14 +820,14 @@ def experts_linear_mx4(x, w: Mx4, d: Dispatch, bias: torch.Tensor | None = None,
     x [T*k, K] has its rows in the dispatch's order (sort_tokens, or what the first half of the experts left), or, with of_tokens, a row
     for each token.  The result [T*k, N] is in the dispatch's order; rows behind the last pair are left as they were.  Types as in
     linear_mx4."""
-    return _product_mx4("experts_linear_mx4", x, (w,), (bias,), act, None, out, out_dtype, d, of_tokens)
+    return _product_mx4("experts_linear_mx4", x, w, None, bias, None, act, None, out, out_dtype, d, of_tokens)
 
 
 def experts_gated_mx4(x, w_gate: Mx4, w_up: Mx4, d: Dispatch, b_gate: torch.Tensor | None = None, b_up: torch.Tensor | None = None,
                       act: str = "silu", of_tokens: bool = False, out: torch.Tensor | None = None,
                       out_dtype: torch.dtype | None = None):
     """act(x w_gate[e]^T + b_gate[e]) * (x w_up[e]^T + b_up[e]): the first half of every expert, arguments as in experts_linear_mx4."""
-    return _product_mx4("experts_gated_mx4", x, (w_gate, w_up), (b_gate, b_up), act, None, out, out_dtype, d, of_tokens)
+    return _product_mx4("experts_gated_mx4", x, w_gate, _second(w_up), b_gate, b_up, act, None, out, out_dtype, d, of_tokens)
 
 
 def _sort(x, d, ldx):
