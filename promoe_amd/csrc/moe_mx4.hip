@@ -1256,7 +1256,7 @@ extern "C" int moe_mx4_experts(const void *x, int64_t ldx, const moe_mx4 *xq, co
     return MOE_EINVAL;
   }
   if (int rc = mx_check("moe_mx4_experts", a, xkind, sorted_tok ? T : P, E, dtype, w_up != nullptr)) return rc;
-  if (sorted_tok && T * a.ldx >= 1ll << 31) {
+  if (sorted_tok && T * a.ldx > LT_OUT) {  // (offsets of gathered rows are those of a buffer resource)
     moe_set_error("moe_mx4_experts: %d rows of tokens %lld bytes apart (less than 2 GiB are needed)", T, a.ldx);
     return MOE_EINVAL;
   }

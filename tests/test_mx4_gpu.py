@@ -222,6 +222,77 @@ def test_sizes_of_dense_layers(cuda, M, N, K, gated, kind):
     product(cuda, M, N, K, kind, torch.bfloat16, "silu" if gated else "none", N % 2 == 1, not gated, gated)
 
 
+# Every tile on sizes that end inside it, with K whole and in pieces.
+@pytest.mark.parametrize("kind", ["mx4", "16"])
+@pytest.mark.parametrize("M,N,K,gated", [(24, 2050, 10944, False), (40, 4099, 14336, False), (100, 4094, 14336, False), (260, 2049, 10944, True),
+                                         (500, 2051, 10944, False), (300, 5003, 4128, False), (1000, 2049, 10944, False), (2000, 4097, 2080, True),
+                                         (4100, 4099, 1056, False), (900, 1409, 2080, True), (4000, 1409, 544, False), (3000, 700, 8192, False),
+                                         (1500, 8190, 544, False), (200, 14330, 1056, True), (600, 10941, 2048, False), (2050, 10941, 1056, False),
+                                         (1030, 8203, 4128, False), (2000, 4099, 4128, True), (60, 30, 9984, False)])
+def test_every_tile_on_ragged_sizes(cuda, M, N, K, gated, kind):
+    f16 = N % 2 == 0
+    product(cuda, M, N, K, kind, torch.float16 if f16 else torch.bfloat16, "gelu" if gated else "relu2", True, not gated, gated, gap=1,
+            out_dtype=torch.float32 if M % 100 else None)
+
+
+@pytest.mark.parametrize("kind", ["mx4", "16"])
+@pytest.mark.parametrize("M,N,K", [(1, 64, 512), (12, 80, 288), (30, 80, 288), (40, 130, 9984), (300, 300, 512)])
+def test_residual_in_place_and_aligned_only_to_its_type(cuda, M, N, K, kind):
+    """out is the residual; rows of an odd number of elements from an odd offset on."""
+    from promoe_amd import ops
+    print(f"case mx4_in_place M={M} N={N} K={K} {kind}", flush=True)
+    gen = torch.Generator(device=cuda).manual_seed(M)
+    x, w = rows((M, K), 1.0, torch.bfloat16, gen, cuda), matrix((N, K), gen, cuda)
+    xv = x.double()
+    if kind == "mx4":
+        x = ops.quantize_mx4(x)
+        xv = values(x.codes, x.scales)
+    buf = torch.randn(1 + M * (N + 5), device=cuda, generator=gen).to(torch.bfloat16)
+    res = buf[1:].view(M, N + 5)[:, :N]
+    before = buf.clone()
+    y, e = expect(xv, [values(w.codes, w.scales)], [None], "none", res)
+    assert ops.linear_mx4(x, w, residual=res, out=res) is res
+    torch.cuda.synchronize()
+    check(res, y, e)
+    keep = torch.ones_like(buf, dtype=torch.bool)
+    keep[1:].view(M, N + 5)[:, :N] = False
+    assert torch.equal(buf[keep], before[keep])
+
+
+@pytest.mark.parametrize("kind", ["mx4", "16"])
+@pytest.mark.parametrize("M,N,K,gated", [(5, 1100, 512, False), (450, 1100, 288, False), (1000, 1100, 544, True), (1050, 2050, 4128, False)])
+def test_rows_far_apart(cuda, M, N, K, gated, kind):
+    """Rows nearly 4 MiB apart, so that offsets pass 2^32 bytes: the same bits as from rows side by side."""
+    from promoe_amd import ops
+    print(f"case mx4_far M={M} N={N} K={K} gated={gated} {kind}", flush=True)
+    gen = torch.Generator(device=cuda).manual_seed(M)
+    ld = (1 << 22) - 16
+
+    def far(t):
+        size = t.element_size()
+        v = torch.empty((t.shape[0] - 1) * (ld // size) + t.shape[1], dtype=t.dtype, device=cuda).as_strided(t.shape, (ld // size, 1))
+        v.copy_(t)
+        return v
+
+    x = rows((M, K), 1.0, torch.bfloat16, gen, cuda).contiguous()
+    ws = [matrix((N, K), gen, cuda) for _ in range(2 if gated else 1)]
+    res = None if gated else rows((M, N), 1.0, torch.bfloat16, gen, cuda).contiguous()
+    xq = ops.quantize_mx4(x)
+    assert torch.equal(ops.quantize_mx4(far(x)).codes, xq.codes)
+    fx, fres = (ops.Mx4(far(xq.codes), xq.scales) if kind == "mx4" else far(x)), None if gated else far(res)
+    fw = [ops.Mx4(far(m.codes), m.scales) for m in ws]
+    assert torch.equal(ops.dequantize_mx4(fw[0]), ops.dequantize_mx4(ws[0]))
+    x = xq if kind == "mx4" else x
+    out = torch.empty((M - 1) * (ld // 2) + N, dtype=torch.bfloat16, device=cuda).as_strided((M, N), (ld // 2, 1))
+    if gated:
+        want = ops.linear_gated_mx4(x, *ws)
+        ops.linear_gated_mx4(fx, *fw, out=out)
+    else:
+        want = ops.linear_mx4(x, ws[0], residual=res)
+        ops.linear_mx4(fx, fw[0], residual=fres, out=out)
+    assert torch.equal(out, want)
+
+
 @pytest.mark.parametrize("M", [1, 12, 40, 300])
 def test_nan_and_infinities_stay_in_their_rows_and_columns(cuda, M):
     from promoe_amd import ops
@@ -350,6 +421,15 @@ def test_experts(cuda, T, E, k, N, K, gated, kind):
 
 
 @pytest.mark.parametrize("kind", ["mx4", "16"])
+@pytest.mark.parametrize("T,E,k,N,K,gated,skew", [(900, 700, 3, 130, 288, True, 0.0), (6000, 700, 3, 70, 288, False, 1.0), (3000, 256, 4, 100, 544, True, 2.0),
+                                                  (300, 8, 2, 1000, 2080, False, 0.0), (1100, 8, 2, 1050, 1056, True, 1.0), (5000, 16, 2, 513, 544, False, 0.5),
+                                                  (2000, 64, 1, 260, 96, True, 4.0), (200, 64, 1, 100, 288, False, 20.0)])
+def test_many_experts_and_uneven_ones(cuda, T, E, k, N, K, gated, skew, kind):
+    """More experts than lanes, single rows behind whole tiles, most rows at a few experts."""
+    experts(cuda, T, E, k, N, K, kind, torch.float16 if T % 3 else torch.bfloat16, gated, gated, bias=True, gap=1, skew=skew)
+
+
+@pytest.mark.parametrize("kind", ["mx4", "16"])
 @pytest.mark.parametrize("T,E,k,N,K,gated", [(1, 64, 6, 1408, 2048, True), (1, 64, 6, 2048, 1408, False), (20, 64, 8, 3584, 2560, False),
                                              (300, 64, 6, 1408, 2048, True), (1024, 8, 2, 4096, 2048, False)])
 def test_sizes_of_experts(cuda, T, E, k, N, K, gated, kind):
@@ -472,7 +552,8 @@ def test_empty_other_stream_graphs_and_refusals(cuda):
                  lambda: ops.experts_linear_mx4(x[:39], wg, d), lambda: ops.experts_linear_mx4(x, matrix((E - 1, I, H), gen, cuda), d),
                  lambda: ops.experts_gated_mx4(x, wg, wu, d, b_gate=torch.zeros(I, **bf)), lambda: ops.quantize_mx4(x[:, :200]),
                  lambda: ops.quantize_mx4(x.double()), lambda: ops.quantize_mx4(x[:, 4:36]), lambda: ops.quantize_mx4(x.cpu()),
-                 lambda: ops.quantize_mx4(x.t()), lambda: ops.linear_mx4(x, w2, act="tanh"), lambda: ops.dequantize_mx4(xq, torch.float64)):
+                 lambda: ops.quantize_mx4(x.t()), lambda: ops.linear_mx4(x, w2, act="tanh"), lambda: ops.dequantize_mx4(xq, torch.float64),
+                 lambda: ops.linear_gated_mx4(x, w2, None), lambda: ops.experts_linear_mx4(x, wg, ops.dispatch(torch.zeros(40, 1, dtype=torch.int32, device=cuda), E, max_units=2))):
         with pytest.raises(L.MoeError):
             call()
     x.requires_grad_(True)
