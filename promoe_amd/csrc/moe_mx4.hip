@@ -53,7 +53,7 @@ static __device__ __forceinline__ u32 scale_byte(u32 top) {
 }
 // Four lanes a block, eight values each: one 16-byte load (two of fp32) and four bytes of codes, side by side over the lanes.  The
 // hardware's conversion divides by the scale, rounds to the nearest (ties to the even code) and goes no further than 6.
-// Bound by memory: 4096 x 14336 in bf16 25 us (5.9 TB/s, the last cache helps), back 22.
+// Bound by memory: 4096 x 14336 in bf16 25 to 27 us (5.9 TB/s, the last cache helps), back 22 to 25.
 #define QT_U 4  // pieces of a lane, all of them on their way at once
 template <int DT>
 __global__ __launch_bounds__(256) void k_mx4_quantize(const QuantArgs a) {
@@ -531,8 +531,8 @@ __global__ __launch_bounds__(256) void k_mx4_join(const MxArgs a) {
 // pair's W blocks alternate between the two matrices (block b: matrix b & 1, its columns 32 (b >> 1) ..), so that a lane holds both sums
 // of a column.  K advances 256 at a time (a slab: 128 bytes of codes and 8 of scales a row); slabs go global -> LDS directly, RING of them
 // in LDS.  A lane's operand of a product is one block of 32 columns: half q of the wave takes the blocks 4 q .. 4 q + 3 of a slab, so that
-// the scales of a fragment's four steps are one word, a byte a step.  A slab of 128 x 128 costs as long in LDS as in the matrix cores (512 cycles);
-// two workgroups a compute unit (RING 2) hide each other's start and end where K is short: 2048 tokens of 64 experts 139 / 91 us.
+// the scales of a fragment's four steps are one word, a byte a step.  Where K is short two workgroups a compute unit (RING 2) do
+// better than one with a longer ring: 2048 tokens of 64 experts, WM 1, WN 2, RING 4 / 2: 139 / 94 us.
 #define M4_K 256
 static __device__ __forceinline__ void mx_dma16(unsigned at, int off, lt_rsrc_t rs, int soff) {
   // (assembly: told that a load writes LDS, the compiler would wait for all of them in front of every barrier and LDS read; the waits
@@ -682,8 +682,7 @@ __global__ __launch_bounds__(256, RING * (WM + WN) * 64 * 136 > 80 * 1024 ? 1 : 
 // fragments are read step by step.  Two slabs in LDS.  The fragments of a whole slab fit the registers (four steps of eight), and they are
 // read as early as the slab is there: in the middle of its step 1 everybody has all of it, so its place takes the slab after next from
 // then on, more than a slab's time in front of the first read of that.
-// 4096 x 4096 x 14336 108 to 120 us (4.0 to 4.5 PFLOP/s): 2590 cycles a slab for 2048 of products, at 1.8 GHz (power).  The result leaves at 4.4 TB/s in
-// the end, 7.6 us.
+// 4096 x 4096 x 14336 108 to 124 us (3.9 to 4.5 PFLOP/s): about 2590 cycles a slab for 2048 of products (from counters at two K), at 1.82 GHz (power).
 template <bool F16, bool GATED>
 __global__ __launch_bounds__(256, 1) void k_mx4_wide(const MxArgs a) {
   constexpr int B = 256, NB = 4, NX = 8, NW = 8, NS = 4, NT = NX + NW + NS;
@@ -817,7 +816,7 @@ static __device__ __forceinline__ f32x16_t mx_mfma32_bf16(u32x4_t a, u32x4_t b, 
 // x in 16 bits: the same tile, K 128 at a time (256 bytes of a row of x, 64 of codes, one word of scales).  Half q of the wave takes the
 // columns 64 q .. 64 q + 63 of a slab, eight a step: blocks 2 q and 2 q + 1 of W, which become bf16 in front of their products.
 // Chunk c (16 bytes) of row r of x stands in slot c ^ (r & 15), of W in slot c ^ ((r >> 2) & 3).  Bound by LDS, which x fills: wide tiles are the
-// better ones (2048 tokens of 64 experts, us: 64 x 256 162, 128 x 128 209).  4096 x 4096 x 14336 420 us (1150 TFLOP/s).
+// better ones (2048 tokens of 64 experts, us: 64 x 256 166, 128 x 128 209).  4096 x 4096 x 14336 418 to 441 us (1090 to 1150 TFLOP/s).
 #define M16_K 128
 template <int X, bool GATED, int WM, int WN, int RING>
 __global__ __launch_bounds__(256, RING * (WM * 64 * 256 + WN * 64 * 64 + 1024) > 80 * 1024 ? 1 : 2) void k_mx4_tile16(const MxArgs a) {
@@ -1147,6 +1146,9 @@ static int mx_launch(const MxArgs &a, int units, int most, float *ws, hipStream_
 #define MR_LAUNCH(SH_, NB_, W_)                                                                                                      \
   hipLaunchKernelGGL(HIP_KERNEL_NAME(k_mx4_rows<X, F16, GATED, SH_, NB_, 1, W_>), dim3((a.N + 16 / SH_ * NB_ - 1) / (16 / SH_ * NB_), units), \
                      dim3(64 * W_), 0, s, a)
+    // Two blocks a workgroup share one operand of x where enough workgroups are left (16-bit x, us, NB 2 / 1: gated 8 x 14336 x 4096, SH 1,
+    // 19.1 / 23.5); with few sets eight waves on one block shorten each wave's part of K (1 x 2048 x 10944, NB 1 and 8 waves / NB 2 and 4:
+    // 8.1 / 8.8; 1 x 14336 x 4096 gated, NB 2, 8 / 4: 18.8 / 17.9).
     const long long sets = (a.N + 15) / 16 * (long long)units;  // of 16 rows of W
     if (most <= 8) {
       if (sets >= 256) MR_LAUNCH(2, 2, 4);

@@ -4,7 +4,8 @@
 //   gradients of unsort: dx[p] = w(t, j) dy[t],  dw(t, j) = <dy[t], x[p]>
 // All go by token: a token's row is read (or written) once, its k rows in the experts' order are written (read) whole, and each sum is one
 // lane's, in the order of the choices: no atomics, the same bits every time.  A pair without a place (pos -1: its expert is not one of
-// the E) takes no part; rows behind the last pair are zero in what is written in the experts' order.  Bound by memory.
+// the E) takes no part; rows behind the last pair are zero in what is written in the experts' order.  Bound by memory: 4096 tokens of 2048
+// bf16 columns, 6 choices: sort and unsort (117 MB) 24 us (4.9 TB/s) and 29 to 33 (3.6 to 4.1), the gradients of unsort (218 MB) 36 (6.0, the last cache helps).
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 
