@@ -313,7 +313,14 @@ extern "C" int moe_unsort_rows_grad(const void *dy, int64_t lddy, const void *x,
   if (int rc = move_check("moe_unsort_rows_grad", T, k, H, dtype, lddy, dw ? ldx : lddx,
                           dy && pos_of_pair && w && (dx || dw) && (x || !dw) && (total || !dx))) return rc;
   if (int rc = move_check("moe_unsort_rows_grad", T, k, H, dtype, lddy, dx ? lddx : ldx, true)) return rc;
-  if (!T) return MOE_OK;
+  if (!T || (!H && !dw)) return MOE_OK;
+  if (!H) {  // dw is zero all the same, and no row of dx exists
+    if (!pos_of_pair || !w) {
+      moe_set_error("moe_unsort_rows_grad: a tensor is missing");
+      return MOE_EINVAL;
+    }
+    dx = nullptr;
+  }
   const int size = dtype == MOE_DT_FP32 ? 4 : 2;
   const int64_t P = (int64_t)T * k, len = (int64_t)H * size;
   lddy *= size; ldx *= size; lddx *= size;

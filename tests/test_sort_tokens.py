@@ -43,3 +43,12 @@ def test_nothing_to_do():
     for call in (sort, unsort, grad):
         assert call(T=0, x=None, y=None) == 0 or call is grad
     assert sort(H=0, ldx=0, ldy=0, x=None, y=None) == 0 and unsort(H=0, ldx=0, ldy=0, x=None, y=None) == 0
+
+
+def test_gradient_of_rows_without_columns():
+    """dw is written (zeros) whatever the columns, so places and weights have to be there; without dw nothing is left to do."""
+    from promoe_amd import _lib as L
+    none = dict(H=0, ldx=0, ldy=0, lddy=0)
+    for kw in (dict(pos=None), dict(w=None)):
+        assert grad(**none, **kw) == L.MOE_EINVAL and b"missing" in L.lib.moe_last_error()
+    assert grad(**none, dw=None, pos=None, w=None, total=None, x=None, y=None, dy=None) == 0

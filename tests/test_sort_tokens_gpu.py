@@ -191,3 +191,55 @@ def test_choices_of_no_expert_have_no_place(cuda, T, k, E):
         pos = torch.full((T * k,), -1, dtype=torch.int32, device=cuda)
         pos[order[:n]] = torch.arange(n, dtype=torch.int32, device=cuda)
         assert int(d.offsets[E]) == n and torch.equal(d.pos_of_pair, pos) and torch.equal(d.sorted_pair[:n].long(), order[:n])
+
+
+def test_weights_of_rows_without_columns(cuda):
+    """Rows of no columns: nothing but the weights' gradient, which is zero."""
+    from promoe_amd import ops
+    print("case unsort_no_columns", flush=True)
+    T, k, E = 9, 3, 4
+    gen = torch.Generator(device=cuda).manual_seed(6)
+    d, _ = routing(T, k, E, gen, cuda, 0.0)
+    r = torch.empty(T * k, 0, device=cuda, requires_grad=True)
+    w = torch.ones(T, k, device=cuda, requires_grad=True)
+    y = ops.unsort_tokens(r, d, w)
+    dr, dw = torch.autograd.grad(y, [r, w], torch.empty_like(y))
+    assert y.shape == (T, 0) and dr.shape == r.shape and dw.shape == w.shape and not dw.any()
+
+
+def test_there_and_back_captured_with_gradients(cuda):
+    """Forward and backward in one graph, replayed with new values between eager runs on other leaves: the same bits."""
+    from promoe_amd import ops
+    print("case moves_captured_backward", flush=True)
+    T, H, k, E = 65, 72, 3, 8
+    gen = torch.Generator(device=cuda).manual_seed(7)
+    d, _ = routing(T, k, E, gen, cuda, 0.2)
+    x0, g0 = (rows((T, H), 1.0, torch.bfloat16, gen, cuda) for _ in range(2))
+    w0 = torch.rand(T, k, device=cuda, generator=gen)
+
+    def step(x, w, g):
+        y = ops.unsort_tokens(ops.sort_tokens(x, d), d, w)
+        return (y.detach(), *torch.autograd.grad(y, [x, w], g))
+
+    def eager(x, w, g):
+        return step(x.detach().clone().requires_grad_(), w.detach().clone().requires_grad_(), g.clone())
+
+    x, w, g = x0.clone().requires_grad_(), w0.clone().requires_grad_(), g0.clone()
+    st = torch.cuda.Stream()
+    st.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(st):
+        for _ in range(2):
+            step(x, w, g)
+    torch.cuda.current_stream().wait_stream(st)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = step(x, w, g)
+    for i in range(4):
+        with torch.no_grad():
+            x.copy_(x0 * (i + 1))
+            w.copy_(w0 + i)
+            g.copy_(g0 * (2 - i))
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(got, eager(x, w, g)))
