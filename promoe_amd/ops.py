@@ -850,13 +850,18 @@ def _unsort(x, d, w, ldx):
     return y
 
 
+def _whole_rows(what, t, rows, cols):
+    """A matrix as autograd hands it over (an expanded gradient, a saved tensor that a hook has laid out anew) with rows that the kernels
+    can read, and their distance."""
+    if t.dim() == 2 and (not (t.stride(1) == 1 or t.shape[1] <= 1) or t.stride(0) < t.shape[1]):
+        t = t.contiguous()
+    return t, _rows(what, t, rows, cols)
+
+
 def _gradient_rows(what, t):
-    """A gradient as autograd hands it over (an expanded one, say) with rows that the kernels can read, and their distance."""
     if torch.is_grad_enabled():
         raise L.MoeError("%s has no second gradient" % what)
-    if not (t.stride(1) == 1 or t.shape[1] <= 1) or t.stride(0) < t.shape[1]:
-        t = t.contiguous()
-    return t, _rows(what, t, *t.shape)
+    return _whole_rows(what, t, *t.shape)
 
 
 class _SortTokens(torch.autograd.Function):
@@ -874,7 +879,7 @@ class _SortTokens(torch.autograd.Function):
 class _UnsortTokens(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, w, d, ldx):
-        ctx.d, ctx.ldx = d, ldx
+        ctx.d = d
         if w is not None:
             ctx.save_for_backward(x, w)
         return _unsort(x, d, w, ldx)
@@ -887,10 +892,16 @@ class _UnsortTokens(torch.autograd.Function):
             return _sort(dy, d, ld), None, None, None
         x, w = ctx.saved_tensors
         need_x, need_w = ctx.needs_input_grad[:2]
-        T, k, H = d.T, d.k, x.shape[1]
+        T, k, H = d.T, d.k, dy.shape[1]
+        # (saved-tensor hooks may return other tensors than were saved: neither layout nor type is what forward saw)
+        x, ldx = _whole_rows("unsort_tokens", x, T * k, H)
+        w = w.contiguous()
+        if x.dtype != dy.dtype or w.dtype != torch.float32 or w.shape != (T, k) or x.device != dy.device or w.device != dy.device:
+            raise L.MoeError("unsort_tokens: saved rows and weights came back as %s %s on %s and %s %s on %s"
+                             % (x.dtype, tuple(x.shape), x.device, w.dtype, tuple(w.shape), w.device))
         dx = torch.empty((T * k, H), dtype=x.dtype, device=x.device) if need_x else None
         dw = torch.empty((T, k), dtype=torch.float32, device=x.device) if need_w else None
-        check(lib.moe_unsort_rows_grad(dy.data_ptr(), ld, x.data_ptr(), ctx.ldx, d.pos_of_pair.data_ptr(), w.data_ptr(),
+        check(lib.moe_unsort_rows_grad(dy.data_ptr(), ld, x.data_ptr(), ldx, d.pos_of_pair.data_ptr(), w.data_ptr(),
                                        d.offsets.data_ptr() + 4 * d.E, ptr(dx), H, ptr(dw), T, k, H, L.ROW_DTYPES[x.dtype],
                                        _raw_stream(x.get_device())), "unsort_tokens")
         return dx, dw, None, None
