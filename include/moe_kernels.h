@@ -134,7 +134,7 @@ typedef struct moe_unit {
 
 /* k2: stable dispatch of the P = T*k (token,slot) pairs (pair p = t*k + j).
  * counts[E], offsets[E+1], sorted_pair[P], pos_of_pair[P], sorted_tok[P] (= p / k),
- * (a pair whose idx is none of the E experts has pos_of_pair -1 and no place; moe_combine takes none such)
+ * (a pair whose idx is none of the E experts has pos_of_pair -1 and no place; moe_combine adds nothing for it)
  * units[max_units] (active experts ascending id, rest m = 0), n_active[1],
  * active_ids[max_units] int64 (the `unique expert ids` list the reference's module
  * hands to report_experts, utils/__init__.py:84-88). */
@@ -456,7 +456,7 @@ int moe_experts_prefill_windows(const void *x_bf16, int T, int H, int I, int I_s
 
 /* k5: y[t,:] = sum_j w[t,j] * part_r[pos_of_pair[t*k+j],:] + g_t * part_s[t,:], bf16 out.
  * g_t = sigmoid(shared_gate_logit[t*sg_stride]) when shared_gate_logit != NULL, else 1;
- * part_s may be NULL (no shared expert). */
+ * part_s may be NULL (no shared expert).  A pair whose place is none of 0 .. T*k - 1 (-1: its idx is no expert) adds nothing. */
 int moe_combine(const float *part_r, const float *part_s, const float *topk_w,
                 const int *pos_of_pair, const float *shared_gate_logit, int sg_stride, void *y_bf16,
                 int T, int H, int k, void *stream);

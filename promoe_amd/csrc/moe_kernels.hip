@@ -2882,17 +2882,24 @@ __global__ __launch_bounds__(256) void k_combine(const float *__restrict__ part_
   const int n = (blockIdx.x * 256 + threadIdx.x) * 4;
   if (n >= H) return;
   float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+  const u32 places = gridDim.y * (u32)k;
   // KK partial rows at a time: positions and weights first, then the rows, then the
   // fma chain in pair order (two round trips per KK rows instead of two per row)
   for (int j0 = 0; j0 < k; j0 += KK) {
     float wj[KK];
     int pos[KK];
+    bool in[KK];
     float4 v[KK];
 #pragma unroll
     for (int j = 0; j < KK; ++j) {
       const int jj = j0 + j < k ? j0 + j : k - 1;
       wj[j] = topk_w[(size_t)t * k + jj];
       pos[j] = pos_of_pair[(size_t)t * k + jj];
+    }
+#pragma unroll
+    for (int j = 0; j < KK; ++j) {  // (a pair without a place, -1, reads row 0 and drops it: no condition around a load)
+      in[j] = (u32)pos[j] < places;
+      pos[j] = in[j] ? pos[j] : 0;
     }
 #pragma unroll
     for (int j = 0; j < KK; ++j) v[j] = *(const float4 *)(part_r + (size_t)pos[j] * H + n);
@@ -2907,7 +2914,7 @@ __global__ __launch_bounds__(256) void k_combine(const float *__restrict__ part_
     }
 #pragma unroll
     for (int j = 0; j < KK; ++j)
-      if (j0 + j < k) {
+      if (j0 + j < k && in[j]) {
         acc.x = fmaf(wj[j], v[j].x, acc.x); acc.y = fmaf(wj[j], v[j].y, acc.y);
         acc.z = fmaf(wj[j], v[j].z, acc.z); acc.w = fmaf(wj[j], v[j].w, acc.w);
       }

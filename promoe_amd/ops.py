@@ -483,7 +483,7 @@ def shared_splits(fmt: int, T: int, H: int, I_sh: int) -> int:
 def combine(part_r, part_s, topk_w, pos_of_pair, shared_gate_logit, T: int, H: int, k: int,
             out: torch.Tensor | None = None, pieces: int | None = None, routed_pieces: int = 1):
     """part_s [S*T, H]: S > 1 when the shared expert's reduction was split (piece s = rows s*T .. s*T+T-1).
-    routed_pieces: the same of part_r [R*T*k, H].
+    routed_pieces: the same of part_r [R*T*k, H].  Choices of no expert (place -1) add nothing.
     pieces: S as the expert launch left it (shared_splits / moe_prefill_shared_splits); inferred from the rows of
     part_s when not given, which is only right for a part_s made for exactly this T."""
     dev = (part_r if part_r is not None else part_s).device
