@@ -8,6 +8,7 @@ from __future__ import annotations
 from ctypes import byref
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _lib as L
 from ._lib import lib, ptr, cur_stream, check
@@ -75,8 +76,17 @@ class RouteRule(L.RouteRule):
 _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (lambda index: torch.cuda.current_stream(index).cuda_stream)
 
 
+def _no_tangents(what: str, *tensors) -> None:
+    """None of a call's tensors may have a forward-mode tangent: the result would come without one."""
+    if getattr(forward_ad, "_current_level", 0) >= 0 and torch._C._is_fwd_grad_enabled():  # (-1 outside of every dual level)
+        for t in tensors:
+            if isinstance(t, torch.Tensor) and forward_ad.unpack_dual(t).tangent is not None:
+                raise L.MoeError("%s has no forward-mode gradient: call it with the primal" % what)
+
+
 def _operands(what: str, first: torch.Tensor, *others) -> int:
     """Index of the GPU that all tensors of a call (None among them) are on; none may be one that a gradient is expected of."""
+    _no_tangents(what, first, *others)
     index = first.get_device()
     if index < 0:
         raise L.MoeError("%s: tensors of a GPU are needed, not of %s" % (what, first.device))
@@ -709,6 +719,7 @@ def dequantize_mx4(q: Mx4, dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
 
 
 def _product_mx4(what, x, w, w_up, bias, b_up, act, residual, out, out_dtype, d=None, of_tokens=False):
+    _no_tangents(what, x, bias, b_up, residual, out)
     quantised = type(x) is Mx4
     if type(w) is not Mx4 or len(w.shape) != (2 if d is None else 3) or (w_up is not None and (type(w_up) is not Mx4 or w_up.shape != w.shape)):
         raise L.MoeError("%s: weights must be Mx4 %s, both of a pair of one shape" % (what, "[N, K]" if d is None else "[E, N, K]"))
@@ -909,6 +920,7 @@ class _UnsortTokens(torch.autograd.Function):
 
 def _move_args(what, x, d, rows, w):
     """(GPU, elements between the rows of x)"""
+    _no_tangents(what, x, w)
     if x.dim() != 2 or x.dtype not in L.ROW_DTYPES or x.shape[0] != rows:
         raise L.MoeError("%s: bf16, fp16 or fp32 [%d, H] is needed, not %s %s" % (what, rows, x.dtype, tuple(x.shape)))
     if w is not None and (w.dtype != torch.float32 or w.shape != (d.T, d.k) or not w.is_contiguous()):
@@ -922,7 +934,7 @@ def _move_args(what, x, d, rows, w):
 def sort_tokens(x: torch.Tensor, d: Dispatch) -> torch.Tensor:
     """The tokens' rows x [T, H] in the order of their experts: [T*k, H], a token's row once for each of its choices (moe_sort_rows).
     Choices of no expert (idx outside 0 .. E - 1) have no row; the rows behind the last one are zero.  Any alignment and row stride, bf16,
-    fp16 or fp32.  With a gradient, not a second one (each token the sum of its rows', in fp32): d has to keep its contents until the
+    fp16 or fp32.  With a gradient, not a second or a forward-mode one (each token the sum of its rows', in fp32): d has to keep its contents until the
     backward pass."""
     index, ldx = _move_args("sort_tokens", x, d, d.T, None)
     if index != torch.cuda.current_device():
@@ -936,7 +948,7 @@ def sort_tokens(x: torch.Tensor, d: Dispatch) -> torch.Tensor:
 def unsort_tokens(x: torch.Tensor, d: Dispatch, w: torch.Tensor | None = None) -> torch.Tensor:
     """The experts' rows x [T*k, H] back to their tokens: y[t] = sum over the choices of w[t, j] x[row of (t, j)] (moe_unsort_rows; w fp32
     [T, k], or 1), in fp32 and in the order of the choices, rounded once to x's type.  Choices of no expert add nothing, whatever lies
-    behind the last row.  With gradients of x and w, not second ones: d has to keep its contents until the backward pass."""
+    behind the last row.  With gradients of x and w, not second or forward-mode ones: d has to keep its contents until the backward pass."""
     index, ldx = _move_args("unsort_tokens", x, d, d.T * d.k, w)
     if index != torch.cuda.current_device():
         with torch.cuda.device(index):
