@@ -691,7 +691,7 @@ def quantize_mx4(x: torch.Tensor) -> Mx4:
             return quantize_mx4(x)
     E = shape[0] if len(shape) == 3 else 1
     M, K = shape[-2:]
-    ldx = _rows("quantize_mx4", x if len(shape) == 2 or not E else x[0], M, K)
+    ldx = _rows("quantize_mx4", x if len(shape) == 2 else x[0], M, K) if E else K
     q = Mx4._empty(shape, x.device)
     rc = lib.moe_mx4_quantize(x.data_ptr(), ldx, x.stride(0) if E > 1 else 0, code, E, M, K, byref(q.desc), _raw_stream(index))
     if rc:
