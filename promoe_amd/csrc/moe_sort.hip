@@ -221,10 +221,15 @@ static int move_check(const char *who, int T, int k, int H, int dtype, int64_t l
   }
   return MOE_OK;
 }
-// Do rows of `len` bytes, `la` and `lb` bytes apart, share memory?  (Ranges that meet are taken to.)
-static bool move_shares(const void *a, int64_t na, int64_t la, const void *b, int64_t nb, int64_t lb, int64_t len) {
-  const char *p = (const char *)a, *q = (const char *)b;
-  return p && q && na && nb && len && p < q + (nb - 1) * lb + len && q < p + (na - 1) * la + len;
+// From the first byte of an array to behind its last one (bytes 0: there is none)
+struct Span { const char *at; int64_t bytes; };
+static Span rows_span(const void *p, int64_t rows, int64_t ld, int64_t len) { return Span{(const char *)p, rows && len ? (rows - 1) * ld + len : 0}; }
+static Span words_span(const void *p, int64_t n) { return Span{(const char *)p, 4 * n}; }
+// Does a result share memory with one of the others?  (Spans that meet are taken to.)
+template <class... S>
+static bool move_shares(const Span &a, const S &...others) {
+  auto meets = [&](const Span &b) { return a.at && b.at && a.bytes && b.bytes && a.at < b.at + b.bytes && b.at < a.at + a.bytes; };
+  return (meets(others) || ...);
 }
 static bool move_wide(const void *p, int64_t ld) { return ((uintptr_t)p | (uintptr_t)ld) % 16 == 0; }
 // pieces of a row, and the lanes it gets: a wave, or fewer where a row is shorter
@@ -241,8 +246,9 @@ extern "C" int moe_sort_rows(const void *x, int64_t ldx, void *y, int64_t ldy, c
   if (!T || !H) return MOE_OK;
   const int size = dtype == MOE_DT_FP32 ? 4 : 2;
   ldx *= size; ldy *= size;
-  if (move_shares(x, T, ldx, y, (int64_t)T * k, ldy, (int64_t)H * size)) {
-    moe_set_error("moe_sort_rows: the result overlaps the rows that are read");
+  const int64_t P = (int64_t)T * k, len = (int64_t)H * size;
+  if (move_shares(rows_span(y, P, ldy, len), rows_span(x, T, ldx, len), words_span(pos_of_pair, P), words_span(total, 1))) {
+    moe_set_error("moe_sort_rows: the result overlaps what is read");
     return MOE_EINVAL;
   }
   MoveArgs a{(const char *)x, nullptr, (char *)y, pos_of_pair, total, nullptr, nullptr, ldx, ldy, 0, T, k, H, 0, 0};
@@ -292,8 +298,9 @@ extern "C" int moe_unsort_rows(const void *x, int64_t ldx, void *y, int64_t ldy,
   if (!T || !H) return MOE_OK;
   const int size = dtype == MOE_DT_FP32 ? 4 : 2;
   ldx *= size; ldy *= size;
-  if (move_shares(x, (int64_t)T * k, ldx, y, T, ldy, (int64_t)H * size)) {
-    moe_set_error("moe_unsort_rows: the result overlaps the rows that are read");
+  const int64_t P = (int64_t)T * k, len = (int64_t)H * size;
+  if (move_shares(rows_span(y, T, ldy, len), rows_span(x, P, ldx, len), words_span(pos_of_pair, P), words_span(w, P))) {
+    moe_set_error("moe_unsort_rows: the result overlaps what is read");
     return MOE_EINVAL;
   }
   MoveArgs a{(const char *)x, nullptr, (char *)y, pos_of_pair, nullptr, w, nullptr, ldx, ldy, 0, T, k, H, 0, 0};
@@ -324,8 +331,10 @@ extern "C" int moe_unsort_rows_grad(const void *dy, int64_t lddy, const void *x,
   const int size = dtype == MOE_DT_FP32 ? 4 : 2;
   const int64_t P = (int64_t)T * k, len = (int64_t)H * size;
   lddy *= size; ldx *= size; lddx *= size;
-  if (H && dx && (move_shares(dx, P, lddx, dy, T, lddy, len) || (dw && move_shares(dx, P, lddx, x, P, ldx, len)))) {
-    moe_set_error("moe_unsort_rows_grad: a gradient overlaps the rows that are read");
+  const Span sdx = rows_span(dx, P, lddx, len), sdw = words_span(dw, P), sx = dw ? rows_span(x, P, ldx, len) : Span{nullptr, 0};
+  const Span sdy = rows_span(dy, T, lddy, len), spos = words_span(pos_of_pair, P), sw = words_span(w, P), sn = dx ? words_span(total, 1) : Span{nullptr, 0};
+  if (move_shares(sdx, sdy, sx, spos, sw, sn, sdw) || move_shares(sdw, sdy, sx, spos, sw, sn)) {
+    moe_set_error("moe_unsort_rows_grad: a gradient overlaps what is read, or the other gradient");
     return MOE_EINVAL;
   }
   MoveArgs a{(const char *)x, (const char *)dy, (char *)dx, pos_of_pair, total, w, dw, ldx, lddx, lddy, T, k, H, 0, 0};
