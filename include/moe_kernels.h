@@ -507,8 +507,9 @@ int moe_linear_gated(const void *x, int64_t ldx, const void *w_gate, const void 
  *   moe_unsort_rows_grad  dx[p,:] = w[t,j] dy[t,:] (rows from total on zero) and dw[t,j] = <dy[t,:], x[p,:]> (0 without a place); dx or
  *                         dw may be NULL
  * Rows of H elements of one type (dtype; w and dw fp32), ld elements apart, any alignment (rows on 16-byte boundaries go faster); sums and
- * products in fp32, rounded once.  T below 2^26, T*k below 2^31, H below 2^24 (2^22 off those boundaries).  A result over what is read, or
- * over the other gradient, is refused (arrays whose spans meet are taken to be).  No reference counterpart (its modules index with torch). */
+ * products in fp32, rounded once.  T below 2^26, T*k below 2^31, H below 2^24; moe_sort_rows and moe_unsort_rows also refuse
+ * rows of more than 4194240 pieces (16 bytes each, single elements off those boundaries).  A result over what is read, or over the other
+ * gradient, is refused (arrays whose spans meet are taken to be).  No reference counterpart (its modules index with torch). */
 int moe_sort_rows(const void *x, int64_t ldx, void *y, int64_t ldy, const int *pos_of_pair, const int *total, int T, int k, int H,
                   int dtype, void *stream);
 int moe_unsort_rows(const void *x, int64_t ldx, void *y, int64_t ldy, const int *pos_of_pair, const float *w, int T, int k, int H,

@@ -240,6 +240,14 @@ static dim3 move_grid(MoveArgs &a) {
   return dim3((a.T + rows - 1) / rows, (a.units + (1 << a.cs) - 1) >> a.cs);
 }
 
+// (the second dimension of a grid ends at 65535: 64 pieces each)
+static int move_pieces(const char *who, const MoveArgs &a, dim3 grid) {
+  if (grid.y <= 65535) return MOE_OK;
+  moe_set_error("%s: rows of %d elements are %d pieces (16 bytes each, single elements where rows are not on 16-byte boundaries), 4194240 at most",
+                who, a.H, a.units);
+  return MOE_EINVAL;
+}
+
 extern "C" int moe_sort_rows(const void *x, int64_t ldx, void *y, int64_t ldy, const int *pos_of_pair, const int *total, int T, int k,
                              int H, int dtype, void *stream) {
   if (int rc = move_check("moe_sort_rows", T, k, H, dtype, ldx, ldy, x && y && pos_of_pair && total)) return rc;
@@ -255,10 +263,7 @@ extern "C" int moe_sort_rows(const void *x, int64_t ldx, void *y, int64_t ldy, c
   const bool wide = move_wide(x, ldx) && move_wide(y, ldy) && (long long)H * size % 16 == 0;
   a.units = wide ? H * size / 16 : H;
   const dim3 grid = move_grid(a);
-  if (grid.y > 65535) {
-    moe_set_error("moe_sort_rows: rows of %d elements that are not on 16-byte boundaries", H);
-    return MOE_EINVAL;
-  }
+  if (int rc = move_pieces("moe_sort_rows", a, grid)) return rc;
   if (wide) hipLaunchKernelGGL(k_sort_rows<u32x4_t>, grid, dim3(256), 0, (hipStream_t)stream, a);
   else if (size == 4) hipLaunchKernelGGL(k_sort_rows<u32>, grid, dim3(256), 0, (hipStream_t)stream, a);
   else hipLaunchKernelGGL(k_sort_rows<uint16_t>, grid, dim3(256), 0, (hipStream_t)stream, a);
@@ -307,10 +312,7 @@ extern "C" int moe_unsort_rows(const void *x, int64_t ldx, void *y, int64_t ldy,
   const bool wide = move_wide(x, ldx) && move_wide(y, ldy) && (long long)H * size % 16 == 0;
   a.units = wide ? H * size / 16 : H;
   const dim3 grid = move_grid(a);
-  if (grid.y > 65535) {
-    moe_set_error("moe_unsort_rows: rows of %d elements that are not on 16-byte boundaries", H);
-    return MOE_EINVAL;
-  }
+  if (int rc = move_pieces("moe_unsort_rows", a, grid)) return rc;
   MOVE_TYPES(unsort_launch, wide, a, grid, (hipStream_t)stream)
   return moe_check_launch("k_unsort_rows");
 }

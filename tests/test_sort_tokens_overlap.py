@@ -45,3 +45,13 @@ def test_the_gradient_of_no_tokens_is_nothing():
     from promoe_amd import _lib as L
     assert L.lib.moe_unsort_rows_grad(None, H, None, H, None, None, None, None, H, None, 0, K, H, 0, None) == 0
     assert L.lib.moe_unsort_rows_grad(D, H, X, H, POS, W, N, Y, H, DW, 0, K, H, 0, None) == 0
+
+
+@pytest.mark.parametrize("dtype,h,off", [(2, 16776964, 0), (2, (1 << 24) - 4, 0), (2, 4194241, 4), (0, 4194241, 2), (1, (1 << 24) - 1, 0)])
+def test_rows_of_too_many_pieces_are_refused_by_their_number(dtype, h, off):
+    """One more than 65535 workgroups of 64 pieces, on 16-byte boundaries or not."""
+    from promoe_amd import _lib as L
+    x, y, ld = (1 << 40) + off, 1 << 42, (h + 7) // 8 * 8
+    pieces = h // 4 if dtype == 2 and h % 4 == 0 and not off else h
+    for rc in (L.lib.moe_sort_rows(x, ld, y, ld, POS, N, 1, 1, h, dtype, None), L.lib.moe_unsort_rows(x, ld, y, ld, POS, W, 1, 1, h, dtype, None)):
+        assert rc == L.MOE_EINVAL and b"%d pieces" % pieces in L.lib.moe_last_error(), L.lib.moe_last_error()
