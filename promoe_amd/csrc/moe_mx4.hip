@@ -995,9 +995,14 @@ __global__ __launch_bounds__(256, RING * (WM * 64 * 256 + WN * 64 * 64 + 1024) >
 }
 
 // ---- entry points -------------------------------------------------------------------------------------------------------------
+// Do na rows of len_a bytes, la apart, share a byte with nb rows of len_b bytes, lb apart?  (Rows side by side in one buffer, the same
+// distance apart, do not; rows of different distances whose ranges meet are taken to.)
 static bool mx_meet(const void *a, int64_t na, int64_t la, int64_t len_a, const void *b, int64_t nb, int64_t lb, int64_t len_b) {
   const char *p = (const char *)a, *q = (const char *)b;
-  return p && q && na > 0 && nb > 0 && len_a > 0 && len_b > 0 && p < q + (nb - 1) * lb + len_b && q < p + (na - 1) * la + len_a;
+  if (!p || !q || na <= 0 || nb <= 0 || len_a <= 0 || len_b <= 0 || p >= q + (nb - 1) * lb + len_b || q >= p + (na - 1) * la + len_a) return false;
+  if (la != lb || la <= 0) return true;
+  const int64_t d = ((p - q) % lb + lb) % lb;
+  return d < len_b || d + len_a > lb;
 }
 extern "C" int64_t moe_mx4_scale_bytes(int64_t rows, int K) {
   return rows <= 0 || K <= 0 ? 0 : (rows + 31) / 32 * mx_slabs(K) * 256;
@@ -1080,7 +1085,7 @@ static int mx_check(const char *who, const MxArgs &a, int xkind, int64_t xrows, 
   auto meets = [&](const void *p, int64_t rows, int64_t ld, int64_t len) { return mx_meet(a.y, a.M, yld, ylen, p, rows, ld, len); };
   bool shares = meets(a.x, xrows, a.ldx, xlen) || (xkind == X_MX4 && meets(a.xs, 1, 0, moe_mx4_scale_bytes(xrows, a.K)));
   for (int i = 0; i < (gated ? 2 : 1); ++i) {
-    shares = shares || meets(a.w[i], 1, 0, (experts - 1) * a.ew + (a.N - 1) * a.ldw + wlen) ||
+    shares = shares || (experts == 1 ? meets(a.w[i], a.N, a.ldw, wlen) : meets(a.w[i], 1, 0, (experts - 1) * a.ew + (a.N - 1) * a.ldw + wlen)) ||
              meets(a.ws[i], 1, 0, (experts - 1) * a.ews + moe_mx4_scale_bytes(a.N, a.K)) || meets(a.bias[i], 1, 0, 2ll * experts * a.N);
   }
   const bool in_place = a.res == a.y && !a.y32 && (a.ldr == a.ldy || a.M == 1);
