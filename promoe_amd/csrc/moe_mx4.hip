@@ -1270,6 +1270,11 @@ extern "C" int moe_mx4_experts(const void *x, int64_t ldx, const moe_mx4 *xq, co
     return MOE_EINVAL;
   }
   if (int rc = mx_check("moe_mx4_experts", a, xkind, sorted_tok ? T : P, E, dtype, w_up != nullptr)) return rc;
+  auto meets = [&](const void *p, int64_t bytes) { return mx_meet(y, P, ldy * (a.y32 ? 4 : 2), N * (a.y32 ? 4ll : 2ll), p, 1, 0, bytes); };
+  if (meets(counts, 4ll * E) || meets(offsets, 4ll * E + 4) || meets(units, (int64_t)sizeof(moe_unit) * max_units) || meets(sorted_tok, 4ll * P)) {
+    moe_set_error("moe_mx4_experts: the result overlaps the dispatch");
+    return MOE_EINVAL;
+  }
   if (sorted_tok && T * a.ldx > LT_OUT) {  // (offsets of gathered rows are those of a buffer resource)
     moe_set_error("moe_mx4_experts: %d rows of tokens %lld bytes apart (less than 2 GiB are needed)", T, a.ldx);
     return MOE_EINVAL;
