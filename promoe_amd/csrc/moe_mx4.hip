@@ -1254,6 +1254,15 @@ extern "C" int moe_mx4_linear(const void *x, int64_t ldx, const moe_mx4 *xq, con
     moe_set_error("moe_mx4_linear: a workspace of %lld bytes on a 16-byte boundary is needed", (long long)need);
     return MOE_EINVAL;
   }
+  auto meets = [&](const void *p, int64_t rows, int64_t ld, int64_t len) { return mx_meet(ws, 1, 0, need, p, rows, ld, len); };
+  bool shares = meets(y, M, ldy * (a.y32 ? 4 : 2), N * (a.y32 ? 4ll : 2ll)) || meets(a.x, M, a.ldx, xq ? K / 2 : K * 2ll) ||
+                meets(residual, M, ldr * 2, N * 2ll) || (xq && meets(a.xs, 1, 0, moe_mx4_scale_bytes(M, K)));
+  for (int i = 0; i < (w_up ? 2 : 1); ++i)
+    shares = shares || meets(a.w[i], N, a.ldw, K / 2) || meets(a.ws[i], 1, 0, moe_mx4_scale_bytes(N, K)) || meets(a.bias[i], 1, 0, 2ll * N);
+  if (shares) {
+    moe_set_error("moe_mx4_linear: the workspace overlaps an operand or the result");
+    return MOE_EINVAL;
+  }
   return mx_run(a, xkind, dtype, w_up != nullptr, 1, M, (float *)ws, (hipStream_t)stream);
 }
 
