@@ -541,6 +541,10 @@ int moe_mx4_dequantize(const moe_mx4 *q_host, int E, int M, int K, void *y, int6
  * with sorted_tok, of the rows sorted_tok[..] of x (T of them, one for each token; else P), with matrix e; bias [E, N].  Rows behind the last pair are left as
  * they were.  E <= 1024, max_units >= min(E, P). */
 int64_t moe_mx4_linear_workspace_bytes(int M, int N, int K, int x_mx4, int gated);
+/* Which kernel a product takes, for tests and measurements (on the host): plan[0], plan[1] rows of x and of W of a tile (0, 0: W streams
+ * past few rows), plan[2] slabs of K in LDS, plan[3] pieces of K.  rows: of all products together; units: min(E, P) of products by expert,
+ * 0 of a dense one. */
+int moe_mx4_plan(int64_t rows, int units, int N, int K, int x_mx4, int gated, int *plan_host);
 int moe_mx4_linear(const void *x, int64_t ldx, const moe_mx4 *xq_host, const moe_mx4 *w_host, const moe_mx4 *w_up_host, const void *bias,
                    const void *bias_up, const void *residual, int64_t ldr, void *y, int64_t ldy, int M, int N, int K, int dtype, int act,
                    int y_fp32, void *ws, int64_t ws_bytes, void *stream);

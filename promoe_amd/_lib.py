@@ -68,6 +68,7 @@ _sig("moe_unsort_rows_grad", [vp, i64, vp, i64, vp, vp, vp, vp, i64, vp, i32, i3
 _sig("moe_mx4_scale_bytes", [i64, i32], i64)
 _sig("moe_mx4_quantize", [vp, i64, i64, i32, i32, i32, i32, vp, vp])
 _sig("moe_mx4_dequantize", [vp, i32, i32, i32, vp, i64, i64, i32, vp])
+_sig("moe_mx4_plan", [i64, i32, i32, i32, i32, i32, vp])
 _sig("moe_mx4_linear_workspace_bytes", [i32] * 5, i64)
 _sig("moe_mx4_linear", [vp, i64, vp, vp, vp, vp, vp, vp, i64, vp, i64, i32, i32, i32, i32, i32, i32, vp, i64, vp])
 _sig("moe_mx4_experts", [vp, i64, vp, vp, vp, vp, vp, vp, i64, vp, vp, vp, i32, vp, i32, i32, i32, i32, i32, i32, i32, i32, vp])

@@ -1144,6 +1144,15 @@ extern "C" int64_t moe_mx4_linear_workspace_bytes(int M, int N, int K, int x_mx4
   const MxPlan p = mx_plan(x_mx4 ? X_MX4 : X_BF16, M, 0, N, K, gated != 0);
   return p.splits > 1 ? (int64_t)p.splits * (gated ? 2 : 1) * M * ((N + 7) & ~7) * 4 : 0;
 }
+extern "C" int moe_mx4_plan(int64_t rows, int units, int N, int K, int x_mx4, int gated, int *plan) {
+  if (rows <= 0 || units < 0 || N <= 0 || K <= 0 || !plan) {
+    moe_set_error("moe_mx4_plan: bad argument (rows=%lld units=%d N=%d K=%d)", (long long)rows, units, N, K);
+    return MOE_EINVAL;
+  }
+  const MxPlan p = mx_plan(x_mx4 ? X_MX4 : X_BF16, rows, units, N, K, gated != 0);
+  plan[0] = 64 * p.wm; plan[1] = 64 * p.wn; plan[2] = p.ring; plan[3] = p.splits;
+  return MOE_OK;
+}
 template <int X, bool F16, bool GATED>
 static int mx_launch(const MxArgs &a, int units, int most, float *ws, hipStream_t s) {  // most: rows that one expert (or the product) can have
   const MxPlan pl = mx_plan(X, a.M, a.units ? units : 0, a.N, a.K, GATED);
