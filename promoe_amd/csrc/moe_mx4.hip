@@ -21,7 +21,7 @@ typedef _Float16 f16x2_t __attribute__((ext_vector_type(2)));
 // ---- rows into codes and back ---------------------------------------------------------------------------------------------------
 // Scales lie in blocks of 32 rows by 8 bytes (256 columns, a slab of the products below), so that what 32 rows need of a slab is 256 bytes
 // in one piece: byte kb of row r at ((r / 32) slabs + kb / 8) 256 + (r % 32) 8 + kb % 8.  Row by row, as they are exchanged, every row would
-// cost the products a cache line for 8 bytes (4096 x 4096 x 14336 in 4 bits: 216 us, with blocks 167).
+// cost the products a cache line for 8 bytes, by count as much traffic as the codes (not timed by itself).
 static __host__ __device__ __forceinline__ int mx_slabs(int K) { return (K + 255) >> 8; }
 static __device__ __forceinline__ long long mx_scale_row(long long r, int slabs) { return (r >> 5) * (slabs * 256ll) + (r & 31) * 8; }
 struct QuantArgs {
@@ -183,13 +183,14 @@ static __device__ __forceinline__ void mx_split(u32x4_t x, u32x4_t &hi, u32x4_t 
 }
 
 // ---- few rows of x: the matrix streams past them --------------------------------------------------------------------------------
-// A workgroup of eight waves takes R = 16 / SH rows of W (gated: of both matrices), its waves the pieces of K in turn; their sums meet
-// in LDS.  A lane's load is one block, 32 columns of a row: with SH = 1 the 16 rows of the operand are 16 rows of W, with few rows of x
+// A workgroup of four or eight waves takes NB sets of R = 16 / SH rows of W (gated: of both matrices), its waves the pieces of K in turn;
+// their sums meet in LDS.  A lane's load is one block, 32 columns of a row: with SH = 1 the 16 rows of the operand are 16 rows of W, with few rows of x
 // (at most 16 / SH) R rows of W by SH pieces of K: row s R + r and column s R + m hold piece s of both, and the products of unlike
 // pieces are left unread.  By expert the second dimension of the grid is a unit of the dispatch; more than 16 rows go in turn.
 // NB: sets of R rows a workgroup takes, all against the same operand of x; U: loads of a set in flight per wave, twice.  Four waves, U = 1:
 // what counts is how soon a workgroup's trip to memory begins and ends (us, U = 1 / 2: 1 x 14336 x 4096 gated 17.9 / 19.1; waves 4 / 8: 17.9 / 18.8).
-// Bound by memory where it is long enough: 20 tokens of 64 experts, 1408 x 2048 gated, 38 us (4.4 TB/s).
+// Bound by memory where it is long enough: 20 tokens of 64 experts, 1408 x 2048 gated, 35 to 38 us (4.4 TB/s and more); 1 x 2048 x 10944, 6.6 us
+// (floor 2.3), is three trips to memory one behind the other for each wave, and the join.
 template <int X, bool F16, bool GATED, int SH, int NB, int U, int WAVES>
 __global__ __launch_bounds__(64 * WAVES) void k_mx4_rows(const MxArgs a) {
   constexpr int MATS = GATED ? 2 : 1, NM = MATS * NB, R = 16 / SH, STEP = 4 * SH * U, SPAN = STEP * WAVES, NX = X == X_MX4 ? 1 : 4;
@@ -532,7 +533,7 @@ __global__ __launch_bounds__(256) void k_mx4_join(const MxArgs a) {
 // of a column.  K advances 256 at a time (a slab: 128 bytes of codes and 8 of scales a row); slabs go global -> LDS directly, RING of them
 // in LDS.  A lane's operand of a product is one block of 32 columns: half q of the wave takes the blocks 4 q .. 4 q + 3 of a slab, so that
 // the scales of a fragment's four steps are one word, a byte a step.  Where K is short two workgroups a compute unit (RING 2) do
-// better than one with a longer ring: 2048 tokens of 64 experts, WM 1, WN 2, RING 4 / 2: 139 / 94 us.
+// better than one with a longer ring: 2048 tokens of 64 experts, WM 1, WN 2, RING 4 / 2: 139 / 94 us (k_mx4_wide, which the plan takes there: 79).
 #define M4_K 256
 static __device__ __forceinline__ void mx_dma16(unsigned at, int off, lt_rsrc_t rs, int soff) {
   // (assembly: told that a load writes LDS, the compiler would wait for all of them in front of every barrier and LDS read; the waits
@@ -682,7 +683,9 @@ __global__ __launch_bounds__(256, RING * (WM + WN) * 64 * 136 > 80 * 1024 ? 1 : 
 // fragments are read step by step.  Two slabs in LDS.  The fragments of a whole slab fit the registers (four steps of eight), and they are
 // read as early as the slab is there: in the middle of its step 1 everybody has all of it, so its place takes the slab after next from
 // then on, more than a slab's time in front of the first read of that.
-// 4096 x 4096 x 14336 108 to 124 us (3.9 to 4.5 PFLOP/s): about 2590 cycles a slab for 2048 of products (from counters at two K), at 1.82 GHz (power).
+// 4096 x 4096 x 14336 108 to 124 us (3.9 to 4.5 PFLOP/s).  4096 x 4096, one round of tiles, K 1024 / 2048 / 4096 / 8192 / 11264 / 14336: 20.9 / 27.4 / 41.4 /
+// 71.3 / 90.4 / 111.2 us, so 1.7 us a slab (2048 cycles of products, which are 0.85 us at 2.4 GHz) and 14 us of start and write-out, which nothing
+// hides.  Why a slab takes twice its products' cycles is not separated: the clock under this load, LDS and waits all have a part.
 template <bool F16, bool GATED>
 __global__ __launch_bounds__(256, 1) void k_mx4_wide(const MxArgs a) {
   constexpr int B = 256, NB = 4, NX = 8, NW = 8, NS = 4, NT = NX + NW + NS;
@@ -816,7 +819,8 @@ static __device__ __forceinline__ f32x16_t mx_mfma32_bf16(u32x4_t a, u32x4_t b, 
 // x in 16 bits: the same tile, K 128 at a time (256 bytes of a row of x, 64 of codes, one word of scales).  Half q of the wave takes the
 // columns 64 q .. 64 q + 63 of a slab, eight a step: blocks 2 q and 2 q + 1 of W, which become bf16 in front of their products.
 // Chunk c (16 bytes) of row r of x stands in slot c ^ (r & 15), of W in slot c ^ ((r >> 2) & 3).  Bound by LDS, which x fills: wide tiles are the
-// better ones (2048 tokens of 64 experts, us: 64 x 256 166, 128 x 128 209).  4096 x 4096 x 14336 418 to 441 us (1090 to 1150 TFLOP/s).
+// better ones (2048 tokens of 64 experts, us: 64 x 256 166, 128 x 128 209).  4096 x 4096 x 14336 374 to 441 us (1090 to 1290 TFLOP/s);
+// past 2048 rows (fp16: 1024) weights expanded by k_mx4_dequantize and the product of 16-bit matrices are mostly faster (327 together).
 #define M16_K 128
 template <int X, bool GATED, int WM, int WN, int RING>
 __global__ __launch_bounds__(256, RING * (WM * 64 * 256 + WN * 64 * 64 + 1024) > 80 * 1024 ? 1 : 2) void k_mx4_tile16(const MxArgs a) {
@@ -885,7 +889,9 @@ __global__ __launch_bounds__(256, RING * (WM * 64 * 256 + WN * 64 * 64 + 1024) >
   for (int i = 0; i < RING; ++i)
 #pragma unroll
     for (int d = 0; d < NT; ++d) dma(d, kt0 + i, i * SLAB);
-  // fp16: can all weights of this wave be fp16?  Decided by all of their scales (a sixteenth of the codes' bytes) while the ring fills
+  // fp16: can all weights of this wave be fp16?  Decided by all of their scales (a sixteenth of the codes' bytes) while the ring fills.
+  // One scale outside of 104 .. 140, such as the 0 of a block of zeros, sends the wave's rows of W through the split form for all of K:
+  // 4096 x 4096 x 14336 with such a block in every 32 rows 958 us (without 435), 379 x 1409 x 2048 28.8 (9.8).
   bool fits = false;
   if constexpr (F16) {
     u16x2_t least{127, 127}, most{127, 127};
@@ -1096,8 +1102,9 @@ static int mx_check(const char *who, const MxArgs &a, int xkind, int64_t xrows, 
   return MOE_OK;
 }
 // Which kernel a product takes: few rows (wm 0), or tiles of 64 wm x 64 wn with `ring` slabs in LDS (4 x 4: the wide kernel), dense ones
-// with K in `splits` pieces.  The plan of the least time after a model of one launch, us, fitted to 11000 measured times of 140 shapes (17 to 4096
-// rows; the chosen plan is 2 % slower than the best of all on average, 31 % at worst):
+// with K in `splits` pieces.  The plan of the least time after a model of one launch, us, fitted to measured times of dense products (12 matrices, 286
+// products of 17 to 4096 rows for each kind of x, 12000 times in all; the chosen plan is 2.4 % (16-bit x 2.1 %) slower than the best of all
+// on average, 31 % (20 %) at worst).  By expert it is an estimate from the average rows of an expert, not fitted:
 //   start + rounds x (slabs x (c0 + c1 x share of the compute units in use) + f),  with pieces j0 + j1 a piece + j2 per MB of partial sums
 // c0, c1: a slab of a workgroup on an idle chip, and what the others' traffic adds; f: first slab and epilogue.
 struct MxPlan { int wm, wn, ring, splits; float us; };

@@ -809,7 +809,9 @@ def linear_mx4(x, w: Mx4, bias: torch.Tensor | None = None, act: str = "none", r
     """act(x w^T + bias) + residual in one pass (moe_mx4_linear), w [N, K] an Mx4.  x [M, K] either bf16 or fp16, whose values take part
     as they are, or an Mx4 (quantize_mx4), then both operands go to the matrix cores in 4 bits.  bias, residual and the result are of
     x's type, or for an Mx4 all bf16 or all fp16 (the result: out_dtype, else theirs, else bf16); out_dtype fp32 leaves the sums in 32
-    bits.  Activations, strides and the rest as in linear, K a multiple of 32."""
+    bits.  Activations, strides and the rest as in linear, K a multiple of 32.  A 16-bit x of more than 2048 rows (fp16: 1024) is mostly
+    faster through dequantize_mx4 and linear.  With an fp16 x, scales of w outside of 2^-23 .. 2^13 (a block of zeros has 2^-127) cost two to
+    three times the products' time."""
     return _product_mx4("linear_mx4", x, w, None, bias, None, act, residual, out, out_dtype)
 
 
@@ -933,9 +935,9 @@ def _move_args(what, x, d, rows, w):
 
 def sort_tokens(x: torch.Tensor, d: Dispatch) -> torch.Tensor:
     """The tokens' rows x [T, H] in the order of their experts: [T*k, H], a token's row once for each of its choices (moe_sort_rows).
-    Choices of no expert (idx outside 0 .. E - 1) have no row; the rows behind the last one are zero.  Any alignment and row stride, bf16,
-    fp16 or fp32.  With a gradient, not a second or a forward-mode one (each token the sum of its rows', in fp32): d has to keep its contents until the
-    backward pass."""
+    Choices of no expert (idx outside 0 .. E - 1) have no row; the rows behind the last one are zero.  Any alignment, rows whole and at
+    least H elements apart (an expanded row is refused), bf16, fp16 or fp32.  With a gradient (each token the sum of its rows', in fp32),
+    not a second or a forward-mode one: d has to keep its contents until the backward pass."""
     index, ldx = _move_args("sort_tokens", x, d, d.T, None)
     if index != torch.cuda.current_device():
         with torch.cuda.device(index):
